@@ -18,6 +18,9 @@ from .api import (  # noqa: F401
     quantize_block128,
     quantize_rows128,
     dequantize_block128,
+    quantize_mxfp4,
+    dequantize_mxfp4,
+    gemm_mxfp4,
     transpose,
 )
 from . import api  # noqa: F401

@@ -15,6 +15,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 _LIB_PATH = os.path.join(_HERE, "libmoe355.so")
 
 DTYPE_F32, DTYPE_TF32, DTYPE_BF16, DTYPE_FP16, DTYPE_FP8 = 0, 1, 2, 3, 4
+DTYPE_MXFP4 = 16               # operands of the MXFP4 entry points (no layer's torch_dtype)
+FEW_TOKENS = 16                # tokens that MoELayer.forward_few takes at most
 ACT_RELU, ACT_GELU, ACT_SWIGLU, ACT_NONE = 0, 1, 2, 3
 GATE_SOFTMAX, GATE_SIGMOID = 0, 1
 FFN_AUTO, FFN_TILED, FFN_PERSISTENT = 0, 1, 2
@@ -29,7 +31,7 @@ EXPORTS = (
     "moe_set_ffn_mode", "moe_get_ffn_mode", "moe_forward", "moe_forward_static", "moe_set_spin_limit", "moe_clear_stall", "moe_gate", "moe_router_stats", "moe_route", "moe_gemm_bias_act", "moe_combine",
     "moe_set_stage_timing", "moe_get_stage_ms", "moe_get_stage_samples", "moe_get_task_counts", "moe_get_queue_balance", "moe_task_trace_bytes", "moe_set_task_trace", "moe_get_task_trace", "moe_measure_mfma_tflops",
     "moe_measure_hbm_read_gbs", "moe_quant_block128", "moe_dequant_block128", "moe_backward_scratch_bytes", "moe_transpose", "moe_expert_gemm",
-    "moe_expert_gemm_act_backward", "moe_expert_gemm_act_backward_supported", "moe_expert_gemm_kn", "moe_expert_gemm_kn_supported", "moe_expert_gemm_pair", "moe_expert_gemm_kn_pair", "moe_expert_wgrads", "moe_expert_wgrad", "moe_act_backward", "moe_bias_grad", "moe_combine_backward", "moe_dispatch_rows", "moe_act_forward", "moe_dispatch_backward", "moe_router_grad_bytes", "moe_combine_router_backward", "moe_dispatch_router_backward", "moe_gate_wgrad", "moe_gate_wgrad_rows", "moe_last_hip_error", "moe_status_string",
+    "moe_expert_gemm_act_backward", "moe_expert_gemm_act_backward_supported", "moe_expert_gemm_kn", "moe_expert_gemm_kn_supported", "moe_expert_gemm_pair", "moe_expert_gemm_kn_pair", "moe_expert_wgrads", "moe_expert_wgrad", "moe_act_backward", "moe_bias_grad", "moe_combine_backward", "moe_dispatch_rows", "moe_act_forward", "moe_dispatch_backward", "moe_router_grad_bytes", "moe_combine_router_backward", "moe_dispatch_router_backward", "moe_gate_wgrad", "moe_gate_wgrad_rows", "moe_quant_mxfp4", "moe_dequant_mxfp4", "moe_gemm_mxfp4", "moe_expert_gemm_mxfp4", "moe_forward_few", "moe_last_hip_error", "moe_status_string",
     "moe_version",
 )
 
@@ -80,6 +82,10 @@ class _CArch(C.Structure):
 class _CWeights(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("gate_w", "gate_bias", "w_up", "w_gate", "w_down", "b_up", "b_gate",
                                           "b_down", "s_up", "s_gate", "s_down", "prepared")]
+
+
+class _CMxfp4Scales(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("s_up", "s_gate", "s_down")]
 
 
 class _CRouting(C.Structure):
@@ -174,6 +180,11 @@ def load_library():
     L.moe_combine_router_backward.argtypes = [vp] * 10
     L.moe_dispatch_router_backward.argtypes = [vp] * 9
     L.moe_gate_wgrad.argtypes = L.moe_gate_wgrad_rows.argtypes = [vp, vp, vp, vp, vp, C.c_size_t, vp]
+    L.moe_quant_mxfp4.argtypes = [vp, i32, i64, i64, vp, vp, vp]
+    L.moe_dequant_mxfp4.argtypes = [vp, vp, i64, i64, i32, vp, vp]
+    L.moe_gemm_mxfp4.argtypes = [vp, vp, i32, vp, vp, vp, vp, i64, i64, i64, i32, vp]
+    L.moe_expert_gemm_mxfp4.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, vp, vp]
+    L.moe_forward_few.argtypes = [vp, vp, C.POINTER(_CWeights), C.POINTER(_CMxfp4Scales), vp, C.POINTER(_CRouting), vp, C.c_size_t, vp]
     L.moe_last_hip_error.argtypes = [vp]
     L.moe_status_string.argtypes = [C.c_int]; L.moe_status_string.restype = C.c_char_p
     L.moe_version.restype = C.c_int
@@ -259,6 +270,23 @@ def _operand(name, t, dtype, elements=0):
         raise TypeError("%s is %s: expected %s" % (name, t.dtype, dtype))
     if t.numel() < elements:
         raise ValueError("%s holds %d elements: at least %d are read" % (name, t.numel(), elements))
+
+
+def _device_operand(name, t, dtype, shape):
+    """_operand, and a tensor of exactly this shape that lies on the current device in one piece."""
+    if t.dtype != dtype:
+        raise TypeError("%s is %s: expected %s" % (name, t.dtype, dtype))
+    if t.shape != shape:
+        raise ValueError("%s has shape %s: expected %s" % (name, tuple(t.shape), tuple(shape)))
+    if not t.is_contiguous():
+        raise ValueError("%s must be contiguous (row-major, K innermost)" % name)
+    _on_current_device(name, t)
+
+
+def _on_current_device(name, t):
+    import torch
+    if not t.is_cuda or t.get_device() != torch.cuda.current_device():
+        raise ValueError("%s lies on %s: expected the current GPU" % (name, t.device))
 
 
 def _stream():
@@ -488,6 +516,101 @@ class MoELayer:
         else:
             _check(self.L.moe_forward(self._h, _ptr(x), C.byref(w), _ptr(out), rp, _ptr(self.workspace),
                                       self.workspace_bytes, _stream()), "moe_forward")
+        return out
+
+    def _mxfp4_weights(self, weights: dict) -> bool:
+        """Whether the expert weights are MXFP4 codes (their scales are bytes)."""
+        import torch
+        s = weights.get("s_up")
+        return s is not None and s.dtype == torch.uint8
+
+    def forward_few(self, x, weights: dict, out=None, routing: dict | None = None):
+        """out[S,H] = MoE(x) for at most 16 tokens of a bf16 or fp16 layer, in two launches (three with a large router).  Expert weights in
+        the layer's type, or (bf16 layers) in MXFP4: w_* from quantize_mxfp4 as uint8 [E,N,K/2], s_* as uint8 [E,N,K/32].  `routing` (from
+        new_routing()) receives the routing result when given."""
+        import torch
+        cfg, act = self.cfg, self.act_dtype
+        S, H, I, E = self.S, self.H, cfg.intermediate_size, self.E
+        mx = self._mxfp4_weights(weights)
+        unknown = set(weights) - set(self.WEIGHT_KEYS)
+        if unknown:
+            raise ValueError("unknown tensors %s" % sorted(unknown))
+        w, sc = _CWeights(), _CMxfp4Scales()
+        for name, t in weights.items():
+            if t is None:
+                continue
+            if name == "gate_w":
+                _device_operand(name, t, act, (E, H))
+            elif name == "gate_bias":
+                _device_operand(name, t, torch.float32, (E,))
+            else:
+                N, K = (H, I) if name.endswith("down") else (I, H)
+                if name[0] == "b":
+                    _device_operand(name, t, act, (E, N))
+                elif name[0] == "w":
+                    _device_operand(name, t, torch.uint8 if mx else act, (E, N, K // 2 if mx else K))
+                elif mx and name[:2] == "s_":
+                    _device_operand(name, t, torch.uint8, (E, N, K // 32))
+                    setattr(sc, name, t.data_ptr())
+                    continue
+            setattr(w, name, t.data_ptr())
+        _device_operand("x", x, act, (S, H))
+        if out is None:
+            out = torch.empty(S, H, dtype=act, device=x.device)
+        else:
+            _device_operand("out", out, act, (S, H))
+        r = None if routing is None else C.byref(_CRouting(*[routing[n].data_ptr() for n, _ in _CRouting._fields_]))
+        _check(self.L.moe_forward_few(self._h, _ptr(x), C.byref(w), C.byref(sc) if mx else None, _ptr(out), r, _ptr(self.workspace),
+                                      self.workspace_bytes, _stream()), "moe_forward_few")
+        return out
+
+    def forward_mxfp4(self, x, weights: dict):
+        """out[S,H] = MoE(x) of a bf16 layer whose expert weights are in MXFP4, for any number of tokens: forward_few for a few, else the
+        stages one by one, the projections by expert_gemm_mxfp4."""
+        import torch
+        if self.S <= FEW_TOKENS:
+            return self.forward_few(x, weights)
+        if not self._mxfp4_weights(weights):
+            raise TypeError("forward_mxfp4 takes expert weights from quantize_mxfp4")
+        cfg = self.cfg
+        _device_operand("x", x, self.act_dtype, (self.S, self.H))
+        _device_operand("gate_w", weights["gate_w"], self.act_dtype, (self.E, self.H))
+        idx, gate = self.gate(x, weights["gate_w"], weights.get("gate_bias"))
+        r = self.route(idx)
+        count, offset = r["expert_count"], r["expert_offset"]
+        rows = self.dispatch_rows(x, r["token_indices"])
+
+        def project(a, name, act):
+            return self.expert_gemm_mxfp4(a, weights["w_" + name], weights["s_" + name], weights.get("b_" + name), count, offset, act=act)
+
+        if cfg.hidden_act == ACT_SWIGLU:
+            h = self.act_forward(project(rows, "up", ACT_NONE), project(rows, "gate", ACT_NONE), count, offset)
+        else:
+            h = project(rows, "up", cfg.hidden_act)
+        return combine(project(h, "down", ACT_NONE), r["pair_row"], gate)
+
+    def expert_gemm_mxfp4(self, a_rows, w, w_scales, bias, expert_count, expert_offset, act: int = ACT_NONE, a_scales=None, out=None):
+        """expert_gemm on weights in MXFP4: w uint8 [E,N,K/2], w_scales uint8 [E,N,K/32]; a_rows bf16 [S k,K], or uint8 [S k,K/2] with
+        a_scales uint8 [S k,K/32].  Rows of no expert are not written."""
+        import torch
+        N, K, A = w.shape[1], 2 * w.shape[2], self.S * self.k
+        _device_operand("w", w, torch.uint8, (self.E, N, K // 2))
+        _device_operand("w_scales", w_scales, torch.uint8, (self.E, N, K // 32))
+        if a_scales is None:
+            _device_operand("a_rows", a_rows, torch.bfloat16, (A, K))
+        else:
+            _device_operand("a_rows", a_rows, torch.uint8, (A, K // 2))
+            _device_operand("a_scales", a_scales, torch.uint8, (A, K // 32))
+        if bias is not None:
+            _device_operand("bias", bias, torch.bfloat16, (self.E, N))
+        for name, t in (("expert_count", expert_count), ("expert_offset", expert_offset)):
+            _device_operand(name, t, torch.int32, (self.E,))
+        if out is None:
+            out = torch.empty(A, N, dtype=torch.bfloat16, device=w.device)
+        else:
+            _device_operand("out", out, torch.bfloat16, (A, N))
+        _check(self.L.moe_expert_gemm_mxfp4(self._h, _ptr(a_rows), _ptr(a_scales), _ptr(w), _ptr(w_scales), _ptr(bias), _ptr(expert_count),
+                                            _ptr(expert_offset), N, K, act, _ptr(out), _stream()), "moe_expert_gemm_mxfp4")
         return out
 
     def set_spin_limit(self, polls: int):
@@ -849,6 +972,72 @@ def dequantize_block128(q, s):
     out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
     _check(load_library().moe_dequant_block128(_ptr(q), _ptr(s), mats, N, K, _ptr(out), _stream()),
            "moe_dequant_block128")
+    return out
+
+
+def _mx_dtype(dtype):
+    import torch
+    known = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_FP16}
+    if dtype not in known:
+        raise TypeError("%s: MXFP4 values come from and go to fp32, bf16 or fp16" % dtype)
+    return known[dtype]
+
+
+def quantize_mxfp4(x):
+    """[.., K] fp32, bf16 or fp16 values on the GPU, K a multiple of 32 -> (uint8 codes [.., K/2], uint8 scales [.., K/32]): MXFP4, two
+    e2m1 values a byte (the even index in the low half) and one power of two for 32 of them."""
+    import torch
+    dtype, K = _mx_dtype(x.dtype), x.shape[-1] if x.dim() else 0
+    if K < 32 or K % 32:
+        raise ValueError("quantize_mxfp4 takes rows of a multiple of 32 values, not %d" % K)
+    _on_current_device("x", x)
+    x = x.contiguous()
+    if x.data_ptr() % 16:
+        x = x.clone()
+    codes = torch.empty(*x.shape[:-1], K // 2, dtype=torch.uint8, device=x.device)
+    scales = torch.empty(*x.shape[:-1], K // 32, dtype=torch.uint8, device=x.device)
+    _check(load_library().moe_quant_mxfp4(_ptr(x), dtype, x.numel() // K, K, _ptr(codes), _ptr(scales), _stream()), "moe_quant_mxfp4")
+    return codes, scales
+
+
+def dequantize_mxfp4(codes, scales, dtype=None):
+    """The values of codes [.., K/2] and scales [.., K/32] (as quantize_mxfp4 gives them) in `dtype`: bf16 unless given, fp32 or fp16."""
+    import torch
+    dtype = dtype or torch.bfloat16
+    kind = _mx_dtype(dtype)
+    K = 2 * codes.shape[-1] if codes.dim() else 0
+    if K < 32 or K % 32:
+        raise ValueError("rows of %d codes: MXFP4 rows hold a multiple of 32 values" % K)
+    codes, scales = codes.contiguous(), scales.contiguous()
+    _device_operand("codes", codes, torch.uint8, codes.shape)
+    _device_operand("scales", scales, torch.uint8, (*codes.shape[:-1], K // 32))
+    if codes.data_ptr() % 4:
+        codes = codes.clone()
+    out = torch.empty(*codes.shape[:-1], K, dtype=dtype, device=codes.device)
+    _check(load_library().moe_dequant_mxfp4(_ptr(codes), _ptr(scales), out.numel() // K, K, kind, _ptr(out), _stream()), "moe_dequant_mxfp4")
+    return out
+
+
+def gemm_mxfp4(A, w, w_scales, bias=None, act: int = ACT_NONE, a_scales=None):
+    """C [M,N] (bf16) = act(A.W^T + bias), W [N,K] in MXFP4 (codes [N,K/2], scales [N,K/32]); A bf16 [M,K], or in MXFP4 too: codes [M,K/2]
+    with a_scales [M,K/32]."""
+    import torch
+    if w.dim() != 2 or A.dim() != 2:
+        raise ValueError("gemm_mxfp4 takes matrices")
+    M, N, K = A.shape[0], w.shape[0], 2 * w.shape[1]
+    _device_operand("w", w, torch.uint8, (N, K // 2))
+    _device_operand("w_scales", w_scales, torch.uint8, (N, K // 32))
+    A = A.contiguous()
+    if a_scales is None:
+        _device_operand("A", A, torch.bfloat16, (M, K))
+    else:
+        _device_operand("A", A, torch.uint8, (M, K // 2))
+        _device_operand("a_scales", a_scales, torch.uint8, (M, K // 32))
+    if bias is not None:
+        _device_operand("bias", bias, torch.bfloat16, (N,))
+    out = torch.empty(M, N, dtype=torch.bfloat16, device=A.device)
+    _check(load_library().moe_gemm_mxfp4(_ptr(A), _ptr(a_scales), DTYPE_BF16 if a_scales is None else DTYPE_MXFP4, _ptr(w), _ptr(w_scales), _ptr(bias),
+                                         _ptr(out), M, N, K, act, _stream()), "moe_gemm_mxfp4")
     return out
 
 

@@ -968,6 +968,39 @@ int moe_forward_static(moe_handle* h, const void* x, const moe_weights* w, void*
     return forward_on(h, x, w, out, routing, g_scratch_ptr[dev], kStaticScratchBytes, stream);
 }
 
+int moe_forward_few(moe_handle* h, const void* x, const moe_weights* w, const moe_mxfp4_scales* mx, void* out, const moe_routing_out* routing,
+                    void* workspace, size_t workspace_bytes, void* stream) {
+    if (!h || !x || !w || !out) return MOE_ERR_BAD_ARGUMENT;
+    int dev = -1;
+    if (hipGetDevice(&dev) != hipSuccess || dev != h->arch.device) return MOE_ERR_BAD_ARGUMENT;
+    const Derived& d = h->d;
+    const bool sw = h->cfg.hidden_act == MOE_ACT_SWIGLU, f16 = d.act_dtype == MOE_DTYPE_FP16;
+    if (d.act_dtype == MOE_DTYPE_F32 || h->cfg.torch_dtype == MOE_DTYPE_FP8_E4M3_B128 || d.S > kFewTokens || (mx && f16)) return MOE_ERR_UNSUPPORTED;
+    if (!w->gate_w || !w->w_up || !w->w_down || sw != (w->w_gate != nullptr) || (!sw && w->b_gate)) return MOE_ERR_BAD_ARGUMENT;
+    if (w->s_up || w->s_down || w->s_gate || w->prepared) return MOE_ERR_BAD_ARGUMENT;
+    if (mx && (!mx->s_up || !mx->s_down || sw != (mx->s_gate != nullptr))) return MOE_ERR_BAD_ARGUMENT;
+    for (const void* p : {x, w->gate_w, w->w_up, w->w_gate, w->w_down, (const void*)out})
+        if ((uintptr_t)p % 16) return MOE_ERR_BAD_ARGUMENT;       // the kernels read and write 16 and 8 bytes at a time
+    const int rc = check_ws(h, workspace, workspace_bytes);
+    if (rc) return rc;
+    FewArgs a{};
+    a.x = x, a.gate_w = w->gate_w, a.gate_bias = w->gate_bias;
+    a.w_up = w->w_up, a.w_gate = w->w_gate, a.w_down = w->w_down;
+    if (mx) a.s_up = mx->s_up, a.s_gate = mx->s_gate, a.s_down = mx->s_down;
+    a.b_up = w->b_up, a.b_gate = w->b_gate, a.b_down = w->b_down;
+    a.logits = at<float>(workspace, h->ws.logits);
+    a.topk_idx = at<int32_t>(workspace, h->ws.topk_idx);
+    a.topk_w = at<float>(workspace, h->ws.topk_w);
+    a.h = at<char>(workspace, h->ws.h);
+    a.out = out;
+    if (routing) a.r = *routing;
+    a.S = d.S, a.H = d.H, a.I = d.I, a.E = d.E, a.k = d.k;
+    a.act = h->cfg.hidden_act, a.gate_fn = h->cfg.gate_fn, a.norm = h->cfg.norm_topk_prob;
+    a.drop = h->cfg.drop_tokens, a.capacity = (int32_t)d.capacity;
+    const hipError_t e = launch_few(a, f16, mx != nullptr, (hipStream_t)stream);
+    return e == hipSuccess ? MOE_OK : hip_fail(h, e);
+}
+
 int moe_prepared_bytes(const moe_handle* h, size_t* bytes) {
     if (!h || !bytes) return MOE_ERR_BAD_ARGUMENT;
     *bytes = h->d.plan.widen ? (size_t)h->d.wide_mats * h->d.E * h->d.I * h->d.H * 2 : 0;
@@ -1181,6 +1214,20 @@ int moe_expert_gemm(moe_handle* h, const void* a_rows, const void* w, const void
     if (rc) return rc;
     const hipError_t e = launch_expert_gemm(a_rows, w, bias, expert_count, expert_offset, h->d.A, h->d.E, N, K, act,
                                             h->d.act_dtype, h->opt, out_rows, scratch, (hipStream_t)stream);
+    return e == hipSuccess ? MOE_OK : hip_fail(h, e);
+}
+
+int moe_expert_gemm_mxfp4(moe_handle* h, const void* a_rows, const uint8_t* a_scales, const void* w, const uint8_t* w_scales, const void* bias,
+                          const int32_t* expert_count, const int32_t* expert_offset, int32_t N, int32_t K, int32_t act, void* out_rows, void* stream) {
+    if (!h || !expert_count || !expert_offset) return MOE_ERR_BAD_ARGUMENT;
+    int dev = -1;
+    if (hipGetDevice(&dev) != hipSuccess || dev != h->arch.device) return MOE_ERR_BAD_ARGUMENT;
+    if (h->cfg.torch_dtype != MOE_DTYPE_BF16) return MOE_ERR_UNSUPPORTED;
+    if (!((N == h->d.H && K == h->d.I) || (N == h->d.I && K == h->d.H))) return MOE_ERR_BAD_ARGUMENT;
+    const MxProduct p{a_rows, a_scales, w, w_scales, (const uint16_t*)bias, expert_count, expert_offset, (uint16_t*)out_rows, h->d.A, N, K, h->d.E, act};
+    const int rc = check_product_mxfp4(p, a_scales ? MOE_DTYPE_MXFP4 : MOE_DTYPE_BF16);
+    if (rc) return rc;
+    const hipError_t e = launch_product_mxfp4(p, MOE_OPT_AUTO, (hipStream_t)stream);
     return e == hipSuccess ? MOE_OK : hip_fail(h, e);
 }
 

@@ -222,6 +222,47 @@ hipError_t launch_ffn_tiled(const FfnArgs& a, const ExpertRows& rows, int dtype,
 hipError_t launch_ffn_persistent(const FfnArgs& a, int dtype, const FfnPlan& p, int blocks, bool early, hipStream_t st);
 int ffn_persistent_blocks(int dtype, int tile, int compute_units);
 
+// ---- MXFP4 (csrc/mxfp4_quant.hip, csrc/mxfp4_product.hip) and the layer for a few tokens (csrc/few.hip) ----
+hipError_t launch_quant_mxfp4(const void* x, int dtype, int64_t values, void* codes, uint8_t* scales, hipStream_t st);
+hipError_t launch_dequant_mxfp4(const void* codes, const uint8_t* scales, int64_t values, int dtype, void* out, hipStream_t st);
+struct MxProduct {              // out = act(a . w^T + bias), one matrix or (count, offset) one an expert over packed rows
+    const void* a;              // [M, K] bf16, or codes [M, K / 2] with a_scales
+    const uint8_t* a_scales;    // [M, K / 32], or null: bf16
+    const void* w;              // [E, N, K / 2] codes
+    const uint8_t* s;           // [E, N, K / 32]
+    const uint16_t* bias;       // [E, N] bf16, or null
+    const int32_t* count;       // [E] rows of every expert, or null: one matrix, M rows
+    const int32_t* offset;
+    uint16_t* out;              // [M, N]
+    int64_t M;
+    int N, K, E, act;
+};
+int check_product_mxfp4(const MxProduct& p, int a_dtype);       // moe_status
+hipError_t launch_product_mxfp4(const MxProduct& p, int form, hipStream_t st);
+constexpr int kFewTokens = 16;  // tokens a call of the layer for a few tokens takes: columns of a matrix instruction
+struct FewArgs {
+    const void* x;              // [S, H]
+    const void* gate_w;         // [E, H]
+    const float* gate_bias;     // [E] or null
+    const void* w_up;           // [E, I, H], or MXFP4 codes
+    const void* w_gate;
+    const void* w_down;
+    const uint8_t* s_up;        // MXFP4: scales
+    const uint8_t* s_gate;
+    const uint8_t* s_down;
+    const void* b_up;
+    const void* b_gate;
+    const void* b_down;
+    float* logits;              // [S, E] in the workspace
+    int32_t* topk_idx;          // [S, k] in the workspace
+    float* topk_w;
+    void* h;                    // [S k, I] in the workspace
+    void* out;                  // [S, H]
+    moe_routing_out r;          // the caller's copies (members may be null)
+    int32_t S, H, I, E, k, act, gate_fn, norm, drop, capacity, fold;
+};
+hipError_t launch_few(FewArgs a, bool f16, bool mxfp4, hipStream_t st);
+
 // ---- backward building blocks (csrc/backward.hip) ----
 size_t backward_scratch_bytes(int64_t A, int E, int H, int I, int elem_bytes);
 hipError_t launch_transpose(const void* src, void* dst, int64_t batch, int64_t rows, int64_t cols, int elem_bytes,

@@ -1,0 +1,531 @@
+// Products whose weights are MXFP4 (mxfp4.hpp): out = act(a . w^T + bias), w [N][K] codes with a scale for 32 values of a row, the rows a
+// in bf16 or in MXFP4 too; one matrix, or a matrix per expert over packed rows.  Sums in fp32, rounded once on store.
+#include "act_deriv.hpp"
+#include "grouped_task.hpp"
+#include "skinny.hpp"
+
+namespace moe355 {
+namespace {
+
+typedef __attribute__((address_space(1))) void mx_gbl_void;
+typedef __attribute__((address_space(3))) void mx_lds_void;
+
+struct MxTask {
+    const char* a;            // the block's first row
+    const uint8_t* a_scales;  // ... and its scales (rows in MXFP4)
+    const char* w;            // the expert's matrix
+    const uint8_t* s;
+    const uint16_t* bias;     // of the expert, or null
+    uint16_t* out;            // at the block's first row
+    int rows, n0;
+};
+
+// Which block of BM rows and which BN columns a workgroup takes.
+template <int BM, bool ROWS4>
+__device__ __forceinline__ bool mx_task(const MxProduct& p, int BN, MxTask& t) {
+    const int ncol = (p.N + BN - 1) / BN;
+    int expert = 0, ctile, rows;
+    int64_t row0;
+    if (p.count) {
+        GroupedTask g;
+        if (!grouped_task<BM>(p.count, p.offset, p.E, ncol, (int)blockIdx.x, g)) return false;
+        expert = g.expert, ctile = g.ctile, row0 = g.row0, rows = g.rows;
+        if (row0 < 0 || row0 + rows > p.M) return false;          // tables that are not this layer's: nothing behind the buffers is touched
+    } else {
+        // an eighth of the tiles in a row for each XCD, kRowChunk row blocks at a time, as for the experts
+        const int blocks = (int)((p.M + BM - 1) / BM);
+        const int64_t total = (int64_t)blocks * ncol, share = (total + 7) / 8;
+        const int64_t id = (int64_t)(blockIdx.x & 7) * share + (blockIdx.x >> 3);
+        if ((int64_t)(blockIdx.x >> 3) >= share || id >= total) return false;
+        int rb = (int)(id / ((int64_t)kRowChunk * ncol)) * kRowChunk;
+        const int width = min(kRowChunk, blocks - rb), local = (int)(id - (int64_t)rb * ncol);
+        ctile = local / width;
+        rb += local - ctile * width;
+        row0 = (int64_t)rb * BM;
+        rows = (int)min((int64_t)BM, p.M - row0);
+    }
+    const int64_t arow = ROWS4 ? p.K >> 1 : 2 * (int64_t)p.K;
+    t.a = static_cast<const char*>(p.a) + row0 * arow;
+    t.a_scales = ROWS4 ? p.a_scales + row0 * (p.K >> 5) : nullptr;
+    t.w = static_cast<const char*>(p.w) + (int64_t)expert * p.N * (p.K >> 1);
+    t.s = p.s + (int64_t)expert * p.N * (p.K >> 5);
+    t.bias = p.bias ? p.bias + (int64_t)expert * p.N : nullptr;
+    t.out = p.out + row0 * p.N;
+    t.rows = rows;
+    t.n0 = ctile * BN;
+    return true;
+}
+
+__device__ __forceinline__ float mx_activate(float u, int act) {
+    if (act == MOE_ACT_GELU) return gelu16(u);
+    return act == MOE_ACT_RELU && u < 0.0f ? 0.0f : u;           // a NaN stays a NaN
+}
+
+// Four neighbouring columns of a token row, as the matrix instructions leave them in a lane.
+__device__ __forceinline__ void mx_store4(const MxProduct& p, const MxTask& t, int row, int col, const mx_f32x4& acc) {
+    float v[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = mx_activate(acc[r] + (t.bias && col + r < p.N ? bf16_bits_to_f32(t.bias[col + r]) : 0.0f), p.act);
+    const uint32_t lo = pack2_bf16(v[0], v[1]), hi = pack2_bf16(v[2], v[3]);
+    uint16_t* o = t.out + (int64_t)row * p.N + col;
+    if (col + 3 < p.N && (p.N & 3) == 0) {
+        *reinterpret_cast<uint2*>(o) = uint2{lo, hi};
+    } else {
+        const uint32_t w[4] = {lo, lo >> 16, hi, hi >> 16};
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (col + r < p.N) o[r] = (uint16_t)w[r];
+    }
+}
+
+// ---- up to 16 rows a block: a weight streamer ----
+constexpr int kStreamWaves = 8;
+
+// One chunk of the token rows.
+template <bool ROWS4>
+struct StreamTokens {
+    mx_u32x4 x[ROWS4 ? 2 : 8];
+    uint32_t s[2];
+};
+
+// KS wavefronts share a contraction (chunks in turn), 8 / KS sets of 16 CG columns a workgroup.
+template <bool ROWS4, int CG, bool COLD>
+__global__ __launch_bounds__(64 * kStreamWaves) void mx_stream_kernel(MxProduct p, int KS) {
+    __shared__ mx_f32x4 red[(kStreamWaves - 1) * CG * 64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int ks = wave % KS, set = wave / KS;
+    MxTask t;
+    if (!mx_task<16, ROWS4>(p, 16 * CG * (kStreamWaves / KS), t)) return;
+    const int n0 = t.n0 + 16 * CG * set, K = p.K;
+    const int idx = lane & 15, q = lane >> 4;
+    SkinnyRows rows[CG];
+#pragma unroll
+    for (int g = 0; g < CG; ++g) rows[g] = skinny_rows<WeightsMx>(t.w, t.s, n0 + 16 * g, p.N, K, lane);
+    const int64_t ar = idx < t.rows ? idx : 0;                   // rows behind the block's last one read row 0 again and are not stored
+    const uint16_t* x16 = reinterpret_cast<const uint16_t*>(t.a) + ar * K;
+    const char* x4 = t.a + ar * (K >> 1) + 16 * q;
+    const uint8_t* xs = ROWS4 ? t.a_scales + ar * (K >> 5) : nullptr;
+
+    mx_f32x4 acc[CG];
+#pragma unroll
+    for (int g = 0; g < CG; ++g) acc[g] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
+    SkinnyChunk<WeightsMx, CG> d[2];
+    StreamTokens<ROWS4> x[2];
+    auto load = [&](int b, int c) {
+        skinny_load<WeightsMx, CG, COLD>(d[b], rows, c);
+        if constexpr (ROWS4) {
+            x[b].x[0] = *reinterpret_cast<const mx_u32x4*>(x4 + 128 * (int64_t)c);
+            x[b].x[1] = *reinterpret_cast<const mx_u32x4*>(x4 + 128 * (int64_t)c + 64);
+            __builtin_memcpy(x[b].s, xs + 8 * (int64_t)c, 8);
+        } else {
+            skinny_tokens<WeightsMx>(x[b].x, x16, c, lane);
+        }
+    };
+    auto multiply = [&](int b) {
+        if constexpr (ROWS4) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int g = 0; g < CG; ++g)
+                    acc[g] = mx_mfma(d[b].v[g][h], skinny_scale(d[b].s[g], h, lane), x[b].x[h], skinny_scale(x[b].s, h, lane), acc[g]);
+        } else {
+            skinny_multiply<WeightsMx, CG>(acc, d[b], x[b].x, lane);
+        }
+    };
+    auto take = [&](int b) {
+        skinny_settle(d[b]);
+        multiply(b);
+    };
+    const int full = K >> 8, n = full > ks ? (full - ks + KS - 1) / KS : 0;
+    if (n > 0) load(0, ks);
+    if (n > 1) load(1, ks + KS);
+    int i = 0;
+    for (; i + 3 < n; i += 2) {
+        take(0);
+        load(0, ks + (i + 2) * KS);
+        take(1);
+        load(1, ks + (i + 3) * KS);
+    }
+    if (n - i > 0) take(0);
+    if (n - i > 2) load(0, ks + (i + 2) * KS);
+    if (n - i > 1) take(1);
+    if (n - i > 2) take(0);
+    if ((K & 255) && full % KS == ks) {          // the rows' last chunk, cut off
+        const int left = K & 255;
+        skinny_load_tail<WeightsMx, CG, COLD>(d[0], rows, full, left >> 1, lane);
+        if constexpr (ROWS4) {
+            x[0].s[0] = x[0].s[1] = 0;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int b = 4 * h + q;
+                x[0].x[h] = mx_u32x4{0u, 0u, 0u, 0u};
+                if (b < (left >> 5)) {
+                    x[0].x[h] = *reinterpret_cast<const mx_u32x4*>(x4 + 128 * (int64_t)full + 64 * h);
+                    x[0].s[h] = (uint32_t)xs[8 * (int64_t)full + b] << (8 * q);
+                }
+            }
+        } else {
+            skinny_tokens_tail<WeightsMx>(x[0].x, x16, full, left, lane);
+        }
+        skinny_settle(d[0]);
+        skinny_zero_tail(d[0], left >> 1, lane);
+        multiply(0);
+    }
+    if (!skinny_join<CG>(acc, ks, KS, red + set * (KS - 1) * CG * 64, lane)) return;
+    if (idx >= t.rows) return;
+#pragma unroll
+    for (int g = 0; g < CG; ++g) {
+        const int col = n0 + 16 * g + 4 * q;
+        if (col < p.N) mx_store4(p, t, idx, col, acc[g]);
+    }
+}
+
+// ---- more rows: tiles ----
+//
+// RH x CW wavefronts of 16 NT rows x 16 CG columns each, KS sets of them that share the contraction.  Token rows go straight into LDS, a
+// slab of 256 (bf16: 256 bytes a row) or 128 bytes (MXFP4) a row at a time, one slab ahead; every fragment of theirs serves CG groups of
+// columns.  Weights go straight into the registers of the wavefront that multiplies them, 64 bytes of a row a step of 128 values, a step
+// ahead: a lane's 16 bytes are a whole block and already the fragment (skinny.hpp).
+template <bool ROWS4_, int RH_, int NT_, int CW_, int CG_, int KS_>
+struct MxTile {
+    static constexpr bool ROWS4 = ROWS4_;
+    static constexpr int RH = RH_, NT = NT_, CW = CW_, CG = CG_, KS = KS_;
+    static constexpr int BM = 16 * NT * RH, BN = 16 * CG * CW;
+    static constexpr int SET = RH * CW;                        // wavefronts of a set
+    static constexpr int THREADS = 64 * SET * KS;
+    static constexpr int PITCH = ROWS4 ? 128 : 256;            // bytes of a row in a slab
+    static constexpr int STEPS = ROWS4 ? 2 : 1;                // steps of 128 values in a slab
+    static constexpr int ROWS_A_LOAD = 1024 / PITCH;           // rows that one instruction of a wavefront brings
+    static constexpr int LOADS = BM / ROWS_A_LOAD / SET;
+    static constexpr int SCALES = ROWS4 ? BM * 8 : 0;          // bytes of the rows' scales in a slab
+    static constexpr int STAGE = BM * PITCH + SCALES;
+    static constexpr int SUMS = (KS - 1) * SET * NT * CG * 1024;
+    static constexpr int LDS = 2 * KS * STAGE > SUMS ? 2 * KS * STAGE : SUMS;
+    static constexpr int BLOCKS = NT * CG >= 32 ? 1 : NT * CG >= 16 ? 2 : 160 * 1024 / LDS;      // workgroups of a compute unit
+    static constexpr int WAVES_PER_SIMD = BLOCKS * THREADS / 256 < 4 ? BLOCKS * THREADS / 256 : 4;
+    static_assert(SET % 4 == 0 && LOADS >= 1 && BM % (ROWS_A_LOAD * SET) == 0, "every wavefront of a set brings as many rows, in steps of 16");
+    static_assert(!ROWS4 || BM <= 64 * SET, "a row's scales a thread");
+    static_assert(LDS <= 160 * 1024, "LDS of a compute unit");
+};
+
+template <class T>
+__global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void mx_tile_kernel(MxProduct p) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    constexpr int NT = T::NT, CG = T::CG, PITCH = T::PITCH;
+    constexpr bool ROWS4 = T::ROWS4;
+    MxTask t;
+    if (!mx_task<T::BM, ROWS4>(p, T::BN, t)) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int ks = wave / T::SET, sw = wave % T::SET;            // set and place in it
+    const int wm = sw / T::CW, wn = sw % T::CW;
+    const int idx = lane & 15, q = lane >> 4;
+    const int K = p.K, N = p.N;
+    const uint32_t arow = ROWS4 ? (uint32_t)K >> 1 : 2 * (uint32_t)K, wrow = (uint32_t)K >> 1, srow = (uint32_t)K >> 5;
+
+    // Rows into LDS: an instruction of a wavefront writes 1 KB of LDS in the order of its lanes, so what a slot holds is decided by the
+    // address its lane reads.  The LDS serves a 16-byte read to lanes 0-3, 12-15 and 20-27 in one cycle, to 4-11, 16-19 and 28-31 in the
+    // next: with 256-byte rows chunk 4 q + j, the one that lane (row, q) reads as its j-th, lies in slot (q + 4 j) ^ row, with 128-byte rows
+    // chunk c in slot c ^ (row / 2): no two of a cycle meet.
+    int chunk;
+    uint32_t a_off[T::LOADS];
+    {
+        const int slots = PITCH / 16, r_in = lane / slots, slot = lane % slots;
+        const int r = (sw * T::ROWS_A_LOAD + r_in) & 15;
+        if constexpr (ROWS4) {
+            chunk = slot ^ ((r >> 1) & 7);
+        } else {
+            const int o = slot ^ r;
+            chunk = 4 * (o & 3) + (o >> 2);
+        }
+#pragma unroll
+        for (int i = 0; i < T::LOADS; ++i) {
+            const int row = (i * T::SET + sw) * T::ROWS_A_LOAD + r_in;
+            a_off[i] = (uint32_t)(row < t.rows ? row : 0) * arow;              // rows behind the block's last one read row 0 again
+        }
+    }
+    unsigned char* const stages = smem + ks * 2 * T::STAGE;
+    const int slabs_all = (int)((arow + PITCH - 1) / PITCH);                   // of a row; set ks takes ks, ks + KS, ...
+    const int slabs = slabs_all > ks ? (slabs_all - ks + T::KS - 1) / T::KS : 0;
+    const int slabs_most = (slabs_all + T::KS - 1) / T::KS;
+    // slab number s of this set into stage s & 1; pieces behind the row's end: its first again (and never multiplied)
+    auto issue = [&](int s) {
+        unsigned char* const st = stages + (s & 1) * T::STAGE;
+        const uint32_t at = (uint32_t)(s * T::KS + ks) * PITCH + 16 * chunk;
+        const uint32_t o = at < arow ? at : 0;
+#pragma unroll
+        for (int i = 0; i < T::LOADS; ++i)
+            __builtin_amdgcn_global_load_lds((mx_gbl_void*)(t.a + (a_off[i] + o)), (mx_lds_void*)(st + (i * T::SET + sw) * 1024), 16, 0, 0);
+    };
+    // the rows' scales: a row a thread, through a register (their addresses have no alignment)
+    uint32_t rs[2] = {0, 0};
+    const int srow_of = (int)(threadIdx.x - ks * T::SET * 64);
+    auto load_row_scales = [&](int s) {
+        if constexpr (ROWS4) {
+            if (srow_of < T::BM) {
+                const uint8_t* at = t.a_scales + (uint32_t)(srow_of < t.rows ? srow_of : 0) * srow;
+                const int b0 = (s * T::KS + ks) * 8;
+                if (b0 + 8 <= (int)srow) {
+                    __builtin_memcpy(rs, at + b0, 8);
+                } else {
+                    rs[0] = rs[1] = 0;
+#pragma unroll
+                    for (int b = 0; b < 8; ++b)
+                        if (b0 + b < (int)srow) rs[b >> 2] |= (uint32_t)at[b0 + b] << (8 * (b & 3));
+                }
+            }
+        }
+    };
+    auto store_row_scales = [&](int s) {
+        if constexpr (ROWS4) {
+            if (srow_of < T::BM) *reinterpret_cast<uint2*>(stages + (s & 1) * T::STAGE + T::BM * PITCH + srow_of * 8) = uint2{rs[0], rs[1]};
+        }
+    };
+
+    // weights: rows of 16 columns a group; columns behind the last one read it again
+    const int c0 = t.n0 + 16 * CG * wn;
+    uint32_t w_off[CG], s_off[CG];
+#pragma unroll
+    for (int g = 0; g < CG; ++g) {
+        const uint32_t n = (uint32_t)min(c0 + 16 * g + idx, N - 1);
+        w_off[g] = n * wrow + 16 * q;
+        s_off[g] = n * srow;
+    }
+    mx_u32x4 w[2][CG];
+    uint32_t ws[2][CG];
+    const int steps_all = (K + 127) >> 7;
+    auto load_w = [&](int b, int step) {          // step: of 128 values, counted over the whole row
+        if (step * 128 + 128 <= K) {
+#pragma unroll
+            for (int g = 0; g < CG; ++g) {
+                w[b][g] = *reinterpret_cast<const mx_u32x4*>(t.w + (w_off[g] + 64 * (uint32_t)step));
+                uint32_t v;
+                __builtin_memcpy(&v, t.s + (s_off[g] + 4 * (uint32_t)step), 4);
+                ws[b][g] = v >> (8 * q);
+            }
+        } else {                                  // the row's last step, cut off: zeros behind its end
+            const bool in = step * 128 + 32 * q < K;
+#pragma unroll
+            for (int g = 0; g < CG; ++g) {
+                w[b][g] = mx_u32x4{0u, 0u, 0u, 0u};
+                ws[b][g] = 0;
+                if (in) {
+                    w[b][g] = *reinterpret_cast<const mx_u32x4*>(t.w + (w_off[g] + 64 * (uint32_t)step));
+                    ws[b][g] = t.s[s_off[g] + 4 * (uint32_t)step + q];
+                }
+            }
+        }
+    };
+
+    mx_f32x4 acc[NT][CG];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int g = 0; g < CG; ++g) acc[i][g] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
+    const int mine = min(NT, max(0, (t.rows - wm * 16 * NT + 15) >> 4));       // groups of 16 rows that exist
+
+    // One step: weights b, rows of stage st, half h of the slab (MXFP4).  CUT: zeros for what lies behind the rows' end (an infinity there
+    // would make a NaN of the weights' zeros).
+    auto step = [&](int b, const unsigned char* st, int h, int number, auto cut_c, auto all_c) {
+        constexpr bool CUT = decltype(cut_c)::value, ALL = decltype(all_c)::value;
+        const bool in = !CUT || number * 128 + 32 * q < K;
+        const unsigned char* base = st + (wm * 16 * NT + idx) * PITCH;
+        if constexpr (ROWS4) {
+            const int at = ((4 * h + q) ^ ((idx >> 1) & 7)) << 4;
+            const unsigned char* sc = st + T::BM * PITCH + (wm * 16 * NT + idx) * 8 + 4 * h;
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                if (!ALL && i >= mine) continue;
+                mx_u32x4 x = *reinterpret_cast<const mx_u32x4*>(base + i * 16 * PITCH + at);
+                uint32_t xs = *reinterpret_cast<const uint32_t*>(sc + i * 128) >> (8 * q);
+                if (CUT && !in) x = mx_u32x4{0u, 0u, 0u, 0u}, xs = 0;
+#pragma unroll
+                for (int g = 0; g < CG; ++g) acc[i][g] = mx_mfma(w[b][g], ws[b][g], x, xs, acc[i][g]);
+            }
+        } else {
+            float s[CG];
+#pragma unroll
+            for (int g = 0; g < CG; ++g) s[g] = mx_scale(ws[b][g] & 255u);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                mx_bf16x8 wf[CG];
+#pragma unroll
+                for (int g = 0; g < CG; ++g) wf[g] = mx_widen8(w[b][g][j], s[g]);
+                const int at = ((q + 4 * j) ^ idx) << 4;
+#pragma unroll
+                for (int i = 0; i < NT; ++i) {
+                    if (!ALL && i >= mine) continue;
+                    mx_u32x4 x = *reinterpret_cast<const mx_u32x4*>(base + i * 16 * PITCH + at);
+                    if (CUT && !in) x = mx_u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+                    for (int g = 0; g < CG; ++g)
+                        acc[i][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[g], __builtin_bit_cast(mx_bf16x8, x), acc[i][g], 0, 0, 0);
+                }
+            }
+        }
+    };
+    typedef std::true_type Yes;
+    typedef std::false_type No;
+    auto run_step = [&](int b, const unsigned char* st, int h, int number) {
+        if (mine == 0) return;
+        if (number * 128 + 128 > K) step(b, st, h, number, Yes{}, No{});
+        else if (mine == NT) step(b, st, h, number, No{}, Yes{});
+        else step(b, st, h, number, No{}, No{});
+    };
+    // Every request of this wavefront for the slab has landed and its reads of the other stage are done, then so have everybody's.
+    auto meet = [&]() {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+
+    if (slabs > 0) {
+        issue(0);
+        load_row_scales(0);
+        load_w(0, ks * T::STEPS);
+        store_row_scales(0);
+    }
+    for (int s = 0; s < slabs_most; s += 2) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {             // stage u; weights: bf16 rows' buffer u, MXFP4 rows' buffer of the half
+            if (s + u >= slabs_most) break;
+            meet();
+            const bool here = s + u < slabs, more = s + u + 1 < slabs;
+            const int number = ((s + u) * T::KS + ks) * T::STEPS;
+            const unsigned char* st = stages + u * T::STAGE;
+            if (more) {
+                issue(s + u + 1);
+                load_row_scales(s + u + 1);
+            }
+            if constexpr (ROWS4) {
+                if (here && number + 1 < steps_all) load_w(1, number + 1);
+                if (here) run_step(0, st, 0, number);
+                if (more) load_w(0, number + 2 * T::KS);
+                if (here && number + 1 < steps_all) run_step(1, st, 1, number + 1);
+                if (more) store_row_scales(s + u + 1);
+            } else {
+                if (more) load_w(u ^ 1, number + T::KS);
+                if (here) run_step(u, st, 0, number);
+            }
+        }
+    }
+
+    if constexpr (T::KS > 1) {                    // the sets' sums, in their order
+        meet();
+        mx_f32x4* red = reinterpret_cast<mx_f32x4*>(smem) + sw * NT * CG * 64 + lane;
+        if (ks > 0) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int g = 0; g < CG; ++g) red[((ks - 1) * T::SET * NT * CG + i * CG + g) * 64] = acc[i][g];
+        }
+        __syncthreads();
+        if (ks > 0) return;
+        for (int k = 0; k < T::KS - 1; ++k)
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int g = 0; g < CG; ++g) acc[i][g] += red[(k * T::SET * NT * CG + i * CG + g) * 64];
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        const int row = 16 * (wm * NT + i) + idx;
+        if (row >= t.rows) continue;
+#pragma unroll
+        for (int g = 0; g < CG; ++g) {
+            const int col = c0 + 16 * g + 4 * q;
+            if (col < N) mx_store4(p, t, row, col, acc[i][g]);
+        }
+    }
+}
+
+// Workgroups of a launch: blocks of BM rows (an expert's last one is its own) times column tiles, in eight equal shares.
+int64_t mx_grid(const MxProduct& p, int BM, int BN) {
+    const int64_t ncol = (p.N + BN - 1) / BN, blocks = p.count ? p.M / BM + p.E : (p.M + BM - 1) / BM;
+    return (blocks * ncol + 7) / 8 * 8 + (p.count ? 16 : 0);
+}
+
+template <class T>
+hipError_t launch_tile(const MxProduct& p, hipStream_t st) {
+    static const hipError_t ready = hipFuncSetAttribute(reinterpret_cast<const void*>(mx_tile_kernel<T>), hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
+    if (ready != hipSuccess) return ready;
+    mx_tile_kernel<T><<<(unsigned)mx_grid(p, T::BM, T::BN), T::THREADS, T::LDS, st>>>(p);
+    return hipGetLastError();
+}
+
+template <bool ROWS4>
+hipError_t launch_stream(const MxProduct& p, hipStream_t st) {
+    const int64_t blocks = p.count ? std::min<int64_t>(p.E, p.M) : (p.M + 15) / 16;
+    const int chunks = (p.K + 255) / 256;
+    const int64_t groups = blocks * ((p.N + 15) / 16);         // wavefronts if each had 16 columns and the whole contraction
+    const bool wide = groups >= 4096 && chunks <= 64;
+    int KS = 1;
+    while (KS < 8 && KS * 2 <= chunks && groups / (wide ? 2 : 1) * KS < 4096) KS *= 2;
+    const bool cold = blocks * p.N * p.K / 2 > ((int64_t)256 << 20);
+    const int BN = 16 * (wide ? 2 : 1) * (kStreamWaves / KS);
+    const unsigned grid = (unsigned)mx_grid(p, 16, BN);
+    if (wide && cold) mx_stream_kernel<ROWS4, 2, true><<<grid, 64 * kStreamWaves, 0, st>>>(p, KS);
+    else if (wide) mx_stream_kernel<ROWS4, 2, false><<<grid, 64 * kStreamWaves, 0, st>>>(p, KS);
+    else if (cold) mx_stream_kernel<ROWS4, 1, true><<<grid, 64 * kStreamWaves, 0, st>>>(p, KS);
+    else mx_stream_kernel<ROWS4, 1, false><<<grid, 64 * kStreamWaves, 0, st>>>(p, KS);
+    return hipGetLastError();
+}
+
+template <bool ROWS4>
+hipError_t launch_product(const MxProduct& p, int form, hipStream_t st) {
+    switch (form) {
+        case 0: return launch_stream<ROWS4>(p, st);
+        case 1: return launch_tile<MxTile<ROWS4, 1, 2, 4, 1, 2>>(p, st);     // 32 x 64
+        case 2: return launch_tile<MxTile<ROWS4, 1, 4, 4, 1, 2>>(p, st);     // 64 x 64
+        case 3: return launch_tile<MxTile<ROWS4, 2, 4, 2, 4, 1>>(p, st);     // 128 x 128
+        default: return launch_tile<MxTile<ROWS4, 2, 8, 4, 4, 1>>(p, st);    // 256 x 256
+    }
+}
+
+int product_form(const MxProduct& p) {
+    const int64_t rows = p.count ? (p.M + p.E - 1) / p.E : p.M;
+    if (rows <= 16) return 0;
+    if (rows <= 32) return 1;
+    if (rows <= 64) return 2;
+    const int64_t tiles = (p.count ? p.M / 256 + p.E : (p.M + 255) / 256) * ((p.N + 255) / 256);
+    return rows >= 256 && tiles >= 192 ? 4 : 3;
+}
+
+int64_t product_workgroups(const MxProduct& p, int form) {
+    constexpr int BM[] = {16, 32, 64, 128, 256}, BN[] = {16, 64, 64, 128, 256};      // (the streamer's narrowest)
+    return mx_grid(p, BM[form], BN[form]);
+}
+
+}  // namespace
+
+// form: MOE_OPT_AUTO, or the kernel asked for
+hipError_t launch_product_mxfp4(const MxProduct& p, int form, hipStream_t st) {
+    if (p.M == 0) return hipSuccess;
+    if (form < 0) form = product_form(p);
+    return p.a_scales ? launch_product<true>(p, form, st) : launch_product<false>(p, form, st);
+}
+
+// What the kernels read and write at a time, their 32-bit offsets and the launches' sizes.
+int check_product_mxfp4(const MxProduct& p, int a_dtype) {
+    auto aligned = [](const void* a) { return (uintptr_t)a % 16 == 0; };
+    if (p.M < 0 || p.N < 1 || p.K < kMxBlock || p.K % kMxBlock || !p.w || !p.s) return MOE_ERR_BAD_ARGUMENT;
+    if (p.act != MOE_ACT_RELU && p.act != MOE_ACT_GELU && p.act != MOE_ACT_NONE) return MOE_ERR_BAD_ARGUMENT;
+    if (a_dtype != MOE_DTYPE_BF16 && a_dtype != MOE_DTYPE_MXFP4) return MOE_ERR_UNSUPPORTED;
+    if (p.M > 0 && (!p.a || !p.out || (a_dtype == MOE_DTYPE_MXFP4) != (p.a_scales != nullptr))) return MOE_ERR_BAD_ARGUMENT;
+    if (!aligned(p.a) || !aligned(p.w) || !aligned(p.out) || (uintptr_t)p.bias % 2) return MOE_ERR_BAD_ARGUMENT;
+    if (p.K > (1 << 20) || (int64_t)p.N * (p.K / 2) >= ((int64_t)1 << 32) || p.M > INT32_MAX) return MOE_ERR_UNSUPPORTED;
+    return product_workgroups(p, product_form(p)) < ((int64_t)1 << 22) ? MOE_OK : MOE_ERR_UNSUPPORTED;      // 1024 threads each: 2^32
+}
+
+}  // namespace moe355
+
+using namespace moe355;
+
+extern "C" int moe_gemm_mxfp4(const void* a, const uint8_t* a_scales, int32_t a_dtype, const void* w, const uint8_t* w_scales, const void* bias, void* out,
+                              int64_t M, int64_t N, int64_t K, int32_t act, void* stream) {
+    if (M < 0 || N < 1 || K < 1) return MOE_ERR_BAD_ARGUMENT;
+    if (N > INT32_MAX / 2 || K > INT32_MAX / 2) return MOE_ERR_UNSUPPORTED;
+    const MxProduct p{a, a_scales, w, w_scales, (const uint16_t*)bias, nullptr, nullptr, (uint16_t*)out, M, (int)N, (int)K, 1, act};
+    const int rc = check_product_mxfp4(p, a_dtype);
+    if (rc) return rc;
+    return launch_product_mxfp4(p, MOE_OPT_AUTO, (hipStream_t)stream) == hipSuccess ? MOE_OK : MOE_ERR_HIP;
+}

@@ -53,6 +53,11 @@ def _forward_cuda(x, gate_w, w_up, w_gate, w_down, config, gate_bias=None, b_up=
     S, H, I, E = cfg.tokens, cfg.hidden_size, cfg.intermediate_size, cfg.num_experts
     act = layer.act_dtype
     fp8 = cfg.torch_dtype == api.DTYPE_FP8
+    if s_up is not None and s_up.dtype == torch.uint8:        # expert weights in MXFP4: forward_mxfp4 checks the operands
+        weights = dict(gate_w=gate_w, gate_bias=gate_bias, w_up=w_up, w_gate=w_gate, w_down=w_down, b_up=b_up, b_gate=b_gate,
+                       b_down=b_down, s_up=s_up, s_gate=s_gate, s_down=s_down)
+        with torch.cuda.device(x.device):
+            return layer.forward_mxfp4(x, {n: t for n, t in weights.items() if t is not None})
     wdt = (torch.float8_e4m3fn, torch.uint8) if fp8 else (act,)
     _check_tensor("x", x, (S, H), (act,))
     _check_tensor("gate_w", gate_w, (E, H), (act,))
@@ -91,7 +96,7 @@ class MoE355(torch.nn.Module):
 
     Built either with random weights (`MoE355(cfg)`, bf16/f32 only) or from packed tensors under the argument names of
     `moe_forward` (`MoE355.from_packed(cfg, tensors)`; see `cuplayground_amd.weights` for packing, quantising and
-    loading them), which also covers the block-scaled e4m3 layers."""
+    loading them), which also covers the block-scaled e4m3 layers and bf16 layers whose expert weights are in MXFP4."""
 
     _NAMES = ("gate_w", "gate_bias", "w_up", "w_gate", "w_down", "b_up", "b_gate", "b_down", "s_up", "s_gate", "s_down")
 

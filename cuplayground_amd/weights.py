@@ -8,7 +8,8 @@ small matrix per expert and projection instead.  This module
 * packs such per-expert matrices into the stacked tensors (`pack_experts`), with the name mapping of Mixtral-style
   checkpoints built in (`pack_mixtral_block`: `experts.{e}.w1` is the SiLU-gated projection = `w_gate`, `w3` = `w_up`,
   `w2` = `w_down`, `gate.weight` = the router);
-* quantises a packed set to the block-scaled e4m3 form on the GPU (`quantize_packed`, through `moe_quant_block128`);
+* quantises a packed set to the block-scaled e4m3 form or to MXFP4 on the GPU (`quantize_packed`, through `moe_quant_block128` or
+  `moe_quant_mxfp4`);
 * writes and reads a packed set as one safetensors file whose metadata carries the layer's knob file (`save_packed`,
   `load_packed`), so that a serving process maps the file and calls `moe_forward` without touching the weights again.
 
@@ -69,20 +70,26 @@ def mixtral_config(packed: Mapping[str, torch.Tensor], tokens: int, top_k: int =
     """The knob file of a Mixtral-style block for `tokens` rows per call: softmax router, top-k renormalised,
     SwiGLU, no token dropping."""
     E, I, H = packed["w_up"].shape
-    fp8 = packed["w_up"].dtype in (torch.uint8, torch.float8_e4m3fn)
+    mxfp4 = "s_up" in packed and packed["s_up"].dtype == torch.uint8        # a bf16 layer that holds its experts' weights in 4 bits
+    fp8 = not mxfp4 and packed["w_up"].dtype in (torch.uint8, torch.float8_e4m3fn)
+    H = 2 * H if mxfp4 else H
     return api.MoEConfig(capacity_factor=1.0, drop_tokens=0, expert_top_k=top_k, hidden_act=api.ACT_SWIGLU,
                          hidden_size=H, intermediate_size=I, micro_batch=1, num_experts=E, sequence_len=tokens,
                          torch_dtype=api.DTYPE_FP8 if fp8 else api.DTYPE_BF16, gate_fn=api.GATE_SOFTMAX,
                          norm_topk_prob=1)
 
 
-def quantize_packed(packed: Mapping[str, torch.Tensor]) -> Dict[str, torch.Tensor]:
-    """bf16/fp32 expert matrices -> e4m3 codes + one fp32 scale per 128 x 128 block (scale = amax / 448); the router
-    and the biases keep their dtype.  Runs on the GPU through `moe_quant_block128`."""
+def quantize_packed(packed: Mapping[str, torch.Tensor], form: str = "e4m3") -> Dict[str, torch.Tensor]:
+    """bf16/fp32 expert matrices -> e4m3 codes + one fp32 scale per 128 x 128 block (scale = amax / 448), or with form = "mxfp4" 4-bit
+    codes + a power of two for 32 values of a row (`MoELayer.forward_mxfp4`); the router and the biases keep their dtype.  Runs on the GPU
+    through `moe_quant_block128` / `moe_quant_mxfp4`."""
+    if form not in ("e4m3", "mxfp4"):
+        raise ValueError(f"unknown form {form!r}: e4m3 or mxfp4")
+    quantize = api.quantize_block128 if form == "e4m3" else api.quantize_mxfp4
     out = {k: v for k, v in packed.items() if not k.startswith("w_")}
     for k in ("w_up", "w_gate", "w_down"):
         if k in packed:
-            q, s = api.quantize_block128(packed[k])
+            q, s = quantize(packed[k])
             out[k] = q
             out["s_" + k[2:]] = s
     return out

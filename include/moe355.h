@@ -47,6 +47,8 @@ typedef enum moe_status {
  * type, except: tf32 layers are fp32 in memory and are computed in full fp32 (gfx950 has no tf32 matrix instruction;
  * the reference's tf32 atoms, processor/tiling.cuh:131-143, keep fp32 storage too), e4m3 layers keep bf16 activations. */
 enum { MOE_DTYPE_F32 = 0, MOE_DTYPE_TF32 = 1, MOE_DTYPE_BF16 = 2, MOE_DTYPE_FP16 = 3, MOE_DTYPE_FP8_E4M3_B128 = 4 };
+/* Operands of the MXFP4 entry points only (no layer's torch_dtype). */
+enum { MOE_DTYPE_MXFP4 = 16 };
 /* hidden_act: the reference enum (aristos_config.schema.json:24-28) plus 2 */
 enum { MOE_ACT_RELU = 0, MOE_ACT_GELU = 1, MOE_ACT_SWIGLU = 2, MOE_ACT_NONE = 3 /* moe_gemm_bias_act only */ };
 enum { MOE_GATE_SOFTMAX = 0, MOE_GATE_SIGMOID = 1 };
@@ -399,6 +401,45 @@ int moe_quant_rows128(const void* x, int64_t rows, int64_t K, void* q, float* sc
  * the reference (same reason). */
 int moe_dequant_block128(const void* q, const float* scales, int64_t matrices, int64_t N, int64_t K, void* out,
                          void* stream);
+
+/* ---- Weights (and rows) in MXFP4 -----------------------------------------------------------------------------------
+ * The 4-bit format of OCP Microscaling Formats 1.0: values of e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), 32 consecutive ones
+ * of a row with one scale of e8m0 (the byte s is 2^(s - 127), 255 is NaN).  [rows, K] values, K a multiple of 32, are codes
+ * [rows, K / 2] bytes, the value of the even index in the low half of its byte, and scales [rows, K / 32] bytes, both row-major.  A layer
+ * whose expert weights are held so is a bf16 layer (torch_dtype = 2) as far as its handle goes.  No counterpart in the reference, whose
+ * dtypes stop at fp16 (aristos_config.schema.json:49-53).  Everything here is asynchronous on `stream`, allocates nothing and can be
+ * captured into a graph.
+ *
+ * moe_quant_mxfp4: x [rows, K] (fp32, bf16 or fp16; 16-byte aligned) -> codes (4-byte aligned), scales.  scale = 2^(floor(log2 amax) - 2), not
+ *   below 2^-127, amax the largest magnitude of the 32 values (1 where all are zero); a value is x / scale rounded to the nearest, ties to
+ *   the even code, at most +-6.  A block that holds an infinity or a NaN gets the scale NaN (and codes 0): all of it reads as NaN.
+ * moe_dequant_mxfp4: the values, in fp32, bf16 or fp16 (exact in the first two up to their overflow; one rounding in fp16). */
+int moe_quant_mxfp4(const void* x, int32_t src_dtype, int64_t rows, int64_t K, void* codes, uint8_t* scales, void* stream);
+int moe_dequant_mxfp4(const void* codes, const uint8_t* scales, int64_t rows, int64_t K, int32_t dst_dtype, void* out, void* stream);
+/* moe_gemm_bias_act on such a matrix: out [M, N] (bf16) = act(a . w^T + bias), w [N, K] in MXFP4, bias [N] bf16 or null, act RELU, GELU or
+ * NONE.  a [M, K]: bf16 (a_dtype = MOE_DTYPE_BF16, a_scales null; the weights are widened exactly, the products are bf16's) or MXFP4
+ * (a_dtype = MOE_DTYPE_MXFP4, codes with a_scales).  Sums in fp32, rounded once.  a, w and out 16-byte aligned; any M (0: nothing is done)
+ * and N, K a multiple of 32.  MOE_ERR_UNSUPPORTED: other types, a matrix of 4 GiB and more. */
+int moe_gemm_mxfp4(const void* a, const uint8_t* a_scales, int32_t a_dtype, const void* w, const uint8_t* w_scales, const void* bias, void* out,
+                   int64_t M, int64_t N, int64_t K, int32_t act, void* stream);
+/* moe_expert_gemm (below) on such weights: the rows of every expert of a bf16 layer through its matrix, w [E, N, K] in MXFP4, bias [E, N] or
+ * null, rows as above (a_scales null: bf16, else MXFP4).  (N, K) is (H, I) or (I, H).  Rows of no expert are neither read nor written.  No
+ * scratch. */
+int moe_expert_gemm_mxfp4(moe_handle* h, const void* a_rows, const uint8_t* a_scales, const void* w, const uint8_t* w_scales, const void* bias,
+                          const int32_t* expert_count, const int32_t* expert_offset, int32_t N, int32_t K, int32_t act, void* out_rows, void* stream);
+/* The whole layer for a few tokens (S <= 16; a decoding step): what moe_forward computes, in two launches -- three where the router is large
+ * -- instead of six.  bf16 and fp16 layers on their own weights (mx = NULL), or bf16 layers on weights in MXFP4: then w_up, w_gate and
+ * w_down of *w are codes and *mx has their scales (s_* of *w stay NULL); the router and the biases keep the activations' type.  The routing
+ * is moe_forward's to the bit, and so are capacity, drops and what `routing` receives.  Sums in fp32; the intermediate rows are rounded to the
+ * activations' type, an expert's output rows are not rounded before the combine, so `out` differs from moe_forward's by that rounding.
+ * The workspace is the handle's; one call at a time per workspace.  MOE_ERR_UNSUPPORTED: more tokens, another type of layer. */
+typedef struct moe_mxfp4_scales {
+    const uint8_t* s_up;      /* [E, I, H / 32] */
+    const uint8_t* s_gate;    /* SwiGLU only, else NULL */
+    const uint8_t* s_down;    /* [E, H, I / 32] */
+} moe_mxfp4_scales;
+int moe_forward_few(moe_handle* h, const void* x, const moe_weights* w, const moe_mxfp4_scales* mx, void* out, const moe_routing_out* routing,
+                    void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- Backward building blocks (fp32, tf32, bf16 and fp16 layers; e4m3 layers: MOE_ERR_UNSUPPORTED) ------------------
  * The reference declares a training knob (is_training, aristos_config.schema.json:20-23) that none of its code reads

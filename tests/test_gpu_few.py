@@ -1,0 +1,214 @@
+"""The layer for a few tokens: against 64 bits, and its routing against the general path's to the bit."""
+import math
+
+import pytest
+import torch
+
+import cuplayground_amd as moe
+from cuplayground_amd import api
+import mxfp4_plain as plain
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+ROUTING = ("topk_idx", "topk_w", "slot", "expert_count", "expert_offset")
+
+
+def _config(S, H, I, E, k, act, dtype=api.DTYPE_BF16, gate=api.GATE_SOFTMAX, norm=1, capacity=0.0):
+    return moe.MoEConfig(capacity_factor=capacity or 1.0, drop_tokens=int(capacity > 0), expert_top_k=k, hidden_act=act, hidden_size=H, intermediate_size=I,
+                         micro_batch=1, num_experts=E, sequence_len=S, torch_dtype=dtype, gate_fn=gate, norm_topk_prob=norm)
+
+
+def _inputs(cfg, weights, bias, seed, gate_bias=False):
+    """(x, the layer's tensors, its expert matrices in 64 bits)."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    dt = torch.float16 if cfg.torch_dtype == api.DTYPE_FP16 else torch.bfloat16
+    S, H, I, E = cfg.tokens, cfg.hidden_size, cfg.intermediate_size, cfg.num_experts
+
+    def normal(*shape, std=1.0):
+        return torch.randn(*shape, generator=g, device=DEV) * std
+
+    w, exact = {"gate_w": normal(E, H, std=0.05).to(dt)}, {}
+    if gate_bias:
+        w["gate_bias"] = normal(E)
+    for m in ("up", "down") + (("gate",) if cfg.hidden_act == api.ACT_SWIGLU else ()):
+        N, K = (H, I) if m == "down" else (I, H)
+        full = normal(E, N, K, std=K ** -0.5)
+        if weights == "mxfp4":
+            w["w_" + m], w["s_" + m] = moe.quantize_mxfp4(full)
+            exact[m] = plain.values(w["w_" + m], w["s_" + m])
+        else:
+            w["w_" + m] = full.to(dt)
+            exact[m] = w["w_" + m].double()
+        if bias:
+            w["b_" + m] = normal(E, N, std=0.3).to(dt)
+    return normal(S, H).to(dt), w, exact
+
+
+def _close(got, x, cfg, w, exact, idx, wts, slot):
+    """The layer in 64 bits with the routing that the call reported.  Of a value: the rounding of the output and that of the intermediate
+    (half a unit in the last place of each, eps / 2), the latter weighted as the down projection weights it; what the fp32 sums and gate
+    weights add is smaller by their 2^-24 and H + I + k terms.  Of all values together: two roundings of eps / 2 each at most."""
+    F = torch.nn.functional
+    half = torch.finfo(x.dtype).eps / 2
+    xd = x.double()
+    want, room = torch.zeros_like(xd), torch.zeros_like(xd)
+    for t in range(cfg.tokens):
+        for r in range(cfg.expert_top_k):
+            if slot[t, r] < 0:
+                continue
+            e, p = int(idx[t, r]), wts[t, r].double()
+
+            def project(v, m):
+                y = exact[m][e] @ v
+                return y + w["b_" + m][e].double() if "b_" + m in w else y
+
+            u = project(xd[t], "up")
+            h = F.silu(project(xd[t], "gate")) * u if cfg.hidden_act == api.ACT_SWIGLU else plain.activate(u, cfg.hidden_act)
+            want[t] += p * project(h, "down")
+            room[t] += p * (exact["down"][e].abs() @ (h.abs() + 1e-3))
+    off = (got.double() - want).abs()
+    sums = (cfg.hidden_size + cfg.intermediate_size) * 2.0 ** -23
+    tol = half * want.abs() + (half + 4 * sums) * 1.02 * room + 1e-6
+    assert (off <= tol).all(), float((off - tol).max())
+    assert off.norm() <= 2 * half * want.norm() + 1e-5 * want.numel() ** 0.5, float(off.norm() / want.norm())
+
+
+def _check(cfg, weights, bias, seed, gate_bias=False):
+    x, w, exact = _inputs(cfg, weights, bias, seed, gate_bias)
+    layer = moe.MoELayer(cfg)
+    routing = layer.new_routing()
+    got = layer.forward_few(x, w, routing=routing)
+    # the general path routes the same tokens: its gate and its slots
+    idx, wts = layer.gate(x, w["gate_w"], w.get("gate_bias"))
+    r = layer.route(idx)
+    want = dict(r, topk_idx=idx, topk_w=wts)
+    for key in ROUTING:
+        assert torch.equal(routing[key], want[key]), key
+    kept = int(want["expert_count"].sum())
+    assert torch.equal(routing["token_indices"][:kept], want["token_indices"][:kept]) and bool((routing["token_indices"][kept:] == -1).all())
+    _close(got, x, cfg, w, exact, idx.cpu(), wts.cpu(), r["slot"].cpu())
+    return layer, x, w, got
+
+
+KINDS = [("mxfp4", api.DTYPE_BF16), ("own", api.DTYPE_BF16), ("own", api.DTYPE_FP16)]
+
+
+@pytest.mark.parametrize("weights,dtype", KINDS)
+@pytest.mark.parametrize("S,H,I,E,k,act,gate,norm,capacity,bias", [
+    (1, 64, 64, 1, 1, api.ACT_RELU, api.GATE_SOFTMAX, 0, 0.0, False),
+    (1, 512, 1024, 8, 2, api.ACT_SWIGLU, api.GATE_SOFTMAX, 1, 0.0, False),
+    (1, 2048, 192, 4, 4, api.ACT_GELU, api.GATE_SIGMOID, 0, 0.0, True),
+    (2, 448, 320, 300, 5, api.ACT_SWIGLU, api.GATE_SIGMOID, 1, 0.0, True),
+    (5, 256, 832, 16, 3, api.ACT_GELU, api.GATE_SOFTMAX, 1, 1.0, True),
+    (7, 1344, 448, 12, 3, api.ACT_RELU, api.GATE_SOFTMAX, 1, 0.0, True),
+    (9, 1024, 512, 64, 8, api.ACT_SWIGLU, api.GATE_SOFTMAX, 0, 1.25, False),
+    (16, 576, 576, 128, 16, api.ACT_SWIGLU, api.GATE_SIGMOID, 1, 0.0, False),
+    (16, 512, 256, 2, 2, api.ACT_GELU, api.GATE_SOFTMAX, 1, 0.5, True),
+    (16, 256, 2112, 512, 8, api.ACT_SWIGLU, api.GATE_SOFTMAX, 1, 1.0, True),
+])
+def test_few(S, H, I, E, k, act, gate, norm, capacity, bias, weights, dtype):
+    _check(_config(S, H, I, E, k, act, dtype, gate, norm, capacity), weights, bias, seed=S + E + k, gate_bias=E % 3 == 0)
+
+
+@pytest.mark.parametrize("weights", ["mxfp4", "own"])
+def test_few_where_all_tokens_choose_the_same_experts(weights):
+    """Sixteen rows in two experts, the others hit by none; and with room for three rows an expert, tokens that lose every pair."""
+    for capacity in (0.0, 0.75):
+        cfg = _config(16, 256, 320, 8, 2, api.ACT_SWIGLU, capacity=capacity)
+        x, w, exact = _inputs(cfg, weights, True, seed=5)
+        w["gate_bias"] = torch.tensor([0, 0, 60.0, 0, 0, 50.0, 0, 0], device=DEV)
+        layer = moe.MoELayer(cfg)
+        routing = layer.new_routing()
+        got = layer.forward_few(x, w, routing=routing)
+        assert torch.equal(routing["topk_idx"], torch.tensor([[2, 5]] * 16, dtype=torch.int32, device=DEV))
+        room = 16 if not capacity else math.ceil(0.75 * 32 / 8)
+        assert int(routing["expert_count"][2]) == room and int(routing["expert_count"].sum()) == 2 * room
+        _close(got, x, cfg, w, exact, routing["topk_idx"].cpu(), routing["topk_w"].cpu(), routing["slot"].cpu())
+        assert bool((got[room:] == 0).all())
+
+
+@pytest.mark.parametrize("weights,dtype", KINDS)
+def test_few_against_the_general_path(weights, dtype):
+    """The same layer by moe_forward (on the widened weights): rounded once more, an expert's rows, so three roundings apart at most."""
+    cfg = _config(16, 512, 768, 16, 4, api.ACT_SWIGLU, dtype)
+    layer, x, w, got = _check(cfg, weights, False, seed=3)
+    if weights == "mxfp4":
+        w = {n: moe.dequantize_mxfp4(t, w["s_" + n[2:]]) if n[:2] == "w_" else t for n, t in w.items() if n[:2] != "s_"}
+    want = layer.forward(x, w)
+    half = torch.finfo(x.dtype).eps / 2
+    assert (got.double() - want.double()).norm() <= 5 * half * want.double().norm()
+
+
+def test_few_keeps_a_token_that_is_not_finite_to_itself():
+    cfg = _config(6, 320, 192, 16, 2, api.ACT_SWIGLU)
+    x, w, exact = _inputs(cfg, "mxfp4", False, seed=8)
+    layer = moe.MoELayer(cfg)
+    clean = layer.forward_few(x, w)
+    x[2, 319], x[4, 0] = float("nan"), float("inf")
+    got = layer.forward_few(x, w)
+    others = [0, 1, 3, 5]
+    assert torch.isnan(got[2]).all() and not torch.isfinite(got[4]).all()
+    assert torch.isfinite(got[others]).all()
+    # the others' experts and sums are what they were; which experts are hit may shift the order of the down projection's sums
+    assert (got[others].double() - clean[others].double()).norm() <= 2.0 ** -8 * clean[others].double().norm()
+
+
+@pytest.mark.parametrize("weights", ["mxfp4", "own"])
+def test_few_repeats_in_a_graph_and_on_another_stream(weights):
+    cfg = _config(4, 512, 1408, 64, 6, api.ACT_SWIGLU)
+    x, w, _ = _inputs(cfg, weights, False, seed=2)
+    layer, other = moe.MoELayer(cfg), moe.MoELayer(cfg)
+    xs = [x, -x, x.roll(1, 0)]
+    want = [layer.forward_few(v, w) for v in xs]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):                             # two handles, two workspaces, at the same time
+        there = [other.forward_few(v, w) for v in xs]
+    here = [layer.forward_few(v, w) for v in xs]
+    torch.cuda.synchronize()
+    for a, b, c in zip(want, there, here):
+        assert torch.equal(a, b) and torch.equal(a, c)
+    held, out = x.clone(), torch.empty_like(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        layer.forward_few(held, w, out=out)
+    for v, y in zip(xs * 2, want * 2):
+        held.copy_(v)
+        graph.replay()
+        other.forward_few(xs[1], w)
+        torch.cuda.synchronize()
+        assert torch.equal(out, y)
+
+
+def test_mxfp4_layer_from_a_checkpoint_to_its_answers(tmp_path):
+    """Expert matrices packed, quantised, saved and loaded; a prompt by the stages, a decoding step by the few-token launches, and the
+    torch operator over both."""
+    from cuplayground_amd import torch_op, weights as W
+    E, H, I, k = 8, 256, 384, 2
+    g = torch.Generator().manual_seed(1)
+
+    def mats(n, r, c):
+        return [torch.randn(r, c, generator=g) * c ** -0.5 for _ in range(n)]
+
+    packed = W.pack_experts(torch.randn(E, H, generator=g) * 0.1, mats(E, I, H), mats(E, H, I), mats(E, I, H), device=DEV)
+    held = W.quantize_packed(packed, form="mxfp4")
+    exact = {m: plain.values(held["w_" + m], held["s_" + m]) for m in ("up", "gate", "down")}
+    for tokens in (3, 70):
+        cfg = W.mixtral_config(held, tokens=tokens, top_k=k)
+        assert (cfg.hidden_size, cfg.intermediate_size, cfg.torch_dtype) == (H, I, api.DTYPE_BF16)
+        path = str(tmp_path / ("layer%d.safetensors" % tokens))
+        W.save_packed(path, held, cfg)
+        loaded, cfg = W.load_packed(path)
+        x = torch.randn(tokens, H, generator=g).to(DEV).bfloat16()
+        layer = moe.MoELayer(cfg)
+        got = layer.forward_mxfp4(x, loaded)
+        idx, wts = layer.gate(x, loaded["gate_w"])
+        slot = layer.route(idx)["slot"]
+        if tokens <= api.FEW_TOKENS:
+            _close(got, x, cfg, loaded, exact, idx.cpu(), wts.cpu(), slot.cpu())
+        # the general path on the widened weights: at most three roundings of each apart (the projections', the intermediate's, the rows')
+        wide = {n: moe.dequantize_mxfp4(t, loaded["s_" + n[2:]]) if n[:2] == "w_" else t for n, t in loaded.items() if n[:2] != "s_"}
+        want = layer.forward(x, wide)
+        assert (got.double() - want.double()).norm() <= 6 * 2.0 ** -8 * want.double().norm()
+        module = torch_op.MoE355.from_packed(cfg, loaded)
+        assert torch.equal(module(x), got)
