@@ -183,9 +183,10 @@ __global__ __launch_bounds__(64 * kStreamWaves) void mx_stream_kernel(MxProduct 
 // ---- more rows: tiles ----
 //
 // RH x CW wavefronts of 16 NT rows x 16 CG columns each, KS sets of them that share the contraction.  Token rows go straight into LDS, a
-// slab of 256 (bf16: 256 bytes a row) or 128 bytes (MXFP4) a row at a time, one slab ahead; every fragment of theirs serves CG groups of
-// columns.  Weights go straight into the registers of the wavefront that multiplies them, 64 bytes of a row a step of 128 values, a step
-// ahead: a lane's 16 bytes are a whole block and already the fragment (skinny.hpp).
+// slab of 256 (bf16) or 128 bytes (MXFP4) a row at a time, one slab ahead; every fragment of theirs serves CG groups of columns.  Weights go
+// straight into the registers of the wavefront that multiplies them, 64 bytes of a row a step of 128 values, a step ahead: a lane's 16
+// bytes are a whole block and already the fragment (skinny.hpp).  All operands are read through buffers that end where they end, so rows
+// behind the block's last one, columns behind the matrix's and what lies behind K are zeros without a branch.
 template <bool ROWS4_, int RH_, int NT_, int CW_, int CG_, int KS_>
 struct MxTile {
     static constexpr bool ROWS4 = ROWS4_;
@@ -194,10 +195,10 @@ struct MxTile {
     static constexpr int SET = RH * CW;                        // wavefronts of a set
     static constexpr int THREADS = 64 * SET * KS;
     static constexpr int PITCH = ROWS4 ? 128 : 256;            // bytes of a row in a slab
-    static constexpr int STEPS = ROWS4 ? 2 : 1;                // steps of 128 values in a slab
     static constexpr int ROWS_A_LOAD = 1024 / PITCH;           // rows that one instruction of a wavefront brings
     static constexpr int LOADS = BM / ROWS_A_LOAD / SET;
-    static constexpr int SCALES = ROWS4 ? BM * 8 : 0;          // bytes of the rows' scales in a slab
+    static constexpr int RB = NT < 4 ? NT : 4;                 // groups of 16 rows whose fragments are in registers at once (twice)
+    static constexpr int SCALES = ROWS4 ? 8 * (BM / RB) * 4 : 0;   // bytes of the rows' scales in a slab: a dword has those of RB rows
     static constexpr int STAGE = BM * PITCH + SCALES;
     static constexpr int SUMS = (KS - 1) * SET * NT * CG * 1024;
     static constexpr int LDS = 2 * KS * STAGE > SUMS ? 2 * KS * STAGE : SUMS;
@@ -208,10 +209,17 @@ struct MxTile {
     static_assert(LDS <= 160 * 1024, "LDS of a compute unit");
 };
 
+// An offset behind the end of every buffer here, also with a tile's rows added to it.  (Offsets are whole in the vector register: the range
+// check is against what a scalar offset leaves of the buffer, and that may be less than nothing.)
+constexpr uint32_t kBehind = 0xD0000000u;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_buffer(const void* p, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00020000);
+}
+
 template <class T>
 __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void mx_tile_kernel(MxProduct p) {
     extern __shared__ __align__(16) unsigned char smem[];
-    constexpr int NT = T::NT, CG = T::CG, PITCH = T::PITCH;
+    constexpr int NT = T::NT, CG = T::CG, PITCH = T::PITCH, RB = T::RB, KS = T::KS;
     constexpr bool ROWS4 = T::ROWS4;
     MxTask t;
     if (!mx_task<T::BM, ROWS4>(p, T::BN, t)) return;
@@ -226,8 +234,7 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void mx_tile_kernel(
     // address its lane reads.  The LDS serves a 16-byte read to lanes 0-3, 12-15 and 20-27 in one cycle, to 4-11, 16-19 and 28-31 in the
     // next: with 256-byte rows chunk 4 q + j, the one that lane (row, q) reads as its j-th, lies in slot (q + 4 j) ^ row, with 128-byte rows
     // chunk c in slot c ^ (row / 2): no two of a cycle meet.
-    int chunk;
-    uint32_t a_off[T::LOADS];
+    uint32_t chunk, a_off;
     {
         const int slots = PITCH / 16, r_in = lane / slots, slot = lane % slots;
         const int r = (sw * T::ROWS_A_LOAD + r_in) & 15;
@@ -237,82 +244,63 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void mx_tile_kernel(
             const int o = slot ^ r;
             chunk = 4 * (o & 3) + (o >> 2);
         }
-#pragma unroll
-        for (int i = 0; i < T::LOADS; ++i) {
-            const int row = (i * T::SET + sw) * T::ROWS_A_LOAD + r_in;
-            a_off[i] = (uint32_t)(row < t.rows ? row : 0) * arow;              // rows behind the block's last one read row 0 again
-        }
+        a_off = (uint32_t)(sw * T::ROWS_A_LOAD + r_in) * arow;
     }
     unsigned char* const stages = smem + ks * 2 * T::STAGE;
     const int slabs_all = (int)((arow + PITCH - 1) / PITCH);                   // of a row; set ks takes ks, ks + KS, ...
-    const int slabs = slabs_all > ks ? (slabs_all - ks + T::KS - 1) / T::KS : 0;
-    const int slabs_most = (slabs_all + T::KS - 1) / T::KS;
-    // slab number s of this set into stage s & 1; pieces behind the row's end: its first again (and never multiplied)
+    const int slabs = slabs_all > ks ? (slabs_all - ks + KS - 1) / KS : 0;
+    const int slabs_most = (slabs_all + KS - 1) / KS;
+    const __amdgpu_buffer_rsrc_t a_buf = mx_buffer(t.a, (uint32_t)t.rows * arow);
+    // slab number s of this set into stage s & 1
     auto issue = [&](int s) {
         unsigned char* const st = stages + (s & 1) * T::STAGE;
-        const uint32_t at = (uint32_t)(s * T::KS + ks) * PITCH + 16 * chunk;
-        const uint32_t o = at < arow ? at : 0;
+        const uint32_t at = (uint32_t)(s * KS + ks) * PITCH + 16 * chunk;
+        const uint32_t v = at < arow ? a_off + at : kBehind;
 #pragma unroll
         for (int i = 0; i < T::LOADS; ++i)
-            __builtin_amdgcn_global_load_lds((mx_gbl_void*)(t.a + (a_off[i] + o)), (mx_lds_void*)(st + (i * T::SET + sw) * 1024), 16, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(a_buf, (mx_lds_void*)(st + (i * T::SET + sw) * 1024), 16, (int)(v + i * T::SET * T::ROWS_A_LOAD * arow), 0, 0, 0);
     };
-    // the rows' scales: a row a thread, through a register (their addresses have no alignment)
+    // The rows' scales, a row a thread, through a register (their addresses have no alignment), into LDS as the matrix instruction picks
+    // them: it takes one byte of a register, so the dword for (block, 64 rows, lane) has those of rows lane, 16 + lane, 32 + lane, 48 + lane.
     uint32_t rs[2] = {0, 0};
-    const int srow_of = (int)(threadIdx.x - ks * T::SET * 64);
-    auto load_row_scales = [&](int s) {
-        if constexpr (ROWS4) {
-            if (srow_of < T::BM) {
-                const uint8_t* at = t.a_scales + (uint32_t)(srow_of < t.rows ? srow_of : 0) * srow;
-                const int b0 = (s * T::KS + ks) * 8;
-                if (b0 + 8 <= (int)srow) {
-                    __builtin_memcpy(rs, at + b0, 8);
-                } else {
-                    rs[0] = rs[1] = 0;
+    const int my_row = (int)threadIdx.x - ks * T::SET * 64;
+    auto load8 = [&](uint32_t (&d)[2], const uint8_t* at, int b0) {            // blocks b0 .. b0 + 7 of a row of srow
+        if (b0 + 8 <= (int)srow) {
+            __builtin_memcpy(d, at + b0, 8);
+        } else {
+            d[0] = d[1] = 0;
 #pragma unroll
-                    for (int b = 0; b < 8; ++b)
-                        if (b0 + b < (int)srow) rs[b >> 2] |= (uint32_t)at[b0 + b] << (8 * (b & 3));
-                }
-            }
+            for (int b = 0; b < 8; ++b)
+                if (b0 + b < (int)srow) d[b >> 2] |= (uint32_t)at[b0 + b] << (8 * (b & 3));
         }
+    };
+    auto load_row_scales = [&](int s) {
+        if constexpr (ROWS4)
+            if (my_row < T::BM) load8(rs, t.a_scales + (uint32_t)(my_row < t.rows ? my_row : 0) * srow, (s * KS + ks) * 8);
     };
     auto store_row_scales = [&](int s) {
         if constexpr (ROWS4) {
-            if (srow_of < T::BM) *reinterpret_cast<uint2*>(stages + (s & 1) * T::STAGE + T::BM * PITCH + srow_of * 8) = uint2{rs[0], rs[1]};
+            if (my_row < T::BM) {
+                unsigned char* at = stages + (s & 1) * T::STAGE + T::BM * PITCH + (my_row / (16 * RB) * 16 + my_row % 16) * 4 + my_row / 16 % RB;
+#pragma unroll
+                for (int b = 0; b < 8; ++b) at[b * (T::BM / RB * 4)] = (unsigned char)(rs[b >> 2] >> (8 * (b & 3)));
+            }
         }
     };
 
-    // weights: rows of 16 columns a group; columns behind the last one read it again
+    // weights: rows of 16 columns a group
     const int c0 = t.n0 + 16 * CG * wn;
-    uint32_t w_off[CG], s_off[CG];
-#pragma unroll
-    for (int g = 0; g < CG; ++g) {
-        const uint32_t n = (uint32_t)min(c0 + 16 * g + idx, N - 1);
-        w_off[g] = n * wrow + 16 * q;
-        s_off[g] = n * srow;
-    }
+    const __amdgpu_buffer_rsrc_t w_buf = mx_buffer(t.w, (uint32_t)N * wrow), s_buf = mx_buffer(t.s, (uint32_t)N * srow);
+    const uint32_t w_off = (uint32_t)(c0 + idx) * wrow + 16 * q, s_off = (uint32_t)(c0 + idx) * srow + q;
     mx_u32x4 w[2][CG];
     uint32_t ws[2][CG];
-    const int steps_all = (K + 127) >> 7;
     auto load_w = [&](int b, int step) {          // step: of 128 values, counted over the whole row
-        if (step * 128 + 128 <= K) {
+        const bool in = step * 128 + 32 * q < K;
+        const uint32_t wv = in ? w_off + 64 * (uint32_t)step : kBehind, sv = in ? s_off + 4 * (uint32_t)step : kBehind;
 #pragma unroll
-            for (int g = 0; g < CG; ++g) {
-                w[b][g] = *reinterpret_cast<const mx_u32x4*>(t.w + (w_off[g] + 64 * (uint32_t)step));
-                uint32_t v;
-                __builtin_memcpy(&v, t.s + (s_off[g] + 4 * (uint32_t)step), 4);
-                ws[b][g] = v >> (8 * q);
-            }
-        } else {                                  // the row's last step, cut off: zeros behind its end
-            const bool in = step * 128 + 32 * q < K;
-#pragma unroll
-            for (int g = 0; g < CG; ++g) {
-                w[b][g] = mx_u32x4{0u, 0u, 0u, 0u};
-                ws[b][g] = 0;
-                if (in) {
-                    w[b][g] = *reinterpret_cast<const mx_u32x4*>(t.w + (w_off[g] + 64 * (uint32_t)step));
-                    ws[b][g] = t.s[s_off[g] + 4 * (uint32_t)step + q];
-                }
-            }
+        for (int g = 0; g < CG; ++g) {
+            w[b][g] = __builtin_bit_cast(mx_u32x4, __builtin_amdgcn_raw_buffer_load_b128(w_buf, (int)(wv + g * 16 * wrow), 0, 0));
+            ws[b][g] = __builtin_amdgcn_raw_buffer_load_b8(s_buf, (int)(sv + g * 16 * srow), 0, 0);
         }
     };
 
@@ -321,55 +309,57 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void mx_tile_kernel(
     for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int g = 0; g < CG; ++g) acc[i][g] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
-    const int mine = min(NT, max(0, (t.rows - wm * 16 * NT + 15) >> 4));       // groups of 16 rows that exist
+    const bool any = t.rows > wm * 16 * NT;       // rows of this wavefront that exist
 
-    // One step: weights b, rows of stage st, half h of the slab (MXFP4).  CUT: zeros for what lies behind the rows' end (an infinity there
-    // would make a NaN of the weights' zeros).
-    auto step = [&](int b, const unsigned char* st, int h, int number, auto cut_c, auto all_c) {
-        constexpr bool CUT = decltype(cut_c)::value, ALL = decltype(all_c)::value;
-        const bool in = !CUT || number * 128 + 32 * q < K;
+    // A slab, in blocks of RB groups of rows: the next block's fragments are read (and, with bf16 rows, the next weights widened) under the
+    // products of the one before.  Parts: the quarters j of a step (bf16), the steps of a slab (MXFP4).
+    constexpr int PARTS = ROWS4 ? 2 : 4, NB = NT / RB, SEQ = PARTS * NB;
+    auto slab = [&](const unsigned char* st, int wb) {
         const unsigned char* base = st + (wm * 16 * NT + idx) * PITCH;
-        if constexpr (ROWS4) {
-            const int at = ((4 * h + q) ^ ((idx >> 1) & 7)) << 4;
-            const unsigned char* sc = st + T::BM * PITCH + (wm * 16 * NT + idx) * 8 + 4 * h;
+        mx_u32x4 x[2][RB];
+        uint32_t xs[2];
+        mx_bf16x8 wf[2][CG];
+        auto read = [&](int n) {
+            const int part = n / NB, ib = n % NB;
+            const int at = ROWS4 ? ((4 * part + q) ^ ((idx >> 1) & 7)) << 4 : ((q + 4 * part) ^ idx) << 4;
 #pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                if (!ALL && i >= mine) continue;
-                mx_u32x4 x = *reinterpret_cast<const mx_u32x4*>(base + i * 16 * PITCH + at);
-                uint32_t xs = *reinterpret_cast<const uint32_t*>(sc + i * 128) >> (8 * q);
-                if (CUT && !in) x = mx_u32x4{0u, 0u, 0u, 0u}, xs = 0;
+            for (int i = 0; i < RB; ++i) x[n & 1][i] = *reinterpret_cast<const mx_u32x4*>(base + (ib * RB + i) * 16 * PITCH + at);
+            if constexpr (ROWS4)
+                xs[n & 1] = *reinterpret_cast<const uint32_t*>(st + T::BM * PITCH + (4 * part + q) * (T::BM / RB * 4) + ((wm * NB + ib) * 16 + idx) * 4);
+        };
+        auto widen = [&](int part) {
+            if constexpr (!ROWS4) {
 #pragma unroll
-                for (int g = 0; g < CG; ++g) acc[i][g] = mx_mfma(w[b][g], ws[b][g], x, xs, acc[i][g]);
-            }
-        } else {
-            float s[CG];
-#pragma unroll
-            for (int g = 0; g < CG; ++g) s[g] = mx_scale(ws[b][g] & 255u);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                mx_bf16x8 wf[CG];
-#pragma unroll
-                for (int g = 0; g < CG; ++g) wf[g] = mx_widen8(w[b][g][j], s[g]);
-                const int at = ((q + 4 * j) ^ idx) << 4;
-#pragma unroll
-                for (int i = 0; i < NT; ++i) {
-                    if (!ALL && i >= mine) continue;
-                    mx_u32x4 x = *reinterpret_cast<const mx_u32x4*>(base + i * 16 * PITCH + at);
-                    if (CUT && !in) x = mx_u32x4{0u, 0u, 0u, 0u};
-#pragma unroll
-                    for (int g = 0; g < CG; ++g)
-                        acc[i][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[g], __builtin_bit_cast(mx_bf16x8, x), acc[i][g], 0, 0, 0);
+                for (int g = 0; g < CG; ++g) {
+                    const uint32_t codes = w[wb][g][part];
+                    wf[part & 1][g] = mx_widen8(codes, mx_scale(ws[wb][g]));
                 }
             }
+        };
+        read(0);
+        widen(0);
+#pragma unroll
+        for (int n = 0; n < SEQ; ++n) {
+            const int part = n / NB, ib = n % NB;
+            if (n + 1 < SEQ) read(n + 1);
+            if (ib == NB - 1 && part + 1 < PARTS) widen(part + 1);
+#pragma unroll
+            for (int i = 0; i < RB; ++i) {
+#pragma unroll
+                for (int g = 0; g < CG; ++g) {
+                    mx_f32x4& a = acc[ib * RB + i][g];
+                    if constexpr (ROWS4) {
+                        if (i == 0) a = mx_mfma<0>(w[part][g], ws[part][g], x[n & 1][i], xs[n & 1], a);
+                        else if (i == 1) a = mx_mfma<1>(w[part][g], ws[part][g], x[n & 1][i], xs[n & 1], a);
+                        else if (i == 2) a = mx_mfma<2>(w[part][g], ws[part][g], x[n & 1][i], xs[n & 1], a);
+                        else a = mx_mfma<3>(w[part][g], ws[part][g], x[n & 1][i], xs[n & 1], a);
+                    } else {
+                        a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[part & 1][g], __builtin_bit_cast(mx_bf16x8, x[n & 1][i]), a, 0, 0, 0);
+                    }
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
-    };
-    typedef std::true_type Yes;
-    typedef std::false_type No;
-    auto run_step = [&](int b, const unsigned char* st, int h, int number) {
-        if (mine == 0) return;
-        if (number * 128 + 128 > K) step(b, st, h, number, Yes{}, No{});
-        else if (mine == NT) step(b, st, h, number, No{}, Yes{});
-        else step(b, st, h, number, No{}, No{});
     };
     // Every request of this wavefront for the slab has landed and its reads of the other stage are done, then so have everybody's.
     auto meet = [&]() {
@@ -381,35 +371,35 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void mx_tile_kernel(
     if (slabs > 0) {
         issue(0);
         load_row_scales(0);
-        load_w(0, ks * T::STEPS);
+        load_w(0, ks * (ROWS4 ? 2 : 1));
+        if constexpr (ROWS4) load_w(1, ks * 2 + 1);
         store_row_scales(0);
     }
     for (int s = 0; s < slabs_most; s += 2) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {             // stage u; weights: bf16 rows' buffer u, MXFP4 rows' buffer of the half
+        for (int u = 0; u < 2; ++u) {             // stage u; weights: buffer u (bf16 rows), both (MXFP4 rows)
             if (s + u >= slabs_most) break;
             meet();
             const bool here = s + u < slabs, more = s + u + 1 < slabs;
-            const int number = ((s + u) * T::KS + ks) * T::STEPS;
+            const int next = (s + u + 1) * KS + ks;
             const unsigned char* st = stages + u * T::STAGE;
             if (more) {
                 issue(s + u + 1);
                 load_row_scales(s + u + 1);
+                if constexpr (!ROWS4) load_w(u ^ 1, next);
             }
+            if (here && any) slab(st, u);
             if constexpr (ROWS4) {
-                if (here && number + 1 < steps_all) load_w(1, number + 1);
-                if (here) run_step(0, st, 0, number);
-                if (more) load_w(0, number + 2 * T::KS);
-                if (here && number + 1 < steps_all) run_step(1, st, 1, number + 1);
-                if (more) store_row_scales(s + u + 1);
-            } else {
-                if (more) load_w(u ^ 1, number + T::KS);
-                if (here) run_step(u, st, 0, number);
+                if (more) {
+                    load_w(0, 2 * next);
+                    load_w(1, 2 * next + 1);
+                    store_row_scales(s + u + 1);
+                }
             }
         }
     }
 
-    if constexpr (T::KS > 1) {                    // the sets' sums, in their order
+    if constexpr (KS > 1) {                       // the sets' sums, in their order
         meet();
         mx_f32x4* red = reinterpret_cast<mx_f32x4*>(smem) + sw * NT * CG * 64 + lane;
         if (ks > 0) {
@@ -420,7 +410,7 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void mx_tile_kernel(
         }
         __syncthreads();
         if (ks > 0) return;
-        for (int k = 0; k < T::KS - 1; ++k)
+        for (int k = 0; k < KS - 1; ++k)
 #pragma unroll
             for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -512,7 +502,7 @@ int check_product_mxfp4(const MxProduct& p, int a_dtype) {
     if (a_dtype != MOE_DTYPE_BF16 && a_dtype != MOE_DTYPE_MXFP4) return MOE_ERR_UNSUPPORTED;
     if (p.M > 0 && (!p.a || !p.out || (a_dtype == MOE_DTYPE_MXFP4) != (p.a_scales != nullptr))) return MOE_ERR_BAD_ARGUMENT;
     if (!aligned(p.a) || !aligned(p.w) || !aligned(p.out) || (uintptr_t)p.bias % 2) return MOE_ERR_BAD_ARGUMENT;
-    if (p.K > (1 << 20) || (int64_t)p.N * (p.K / 2) >= ((int64_t)1 << 32) || p.M > INT32_MAX) return MOE_ERR_UNSUPPORTED;
+    if (p.K > (1 << 20) || (int64_t)p.N * (p.K / 2) >= ((int64_t)3 << 30) || p.M > INT32_MAX) return MOE_ERR_UNSUPPORTED;
     return product_workgroups(p, product_form(p)) < ((int64_t)1 << 22) ? MOE_OK : MOE_ERR_UNSUPPORTED;      // 1024 threads each: 2^32
 }
 

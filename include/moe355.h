@@ -419,7 +419,7 @@ int moe_dequant_mxfp4(const void* codes, const uint8_t* scales, int64_t rows, in
 /* moe_gemm_bias_act on such a matrix: out [M, N] (bf16) = act(a . w^T + bias), w [N, K] in MXFP4, bias [N] bf16 or null, act RELU, GELU or
  * NONE.  a [M, K]: bf16 (a_dtype = MOE_DTYPE_BF16, a_scales null; the weights are widened exactly, the products are bf16's) or MXFP4
  * (a_dtype = MOE_DTYPE_MXFP4, codes with a_scales).  Sums in fp32, rounded once.  a, w and out 16-byte aligned; any M (0: nothing is done)
- * and N, K a multiple of 32.  MOE_ERR_UNSUPPORTED: other types, a matrix of 4 GiB and more. */
+ * and N, K a multiple of 32.  MOE_ERR_UNSUPPORTED: other types, a matrix of 3 GiB and more. */
 int moe_gemm_mxfp4(const void* a, const uint8_t* a_scales, int32_t a_dtype, const void* w, const uint8_t* w_scales, const void* bias, void* out,
                    int64_t M, int64_t N, int64_t K, int32_t act, void* stream);
 /* moe_expert_gemm (below) on such weights: the rows of every expert of a bf16 layer through its matrix, w [E, N, K] in MXFP4, bias [E, N] or
