@@ -17,8 +17,13 @@ struct MxTask {
     const uint8_t* s;
     const uint16_t* bias;     // of the expert, or null
     uint16_t* out;            // at the block's first row
+    int64_t row0;
     int rows, n0;
 };
+
+__device__ __forceinline__ int64_t mx_uniform(int64_t v) {
+    return (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)v) | (int64_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32;
+}
 
 // Which block of BM rows and which BN columns a workgroup takes.
 template <int BM, bool ROWS4>
@@ -44,7 +49,10 @@ __device__ __forceinline__ bool mx_task(const MxProduct& p, int BN, MxTask& t) {
         row0 = (int64_t)rb * BM;
         rows = (int)min((int64_t)BM, p.M - row0);
     }
+    // the same in every lane, and said so
+    row0 = mx_uniform(row0), expert = __builtin_amdgcn_readfirstlane(expert), ctile = __builtin_amdgcn_readfirstlane(ctile), rows = __builtin_amdgcn_readfirstlane(rows);
     const int64_t arow = ROWS4 ? p.K >> 1 : 2 * (int64_t)p.K;
+    t.row0 = row0;
     t.a = static_cast<const char*>(p.a) + row0 * arow;
     t.a_scales = ROWS4 ? p.a_scales + row0 * (p.K >> 5) : nullptr;
     t.w = static_cast<const char*>(p.w) + (int64_t)expert * p.N * (p.K >> 1);
@@ -56,26 +64,57 @@ __device__ __forceinline__ bool mx_task(const MxProduct& p, int BN, MxTask& t) {
     return true;
 }
 
-__device__ __forceinline__ float mx_activate(float u, int act) {
-    if (act == MOE_ACT_GELU) return gelu16(u);
-    return act == MOE_ACT_RELU && u < 0.0f ? 0.0f : u;           // a NaN stays a NaN
+// The bias of four neighbouring columns.
+__device__ __forceinline__ mx_f32x4 mx_bias4(const MxProduct& p, const MxTask& t, int col) {
+    mx_f32x4 b = {0.f, 0.f, 0.f, 0.f};
+    if (t.bias) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (col + r < p.N) b[r] = bf16_bits_to_f32(t.bias[col + r]);
+    }
+    return b;
 }
-
-// Four neighbouring columns of a token row, as the matrix instructions leave them in a lane.
-__device__ __forceinline__ void mx_store4(const MxProduct& p, const MxTask& t, int row, int col, const mx_f32x4& acc) {
+// Four neighbouring columns of a token row, as the matrix instructions leave them in a lane.  whole: N is a multiple of 4.
+template <int ACT>
+__device__ __forceinline__ void mx_store4(const MxTask& t, int N, bool whole, int row, int col, const mx_f32x4& u) {
     float v[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) v[r] = mx_activate(acc[r] + (t.bias && col + r < p.N ? bf16_bits_to_f32(t.bias[col + r]) : 0.0f), p.act);
+    for (int r = 0; r < 4; ++r) v[r] = ACT == MOE_ACT_GELU ? gelu16(u[r]) : ACT == MOE_ACT_RELU && u[r] < 0.0f ? 0.0f : u[r];      // a NaN stays a NaN
     const uint32_t lo = pack2_bf16(v[0], v[1]), hi = pack2_bf16(v[2], v[3]);
-    uint16_t* o = t.out + (int64_t)row * p.N + col;
-    if (col + 3 < p.N && (p.N & 3) == 0) {
+    uint16_t* o = t.out + (int64_t)row * N + col;
+    if (whole) {
         *reinterpret_cast<uint2*>(o) = uint2{lo, hi};
     } else {
         const uint32_t w[4] = {lo, lo >> 16, hi, hi >> 16};
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-            if (col + r < p.N) o[r] = (uint16_t)w[r];
+            if (col + r < N) o[r] = (uint16_t)w[r];
     }
+}
+// ... for NT x CG of them: rows row0 + 16 i, columns col0 + 16 g.  One activation for all: a switch at every value costs more than the values.
+template <int NT, int CG>
+__device__ __forceinline__ void mx_store_tile(const MxProduct& p, const MxTask& t, int row0, int col0, const mx_f32x4 (&acc)[NT][CG]) {
+    const int N = p.N;
+    mx_f32x4 b[CG];
+#pragma unroll
+    for (int g = 0; g < CG; ++g) b[g] = mx_bias4(p, t, col0 + 16 * g);
+    auto all = [&](auto act_c, auto whole_c) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            if (row0 + 16 * i >= t.rows) break;
+#pragma unroll
+            for (int g = 0; g < CG; ++g)
+                if (col0 + 16 * g < N) mx_store4<decltype(act_c)::value>(t, N, decltype(whole_c)::value, row0 + 16 * i, col0 + 16 * g, acc[i][g] + b[g]);
+        }
+    };
+    typedef std::true_type Whole;
+    if (N & 3) {
+        if (p.act == MOE_ACT_GELU) all(std::integral_constant<int, MOE_ACT_GELU>{}, std::false_type{});
+        else if (p.act == MOE_ACT_RELU) all(std::integral_constant<int, MOE_ACT_RELU>{}, std::false_type{});
+        else all(std::integral_constant<int, MOE_ACT_NONE>{}, std::false_type{});
+    } else if (p.act == MOE_ACT_GELU) all(std::integral_constant<int, MOE_ACT_GELU>{}, Whole{});
+    else if (p.act == MOE_ACT_RELU) all(std::integral_constant<int, MOE_ACT_RELU>{}, Whole{});
+    else all(std::integral_constant<int, MOE_ACT_NONE>{}, Whole{});
 }
 
 // ---- up to 16 rows a block: a weight streamer ----
@@ -172,12 +211,10 @@ __global__ __launch_bounds__(64 * kStreamWaves) void mx_stream_kernel(MxProduct 
         multiply(0);
     }
     if (!skinny_join<CG>(acc, ks, KS, red + set * (KS - 1) * CG * 64, lane)) return;
-    if (idx >= t.rows) return;
+    mx_f32x4 sum[1][CG];
 #pragma unroll
-    for (int g = 0; g < CG; ++g) {
-        const int col = n0 + 16 * g + 4 * q;
-        if (col < p.N) mx_store4(p, t, idx, col, acc[g]);
-    }
+    for (int g = 0; g < CG; ++g) sum[0][g] = acc[g];
+    mx_store_tile<1, CG>(p, t, idx, n0 + 4 * q, sum);
 }
 
 // ---- more rows: tiles ----
@@ -198,14 +235,15 @@ struct MxTile {
     static constexpr int ROWS_A_LOAD = 1024 / PITCH;           // rows that one instruction of a wavefront brings
     static constexpr int LOADS = BM / ROWS_A_LOAD / SET;
     static constexpr int RB = NT < 4 ? NT : 4;                 // groups of 16 rows whose fragments are in registers at once (twice)
-    static constexpr int SCALES = ROWS4 ? 8 * (BM / RB) * 4 : 0;   // bytes of the rows' scales in a slab: a dword has those of RB rows
+    static constexpr int GROUPS = (BM + 63) / 64;              // of 64 rows, whose scales share dwords
+    static constexpr int SCALES = ROWS4 ? 8 * GROUPS * 64 : 0;
     static constexpr int STAGE = BM * PITCH + SCALES;
     static constexpr int SUMS = (KS - 1) * SET * NT * CG * 1024;
     static constexpr int LDS = 2 * KS * STAGE > SUMS ? 2 * KS * STAGE : SUMS;
     static constexpr int BLOCKS = NT * CG >= 32 ? 1 : NT * CG >= 16 ? 2 : 160 * 1024 / LDS;      // workgroups of a compute unit
     static constexpr int WAVES_PER_SIMD = BLOCKS * THREADS / 256 < 4 ? BLOCKS * THREADS / 256 : 4;
     static_assert(SET % 4 == 0 && LOADS >= 1 && BM % (ROWS_A_LOAD * SET) == 0, "every wavefront of a set brings as many rows, in steps of 16");
-    static_assert(!ROWS4 || BM <= 64 * SET, "a row's scales a thread");
+    static_assert(!ROWS4 || (GROUPS <= SET && (RH == 1 || 16 * NT % 64 == 0)), "a row's scales a thread; a wavefront's rows begin a group");
     static_assert(LDS <= 160 * 1024, "LDS of a compute unit");
 };
 
@@ -248,7 +286,6 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void mx_tile_kernel(
     }
     unsigned char* const stages = smem + ks * 2 * T::STAGE;
     const int slabs_all = (int)((arow + PITCH - 1) / PITCH);                   // of a row; set ks takes ks, ks + KS, ...
-    const int slabs = slabs_all > ks ? (slabs_all - ks + KS - 1) / KS : 0;
     const int slabs_most = (slabs_all + KS - 1) / KS;
     const __amdgpu_buffer_rsrc_t a_buf = mx_buffer(t.a, (uint32_t)t.rows * arow);
     // slab number s of this set into stage s & 1
@@ -260,30 +297,32 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void mx_tile_kernel(
         for (int i = 0; i < T::LOADS; ++i)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(a_buf, (mx_lds_void*)(st + (i * T::SET + sw) * 1024), 16, (int)(v + i * T::SET * T::ROWS_A_LOAD * arow), 0, 0, 0);
     };
-    // The rows' scales, a row a thread, through a register (their addresses have no alignment), into LDS as the matrix instruction picks
-    // them: it takes one byte of a register, so the dword for (block, 64 rows, lane) has those of rows lane, 16 + lane, 32 + lane, 48 + lane.
-    uint32_t rs[2] = {0, 0};
-    const int my_row = (int)threadIdx.x - ks * T::SET * 64;
-    auto load8 = [&](uint32_t (&d)[2], const uint8_t* at, int b0) {            // blocks b0 .. b0 + 7 of a row of srow
-        if (b0 + 8 <= (int)srow) {
-            __builtin_memcpy(d, at + b0, 8);
-        } else {
-            d[0] = d[1] = 0;
-#pragma unroll
-            for (int b = 0; b < 8; ++b)
-                if (b0 + b < (int)srow) d[b >> 2] |= (uint32_t)at[b0 + b] << (8 * (b & 3));
-        }
-    };
+    // The rows' scales, a row a lane, through registers (their addresses have no alignment), into LDS as the matrix instruction picks them: it
+    // takes one byte of a register, so the dword for (block, 64 rows, idx) has those of rows idx, 16 + idx, 32 + idx, 48 + idx.  Every
+    // wavefront does so, some for the same rows: without a branch, behind which the compiler would move products.
+    uint64_t rs = 0;
+    const int group = sw % T::GROUPS, my_row = min(64 * group + lane, t.rows - 1);
     auto load_row_scales = [&](int s) {
-        if constexpr (ROWS4)
-            if (my_row < T::BM) load8(rs, t.a_scales + (uint32_t)(my_row < t.rows ? my_row : 0) * srow, (s * KS + ks) * 8);
+        if constexpr (ROWS4) {                     // eight bytes, of which those of this row count; inside the whole array, which is longer
+            const int b0 = (s * KS + ks) * 8, n = min(max((int)srow - b0, 0), 8);
+            const int64_t want = (t.row0 + my_row) * srow + min(b0, (int)srow), at = min(want, p.M * srow - 8);
+            uint64_t v;
+            __builtin_memcpy(&v, p.a_scales + at, 8);
+            v = n > 0 ? v >> (8 * (want - at)) : 0;
+            rs = n < 8 ? v & (((uint64_t)1 << (8 * n)) - 1) : v;
+        }
     };
     auto store_row_scales = [&](int s) {
         if constexpr (ROWS4) {
-            if (my_row < T::BM) {
-                unsigned char* at = stages + (s & 1) * T::STAGE + T::BM * PITCH + (my_row / (16 * RB) * 16 + my_row % 16) * 4 + my_row / 16 % RB;
+            uint32_t* at = reinterpret_cast<uint32_t*>(stages + (s & 1) * T::STAGE + T::BM * PITCH) + group * 16 + idx;
 #pragma unroll
-                for (int b = 0; b < 8; ++b) at[b * (T::BM / RB * 4)] = (unsigned char)(rs[b >> 2] >> (8 * (b & 3)));
+            for (int h = 0; h < 2; ++h) {          // blocks 4 h + q: four lanes, sixteen apart, turn their four bytes round
+                const uint32_t mine = (uint32_t)(rs >> (32 * h));
+                const auto a = __builtin_amdgcn_permlane16_swap(mine, mine, false, false);       // lanes' rows 0 0 2 2 and 1 1 3 3
+                const auto even = __builtin_amdgcn_permlane32_swap(a[0], a[0], false, false), odd = __builtin_amdgcn_permlane32_swap(a[1], a[1], false, false);
+                const uint32_t sel = 0x0C0C0400u + 0x0101u * q;                                  // byte q of the second operand, then of the first
+                const uint32_t lo = __builtin_amdgcn_perm(odd[0], even[0], sel), hi = __builtin_amdgcn_perm(odd[1], even[1], sel);
+                at[(4 * h + q) * T::GROUPS * 16] = lo | hi << 16;
             }
         }
     };
@@ -292,8 +331,9 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void mx_tile_kernel(
     const int c0 = t.n0 + 16 * CG * wn;
     const __amdgpu_buffer_rsrc_t w_buf = mx_buffer(t.w, (uint32_t)N * wrow), s_buf = mx_buffer(t.s, (uint32_t)N * srow);
     const uint32_t w_off = (uint32_t)(c0 + idx) * wrow + 16 * q, s_off = (uint32_t)(c0 + idx) * srow + q;
-    mx_u32x4 w[2][CG];
-    uint32_t ws[2][CG];
+    mx_u32x4 w[ROWS4 ? 2 : 1][CG], cur[CG];
+    uint32_t ws[ROWS4 ? 2 : 1][CG];
+    float cur_s[CG];
     auto load_w = [&](int b, int step) {          // step: of 128 values, counted over the whole row
         const bool in = step * 128 + 32 * q < K;
         const uint32_t wv = in ? w_off + 64 * (uint32_t)step : kBehind, sv = in ? s_off + 4 * (uint32_t)step : kBehind;
@@ -309,15 +349,14 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void mx_tile_kernel(
     for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int g = 0; g < CG; ++g) acc[i][g] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
-    const bool any = t.rows > wm * 16 * NT;       // rows of this wavefront that exist
-
     // A slab, in blocks of RB groups of rows: the next block's fragments are read (and, with bf16 rows, the next weights widened) under the
     // products of the one before.  Parts: the quarters j of a step (bf16), the steps of a slab (MXFP4).
     constexpr int PARTS = ROWS4 ? 2 : 4, NB = NT / RB, SEQ = PARTS * NB;
-    auto slab = [&](const unsigned char* st, int wb) {
+    mx_u32x4 x[2][RB];
+    uint32_t xs[2];
+    // behind(part): what is requested once the weights of a part are done with
+    auto slab = [&](const unsigned char* st, auto behind) {
         const unsigned char* base = st + (wm * 16 * NT + idx) * PITCH;
-        mx_u32x4 x[2][RB];
-        uint32_t xs[2];
         mx_bf16x8 wf[2][CG];
         auto read = [&](int n) {
             const int part = n / NB, ib = n % NB;
@@ -325,14 +364,14 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void mx_tile_kernel(
 #pragma unroll
             for (int i = 0; i < RB; ++i) x[n & 1][i] = *reinterpret_cast<const mx_u32x4*>(base + (ib * RB + i) * 16 * PITCH + at);
             if constexpr (ROWS4)
-                xs[n & 1] = *reinterpret_cast<const uint32_t*>(st + T::BM * PITCH + (4 * part + q) * (T::BM / RB * 4) + ((wm * NB + ib) * 16 + idx) * 4);
+                xs[n & 1] = reinterpret_cast<const uint32_t*>(st + T::BM * PITCH)[((4 * part + q) * T::GROUPS + wm * NB + ib) * 16 + idx];
         };
         auto widen = [&](int part) {
             if constexpr (!ROWS4) {
 #pragma unroll
                 for (int g = 0; g < CG; ++g) {
-                    const uint32_t codes = w[wb][g][part];
-                    wf[part & 1][g] = mx_widen8(codes, mx_scale(ws[wb][g]));
+                    const uint32_t codes = cur[g][part];
+                    wf[part & 1][g] = mx_widen8(codes, cur_s[g]);
                 }
             }
         };
@@ -359,48 +398,60 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void mx_tile_kernel(
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
+            if (ib == NB - 1) behind(part);
         }
     };
-    // Every request of this wavefront for the slab has landed and its reads of the other stage are done, then so have everybody's.
-    auto meet = [&]() {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    // Every request of this wavefront for the slab's rows has landed (LATER requests behind them may be on their way) and its reads of the
+    // other stage are done, then so have everybody's.
+    auto meet = [&](auto later) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(decltype(later)::value) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
+    typedef std::integral_constant<int, 0> None;
+    typedef std::integral_constant<int, 4 * CG> Weights;       // MXFP4 rows: the two steps' loads, which come last
 
-    if (slabs > 0) {
-        issue(0);
-        load_row_scales(0);
-        load_w(0, ks * (ROWS4 ? 2 : 1));
-        if constexpr (ROWS4) load_w(1, ks * 2 + 1);
-        store_row_scales(0);
-    }
-    for (int s = 0; s < slabs_most; s += 2) {
+    // One path for every slab: what is requested behind the last one lies behind the operands' ends, and every set runs as many slabs as the
+    // longest (of zeros).  Where paths with and without requests met, every wait would be one for all of them.
+    constexpr int STEPS = ROWS4 ? 2 : 1;
+    issue(0);
+    load_row_scales(0);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {             // stage u; weights: buffer u (bf16 rows), both (MXFP4 rows)
-            if (s + u >= slabs_most) break;
-            meet();
-            const bool here = s + u < slabs, more = s + u + 1 < slabs;
-            const int next = (s + u + 1) * KS + ks;
-            const unsigned char* st = stages + u * T::STAGE;
-            if (more) {
-                issue(s + u + 1);
-                load_row_scales(s + u + 1);
-                if constexpr (!ROWS4) load_w(u ^ 1, next);
-            }
-            if (here && any) slab(st, u);
+    for (int h = 0; h < STEPS; ++h) load_w(h, ks * STEPS + h);
+    store_row_scales(0);
+    if (t.rows > wm * 16 * NT) {
+        for (int s = 0; s < slabs_most; ++s) {
+            const int next = ((s + 1) * KS + ks) * STEPS;
+            const unsigned char* st = stages + (s & 1) * T::STAGE;
             if constexpr (ROWS4) {
-                if (more) {
-                    load_w(0, 2 * next);
-                    load_w(1, 2 * next + 1);
-                    store_row_scales(s + u + 1);
+                meet(Weights{});
+                issue(s + 1);
+                load_row_scales(s + 1);
+                slab(st, [&](int part) { load_w(part, next + part); });
+                store_row_scales(s + 1);
+            } else {
+                meet(None{});
+#pragma unroll
+                for (int g = 0; g < CG; ++g) {
+                    cur[g] = w[0][g];
+                    cur_s[g] = mx_scale(ws[0][g]);
                 }
+                issue(s + 1);
+                load_w(0, next);
+                slab(st, [](int) {});
             }
+        }
+    } else {                                      // no rows for this wavefront: it brings the others theirs
+        for (int s = 0; s < slabs_most; ++s) {
+            meet(None{});
+            issue(s + 1);
+            load_row_scales(s + 1);
+            store_row_scales(s + 1);
         }
     }
 
     if constexpr (KS > 1) {                       // the sets' sums, in their order
-        meet();
+        meet(None{});
         mx_f32x4* red = reinterpret_cast<mx_f32x4*>(smem) + sw * NT * CG * 64 + lane;
         if (ks > 0) {
 #pragma unroll
@@ -416,16 +467,7 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void mx_tile_kernel(
 #pragma unroll
                 for (int g = 0; g < CG; ++g) acc[i][g] += red[(k * T::SET * NT * CG + i * CG + g) * 64];
     }
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-        const int row = 16 * (wm * NT + i) + idx;
-        if (row >= t.rows) continue;
-#pragma unroll
-        for (int g = 0; g < CG; ++g) {
-            const int col = c0 + 16 * g + 4 * q;
-            if (col < N) mx_store4(p, t, row, col, acc[i][g]);
-        }
-    }
+    mx_store_tile<NT, CG>(p, t, 16 * wm * NT + idx, c0 + 4 * q, acc);
 }
 
 // Workgroups of a launch: blocks of BM rows (an expert's last one is its own) times column tiles, in eight equal shares.

@@ -170,7 +170,9 @@ __device__ __forceinline__ void skinny_multiply(mx_f32x4 (&acc)[G], const Skinny
 // Both operands in MXFP4: the scaled instruction over 128 values.  A scale is a byte of its register: the lowest of sa, byte BYTE of sb.
 template <int BYTE = 0>
 __device__ __forceinline__ mx_f32x4 mx_mfma(mx_u32x4 a, uint32_t sa, mx_u32x4 b, uint32_t sb, mx_f32x4 c) {
-    const mx_i32x8 av = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0}, bv = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
+    // (the upper half, which 4-bit operands do not have, is left open)
+    const mx_i32x8 av = __builtin_bit_cast(mx_i32x8, __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1));
+    const mx_i32x8 bv = __builtin_bit_cast(mx_i32x8, __builtin_shufflevector(b, b, 0, 1, 2, 3, -1, -1, -1, -1));
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4 /* e2m1 */, 4, 0, (int)sa, BYTE, (int)sb);
 }
 
