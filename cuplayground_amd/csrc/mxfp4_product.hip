@@ -219,128 +219,256 @@ __global__ __launch_bounds__(64 * kStreamWaves) void mx_stream_kernel(MxProduct 
 
 // ---- more rows: tiles ----
 //
-// RH x CW wavefronts of 16 NT rows x 16 CG columns each, KS sets of them that share the contraction.  Token rows go straight into LDS, a
-// slab of 256 (bf16) or 128 bytes (MXFP4) a row at a time, one slab ahead; every fragment of theirs serves CG groups of columns.  Weights go
-// straight into the registers of the wavefront that multiplies them, 64 bytes of a row a step of 128 values, a step ahead: a lane's 16
-// bytes are a whole block and already the fragment (skinny.hpp).  All operands are read through buffers that end where they end, so rows
-// behind the block's last one, columns behind the matrix's and what lies behind K are zeros without a branch.
-template <bool ROWS4_, int RH_, int NT_, int CW_, int CG_, int KS_>
+// RH x CW wavefronts of 16 NT rows x 16 CG columns each, KS sets of them that share the contraction.  Operands go straight into LDS a slab of
+// the contraction at a time, one slab ahead, and are read through buffers that end where they end: rows behind the block's last one,
+// columns behind the matrix's and what lies behind K are zeros without a branch.  Every slab takes the same path: what is requested behind
+// the last one lies behind the operands' ends, and every set runs as many slabs as the longest (of zeros).  Where paths with and without
+// requests met, every wait would be one for all of them.
+constexpr uint32_t kBehind = 0xD0000000u;      // an offset behind the end of every buffer here, also with a tile's rows added to it (offsets
+                                               // are whole in the vector register: the range check is against what a scalar offset leaves of the
+                                               // buffer, and that may be less than nothing)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_buffer(const void* p, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00020000);
+}
+// Every request of this wavefront for the slab has landed and its reads of the other stage are done, then so have everybody's.
+__device__ __forceinline__ void mx_meet() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+// The sets' sums, in their order, through LDS: returns whether this wavefront holds them.
+template <int KS, int SET, int NT, int CG>
+__device__ __forceinline__ bool mx_join(mx_f32x4 (&acc)[NT][CG], int ks, int sw, unsigned char* smem, int lane) {
+    if constexpr (KS > 1) {
+        mx_meet();
+        mx_f32x4* red = reinterpret_cast<mx_f32x4*>(smem) + sw * NT * CG * 64 + lane;
+        if (ks > 0) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int g = 0; g < CG; ++g) red[((ks - 1) * SET * NT * CG + i * CG + g) * 64] = acc[i][g];
+        }
+        __syncthreads();
+        if (ks > 0) return false;
+        for (int k = 0; k < KS - 1; ++k)
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int g = 0; g < CG; ++g) acc[i][g] += red[(k * SET * NT * CG + i * CG + g) * 64];
+    }
+    return true;
+}
+
+// -- rows in bf16 --
+// A slab is 128 values: 256 bytes of a token row, 64 of a weight row, of which a lane's 16 are a whole block and, widened, four fragments
+// (skinny.hpp).  Scales go through registers: two stages of a 128 x 128 tile's operands are half of the LDS to the byte.
+template <int RH_, int NT_, int CW_, int CG_, int KS_>
 struct MxTile {
-    static constexpr bool ROWS4 = ROWS4_;
+    static constexpr bool ROWS4 = false;
     static constexpr int RH = RH_, NT = NT_, CW = CW_, CG = CG_, KS = KS_;
     static constexpr int BM = 16 * NT * RH, BN = 16 * CG * CW;
     static constexpr int SET = RH * CW;                        // wavefronts of a set
     static constexpr int THREADS = 64 * SET * KS;
-    static constexpr int PITCH = ROWS4 ? 128 : 256;            // bytes of a row in a slab
-    static constexpr int ROWS_A_LOAD = 1024 / PITCH;           // rows that one instruction of a wavefront brings
-    static constexpr int LOADS = BM / ROWS_A_LOAD / SET;
+    static constexpr int LOADS_A = BM / 4 / SET, LOADS_W = BN / 16 / SET;      // an instruction of a wavefront brings 4 and 16 rows
     static constexpr int RB = NT < 4 ? NT : 4;                 // groups of 16 rows whose fragments are in registers at once (twice)
-    static constexpr int GROUPS = (BM + 63) / 64;              // of 64 rows, whose scales share dwords
-    static constexpr int SCALES = ROWS4 ? 8 * GROUPS * 64 : 0;
-    static constexpr int STAGE = BM * PITCH + SCALES;
+    static constexpr int STAGE = BM * 256 + BN * 64;
     static constexpr int SUMS = (KS - 1) * SET * NT * CG * 1024;
     static constexpr int LDS = 2 * KS * STAGE > SUMS ? 2 * KS * STAGE : SUMS;
     static constexpr int BLOCKS = NT * CG >= 32 ? 1 : NT * CG >= 16 ? 2 : 160 * 1024 / LDS;      // workgroups of a compute unit
     static constexpr int WAVES_PER_SIMD = BLOCKS * THREADS / 256 < 4 ? BLOCKS * THREADS / 256 : 4;
-    static_assert(SET % 4 == 0 && LOADS >= 1 && BM % (ROWS_A_LOAD * SET) == 0, "every wavefront of a set brings as many rows, in steps of 16");
-    static_assert(!ROWS4 || (GROUPS <= SET && (RH == 1 || 16 * NT % 64 == 0)), "a row's scales a thread; a wavefront's rows begin a group");
+    static_assert(SET % 4 == 0 && BM % (4 * SET) == 0 && BN % (16 * SET) == 0, "every wavefront of a set brings as many rows, in steps of 16");
     static_assert(LDS <= 160 * 1024, "LDS of a compute unit");
 };
-
-// An offset behind the end of every buffer here, also with a tile's rows added to it.  (Offsets are whole in the vector register: the range
-// check is against what a scalar offset leaves of the buffer, and that may be less than nothing.)
-constexpr uint32_t kBehind = 0xD0000000u;
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_buffer(const void* p, uint32_t bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00020000);
-}
 
 template <class T>
 __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void mx_tile_kernel(MxProduct p) {
     extern __shared__ __align__(16) unsigned char smem[];
-    constexpr int NT = T::NT, CG = T::CG, PITCH = T::PITCH, RB = T::RB, KS = T::KS;
-    constexpr bool ROWS4 = T::ROWS4;
+    constexpr int NT = T::NT, CG = T::CG, RB = T::RB, KS = T::KS;
     MxTask t;
-    if (!mx_task<T::BM, ROWS4>(p, T::BN, t)) return;
+    if (!mx_task<T::BM, false>(p, T::BN, t)) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ks = wave / T::SET, sw = wave % T::SET;            // set and place in it
     const int wm = sw / T::CW, wn = sw % T::CW;
     const int idx = lane & 15, q = lane >> 4;
     const int K = p.K, N = p.N;
-    const uint32_t arow = ROWS4 ? (uint32_t)K >> 1 : 2 * (uint32_t)K, wrow = (uint32_t)K >> 1, srow = (uint32_t)K >> 5;
+    const uint32_t arow = 2 * (uint32_t)K, wrow = (uint32_t)K >> 1, srow = (uint32_t)K >> 5;
 
     // Rows into LDS: an instruction of a wavefront writes 1 KB of LDS in the order of its lanes, so what a slot holds is decided by the
     // address its lane reads.  The LDS serves a 16-byte read to lanes 0-3, 12-15 and 20-27 in one cycle, to 4-11, 16-19 and 28-31 in the
-    // next: with 256-byte rows chunk 4 q + j, the one that lane (row, q) reads as its j-th, lies in slot (q + 4 j) ^ row, with 128-byte rows
-    // chunk c in slot c ^ (row / 2): no two of a cycle meet.
-    uint32_t chunk, a_off;
-    {
-        const int slots = PITCH / 16, r_in = lane / slots, slot = lane % slots;
-        const int r = (sw * T::ROWS_A_LOAD + r_in) & 15;
-        if constexpr (ROWS4) {
-            chunk = slot ^ ((r >> 1) & 7);
-        } else {
-            const int o = slot ^ r;
-            chunk = 4 * (o & 3) + (o >> 2);
-        }
-        a_off = (uint32_t)(sw * T::ROWS_A_LOAD + r_in) * arow;
-    }
+    // next: chunk 4 q + j of a row, the one that lane (row, q) reads as its j-th, lies in slot (q + 4 j) ^ row: no two of a cycle meet.
+    const int swapped = (lane & 15) ^ ((4 * sw + q) & 15);
+    const uint32_t chunk = 4 * (swapped & 3) + (swapped >> 2), a_off = (uint32_t)(4 * sw + q) * arow;
     unsigned char* const stages = smem + ks * 2 * T::STAGE;
-    const int slabs_all = (int)((arow + PITCH - 1) / PITCH);                   // of a row; set ks takes ks, ks + KS, ...
-    const int slabs_most = (slabs_all + KS - 1) / KS;
-    const __amdgpu_buffer_rsrc_t a_buf = mx_buffer(t.a, (uint32_t)t.rows * arow);
-    // slab number s of this set into stage s & 1
-    auto issue = [&](int s) {
+    const int slabs_all = (K + 127) >> 7, slabs = (slabs_all + KS - 1) / KS;       // of a row; set ks takes ks, ks + KS, ...
+    // (a weight row's chunk c lies in slot c ^ w_turn: of rows four apart, which meet the same banks, two take chunk q and two q ^ 1)
+    auto w_turn = [](int row) { return (4 - (row >> 2)) & 3; };
+    const int c0 = t.n0 + 16 * CG * wn;
+    const uint32_t w_chunk = (lane & 3) ^ w_turn(lane >> 2), w_off = (uint32_t)(t.n0 + 16 * sw + (lane >> 2)) * wrow, s_off = (uint32_t)(c0 + idx) * srow + q;
+    const __amdgpu_buffer_rsrc_t a_buf = mx_buffer(t.a, (uint32_t)t.rows * arow), w_buf = mx_buffer(t.w, (uint32_t)N * wrow), s_buf = mx_buffer(t.s, (uint32_t)N * srow);
+    auto issue = [&](int s) {                     // slab number s of this set into stage s & 1
         unsigned char* const st = stages + (s & 1) * T::STAGE;
-        const uint32_t at = (uint32_t)(s * KS + ks) * PITCH + 16 * chunk;
-        const uint32_t v = at < arow ? a_off + at : kBehind;
+        const uint32_t slab = s * KS + ks, at = slab * 256 + 16 * chunk, w_at = slab * 64 + 16 * w_chunk;
+        const uint32_t v = at < arow ? a_off + at : kBehind, vw = w_at < wrow ? w_off + w_at : kBehind;
 #pragma unroll
-        for (int i = 0; i < T::LOADS; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(a_buf, (mx_lds_void*)(st + (i * T::SET + sw) * 1024), 16, (int)(v + i * T::SET * T::ROWS_A_LOAD * arow), 0, 0, 0);
-    };
-    // The rows' scales, a row a lane, through registers (their addresses have no alignment), into LDS as the matrix instruction picks them: it
-    // takes one byte of a register, so the dword for (block, 64 rows, idx) has those of rows idx, 16 + idx, 32 + idx, 48 + idx.  Every
-    // wavefront does so, some for the same rows: without a branch, behind which the compiler would move products.
-    uint64_t rs = 0;
-    const int group = sw % T::GROUPS, my_row = min(64 * group + lane, t.rows - 1);
-    auto load_row_scales = [&](int s) {
-        if constexpr (ROWS4) {                     // eight bytes, of which those of this row count; inside the whole array, which is longer
-            const int b0 = (s * KS + ks) * 8, n = min(max((int)srow - b0, 0), 8);
-            const int64_t want = (t.row0 + my_row) * srow + min(b0, (int)srow), at = min(want, p.M * srow - 8);
-            uint64_t v;
-            __builtin_memcpy(&v, p.a_scales + at, 8);
-            v = n > 0 ? v >> (8 * (want - at)) : 0;
-            rs = n < 8 ? v & (((uint64_t)1 << (8 * n)) - 1) : v;
-        }
-    };
-    auto store_row_scales = [&](int s) {
-        if constexpr (ROWS4) {
-            uint32_t* at = reinterpret_cast<uint32_t*>(stages + (s & 1) * T::STAGE + T::BM * PITCH) + group * 16 + idx;
+        for (int i = 0; i < T::LOADS_A; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(a_buf, (mx_lds_void*)(st + (i * T::SET + sw) * 1024), 16, (int)(v + i * T::SET * 4 * arow), 0, 0, 0);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {          // blocks 4 h + q: four lanes, sixteen apart, turn their four bytes round
-                const uint32_t mine = (uint32_t)(rs >> (32 * h));
-                const auto a = __builtin_amdgcn_permlane16_swap(mine, mine, false, false);       // lanes' rows 0 0 2 2 and 1 1 3 3
-                const auto even = __builtin_amdgcn_permlane32_swap(a[0], a[0], false, false), odd = __builtin_amdgcn_permlane32_swap(a[1], a[1], false, false);
-                const uint32_t sel = 0x0C0C0400u + 0x0101u * q;                                  // byte q of the second operand, then of the first
-                const uint32_t lo = __builtin_amdgcn_perm(odd[0], even[0], sel), hi = __builtin_amdgcn_perm(odd[1], even[1], sel);
-                at[(4 * h + q) * T::GROUPS * 16] = lo | hi << 16;
+        for (int i = 0; i < T::LOADS_W; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(w_buf, (mx_lds_void*)(st + T::BM * 256 + (i * T::SET + sw) * 1024), 16, (int)(vw + i * T::SET * 16 * wrow), 0, 0, 0);
+    };
+    uint32_t ws[CG];
+    auto load_scales = [&](int s) {
+        const uint32_t slab = s * KS + ks, v = slab * 4 + q < srow ? s_off + 4 * slab : kBehind;
+#pragma unroll
+        for (int g = 0; g < CG; ++g) ws[g] = __builtin_amdgcn_raw_buffer_load_b8(s_buf, (int)(v + g * 16 * srow), 0, 0);
+    };
+
+    mx_f32x4 acc[NT][CG];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int g = 0; g < CG; ++g) acc[i][g] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
+
+    // A slab, in blocks of RB groups of rows of a quarter (32 values a lane group): the next block's fragments are read, and the next quarter's
+    // weights widened, under the products of the one before.
+    constexpr int NB = NT / RB, SEQ = 4 * NB;
+    float scale[CG];
+    auto slab = [&](const unsigned char* st) {
+        const unsigned char* base = st + (wm * 16 * NT + idx) * 256;
+        mx_u32x4 x[2][RB], w[CG];
+        mx_bf16x8 wf[2][CG];
+#pragma unroll
+        for (int g = 0; g < CG; ++g) w[g] = *reinterpret_cast<const mx_u32x4*>(st + T::BM * 256 + (wn * 16 * CG + 16 * g + idx) * 64 + ((q ^ w_turn(idx)) << 4));
+        auto read = [&](int n) {
+            const int at = ((q + 4 * (n / NB)) ^ idx) << 4;
+#pragma unroll
+            for (int i = 0; i < RB; ++i) x[n & 1][i] = *reinterpret_cast<const mx_u32x4*>(base + (n % NB * RB + i) * 16 * 256 + at);
+        };
+        auto widen = [&](int quarter) {
+#pragma unroll
+            for (int g = 0; g < CG; ++g) {
+                const uint32_t codes = w[g][quarter];
+                wf[quarter & 1][g] = mx_widen8(codes, scale[g]);
             }
+        };
+        read(0);
+        widen(0);
+#pragma unroll
+        for (int n = 0; n < SEQ; ++n) {
+            const int quarter = n / NB, ib = n % NB;
+            if (n + 1 < SEQ) read(n + 1);
+            if (ib == NB - 1 && quarter < 3) widen(quarter + 1);
+#pragma unroll
+            for (int i = 0; i < RB; ++i)
+#pragma unroll
+                for (int g = 0; g < CG; ++g)
+                    acc[ib * RB + i][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[quarter & 1][g], __builtin_bit_cast(mx_bf16x8, x[n & 1][i]), acc[ib * RB + i][g], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
 
-    // weights: rows of 16 columns a group
-    const int c0 = t.n0 + 16 * CG * wn;
-    const __amdgpu_buffer_rsrc_t w_buf = mx_buffer(t.w, (uint32_t)N * wrow), s_buf = mx_buffer(t.s, (uint32_t)N * srow);
-    const uint32_t w_off = (uint32_t)(c0 + idx) * wrow + 16 * q, s_off = (uint32_t)(c0 + idx) * srow + q;
-    mx_u32x4 w[ROWS4 ? 2 : 1][CG], cur[CG];
-    uint32_t ws[ROWS4 ? 2 : 1][CG];
-    float cur_s[CG];
-    auto load_w = [&](int b, int step) {          // step: of 128 values, counted over the whole row
-        const bool in = step * 128 + 32 * q < K;
-        const uint32_t wv = in ? w_off + 64 * (uint32_t)step : kBehind, sv = in ? s_off + 4 * (uint32_t)step : kBehind;
+    issue(0);
+    if (t.rows > wm * 16 * NT) {
+        load_scales(0);
+        for (int s = 0; s < slabs; ++s) {
+            mx_meet();
 #pragma unroll
-        for (int g = 0; g < CG; ++g) {
-            w[b][g] = __builtin_bit_cast(mx_u32x4, __builtin_amdgcn_raw_buffer_load_b128(w_buf, (int)(wv + g * 16 * wrow), 0, 0));
-            ws[b][g] = __builtin_amdgcn_raw_buffer_load_b8(s_buf, (int)(sv + g * 16 * srow), 0, 0);
+            for (int g = 0; g < CG; ++g) scale[g] = mx_scale(ws[g]);
+            issue(s + 1);
+            load_scales(s + 1);
+            slab(stages + (s & 1) * T::STAGE);
+        }
+    } else {                                      // no rows for this wavefront: it brings the others theirs
+        for (int s = 0; s < slabs; ++s) {
+            mx_meet();
+            issue(s + 1);
+        }
+    }
+    if (!mx_join<KS, T::SET, NT, CG>(acc, ks, sw, smem, lane)) return;
+    mx_store_tile<NT, CG>(p, t, 16 * wm * NT + idx, c0 + 4 * q, acc);
+}
+
+// -- rows in MXFP4 too --
+// A slab is 256 values, 128 bytes of every row, both operands in LDS: the products are so fast that a fragment of weights fetched by each of
+// the RH wavefronts that use it, half a line at a time, costs five times their time.
+template <int RH_, int NT_, int CW_, int CG_, int KS_>
+struct MxTile4 {
+    static constexpr bool ROWS4 = true;
+    static constexpr int RH = RH_, NT = NT_, CW = CW_, CG = CG_, KS = KS_;
+    static constexpr int BM = 16 * NT * RH, BN = 16 * CG * CW;
+    static constexpr int SET = RH * CW;
+    static constexpr int THREADS = 64 * SET * KS;
+    static constexpr int LOADS_A = BM / 8 / SET, LOADS_W = BN / 8 / SET;       // an instruction of a wavefront brings 8 rows
+    static constexpr int RB = NT < 4 ? NT : 4;
+    static constexpr int GROUPS_A = (BM + 63) / 64, GROUPS = GROUPS_A + (BN + 63) / 64;      // of 64 rows, whose scales share dwords: tokens, then weights
+    static constexpr int SCALES = 8 * GROUPS * 64;
+    static constexpr int STAGE = (BM + BN) * 128 + SCALES;
+    static constexpr int SUMS = (KS - 1) * SET * NT * CG * 1024;
+    static constexpr int LDS = 2 * KS * STAGE > SUMS ? 2 * KS * STAGE : SUMS;
+    static constexpr int BLOCKS = NT * CG >= 32 ? 1 : NT * CG >= 16 ? 2 : 160 * 1024 / LDS;
+    static constexpr int WAVES_PER_SIMD = BLOCKS * THREADS / 256 < 4 ? BLOCKS * THREADS / 256 : 4;
+    static_assert(SET % 2 == 0 && BM % (8 * SET) == 0 && BN % (8 * SET) == 0, "every wavefront of a set brings as many rows, in steps of 16");
+    static_assert(GROUPS <= SET && (RH == 1 || 16 * NT % 64 == 0) && (16 * CG % 64 == 0 || 64 % (16 * CG) == 0),
+                  "a wavefront's scales: a group of 64 rows; its rows and columns begin a group or lie inside one");
+    static_assert(LDS <= 160 * 1024, "LDS of a compute unit");
+};
+
+template <class T>
+__global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void mx_tile4_kernel(MxProduct p) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    constexpr int NT = T::NT, CG = T::CG, RB = T::RB, KS = T::KS, SET = T::SET;
+    MxTask t;
+    if (!mx_task<T::BM, true>(p, T::BN, t)) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int ks = wave / SET, sw = wave % SET;
+    const int wm = sw / T::CW, wn = sw % T::CW;
+    const int idx = lane & 15, q = lane >> 4;
+    const int K = p.K, N = p.N;
+    const uint32_t row = (uint32_t)K >> 1, srow = (uint32_t)K >> 5;
+
+    // Chunk c (16 bytes: a block) of a row lies in slot c ^ (row / 2): the reads below meet no bank twice in a cycle.
+    const uint32_t chunk = (lane & 7) ^ (((8 * sw + (lane >> 3)) >> 1) & 7), off = (uint32_t)(8 * sw + (lane >> 3)) * row;
+    unsigned char* const stages = smem + ks * 2 * T::STAGE;
+    const int slabs_all = (K + 255) >> 8, slabs = (slabs_all + KS - 1) / KS;
+    const __amdgpu_buffer_rsrc_t a_buf = mx_buffer(t.a, (uint32_t)t.rows * row), w_buf = mx_buffer(t.w, (uint32_t)N * row);
+    auto issue = [&](int s) {
+        unsigned char* const st = stages + (s & 1) * T::STAGE;
+        const uint32_t at = (uint32_t)(s * KS + ks) * 128 + 16 * chunk;
+        const uint32_t v = at < row ? off + at : kBehind, vw = at < row ? off + at + (uint32_t)t.n0 * row : kBehind;
+#pragma unroll
+        for (int i = 0; i < T::LOADS_A; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(a_buf, (mx_lds_void*)(st + (i * SET + sw) * 1024), 16, (int)(v + i * SET * 8 * row), 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < T::LOADS_W; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(w_buf, (mx_lds_void*)(st + T::BM * 128 + (i * SET + sw) * 1024), 16, (int)(vw + i * SET * 8 * row), 0, 0, 0);
+    };
+    // The scales, eight of a row a lane, through registers (their addresses have no alignment), into LDS as the matrix instruction picks them:
+    // it takes one byte of a register, so the dword for (block, 64 rows, idx) has those of rows idx, 16 + idx, 32 + idx, 48 + idx.  Every
+    // wavefront does so for one group of 64 rows, some for the same: without a branch, behind which the compiler would move products.
+    const int group = sw % T::GROUPS;
+    const bool of_w = group >= T::GROUPS_A;
+    const uint8_t* const sc = of_w ? t.s : p.a_scales;
+    const int64_t sc_end = (of_w ? (int64_t)N : p.M) * srow;                     // bytes of the whole array
+    const int64_t sc_row = of_w ? min(t.n0 + 64 * (group - T::GROUPS_A) + lane, N - 1) : t.row0 + min(64 * group + lane, t.rows - 1);
+    uint64_t held = 0;
+    auto load_scales = [&](int s) {               // those behind the row's end: 0.  The eight bytes lie inside the array, which has eight
+        const int b0 = (s * KS + ks) * 8, n = min(max((int)srow - b0, 0), 8);
+        const int64_t want = sc_row * srow + min(b0, (int)srow), at = min(want, sc_end - 8);
+        uint64_t v;
+        __builtin_memcpy(&v, sc + at, 8);
+        v = n > 0 ? v >> (8 * (want - at)) : 0;
+        held = n < 8 ? v & (((uint64_t)1 << (8 * n)) - 1) : v;
+    };
+    auto store_scales = [&](int s) {
+        uint32_t* at = reinterpret_cast<uint32_t*>(stages + (s & 1) * T::STAGE + (T::BM + T::BN) * 128) + group * 16 + idx;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {             // blocks 4 h + q: four lanes, sixteen apart, turn their four bytes round
+            const uint32_t mine = (uint32_t)(held >> (32 * h));
+            const auto a = __builtin_amdgcn_permlane16_swap(mine, mine, false, false);       // lanes' rows 0 0 2 2 and 1 1 3 3
+            const auto even = __builtin_amdgcn_permlane32_swap(a[0], a[0], false, false), odd = __builtin_amdgcn_permlane32_swap(a[1], a[1], false, false);
+            const uint32_t sel = 0x0C0C0400u + 0x0101u * q;                                  // byte q of the second operand, then of the first
+            const uint32_t lo = __builtin_amdgcn_perm(odd[0], even[0], sel), hi = __builtin_amdgcn_perm(odd[1], even[1], sel);
+            at[(4 * h + q) * T::GROUPS * 16] = lo | hi << 16;
         }
     };
 
@@ -349,125 +477,61 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void mx_tile_kernel(
     for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int g = 0; g < CG; ++g) acc[i][g] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
-    // A slab, in blocks of RB groups of rows: the next block's fragments are read (and, with bf16 rows, the next weights widened) under the
-    // products of the one before.  Parts: the quarters j of a step (bf16), the steps of a slab (MXFP4).
-    constexpr int PARTS = ROWS4 ? 2 : 4, NB = NT / RB, SEQ = PARTS * NB;
-    mx_u32x4 x[2][RB];
-    uint32_t xs[2];
-    // behind(part): what is requested once the weights of a part are done with
-    auto slab = [&](const unsigned char* st, auto behind) {
-        const unsigned char* base = st + (wm * 16 * NT + idx) * PITCH;
-        mx_bf16x8 wf[2][CG];
+
+    // A slab: halves of 128 values, blocks of RB groups of rows; the next block's fragments are read under the products of the one before.
+    constexpr int NB = NT / RB, SEQ = 2 * NB;
+    constexpr int COLS0 = 16 * CG % 64 == 0 ? 0 : CG;      // narrower wavefronts share a group of 64 columns: whose bytes are theirs
+    auto slab = [&](const unsigned char* st) {
+        const unsigned char* xb = st + (wm * 16 * NT + idx) * 128;
+        const unsigned char* wb = st + (T::BM + wn * 16 * CG + idx) * 128;
+        const uint32_t* scales = reinterpret_cast<const uint32_t*>(st + (T::BM + T::BN) * 128);
+        mx_u32x4 x[2][RB], w[2][CG];
+        uint32_t xs[2], ws[2];
+        const int wgroup = T::GROUPS_A + (wn * 16 * CG) / 64;
         auto read = [&](int n) {
-            const int part = n / NB, ib = n % NB;
-            const int at = ROWS4 ? ((4 * part + q) ^ ((idx >> 1) & 7)) << 4 : ((q + 4 * part) ^ idx) << 4;
+            const int h = n / NB, ib = n % NB;
+            const int at = ((4 * h + q) ^ ((idx >> 1) & 7)) << 4;
+            if (ib == 0) {
 #pragma unroll
-            for (int i = 0; i < RB; ++i) x[n & 1][i] = *reinterpret_cast<const mx_u32x4*>(base + (ib * RB + i) * 16 * PITCH + at);
-            if constexpr (ROWS4)
-                xs[n & 1] = reinterpret_cast<const uint32_t*>(st + T::BM * PITCH)[((4 * part + q) * T::GROUPS + wm * NB + ib) * 16 + idx];
-        };
-        auto widen = [&](int part) {
-            if constexpr (!ROWS4) {
-#pragma unroll
-                for (int g = 0; g < CG; ++g) {
-                    const uint32_t codes = cur[g][part];
-                    wf[part & 1][g] = mx_widen8(codes, cur_s[g]);
-                }
+                for (int g = 0; g < CG; ++g) w[h][g] = *reinterpret_cast<const mx_u32x4*>(wb + g * 16 * 128 + at);
+                ws[h] = scales[((4 * h + q) * T::GROUPS + wgroup) * 16 + idx];
+                if (COLS0) ws[h] >>= 8 * (wn * CG % 4);
             }
+#pragma unroll
+            for (int i = 0; i < RB; ++i) x[n & 1][i] = *reinterpret_cast<const mx_u32x4*>(xb + (ib * RB + i) * 16 * 128 + at);
+            xs[n & 1] = scales[((4 * h + q) * T::GROUPS + wm * NB + ib) * 16 + idx];
         };
         read(0);
-        widen(0);
 #pragma unroll
         for (int n = 0; n < SEQ; ++n) {
-            const int part = n / NB, ib = n % NB;
+            const int h = n / NB, ib = n % NB;
             if (n + 1 < SEQ) read(n + 1);
-            if (ib == NB - 1 && part + 1 < PARTS) widen(part + 1);
-#pragma unroll
-            for (int i = 0; i < RB; ++i) {
-#pragma unroll
-                for (int g = 0; g < CG; ++g) {
-                    mx_f32x4& a = acc[ib * RB + i][g];
-                    if constexpr (ROWS4) {
-                        if (i == 0) a = mx_mfma<0>(w[part][g], ws[part][g], x[n & 1][i], xs[n & 1], a);
-                        else if (i == 1) a = mx_mfma<1>(w[part][g], ws[part][g], x[n & 1][i], xs[n & 1], a);
-                        else if (i == 2) a = mx_mfma<2>(w[part][g], ws[part][g], x[n & 1][i], xs[n & 1], a);
-                        else a = mx_mfma<3>(w[part][g], ws[part][g], x[n & 1][i], xs[n & 1], a);
-                    } else {
-                        a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[part & 1][g], __builtin_bit_cast(mx_bf16x8, x[n & 1][i]), a, 0, 0, 0);
-                    }
-                }
-            }
+            mx_products<RB, CG>(acc, ib * RB, w[h], ws[h], x[n & 1], xs[n & 1]);
             __builtin_amdgcn_sched_barrier(0);
-            if (ib == NB - 1) behind(part);
         }
     };
-    // Every request of this wavefront for the slab's rows has landed (LATER requests behind them may be on their way) and its reads of the
-    // other stage are done, then so have everybody's.
-    auto meet = [&](auto later) {
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(decltype(later)::value) : "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-    };
-    typedef std::integral_constant<int, 0> None;
-    typedef std::integral_constant<int, 4 * CG> Weights;       // MXFP4 rows: the two steps' loads, which come last
 
-    // One path for every slab: what is requested behind the last one lies behind the operands' ends, and every set runs as many slabs as the
-    // longest (of zeros).  Where paths with and without requests met, every wait would be one for all of them.
-    constexpr int STEPS = ROWS4 ? 2 : 1;
     issue(0);
-    load_row_scales(0);
-#pragma unroll
-    for (int h = 0; h < STEPS; ++h) load_w(h, ks * STEPS + h);
-    store_row_scales(0);
+    load_scales(0);
+    store_scales(0);
     if (t.rows > wm * 16 * NT) {
-        for (int s = 0; s < slabs_most; ++s) {
-            const int next = ((s + 1) * KS + ks) * STEPS;
-            const unsigned char* st = stages + (s & 1) * T::STAGE;
-            if constexpr (ROWS4) {
-                meet(Weights{});
-                issue(s + 1);
-                load_row_scales(s + 1);
-                slab(st, [&](int part) { load_w(part, next + part); });
-                store_row_scales(s + 1);
-            } else {
-                meet(None{});
-#pragma unroll
-                for (int g = 0; g < CG; ++g) {
-                    cur[g] = w[0][g];
-                    cur_s[g] = mx_scale(ws[0][g]);
-                }
-                issue(s + 1);
-                load_w(0, next);
-                slab(st, [](int) {});
-            }
-        }
-    } else {                                      // no rows for this wavefront: it brings the others theirs
-        for (int s = 0; s < slabs_most; ++s) {
-            meet(None{});
+        for (int s = 0; s < slabs; ++s) {
+            mx_meet();
             issue(s + 1);
-            load_row_scales(s + 1);
-            store_row_scales(s + 1);
+            load_scales(s + 1);
+            slab(stages + (s & 1) * T::STAGE);
+            store_scales(s + 1);
+        }
+    } else {
+        for (int s = 0; s < slabs; ++s) {
+            mx_meet();
+            issue(s + 1);
+            load_scales(s + 1);
+            store_scales(s + 1);
         }
     }
-
-    if constexpr (KS > 1) {                       // the sets' sums, in their order
-        meet(None{});
-        mx_f32x4* red = reinterpret_cast<mx_f32x4*>(smem) + sw * NT * CG * 64 + lane;
-        if (ks > 0) {
-#pragma unroll
-            for (int i = 0; i < NT; ++i)
-#pragma unroll
-                for (int g = 0; g < CG; ++g) red[((ks - 1) * T::SET * NT * CG + i * CG + g) * 64] = acc[i][g];
-        }
-        __syncthreads();
-        if (ks > 0) return;
-        for (int k = 0; k < KS - 1; ++k)
-#pragma unroll
-            for (int i = 0; i < NT; ++i)
-#pragma unroll
-                for (int g = 0; g < CG; ++g) acc[i][g] += red[(k * T::SET * NT * CG + i * CG + g) * 64];
-    }
-    mx_store_tile<NT, CG>(p, t, 16 * wm * NT + idx, c0 + 4 * q, acc);
+    if (!mx_join<KS, SET, NT, CG>(acc, ks, sw, smem, lane)) return;
+    mx_store_tile<NT, CG>(p, t, 16 * wm * NT + idx, t.n0 + 16 * CG * wn + 4 * q, acc);
 }
 
 // Workgroups of a launch: blocks of BM rows (an expert's last one is its own) times column tiles, in eight equal shares.
@@ -478,9 +542,13 @@ int64_t mx_grid(const MxProduct& p, int BM, int BN) {
 
 template <class T>
 hipError_t launch_tile(const MxProduct& p, hipStream_t st) {
-    static const hipError_t ready = hipFuncSetAttribute(reinterpret_cast<const void*>(mx_tile_kernel<T>), hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
+    void (*const kernel)(MxProduct) = [] {
+        if constexpr (T::ROWS4) return mx_tile4_kernel<T>;
+        else return mx_tile_kernel<T>;
+    }();
+    static const hipError_t ready = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
     if (ready != hipSuccess) return ready;
-    mx_tile_kernel<T><<<(unsigned)mx_grid(p, T::BM, T::BN), T::THREADS, T::LDS, st>>>(p);
+    kernel<<<(unsigned)mx_grid(p, T::BM, T::BN), T::THREADS, T::LDS, st>>>(p);
     return hipGetLastError();
 }
 
@@ -502,20 +570,28 @@ hipError_t launch_stream(const MxProduct& p, hipStream_t st) {
     return hipGetLastError();
 }
 
-template <bool ROWS4>
-hipError_t launch_product(const MxProduct& p, int form, hipStream_t st) {
+hipError_t launch_product16(const MxProduct& p, int form, hipStream_t st) {
     switch (form) {
-        case 0: return launch_stream<ROWS4>(p, st);
-        case 1: return launch_tile<MxTile<ROWS4, 1, 2, 4, 1, 2>>(p, st);     // 32 x 64
-        case 2: return launch_tile<MxTile<ROWS4, 1, 4, 4, 1, 2>>(p, st);     // 64 x 64
-        case 3: return launch_tile<MxTile<ROWS4, 2, 4, 2, 4, 1>>(p, st);     // 128 x 128
-        default: return launch_tile<MxTile<ROWS4, 2, 8, 4, 4, 1>>(p, st);    // 256 x 256
+        case 0: return launch_stream<false>(p, st);
+        case 1: return launch_tile<MxTile<1, 2, 4, 1, 2>>(p, st);     // 32 x 64
+        case 2: return launch_tile<MxTile<1, 4, 4, 1, 2>>(p, st);     // 64 x 64
+        case 3: return launch_tile<MxTile<2, 4, 2, 4, 1>>(p, st);     // 128 x 128
+        default: return launch_tile<MxTile<2, 8, 4, 4, 1>>(p, st);    // 256 x 256
+    }
+}
+hipError_t launch_product4(const MxProduct& p, int form, hipStream_t st) {
+    switch (form) {
+        case 0: return launch_stream<true>(p, st);
+        case 1: return launch_tile<MxTile4<1, 2, 4, 1, 2>>(p, st);
+        case 2: return launch_tile<MxTile4<1, 4, 4, 1, 2>>(p, st);
+        case 3: return launch_tile<MxTile4<2, 4, 2, 4, 1>>(p, st);
+        default: return launch_tile<MxTile4<2, 8, 4, 4, 1>>(p, st);
     }
 }
 
 int product_form(const MxProduct& p) {
     const int64_t rows = p.count ? (p.M + p.E - 1) / p.E : p.M;
-    if (rows <= 16) return 0;
+    if (rows <= 16 || (int64_t)p.N * p.K < 256) return 0;       // (the tiles read eight scales at a time: a matrix has that many)
     if (rows <= 32) return 1;
     if (rows <= 64) return 2;
     const int64_t tiles = (p.count ? p.M / 256 + p.E : (p.M + 255) / 256) * ((p.N + 255) / 256);
@@ -533,7 +609,7 @@ int64_t product_workgroups(const MxProduct& p, int form) {
 hipError_t launch_product_mxfp4(const MxProduct& p, int form, hipStream_t st) {
     if (p.M == 0) return hipSuccess;
     if (form < 0) form = product_form(p);
-    return p.a_scales ? launch_product<true>(p, form, st) : launch_product<false>(p, form, st);
+    return p.a_scales ? launch_product4(p, form, st) : launch_product16(p, form, st);
 }
 
 // What the kernels read and write at a time, their 32-bit offsets and the launches' sizes.
