@@ -91,20 +91,20 @@ __device__ __forceinline__ void mx_store4(const MxTask& t, int N, bool whole, in
             if (col + r < N) o[r] = (uint16_t)w[r];
     }
 }
-// ... for NT x CG of them: rows row0 + 16 i, columns col0 + 16 g.  One activation for all: a switch at every value costs more than the values.
-template <int NT, int CG>
+// ... for NT x CG of them: rows row0 + ROWS i, columns col0 + COLS g.  One activation for all: a switch at every value costs more than the values.
+template <int NT, int CG, int ROWS = 16, int COLS = 16>
 __device__ __forceinline__ void mx_store_tile(const MxProduct& p, const MxTask& t, int row0, int col0, const mx_f32x4 (&acc)[NT][CG]) {
     const int N = p.N;
     mx_f32x4 b[CG];
 #pragma unroll
-    for (int g = 0; g < CG; ++g) b[g] = mx_bias4(p, t, col0 + 16 * g);
+    for (int g = 0; g < CG; ++g) b[g] = mx_bias4(p, t, col0 + COLS * g);
     auto all = [&](auto act_c, auto whole_c) {
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-            if (row0 + 16 * i >= t.rows) break;
+            if (row0 + ROWS * i >= t.rows) break;
 #pragma unroll
             for (int g = 0; g < CG; ++g)
-                if (col0 + 16 * g < N) mx_store4<decltype(act_c)::value>(t, N, decltype(whole_c)::value, row0 + 16 * i, col0 + 16 * g, acc[i][g] + b[g]);
+                if (col0 + COLS * g < N) mx_store4<decltype(act_c)::value>(t, N, decltype(whole_c)::value, row0 + ROWS * i, col0 + COLS * g, acc[i][g] + b[g]);
         }
     };
     typedef std::true_type Whole;
@@ -270,7 +270,7 @@ struct MxTile {
     static constexpr int SET = RH * CW;                        // wavefronts of a set
     static constexpr int THREADS = 64 * SET * KS;
     static constexpr int LOADS_A = BM / 4 / SET, LOADS_W = BN / 16 / SET;      // an instruction of a wavefront brings 4 and 16 rows
-    static constexpr int RB = NT < 4 ? NT : 4;                 // groups of 16 rows whose fragments are in registers at once (twice)
+    static constexpr int RB = NT % 4 == 0 ? 4 : NT % 3 == 0 ? 3 : NT;      // groups of 16 rows whose fragments are in registers at once (twice)
     static constexpr int STAGE = BM * 256 + BN * 64;
     static constexpr int SUMS = (KS - 1) * SET * NT * CG * 1024;
     static constexpr int LDS = 2 * KS * STAGE > SUMS ? 2 * KS * STAGE : SUMS;
@@ -389,40 +389,45 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void mx_tile_kernel(
 }
 
 // -- rows in MXFP4 too --
-// A slab is 256 values, 128 bytes of every row, both operands in LDS: the products are so fast that a fragment of weights fetched by each of
-// the RH wavefronts that use it, half a line at a time, costs five times their time.
+// A slab is 256 values, 128 bytes of every row, both operands in LDS.  Products are 32 x 32 over 64 values: the scaled instruction of that
+// shape takes 33 cycles, that of 16 x 16 over 128 values, half as much work, 31 (measured).  A lane's 16 bytes are the block of its
+// row that it multiplies.  NT, CG: 32-row and 32-column blocks of a wavefront.
 template <int RH_, int NT_, int CW_, int CG_, int KS_>
 struct MxTile4 {
     static constexpr bool ROWS4 = true;
     static constexpr int RH = RH_, NT = NT_, CW = CW_, CG = CG_, KS = KS_;
-    static constexpr int BM = 16 * NT * RH, BN = 16 * CG * CW;
+    static constexpr int BM = 32 * NT * RH, BN = 32 * CG * CW;
     static constexpr int SET = RH * CW;
     static constexpr int THREADS = 64 * SET * KS;
     static constexpr int LOADS_A = BM / 8 / SET, LOADS_W = BN / 8 / SET;       // an instruction of a wavefront brings 8 rows
-    static constexpr int RB = NT < 4 ? NT : 4;
-    static constexpr int GROUPS_A = (BM + 63) / 64, GROUPS = GROUPS_A + (BN + 63) / 64;      // of 64 rows, whose scales share dwords: tokens, then weights
-    static constexpr int SCALES = 8 * GROUPS * 64;
-    static constexpr int STAGE = (BM + BN) * 128 + SCALES;
-    static constexpr int SUMS = (KS - 1) * SET * NT * CG * 1024;
+    static constexpr int STAGE = (BM + BN) * (128 + 8);
+    static constexpr int SUMS = (KS - 1) * SET * NT * CG * 4096;
     static constexpr int LDS = 2 * KS * STAGE > SUMS ? 2 * KS * STAGE : SUMS;
-    static constexpr int BLOCKS = NT * CG >= 32 ? 1 : NT * CG >= 16 ? 2 : 160 * 1024 / LDS;
-    static constexpr int WAVES_PER_SIMD = BLOCKS * THREADS / 256 < 4 ? BLOCKS * THREADS / 256 : 4;
-    static_assert(SET % 2 == 0 && BM % (8 * SET) == 0 && BN % (8 * SET) == 0, "every wavefront of a set brings as many rows, in steps of 16");
-    static_assert(GROUPS <= SET && (RH == 1 || 16 * NT % 64 == 0) && (16 * CG % 64 == 0 || 64 % (16 * CG) == 0),
-                  "a wavefront's scales: a group of 64 rows; its rows and columns begin a group or lie inside one");
+    static constexpr int BLOCKS = NT * CG >= 8 ? 1 : NT * CG >= 4 ? 2 : 160 * 1024 / LDS;
+    static constexpr int WAVES_PER_SIMD = BLOCKS * THREADS / 256 < 1 ? 1 : BLOCKS * THREADS / 256 < 4 ? BLOCKS * THREADS / 256 : 4;
+    static_assert(SET % 2 == 0 && BM % (8 * SET) == 0 && BN % (8 * SET) == 0 && BM + BN <= 64 * SET, "every wavefront of a set brings as many rows, in steps of 16, and a lane the scales of one");
     static_assert(LDS <= 160 * 1024, "LDS of a compute unit");
 };
+typedef float mx_f32x16 __attribute__((ext_vector_type(16)));
+// The scaled instruction, 32 x 32 over 64 values; a scale is byte B of its register.
+template <int B>
+__device__ __forceinline__ mx_f32x16 mx_mfma32(mx_u32x4 a, uint32_t sa, mx_u32x4 b, uint32_t sb, mx_f32x16 c) {
+    // (the upper half, which 4-bit operands do not have, is left open)
+    const mx_i32x8 av = __builtin_bit_cast(mx_i32x8, __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1));
+    const mx_i32x8 bv = __builtin_bit_cast(mx_i32x8, __builtin_shufflevector(b, b, 0, 1, 2, 3, -1, -1, -1, -1));
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, c, 4 /* e2m1 */, 4, B, (int)sa, B, (int)sb);
+}
 
 template <class T>
 __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void mx_tile4_kernel(MxProduct p) {
     extern __shared__ __align__(16) unsigned char smem[];
-    constexpr int NT = T::NT, CG = T::CG, RB = T::RB, KS = T::KS, SET = T::SET;
+    constexpr int NT = T::NT, CG = T::CG, KS = T::KS, SET = T::SET, BM = T::BM, BN = T::BN;
     MxTask t;
-    if (!mx_task<T::BM, true>(p, T::BN, t)) return;
+    if (!mx_task<BM, true>(p, BN, t)) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ks = wave / SET, sw = wave % SET;
     const int wm = sw / T::CW, wn = sw % T::CW;
-    const int idx = lane & 15, q = lane >> 4;
+    const int r32 = lane & 31, b = lane >> 5;
     const int K = p.K, N = p.N;
     const uint32_t row = (uint32_t)K >> 1, srow = (uint32_t)K >> 5;
 
@@ -431,107 +436,116 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void mx_tile4_kernel
     unsigned char* const stages = smem + ks * 2 * T::STAGE;
     const int slabs_all = (K + 255) >> 8, slabs = (slabs_all + KS - 1) / KS;
     const __amdgpu_buffer_rsrc_t a_buf = mx_buffer(t.a, (uint32_t)t.rows * row), w_buf = mx_buffer(t.w, (uint32_t)N * row);
-    auto issue = [&](int s) {
+    // requests [first, last) of a slab's, weights first
+    constexpr int LOADS = T::LOADS_A + T::LOADS_W;
+    auto issue = [&](int s, int first, int last) {
         unsigned char* const st = stages + (s & 1) * T::STAGE;
         const uint32_t at = (uint32_t)(s * KS + ks) * 128 + 16 * chunk;
         const uint32_t v = at < row ? off + at : kBehind, vw = at < row ? off + at + (uint32_t)t.n0 * row : kBehind;
 #pragma unroll
-        for (int i = 0; i < T::LOADS_A; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(a_buf, (mx_lds_void*)(st + (i * SET + sw) * 1024), 16, (int)(v + i * SET * 8 * row), 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < T::LOADS_W; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(w_buf, (mx_lds_void*)(st + T::BM * 128 + (i * SET + sw) * 1024), 16, (int)(vw + i * SET * 8 * row), 0, 0, 0);
-    };
-    // The scales, eight of a row a lane, through registers (their addresses have no alignment), into LDS as the matrix instruction picks them:
-    // it takes one byte of a register, so the dword for (block, 64 rows, idx) has those of rows idx, 16 + idx, 32 + idx, 48 + idx.  Every
-    // wavefront does so for one group of 64 rows, some for the same: without a branch, behind which the compiler would move products.
-    const int group = sw % T::GROUPS;
-    const bool of_w = group >= T::GROUPS_A;
-    const uint8_t* const sc = of_w ? t.s : p.a_scales;
-    const int64_t sc_end = (of_w ? (int64_t)N : p.M) * srow;                     // bytes of the whole array
-    const int64_t sc_row = of_w ? min(t.n0 + 64 * (group - T::GROUPS_A) + lane, N - 1) : t.row0 + min(64 * group + lane, t.rows - 1);
-    uint64_t held = 0;
-    auto load_scales = [&](int s) {               // those behind the row's end: 0.  The eight bytes lie inside the array, which has eight
-        const int b0 = (s * KS + ks) * 8, n = min(max((int)srow - b0, 0), 8);
-        const int64_t want = sc_row * srow + min(b0, (int)srow), at = min(want, sc_end - 8);
-        uint64_t v;
-        __builtin_memcpy(&v, sc + at, 8);
-        v = n > 0 ? v >> (8 * (want - at)) : 0;
-        held = n < 8 ? v & (((uint64_t)1 << (8 * n)) - 1) : v;
-    };
-    auto store_scales = [&](int s) {
-        uint32_t* at = reinterpret_cast<uint32_t*>(stages + (s & 1) * T::STAGE + (T::BM + T::BN) * 128) + group * 16 + idx;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {             // blocks 4 h + q: four lanes, sixteen apart, turn their four bytes round
-            const uint32_t mine = (uint32_t)(held >> (32 * h));
-            const auto a = __builtin_amdgcn_permlane16_swap(mine, mine, false, false);       // lanes' rows 0 0 2 2 and 1 1 3 3
-            const auto even = __builtin_amdgcn_permlane32_swap(a[0], a[0], false, false), odd = __builtin_amdgcn_permlane32_swap(a[1], a[1], false, false);
-            const uint32_t sel = 0x0C0C0400u + 0x0101u * q;                                  // byte q of the second operand, then of the first
-            const uint32_t lo = __builtin_amdgcn_perm(odd[0], even[0], sel), hi = __builtin_amdgcn_perm(odd[1], even[1], sel);
-            at[(4 * h + q) * T::GROUPS * 16] = lo | hi << 16;
+        for (int l = first; l < last && l < LOADS; ++l) {
+            const int i = l - T::LOADS_W;
+            if (l < T::LOADS_W)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(w_buf, (mx_lds_void*)(st + BM * 128 + (l * SET + sw) * 1024), 16, (int)(vw + l * SET * 8 * row), 0, 0, 0);
+            else
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(a_buf, (mx_lds_void*)(st + (i * SET + sw) * 1024), 16, (int)(v + i * SET * 8 * row), 0, 0, 0);
         }
     };
+    // The scales, eight of a row a lane (token rows, then weight rows), through registers: their addresses have no alignment.
+    const int my = min((int)threadIdx.x - ks * SET * 64, BM + BN - 1);
+    const bool of_w = my >= BM;
+    const uint8_t* const sc = of_w ? t.s : p.a_scales;
+    const int64_t sc_last = (of_w ? (int64_t)N : p.M) * srow - 8;                // the last eight bytes of the whole array
+    const int64_t sc_row = (of_w ? min(t.n0 + my - BM, N - 1) : t.row0 + min(my, t.rows - 1)) * (int64_t)srow;
+    uint64_t raw;
+    auto scales_at = [&](int s) { return sc_row + min((s * KS + ks) * 8, (int)srow); };
+    auto load_scales = [&](int s) { __builtin_memcpy(&raw, sc + min(scales_at(s), sc_last), 8); };      // inside the array, which has eight
+    auto store_scales = [&](int s) {              // those behind the row's end: 0
+        const int64_t want = scales_at(s);
+        const int early = (int)(want - min(want, sc_last)) * 4, over = (8 - min(max((int)srow - (s * KS + ks) * 8, 0), 8)) * 4;      // half of the bits, up to 32
+        const uint64_t held = raw >> early >> early << over << over >> over >> over;      // without a condition: the load would move behind it, and wait there
+        *reinterpret_cast<uint64_t*>(stages + (s & 1) * T::STAGE + (BM + BN) * 128 + my * 8) = held;
+    };
 
-    mx_f32x4 acc[NT][CG];
+    mx_f32x16 acc[NT][CG];
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
-        for (int g = 0; g < CG; ++g) acc[i][g] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int g = 0; g < CG; ++g)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][g][r] = 0.0f;
 
-    // A slab: halves of 128 values, blocks of RB groups of rows; the next block's fragments are read under the products of the one before.
-    constexpr int NB = NT / RB, SEQ = 2 * NB;
-    constexpr int COLS0 = 16 * CG % 64 == 0 ? 0 : CG;      // narrower wavefronts share a group of 64 columns: whose bytes are theirs
-    auto slab = [&](const unsigned char* st) {
-        const unsigned char* xb = st + (wm * 16 * NT + idx) * 128;
-        const unsigned char* wb = st + (T::BM + wn * 16 * CG + idx) * 128;
-        const uint32_t* scales = reinterpret_cast<const uint32_t*>(st + (T::BM + T::BN) * 128);
-        mx_u32x4 x[2][RB], w[2][CG];
-        uint32_t xs[2], ws[2];
-        const int wgroup = T::GROUPS_A + (wn * 16 * CG) / 64;
-        auto read = [&](int n) {
-            const int h = n / NB, ib = n % NB;
-            const int at = ((4 * h + q) ^ ((idx >> 1) & 7)) << 4;
-            if (ib == 0) {
+    // A slab in quarters of 64 values: the next quarter's fragments are read under the products of the one before.  Of a row's eight scales a
+    // lane takes those of its blocks, the even or the odd ones; quarter j's is byte j.
+    auto slab = [&](const unsigned char* st, auto request) {       // request(j): in front of quarter j
+        const unsigned char* xb = st + (wm * 32 * NT + r32) * 128;
+        const unsigned char* wb = st + (BM + wn * 32 * CG + r32) * 128;
+        const uint2* scales = reinterpret_cast<const uint2*>(st + (BM + BN) * 128);
+        const uint32_t pick = 0x06040200u + 0x01010101u * b;
+        mx_u32x4 x[2][NT], w[2][CG];
+        uint32_t xs[NT], ws[CG];
+        auto read = [&](int j) {
+            const int at = ((2 * j + b) ^ ((r32 >> 1) & 7)) << 4;
 #pragma unroll
-                for (int g = 0; g < CG; ++g) w[h][g] = *reinterpret_cast<const mx_u32x4*>(wb + g * 16 * 128 + at);
-                ws[h] = scales[((4 * h + q) * T::GROUPS + wgroup) * 16 + idx];
-                if (COLS0) ws[h] >>= 8 * (wn * CG % 4);
-            }
+            for (int g = 0; g < CG; ++g) w[j & 1][g] = *reinterpret_cast<const mx_u32x4*>(wb + g * 32 * 128 + at);
 #pragma unroll
-            for (int i = 0; i < RB; ++i) x[n & 1][i] = *reinterpret_cast<const mx_u32x4*>(xb + (ib * RB + i) * 16 * 128 + at);
-            xs[n & 1] = scales[((4 * h + q) * T::GROUPS + wm * NB + ib) * 16 + idx];
+            for (int i = 0; i < NT; ++i) x[j & 1][i] = *reinterpret_cast<const mx_u32x4*>(xb + i * 32 * 128 + at);
         };
         read(0);
 #pragma unroll
-        for (int n = 0; n < SEQ; ++n) {
-            const int h = n / NB, ib = n % NB;
-            if (n + 1 < SEQ) read(n + 1);
-            mx_products<RB, CG>(acc, ib * RB, w[h], ws[h], x[n & 1], xs[n & 1]);
-            __builtin_amdgcn_sched_barrier(0);
+        for (int g = 0; g < CG; ++g) {
+            const uint2 v = scales[BM + wn * 32 * CG + g * 32 + r32];
+            ws[g] = __builtin_amdgcn_perm(v.y, v.x, pick);
         }
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            const uint2 v = scales[wm * 32 * NT + i * 32 + r32];
+            xs[i] = __builtin_amdgcn_perm(v.y, v.x, pick);
+        }
+        auto quarter = [&](auto j_c) {
+            constexpr int J = decltype(j_c)::value;
+            request(J);
+            if constexpr (J < 3) read(J + 1);
+            __builtin_amdgcn_sched_barrier(0);    // (the compiler would put the reads last)
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int g = 0; g < CG; ++g) acc[i][g] = mx_mfma32<J>(w[J & 1][g], ws[g], x[J & 1][i], xs[i], acc[i][g]);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        quarter(std::integral_constant<int, 0>{});
+        quarter(std::integral_constant<int, 1>{});
+        quarter(std::integral_constant<int, 2>{});
+        quarter(std::integral_constant<int, 3>{});
     };
 
-    issue(0);
+    constexpr int PER = (LOADS + 2) / 3;          // requests in front of a quarter but the last
+    issue(0, 0, LOADS);
     load_scales(0);
     store_scales(0);
-    if (t.rows > wm * 16 * NT) {
+    if (t.rows > wm * 32 * NT) {
         for (int s = 0; s < slabs; ++s) {
             mx_meet();
-            issue(s + 1);
             load_scales(s + 1);
-            slab(stages + (s & 1) * T::STAGE);
+            slab(stages + (s & 1) * T::STAGE, [&](int j) { issue(s + 1, j * PER, j * PER + PER); });
             store_scales(s + 1);
         }
     } else {
         for (int s = 0; s < slabs; ++s) {
             mx_meet();
-            issue(s + 1);
+            issue(s + 1, 0, LOADS);
             load_scales(s + 1);
             store_scales(s + 1);
         }
     }
-    if (!mx_join<KS, SET, NT, CG>(acc, ks, sw, smem, lane)) return;
-    mx_store_tile<NT, CG>(p, t, 16 * wm * NT + idx, t.n0 + 16 * CG * wn + 4 * q, acc);
+    // In four pieces as the 16 x 16 products leave them: 4 b .. + 3 of eight columns each, token row r32.
+    mx_f32x4 sum[NT][4 * CG];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int g = 0; g < 4 * CG; ++g) sum[i][g] = mx_f32x4{acc[i][g / 4][4 * (g % 4)], acc[i][g / 4][4 * (g % 4) + 1], acc[i][g / 4][4 * (g % 4) + 2], acc[i][g / 4][4 * (g % 4) + 3]};
+    if (!mx_join<KS, SET, NT, 4 * CG>(sum, ks, sw, smem, lane)) return;
+    mx_store_tile<NT, 4 * CG, 32, 8>(p, t, wm * 32 * NT + r32, t.n0 + wn * 32 * CG + 4 * b, sum);
 }
 
 // Workgroups of a launch: blocks of BM rows (an expert's last one is its own) times column tiles, in eight equal shares.
@@ -575,17 +589,38 @@ hipError_t launch_product16(const MxProduct& p, int form, hipStream_t st) {
         case 0: return launch_stream<false>(p, st);
         case 1: return launch_tile<MxTile<1, 2, 4, 1, 2>>(p, st);     // 32 x 64
         case 2: return launch_tile<MxTile<1, 4, 4, 1, 2>>(p, st);     // 64 x 64
-        case 3: return launch_tile<MxTile<2, 4, 2, 4, 1>>(p, st);     // 128 x 128
+        case 3: return launch_tile<MxTile<1, 8, 4, 2, 1>>(p, st);     // 128 x 128
+#ifdef TUNE
+        case 6: return launch_tile<MxTile<1, 16, 8, 2, 1>>(p, st);
+        case 7: return launch_tile<MxTile<1, 6, 4, 2, 1>>(p, st);
+        case 8: return launch_tile<MxTile<1, 4, 4, 2, 1>>(p, st);
+        case 9: return launch_tile<MxTile<1, 4, 4, 1, 4>>(p, st);
+        case 10: return launch_tile<MxTile<1, 8, 4, 1, 1>>(p, st);
+        case 11: return launch_tile<MxTile<1, 4, 4, 2, 2>>(p, st);
+        case 12: return launch_tile<MxTile<1, 2, 4, 1, 4>>(p, st);
+        case 13: return launch_tile<MxTile<1, 2, 4, 2, 2>>(p, st);
+        case 14: return launch_tile<MxTile<1, 2, 4, 2, 1>>(p, st);
+        case 15: return launch_tile<MxTile<1, 1, 4, 1, 4>>(p, st);
+        case 16: return launch_tile<MxTile<1, 1, 4, 2, 2>>(p, st);
+#endif
         default: return launch_tile<MxTile<2, 8, 4, 4, 1>>(p, st);    // 256 x 256
     }
 }
 hipError_t launch_product4(const MxProduct& p, int form, hipStream_t st) {
     switch (form) {
         case 0: return launch_stream<true>(p, st);
-        case 1: return launch_tile<MxTile4<1, 2, 4, 1, 2>>(p, st);
-        case 2: return launch_tile<MxTile4<1, 4, 4, 1, 2>>(p, st);
-        case 3: return launch_tile<MxTile4<2, 4, 2, 4, 1>>(p, st);
-        default: return launch_tile<MxTile4<2, 8, 4, 4, 1>>(p, st);
+        case 1: return launch_tile<MxTile4<1, 1, 2, 1, 4>>(p, st);    // 32 x 64
+        case 2: return launch_tile<MxTile4<1, 2, 2, 1, 2>>(p, st);    // 64 x 64
+        case 3: return launch_tile<MxTile4<2, 2, 2, 2, 1>>(p, st);    // 128 x 128
+#ifdef TUNE
+        case 5: return launch_tile<MxTile4<1, 1, 2, 1, 2>>(p, st);
+        case 6: return launch_tile<MxTile4<2, 2, 4, 2, 1>>(p, st);    // 128 x 256
+        case 7: return launch_tile<MxTile4<2, 1, 2, 2, 1>>(p, st);    // 64 x 128
+        case 8: return launch_tile<MxTile4<1, 2, 4, 1, 1>>(p, st);    // 64 x 128
+        case 9: return launch_tile<MxTile4<1, 2, 2, 1, 4>>(p, st);    // 64 x 64
+        case 11: return launch_tile<MxTile4<1, 2, 4, 1, 2>>(p, st);    // 64 x 128
+#endif
+        default: return launch_tile<MxTile4<4, 2, 2, 4, 1>>(p, st);   // 256 x 256
     }
 }
 

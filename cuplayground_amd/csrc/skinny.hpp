@@ -167,20 +167,12 @@ __device__ __forceinline__ void skinny_multiply(mx_f32x4 (&acc)[G], const Skinny
     }
 }
 
-// Both operands in MXFP4: the scaled instruction over 128 values.  A scale is a byte of its register.
-template <int A = 0, int B = 0>
+// Both operands in MXFP4: the scaled instruction over 128 values; a scale is the low byte of its register.
 __device__ __forceinline__ mx_f32x4 mx_mfma(mx_u32x4 a, uint32_t sa, mx_u32x4 b, uint32_t sb, mx_f32x4 c) {
     // (the upper half, which 4-bit operands do not have, is left open)
     const mx_i32x8 av = __builtin_bit_cast(mx_i32x8, __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1));
     const mx_i32x8 bv = __builtin_bit_cast(mx_i32x8, __builtin_shufflevector(b, b, 0, 1, 2, 3, -1, -1, -1, -1));
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4 /* e2m1 */, 4, A, (int)sa, B, (int)sb);
-}
-// acc[at + i][g] += w[g] . x[i], the scales of w[g] and x[i] in byte g and byte i.
-template <int RB, int CG, int I = 0, int G = 0, int NT>
-__device__ __forceinline__ void mx_products(mx_f32x4 (&acc)[NT][CG], int at, const mx_u32x4 (&w)[CG], uint32_t ws, const mx_u32x4 (&x)[RB], uint32_t xs) {
-    acc[at + I][G] = mx_mfma<G, I>(w[G], ws, x[I], xs, acc[at + I][G]);
-    if constexpr (G + 1 < CG) mx_products<RB, CG, I, G + 1>(acc, at, w, ws, x, xs);
-    else if constexpr (I + 1 < RB) mx_products<RB, CG, I + 1, 0>(acc, at, w, ws, x, xs);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4 /* e2m1 */, 4, 0, (int)sa, 0, (int)sb);
 }
 
 // Sums of KS wavefronts that shared a contraction, through LDS, in the order of the wavefronts: returns whether this one holds them.
