@@ -28,6 +28,7 @@ struct FewPlan {
     int16_t base[kMaxExperts];         // packed row of its first one
     int16_t list[kFewPairs];           // experts that are hit, ascending
     float row_w[kFewPairs];            // gate weight of a packed row
+    uint8_t row_t[kFewPairs];          // its token
     int32_t hit, kept;
 };
 
@@ -118,7 +119,11 @@ __device__ __forceinline__ void few_plan(FewPlan& p, const FewArgs& a) {
     __syncthreads();
     if (tid < P) {
         const int e = p.idx[tid], t = tid / a.k;
-        if ((unsigned)e < (unsigned)a.E && ((p.mask[e] >> t) & 1u)) p.row_w[p.base[e] + __popc(p.mask[e] & ((1u << t) - 1u))] = p.w[tid];
+        if ((unsigned)e < (unsigned)a.E && ((p.mask[e] >> t) & 1u)) {
+            const int row = p.base[e] + __popc(p.mask[e] & ((1u << t) - 1u));
+            p.row_w[row] = p.w[tid];
+            p.row_t[row] = (uint8_t)t;
+        }
     }
     __syncthreads();
 }
@@ -146,52 +151,11 @@ __device__ __forceinline__ void few_report(const FewPlan& p, const FewArgs& a) {
     }
 }
 
-// Runs units [0, n) through a ring of two: load(b) fetches the next unit into buffer b, take(b) multiplies what lies there.  (Loads behind a
-// condition in the loop would make every wait one for all of them.)
-template <class LOAD, class TAKE>
-__device__ __forceinline__ void few_ring(int n, LOAD load, TAKE take) {
-    if (n > 0) load(0);
-    if (n > 1) load(1);
-    int i = 0;
-    for (; i + 3 < n; i += 2) {
-        take(0);
-        load(0);
-        take(1);
-        load(1);
-    }
-    if (n - i > 0) take(0);
-    if (n - i > 2) load(0);
-    if (n - i > 1) take(1);
-    if (n - i > 2) take(0);
-}
-
-// What both projections hold of a unit: weights of G groups of 16 rows, the token rows' pieces.
-template <class W, int G>
-struct FewUnit {
-    SkinnyChunk<W, G> w;
-    mx_u32x4 x[W::FRAGS];
-};
-template <class W, int G, bool COLD, bool CUT>
-__device__ __forceinline__ void few_fetch(FewUnit<W, G>& u, const SkinnyRows (&rows)[G], const uint16_t* x, int c, int full, int left, int lane) {
-    if (CUT && c == full) {
-        skinny_load_tail<W, G, COLD>(u.w, rows, c, (int)W::row_bytes(left), lane);
-        skinny_tokens_tail<W>(u.x, x, c, left, lane);
-    } else {
-        skinny_load<W, G, COLD>(u.w, rows, c);
-        skinny_tokens<W>(u.x, x, c, lane);
-    }
-}
-template <class W, int G, bool CUT>
-__device__ __forceinline__ void few_multiply(mx_f32x4 (&acc)[G], FewUnit<W, G>& u, int c, int full, int left, int lane) {
-    skinny_settle(u.w);
-    if (CUT && c == full) skinny_zero_tail(u.w, (int)W::row_bytes(left), lane);
-    skinny_multiply<W, G>(acc, u.w, u.x, lane);
-}
-
 // The up (and gate) projection: a task is 16 columns of both matrices of an expert, or 32 of the one, over the whole of H, by KS wavefronts.
 // With KS = 1 a wavefront goes from task to task without a pause: the next one's weights are requested under the last ones' products.
-template <class W, class ET, bool GATED, bool COLD, bool CUT>
+template <class W, class ET, bool GATED, bool COLD>
 __global__ __launch_bounds__(kFewThreads, 2) void few_up_kernel(FewArgs a, int KS) {
+    extern __shared__ __align__(16) unsigned char smem[];
     __shared__ FewPlan plan;
     __shared__ mx_f32x4 red[(kFewWaves - 1) * 2 * 64];           // first the logits of a small router
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -214,37 +178,39 @@ __global__ __launch_bounds__(kFewThreads, 2) void few_up_kernel(FewArgs a, int K
     if (blockIdx.x == 0) few_report(plan, a);
 
     constexpr int G = 2, COLS = GATED ? 16 : 32;
-    const int H = a.H, I = a.I, full = H / W::K, left = H - full * W::K, chunks = full + (left ? 1 : 0);
+    const int H = a.H, I = a.I, chunks = (H + W::K - 1) / W::K;
     const int ncol = I / COLS, tasks = plan.hit * ncol;
     const int ks = wave % KS, first = blockIdx.x * (kFewWaves / KS) + wave / KS, stride = gridDim.x * (kFewWaves / KS);
-    const int mine = ks < chunks ? (chunks - ks + KS - 1) / KS : 0;                            // chunks of a task that are this wavefront's
+    const int share = (chunks + KS - 1) / KS, begin = min(ks * share, chunks), end = min(begin + share, chunks);      // chunks of a task that are this wavefront's
+    const int units = (end - begin + kUnit - 1) / kUnit;
     const int idx = lane & 15, q = lane >> 4;
     const int64_t mat = W::row_bytes((int64_t)H * I), smat = (int64_t)I * (H >> 5);
 
     // (with KS > 1 the launch has a set of wavefronts for every task there can be)
     const int mytasks = first < tasks ? (KS > 1 ? 1 : (tasks - 1 - first) / stride + 1) : 0;
-    FewUnit<W, G> u[2];
-    SkinnyRows rows[G];
-    const uint16_t* x = nullptr;
-    int lt = first, lc = ks;             // the next unit to load: its task and chunk
-    auto aim = [&]() {
-        const int j = lt / ncol, n0 = (lt - j * ncol) * COLS;
-        const int e = __builtin_amdgcn_readfirstlane(plan.list[j]);
-        const uint32_t m = plan.mask[e];
-        uint32_t rest = m;               // the idx-th token of the mask; lanes behind the last one take the first
-        for (int i = 0; i < idx && (rest & (rest - 1)); ++i) rest &= rest - 1;
-        const int t = __ffs(idx < __popc(m) ? rest : m) - 1;
-        x = (const uint16_t*)a.x + (int64_t)t * H;
+    Skinny<W, G, COLD> st;
+    st.init(smem + wave * skinny_lds<W>(a.S), a.S, H);
+    st.x_buf = mx_buffer(a.x, (uint32_t)a.S * st.x_row);
+    int task = first, unit = 0;          // the next unit to be fetched
+    auto next = [&](int u) {
+        if (u == mytasks * units) {
+            st.chunk_end = 0;
+            return;
+        }
+        if (unit == 0) {
+            const int j = task / ncol, n0 = (task - j * ncol) * COLS;
+            const int e = __builtin_amdgcn_readfirstlane(plan.list[j]), base = __builtin_amdgcn_readfirstlane(plan.base[e]);
 #pragma unroll
-        for (int g = 0; g < G; ++g)
-            rows[g] = skinny_rows<W>(static_cast<const char*>(GATED && g ? a.w_gate : a.w_up) + e * mat, W::MX ? (GATED && g ? a.s_gate : a.s_up) + e * smat : nullptr,
-                                     n0 + (GATED ? 0 : 16 * g), I, H, lane);
-    };
-    auto load = [&](int b) {
-        if (lc == ks) aim();
-        few_fetch<W, G, COLD, CUT>(u[b], rows, x, lc, full, left, lane);
-        lc += KS;
-        if (lc >= chunks) lc = ks, lt += stride;
+            for (int g = 0; g < G; ++g) {
+                st.w_buf[g] = mx_buffer(static_cast<const char*>(GATED && g ? a.w_gate : a.w_up) + e * mat, (uint32_t)mat);
+                if constexpr (W::MX) st.s_at[g] = (GATED && g ? a.s_gate : a.s_up) + e * smat;
+            }
+            st.aim_weights(n0, I, GATED ? 0 : 16);
+            st.aim_tokens(__builtin_amdgcn_readfirstlane(__popc(plan.mask[e])), [&](int r) { return (uint32_t)plan.row_t[base + r] * st.x_row; });
+        }
+        st.chunk0 = begin + kUnit * unit;
+        st.chunk_end = end;
+        if (++unit == units) unit = 0, task += stride;
     };
     mx_f32x4 acc[G] = {};
     auto store = [&](int task) {
@@ -280,29 +246,24 @@ __global__ __launch_bounds__(kFewThreads, 2) void few_up_kernel(FewArgs a, int K
             }
         }
     };
-    int ct = first, cc = ks;             // the next unit to multiply
-    auto take = [&](int b) {
-        few_multiply<W, G, CUT>(acc, u[b], cc, full, left, lane);
-        cc += KS;
-        if (cc >= chunks) {
-            if (KS == 1) {
-                store(ct);
+    int done_task = first, done_unit = 0;
+    st.run(mytasks * units, acc, next, [&](int) {
+        if (KS > 1 || ++done_unit < units) return;
+        store(done_task);
 #pragma unroll
-                for (int g = 0; g < G; ++g) acc[g] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
-            }
-            cc = ks, ct += stride;
-        }
-    };
-    few_ring(mytasks * mine, load, take);
+        for (int g = 0; g < G; ++g) acc[g] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
+        done_unit = 0, done_task += stride;
+    });
     if (KS > 1) {
         const bool holds = skinny_join<G>(acc, ks, KS, red + wave / KS * (KS - 1) * G * 64, lane);
         if (holds && mytasks) store(first);
     }
 }
 
-// The down projection and the combine: a workgroup owns 16 G columns of out; its wavefronts share the (expert, chunk of I) units.
-template <class W, class ET, int G, bool COLD, bool CUT>
+// The down projection and the combine: a workgroup owns 16 G columns of out; its wavefronts share the (expert, unit of I) pairs.
+template <class W, class ET, int G, bool COLD>
 __global__ __launch_bounds__(kFewThreads, 2) void few_down_kernel(FewArgs a) {
+    extern __shared__ __align__(16) unsigned char smem[];
     __shared__ FewPlan plan;
     __shared__ mx_f32x4 red[(kFewWaves - 1) * G * 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -313,95 +274,102 @@ __global__ __launch_bounds__(kFewThreads, 2) void few_down_kernel(FewArgs a) {
     __syncthreads();
     few_plan(plan, a);
 
-    const int H = a.H, I = a.I, full = I / W::K, left = I - full * W::K, chunks = full + (left ? 1 : 0);
+    const int H = a.H, I = a.I, chunks = (I + W::K - 1) / W::K, units = (chunks + kUnit - 1) / kUnit;      // of an expert
     const int n0 = blockIdx.x * 16 * G;
     const int idx = lane & 15, q = lane >> 4;
     const int64_t mat = W::row_bytes((int64_t)H * I), smat = (int64_t)H * (I >> 5);
-    const int units = plan.hit * chunks;
-    const int begin = (int)((int64_t)units * wave / kFewWaves), end = (int)((int64_t)units * (wave + 1) / kFewWaves);
-    FewUnit<W, G> u[2];
-    SkinnyRows rows[G];
-    const uint16_t* x = nullptr;
-    int lj = begin / max(chunks, 1), lc = begin - lj * chunks;
-    auto aim = [&]() {
-        const int e = __builtin_amdgcn_readfirstlane(plan.list[lj]);
-        const uint32_t m = plan.mask[e];
-        // lane idx is token idx; where that is not the expert's, its first row is read and the sum left out
-        const int at = (m >> idx) & 1u ? __popc(m & ((1u << idx) - 1u)) : 0;
-        x = (const uint16_t*)a.h + (int64_t)(plan.base[e] + at) * I;
-#pragma unroll
-        for (int g = 0; g < G; ++g) rows[g] = skinny_rows<W>(static_cast<const char*>(a.w_down) + e * mat, W::MX ? a.s_down + e * smat : nullptr, n0 + 16 * g, H, I, lane);
-    };
+    const int all = plan.hit * units;
+    const int begin = (int)((int64_t)all * wave / kFewWaves), end = (int)((int64_t)all * (wave + 1) / kFewWaves);
+    Skinny<W, G, COLD> st;
+    st.init(smem + wave * skinny_lds<W>(a.S), a.S, I);
+    st.x_buf = mx_buffer(a.h, (uint32_t)plan.kept * st.x_row);
+    st.aim_weights(n0, H, 16);
+    int j = begin / units, unit = begin - j * units;
     bool aimed = false;
-    auto load = [&](int b) {
-        if (!aimed || lc == 0) aim(), aimed = true;
-        few_fetch<W, G, COLD, CUT>(u[b], rows, x, lc, full, left, lane);
-        if (++lc == chunks) lc = 0, ++lj;
-    };
-    mx_f32x4 out[G] = {}, acc[G] = {};
-    int cj = lj, cc = lc, done = begin;
-    auto take = [&](int b) {
-        if (cc == 0 && a.b_down) {       // the expert's bias goes with its first chunk
-            const uint16_t* bd = (const uint16_t*)a.b_down + (int64_t)__builtin_amdgcn_readfirstlane(plan.list[cj]) * H + n0 + 4 * q;
-#pragma unroll
-            for (int g = 0; g < G; ++g)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) acc[g][r] = few_widen<ET>(bd[16 * g + r]);
+    auto next = [&](int u) {
+        if (u == end - begin) {
+            st.chunk_end = 0;
+            return;
         }
-        few_multiply<W, G, CUT>(acc, u[b], cc, full, left, lane);
-        ++done;
-        if (++cc == chunks || done == end) {
-            const int e = __builtin_amdgcn_readfirstlane(plan.list[cj]);
-            const uint32_t m = plan.mask[e];
-            if ((m >> idx) & 1u) {
-                const float w = plan.row_w[plan.base[e] + __popc(m & ((1u << idx) - 1u))];
+        if (!aimed || unit == 0) {
+            const int e = __builtin_amdgcn_readfirstlane(plan.list[j]), base = __builtin_amdgcn_readfirstlane(plan.base[e]);
 #pragma unroll
-                for (int g = 0; g < G; ++g)
+            for (int g = 0; g < G; ++g) {
+                st.w_buf[g] = mx_buffer(static_cast<const char*>(a.w_down) + e * mat, (uint32_t)mat);
+                if constexpr (W::MX) st.s_at[g] = a.s_down + e * smat;
+            }
+            st.aim_tokens(__builtin_amdgcn_readfirstlane(__popc(plan.mask[e])), [&](int r) { return (uint32_t)(base + r) * st.x_row; });
+            aimed = true;
+        }
+        st.chunk0 = kUnit * unit;
+        st.chunk_end = chunks;
+        if (++unit == units) unit = 0, ++j;
+    };
+    mx_f32x4 out[1][G] = {}, acc[G] = {};
+    int done_j = j, done_unit = unit, left = end - begin;
+    bool whole = unit == 0;              // the expert's first unit is among them
+    st.run(left, acc, next, [&](int) {
+        --left;
+        if (++done_unit < units && left > 0) return;
+        // the columns are the expert's rows in order: lane (row, q) hands its sums to the lane of the row's token
+        const int e = __builtin_amdgcn_readfirstlane(plan.list[done_j]);
+        const uint32_t m = plan.mask[e];
+        const bool in = (m >> idx) & 1u;
+        const int r = __popc(m & ((1u << idx) - 1u)), from = 4 * ((lane & 48) + (in ? r : 0));
+        const float w = in ? plan.row_w[plan.base[e] + r] : 0.0f;
+        const uint16_t* bd = a.b_down && whole ? (const uint16_t*)a.b_down + (int64_t)e * H + n0 + 4 * q : nullptr;      // the bias goes with the first unit
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) out[g][r] = __builtin_fmaf(w, acc[g][r], out[g][r]);
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float y = __uint_as_float(__builtin_amdgcn_ds_bpermute(from, (int)__float_as_uint(acc[g][i])));
+                if (bd) y += few_widen<ET>(bd[16 * g + i]);
+                if (in) out[0][g][i] = __builtin_fmaf(w, y, out[0][g][i]);      // a token that is not the expert's: not even a NaN of it
             }
 #pragma unroll
-            for (int g = 0; g < G; ++g) acc[g] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
-            cc = 0, ++cj;
-        }
-    };
-    few_ring(end - begin, load, take);
-    if (!skinny_join<G>(out, wave, kFewWaves, red, lane) || idx >= a.S) return;
+        for (int g = 0; g < G; ++g) acc[g] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
+        done_unit = 0, ++done_j, whole = true;
+    });
+    if (!skinny_join<G>(out[0], wave, kFewWaves, red, lane) || idx >= a.S) return;
 #pragma unroll
     for (int g = 0; g < G; ++g)
-        *reinterpret_cast<uint2*>((uint16_t*)a.out + (int64_t)idx * H + n0 + 16 * g + 4 * q) = uint2{few_pack<ET>(out[g][0], out[g][1]), few_pack<ET>(out[g][2], out[g][3])};
+        *reinterpret_cast<uint2*>((uint16_t*)a.out + (int64_t)idx * H + n0 + 16 * g + 4 * q) = uint2{few_pack<ET>(out[0][g][0], out[0][g][1]), few_pack<ET>(out[0][g][2], out[0][g][3])};
 }
 
 // Router products up to which every workgroup makes the logits itself instead of a launch in front.
 constexpr int64_t kFoldProducts = 1 << 18;
 
-template <class W, class ET, bool COLD, bool CUT_UP, bool CUT_DOWN>
+template <class W, class ET, bool COLD>
 hipError_t launch_few_form(const FewArgs& a, hipStream_t st) {
     const bool gated = a.w_gate != nullptr;
     const int64_t most = std::min<int64_t>(a.E, (int64_t)a.S * a.k) * (a.I / (gated ? 16 : 32));      // tasks there can be
-    const int chunks = (a.H + W::K - 1) / W::K;
+    const int chunks = (a.H + W::K - 1) / W::K, lds = kFewWaves * skinny_lds<W>(a.S);
+    static const hipError_t ready = [] {
+        constexpr int bytes = kFewWaves * skinny_lds<W>(kFewTokens);
+        for (const void* f : {reinterpret_cast<const void*>(few_up_kernel<W, ET, true, COLD>), reinterpret_cast<const void*>(few_up_kernel<W, ET, false, COLD>),
+                              reinterpret_cast<const void*>(few_down_kernel<W, ET, 1, COLD>)}) {
+            const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+            if (e != hipSuccess) return e;
+        }
+        return hipSuccess;
+    }();
+    if (ready != hipSuccess) return ready;
     int KS = 1;
-    while (KS < kFewWaves && 2 * KS <= chunks && most * KS < 1024) KS *= 2;
+    while (KS < kFewWaves && 2 * KS * kUnit <= chunks && most * KS < 1024) KS *= 2;
     const int64_t sets = (most + kFewWaves / KS - 1) / (kFewWaves / KS);
     const unsigned grid = (unsigned)(KS > 1 ? sets : std::min<int64_t>(sets, 512));
-    if (gated) few_up_kernel<W, ET, true, COLD, CUT_UP><<<grid, kFewThreads, 0, st>>>(a, KS);
-    else few_up_kernel<W, ET, false, COLD, CUT_UP><<<grid, kFewThreads, 0, st>>>(a, KS);
+    if (gated) few_up_kernel<W, ET, true, COLD><<<grid, kFewThreads, lds, st>>>(a, KS);
+    else few_up_kernel<W, ET, false, COLD><<<grid, kFewThreads, lds, st>>>(a, KS);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    few_down_kernel<W, ET, 1, COLD, CUT_DOWN><<<a.H / 16, kFewThreads, 0, st>>>(a);
+    few_down_kernel<W, ET, 1, COLD><<<a.H / 16, kFewThreads, lds, st>>>(a);
     return hipGetLastError();
-}
-template <class W, class ET, bool COLD>
-hipError_t launch_few_cut(const FewArgs& a, hipStream_t st) {
-    const bool up = a.H % W::K, down = a.I % W::K;
-    if (up) return down ? launch_few_form<W, ET, COLD, true, true>(a, st) : launch_few_form<W, ET, COLD, true, false>(a, st);
-    return down ? launch_few_form<W, ET, COLD, false, true>(a, st) : launch_few_form<W, ET, COLD, false, false>(a, st);
 }
 template <class W, class ET>
 hipError_t launch_few_weights(const FewArgs& a, hipStream_t st) {
     const int64_t experts = std::min<int64_t>(a.E, (int64_t)a.S * a.k);
     const bool cold = experts * W::row_bytes((int64_t)a.H * a.I) * (a.w_gate ? 3 : 2) > ((int64_t)256 << 20);     // more than the memory-side cache holds
-    return cold ? launch_few_cut<W, ET, true>(a, st) : launch_few_cut<W, ET, false>(a, st);
+    return cold ? launch_few_form<W, ET, true>(a, st) : launch_few_form<W, ET, false>(a, st);
 }
 
 }  // namespace
@@ -415,7 +383,7 @@ hipError_t launch_few(FewArgs a, bool f16, bool mxfp4, hipStream_t st) {
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    if (mxfp4) return launch_few_weights<WeightsMx, bf16_s>(a, st);
+    if (mxfp4) return launch_few_weights<WeightsMx<false>, bf16_s>(a, st);
     return f16 ? launch_few_weights<Weights16<f16_s>, f16_s>(a, st) : launch_few_weights<Weights16<bf16_s>, bf16_s>(a, st);
 }
 

@@ -120,101 +120,59 @@ __device__ __forceinline__ void mx_store_tile(const MxProduct& p, const MxTask& 
 // ---- up to 16 rows a block: a weight streamer ----
 constexpr int kStreamWaves = 8;
 
-// One chunk of the token rows.
-template <bool ROWS4>
-struct StreamTokens {
-    mx_u32x4 x[ROWS4 ? 2 : 8];
-    uint32_t s[2];
-};
-
-// KS wavefronts share a contraction (chunks in turn), 8 / KS sets of 16 CG columns a workgroup.
+// KS wavefronts share a contraction, a share in a row each, 8 / KS sets of 16 CG columns a workgroup.  rows_most: token rows that LDS is there for.
 template <bool ROWS4, int CG, bool COLD>
-__global__ __launch_bounds__(64 * kStreamWaves) void mx_stream_kernel(MxProduct p, int KS) {
+__global__ __launch_bounds__(64 * kStreamWaves) void mx_stream_kernel(MxProduct p, int KS, int rows_most) {
+    typedef WeightsMx<ROWS4> W;
+    extern __shared__ __align__(16) unsigned char smem[];
     __shared__ mx_f32x4 red[(kStreamWaves - 1) * CG * 64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ks = wave % KS, set = wave / KS;
     MxTask t;
     if (!mx_task<16, ROWS4>(p, 16 * CG * (kStreamWaves / KS), t)) return;
     const int n0 = t.n0 + 16 * CG * set, K = p.K;
-    const int idx = lane & 15, q = lane >> 4;
-    SkinnyRows rows[CG];
+    Skinny<W, CG, COLD> st;
+    st.init(smem + wave * skinny_lds<W>(rows_most), rows_most, K);
 #pragma unroll
-    for (int g = 0; g < CG; ++g) rows[g] = skinny_rows<WeightsMx>(t.w, t.s, n0 + 16 * g, p.N, K, lane);
-    const int64_t ar = idx < t.rows ? idx : 0;                   // rows behind the block's last one read row 0 again and are not stored
-    const uint16_t* x16 = reinterpret_cast<const uint16_t*>(t.a) + ar * K;
-    const char* x4 = t.a + ar * (K >> 1) + 16 * q;
-    const uint8_t* xs = ROWS4 ? t.a_scales + ar * (K >> 5) : nullptr;
+    for (int g = 0; g < CG; ++g) {
+        st.w_buf[g] = mx_buffer(t.w, (uint32_t)p.N * st.row);
+        st.s_at[g] = t.s;
+    }
+    st.x_buf = mx_buffer(t.a, (uint32_t)t.rows * st.x_row);
+    st.aim_weights(n0, p.N, 16);
+    st.aim_tokens(t.rows, [&](int r) { return (uint32_t)r * st.x_row; });
+    if constexpr (ROWS4) {
+        st.sx_at = p.a_scales;                    // (the whole array: the eight bytes at the end of a block's may lie behind it)
+        st.sx_base = t.row0 * (K >> 5);
+        st.sx_end = p.M * (K >> 5) - 8;
+        st.sx_row = (uint32_t)min(lane >> 2, t.rows - 1) * (uint32_t)(K >> 5);
+    }
+    const int chunks = (K + W::K - 1) / W::K, share = (chunks + KS - 1) / KS;
+    const int begin = min(ks * share, chunks), end = min(begin + share, chunks), n = (end - begin + kUnit - 1) / kUnit;
+    mx_f32x4 acc[1][CG] = {};
+    st.run(n, acc[0], [&](int u) { st.chunk0 = begin + kUnit * u, st.chunk_end = u < n ? end : 0; }, [](int) {});
+    if (!skinny_join<CG>(acc[0], ks, KS, red + set * (KS - 1) * CG * 64, lane)) return;
+    mx_store_tile<1, CG>(p, t, lane & 15, n0 + 4 * (lane >> 4), acc);
+}
 
-    mx_f32x4 acc[CG];
-#pragma unroll
-    for (int g = 0; g < CG; ++g) acc[g] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
-    SkinnyChunk<WeightsMx, CG> d[2];
-    StreamTokens<ROWS4> x[2];
-    auto load = [&](int b, int c) {
-        skinny_load<WeightsMx, CG, COLD>(d[b], rows, c);
-        if constexpr (ROWS4) {
-            x[b].x[0] = *reinterpret_cast<const mx_u32x4*>(x4 + 128 * (int64_t)c);
-            x[b].x[1] = *reinterpret_cast<const mx_u32x4*>(x4 + 128 * (int64_t)c + 64);
-            __builtin_memcpy(x[b].s, xs + 8 * (int64_t)c, 8);
-        } else {
-            skinny_tokens<WeightsMx>(x[b].x, x16, c, lane);
-        }
+// A matrix of fewer than 256 values, which has no eight scales in a row to fetch: a value of the result a thread.
+template <bool ROWS4>
+__global__ __launch_bounds__(256) void mx_small_kernel(MxProduct p) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= p.M * p.N) return;
+    const int64_t m = i / p.N;
+    const int n = (int)(i - m * p.N);
+    auto value = [&](const void* codes, const uint8_t* scales, int64_t row, int k) {
+        const uint32_t c = static_cast<const uint8_t*>(codes)[row * (p.K >> 1) + (k >> 1)] >> (4 * (k & 1));
+        return __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c & 15u, mx_scale(scales[row * (p.K >> 5) + (k >> 5)]), 0)[0];
     };
-    auto multiply = [&](int b) {
-        if constexpr (ROWS4) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int g = 0; g < CG; ++g)
-                    acc[g] = mx_mfma(d[b].v[g][h], skinny_scale(d[b].s[g], h, lane), x[b].x[h], skinny_scale(x[b].s, h, lane), acc[g]);
-        } else {
-            skinny_multiply<WeightsMx, CG>(acc, d[b], x[b].x, lane);
-        }
-    };
-    auto take = [&](int b) {
-        skinny_settle(d[b]);
-        multiply(b);
-    };
-    const int full = K >> 8, n = full > ks ? (full - ks + KS - 1) / KS : 0;
-    if (n > 0) load(0, ks);
-    if (n > 1) load(1, ks + KS);
-    int i = 0;
-    for (; i + 3 < n; i += 2) {
-        take(0);
-        load(0, ks + (i + 2) * KS);
-        take(1);
-        load(1, ks + (i + 3) * KS);
+    float sum = 0.0f;
+    for (int k = 0; k < p.K; ++k) {
+        const float a = ROWS4 ? value(p.a, p.a_scales, m, k) : bf16_bits_to_f32(static_cast<const uint16_t*>(p.a)[m * p.K + k]);
+        sum = __builtin_fmaf(a, value(p.w, p.s, n, k), sum);
     }
-    if (n - i > 0) take(0);
-    if (n - i > 2) load(0, ks + (i + 2) * KS);
-    if (n - i > 1) take(1);
-    if (n - i > 2) take(0);
-    if ((K & 255) && full % KS == ks) {          // the rows' last chunk, cut off
-        const int left = K & 255;
-        skinny_load_tail<WeightsMx, CG, COLD>(d[0], rows, full, left >> 1, lane);
-        if constexpr (ROWS4) {
-            x[0].s[0] = x[0].s[1] = 0;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int b = 4 * h + q;
-                x[0].x[h] = mx_u32x4{0u, 0u, 0u, 0u};
-                if (b < (left >> 5)) {
-                    x[0].x[h] = *reinterpret_cast<const mx_u32x4*>(x4 + 128 * (int64_t)full + 64 * h);
-                    x[0].s[h] = (uint32_t)xs[8 * (int64_t)full + b] << (8 * q);
-                }
-            }
-        } else {
-            skinny_tokens_tail<WeightsMx>(x[0].x, x16, full, left, lane);
-        }
-        skinny_settle(d[0]);
-        skinny_zero_tail(d[0], left >> 1, lane);
-        multiply(0);
-    }
-    if (!skinny_join<CG>(acc, ks, KS, red + set * (KS - 1) * CG * 64, lane)) return;
-    mx_f32x4 sum[1][CG];
-#pragma unroll
-    for (int g = 0; g < CG; ++g) sum[0][g] = acc[g];
-    mx_store_tile<1, CG>(p, t, idx, n0 + 4 * q, sum);
+    if (p.bias) sum += bf16_bits_to_f32(p.bias[n]);
+    p.out[i] = (uint16_t)pack2_bf16(p.act == MOE_ACT_GELU ? gelu16(sum) : p.act == MOE_ACT_RELU && sum < 0.0f ? 0.0f : sum, 0.0f);
 }
 
 // ---- more rows: tiles ----
@@ -224,12 +182,6 @@ __global__ __launch_bounds__(64 * kStreamWaves) void mx_stream_kernel(MxProduct 
 // columns behind the matrix's and what lies behind K are zeros without a branch.  Every slab takes the same path: what is requested behind
 // the last one lies behind the operands' ends, and every set runs as many slabs as the longest (of zeros).  Where paths with and without
 // requests met, every wait would be one for all of them.
-constexpr uint32_t kBehind = 0xD0000000u;      // an offset behind the end of every buffer here, also with a tile's rows added to it (offsets
-                                               // are whole in the vector register: the range check is against what a scalar offset leaves of the
-                                               // buffer, and that may be less than nothing)
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_buffer(const void* p, uint32_t bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00020000);
-}
 // Every request of this wavefront for the slab has landed and its reads of the other stage are done, then so have everybody's.
 __device__ __forceinline__ void mx_meet() {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -566,21 +518,44 @@ hipError_t launch_tile(const MxProduct& p, hipStream_t st) {
     return hipGetLastError();
 }
 
+template <bool ROWS4, int CG>
+hipError_t launch_stream_form(const MxProduct& p, int KS, bool cold, hipStream_t st) {
+    const int rows = (int)(p.count ? 16 : std::min<int64_t>(p.M, 16)), lds = kStreamWaves * skinny_lds<WeightsMx<ROWS4>>(rows);
+    const unsigned grid = (unsigned)mx_grid(p, 16, 16 * CG * (kStreamWaves / KS));
+    static const hipError_t ready = [] {
+        constexpr int most = kStreamWaves * skinny_lds<WeightsMx<ROWS4>>(16);
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(mx_stream_kernel<ROWS4, CG, true>), hipFuncAttributeMaxDynamicSharedMemorySize, most);
+        return e != hipSuccess ? e : hipFuncSetAttribute(reinterpret_cast<const void*>(mx_stream_kernel<ROWS4, CG, false>), hipFuncAttributeMaxDynamicSharedMemorySize, most);
+    }();
+    if (ready != hipSuccess) return ready;
+    if (cold) mx_stream_kernel<ROWS4, CG, true><<<grid, 64 * kStreamWaves, lds, st>>>(p, KS, rows);
+    else mx_stream_kernel<ROWS4, CG, false><<<grid, 64 * kStreamWaves, lds, st>>>(p, KS, rows);
+    return hipGetLastError();
+}
+
 template <bool ROWS4>
 hipError_t launch_stream(const MxProduct& p, hipStream_t st) {
     const int64_t blocks = p.count ? std::min<int64_t>(p.E, p.M) : (p.M + 15) / 16;
     const int chunks = (p.K + 255) / 256;
     const int64_t groups = blocks * ((p.N + 15) / 16);         // wavefronts if each had 16 columns and the whole contraction
-    const bool wide = groups >= 4096 && chunks <= 64;
+#ifdef TUNE
+    static const int t_wide = getenv("T_WIDE") ? atoi(getenv("T_WIDE")) : -1, t_ks = getenv("T_KS") ? atoi(getenv("T_KS")) : -1;
+    const bool wide = t_wide >= 0 ? t_wide : groups >= 4096;
     int KS = 1;
     while (KS < 8 && KS * 2 <= chunks && groups / (wide ? 2 : 1) * KS < 4096) KS *= 2;
+    if (t_ks > 0) KS = t_ks;
+#else
+    const bool wide = groups >= 4096;
+    int KS = 1;
+    while (KS < 8 && KS * 2 <= chunks && groups / (wide ? 2 : 1) * KS < 4096) KS *= 2;
+#endif
     const bool cold = blocks * p.N * p.K / 2 > ((int64_t)256 << 20);
-    const int BN = 16 * (wide ? 2 : 1) * (kStreamWaves / KS);
-    const unsigned grid = (unsigned)mx_grid(p, 16, BN);
-    if (wide && cold) mx_stream_kernel<ROWS4, 2, true><<<grid, 64 * kStreamWaves, 0, st>>>(p, KS);
-    else if (wide) mx_stream_kernel<ROWS4, 2, false><<<grid, 64 * kStreamWaves, 0, st>>>(p, KS);
-    else if (cold) mx_stream_kernel<ROWS4, 1, true><<<grid, 64 * kStreamWaves, 0, st>>>(p, KS);
-    else mx_stream_kernel<ROWS4, 1, false><<<grid, 64 * kStreamWaves, 0, st>>>(p, KS);
+    return wide ? launch_stream_form<ROWS4, 2>(p, KS, cold, st) : launch_stream_form<ROWS4, 1>(p, KS, cold, st);
+}
+
+template <bool ROWS4>
+hipError_t launch_small(const MxProduct& p, hipStream_t st) {
+    mx_small_kernel<ROWS4><<<(unsigned)((p.M * p.N + 255) / 256), 256, 0, st>>>(p);
     return hipGetLastError();
 }
 
@@ -626,14 +601,16 @@ hipError_t launch_product4(const MxProduct& p, int form, hipStream_t st) {
 
 int product_form(const MxProduct& p) {
     const int64_t rows = p.count ? (p.M + p.E - 1) / p.E : p.M;
-    if (rows <= 16 || (int64_t)p.N * p.K < 256) return 0;       // (the tiles read eight scales at a time: a matrix has that many)
+    if (rows <= 16) return 0;
     if (rows <= 32) return 1;
     if (rows <= 64) return 2;
     const int64_t tiles = (p.count ? p.M / 256 + p.E : (p.M + 255) / 256) * ((p.N + 255) / 256);
     return rows >= 256 && tiles >= 192 ? 4 : 3;
 }
 
+bool is_small(const MxProduct& p) { return (int64_t)p.N * p.K < 256 || (p.a_scales && p.M * p.K < 256); }      // eight scales are fetched at a time
 int64_t product_workgroups(const MxProduct& p, int form) {
+    if (is_small(p)) return (p.M * p.N + 255) / 256;
     constexpr int BM[] = {16, 32, 64, 128, 256}, BN[] = {16, 64, 64, 128, 256};      // (the streamer's narrowest)
     return mx_grid(p, BM[form], BN[form]);
 }
@@ -643,6 +620,7 @@ int64_t product_workgroups(const MxProduct& p, int form) {
 // form: MOE_OPT_AUTO, or the kernel asked for
 hipError_t launch_product_mxfp4(const MxProduct& p, int form, hipStream_t st) {
     if (p.M == 0) return hipSuccess;
+    if (is_small(p)) return p.a_scales ? launch_small<true>(p, st) : launch_small<false>(p, st);
     if (form < 0) form = product_form(p);
     return p.a_scales ? launch_product4(p, form, st) : launch_product16(p, form, st);
 }

@@ -7,6 +7,12 @@
 // does not matter as long as both operands agree: with 16-bit weights a piece is the eight values an instruction takes of a lane.  With
 // MXFP4 a piece is 32 codes, a whole block with one scale: four instructions of bf16, eight of its codes each -- widened exactly, scale
 // included, two an instruction -- or, against rows in MXFP4, the whole operand of one scaled instruction over 128 values.
+//
+// What bounds it is memory, and then the address unit, which takes as long over a request for 64 bytes as over one for a kilobyte.  So
+// nothing but weights is fetched in the shape in which it is used: a chunk's token rows go, as they lie, into LDS of the wavefront's own
+// (for one row an instruction a chunk instead of eight), and scales come for four chunks at a time, 32 bytes of 16 rows an instruction, and
+// find their lanes by a permutation.  One row times 65536 x 4096, us, everything fetched as it is used / scales left out / rows left out /
+// both: 40.2 / 36.6 / 31.9 / 25.6.  All operands are read through buffers that end where they end: what lies behind is zeros, without a branch.
 #pragma once
 
 #include "ffn_common.hpp"
@@ -17,163 +23,246 @@ namespace moe355 {
 namespace {
 
 typedef _Float16 sk_f16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) void sk_lds_void;
 
-// Weights in 16 bits (ET: bf16_s, f16_s).  A chunk is what a wavefront has in flight twice: 256 bytes of each of 16 rows.
+constexpr uint32_t kBehind = 0xD0000000u;      // an offset behind the end of every buffer here, also with a tile's rows added to it (offsets
+                                               // are whole in the vector register: the range check is against what a scalar offset leaves of the
+                                               // buffer, and that may be less than nothing)
+constexpr int64_t kBufferBytes = (int64_t)3 << 30;      // what a buffer may have at most
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_buffer(const void* p, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00020000);
+}
+
+// Weights in 16 bits (ET: bf16_s, f16_s).  A chunk: 256 bytes of each of 16 rows, 256 bytes of a token row.
 template <class ET>
 struct Weights16 {
     static constexpr bool MX = false;
     static constexpr bool F16 = std::is_same<ET, f16_s>::value;
     static constexpr int K = 128;            // values of k of a chunk
-    static constexpr int LINES = 2;          // 128-byte lines of a row
-    static constexpr int FRAGS = 4;          // 16-byte pieces of a token row that a lane multiplies
+    static constexpr int LINES = 2;          // 128-byte lines of a weight row
+    static constexpr int ROWB = 256;         // bytes of a token row
     static __host__ __device__ __forceinline__ int64_t row_bytes(int64_t k) { return 2 * k; }
+    static __device__ __forceinline__ uint32_t token_bytes(uint32_t k) { return 2 * k; }
 };
+// Weights in MXFP4; token rows in bf16, or (ROWS4) in MXFP4 too.
+template <bool ROWS4_>
 struct WeightsMx {
     static constexpr bool MX = true;
+    static constexpr bool ROWS4 = ROWS4_;
     static constexpr bool F16 = false;
     static constexpr int K = 256;
     static constexpr int LINES = 1;
-    static constexpr int FRAGS = 8;
+    static constexpr int ROWB = ROWS4 ? 128 : 512;
     static __host__ __device__ __forceinline__ int64_t row_bytes(int64_t k) { return k >> 1; }
+    static __device__ __forceinline__ uint32_t token_bytes(uint32_t k) { return ROWS4 ? k >> 1 : 2 * k; }
 };
-
-// Where 16 rows of a matrix lie for this lane.
-struct SkinnyRows {
-    const char* first;       // of the line instruction's lower eight rows
-    const char* second;      // ... and of the upper eight
-    const uint8_t* scale;    // of row (lane & 15)
-};
-// Rows n0 .. n0 + 15 of [N][K]; rows behind the last one read it again.
+constexpr int kUnit = 4;                       // chunks that share a fetch of scales
+constexpr uint32_t kNoChunk = 1u << 22;        // a chunk behind every row's end
+// LDS of a wavefront: two chunks of token rows, whole instructions of them.
 template <class W>
-__device__ __forceinline__ SkinnyRows skinny_rows(const void* w, const uint8_t* s, int n0, int N, int K, int lane) {
-    const int64_t rb = W::row_bytes(K);
-    const char* base = static_cast<const char*>(w) + ((lane >> 4) + ((lane & 8) >> 1)) * 16;
-    SkinnyRows r;
-    r.first = base + min(n0 + (lane & 7), N - 1) * rb;
-    r.second = base + min(n0 + 8 + (lane & 7), N - 1) * rb + ((lane & 8) ? -64 : 64);
-    r.scale = W::MX ? s + (int64_t)min(n0 + (lane & 15), N - 1) * (K >> 5) : nullptr;
-    return r;
+__host__ __device__ constexpr int skinny_lds(int rows) {
+    return 2 * ((rows * W::ROWB + 1023) / 1024) * 1024;
 }
 
-template <class W, int G>
-struct SkinnyChunk {
-    mx_u32x4 v[G][2 * W::LINES];
-    uint32_t s[W::MX ? G : 1][2];            // MXFP4: the scales of the row's eight blocks
-};
-
+// One wavefront's stream.  aim() says what the next unit is made of; scales(), fetch() and multiply() go through its chunks.
 template <class W, int G, bool COLD>
-__device__ __forceinline__ void skinny_load(SkinnyChunk<W, G>& d, const SkinnyRows (&r)[G], int c) {
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-#pragma unroll
-        for (int l = 0; l < W::LINES; ++l) {
-            const int64_t at = ((int64_t)c * W::LINES + l) * 128;
-            d.v[g][2 * l] = load_piece<COLD>(r[g].first + at);
-            d.v[g][2 * l + 1] = load_piece<COLD>(r[g].second + at);
-        }
-        if constexpr (W::MX) __builtin_memcpy(d.s[g], r[g].scale + 8 * (int64_t)c, 8);
+struct Skinny {
+    static constexpr bool rows4() { return W::MX && W::ROWB == 128; }
+    static constexpr int PER = 1024 / W::ROWB;             // token rows an instruction brings
+    static constexpr int MOST = 16 / PER;                  // ... and instructions for 16 rows
+    static constexpr int LATER = 2 * W::LINES * G;         // requests for a chunk's weights, its last ones
+
+    mx_u32x4 v[2][G][2 * W::LINES];
+    uint64_t s_raw[G], sx_raw;
+    uint32_t s_early[G], sx_early;                         // bytes that the fetch lies in front of what was wanted
+    uint32_t s[G][2], sx[2];                               // this chunk's scales (MXFP4): blocks 0-3 and 4-7 of row (lane & 15)
+    uint64_t s_held[G], sx_held;
+
+    __amdgpu_buffer_rsrc_t w_buf[G], x_buf;
+    const uint8_t* s_at[G];
+    const uint8_t* sx_at;
+    uint32_t s_last;                                       // the last eight bytes of the matrix's scales
+    int64_t sx_base, sx_end;                               // the token rows' scales: where row 0 begins, the array's last eight bytes
+    uint32_t w1, w2, w_add, s_row[G], x_off[MOST], sx_row, row, x_row;
+    int rows, chunk0, chunk_end;                           // token rows, chunks [chunk0, chunk_end) of the unit
+    int lane;
+    unsigned char* lds;
+    int half;                                              // bytes of one of its two parts
+
+    __device__ __forceinline__ void init(unsigned char* own, int rows_most, int K) {
+        lane = threadIdx.x & 63;
+        lds = own;
+        half = skinny_lds<W>(rows_most) / 2;
+        row = (uint32_t)W::row_bytes(K);
+        x_row = W::token_bytes(K);
     }
-}
-
-// A row's last chunk, cut off: pieces behind its end are read from the chunk's first (which is inside) and become zeros in skinny_settle_tail.
-// left: bytes of the row that the chunk has.
-template <class W, int G, bool COLD>
-__device__ __forceinline__ void skinny_load_tail(SkinnyChunk<W, G>& d, const SkinnyRows (&r)[G], int c, int left, int lane) {
-    const int piece = (lane >> 4) + ((lane & 8) >> 1);
+    // Weight rows n0 .. n0 + 15 of [N][K], and of group g those 16 g further on (or the same ones of another matrix: w_buf, s_at).
+    __device__ __forceinline__ void aim_weights(int n0, int N, int step) {
+        w1 = (uint32_t)(n0 + (lane & 7)) * row;
+        w2 = w1 + 8 * row;
+        w_add = (uint32_t)step * row;
+        if constexpr (W::MX) {
+            const uint32_t sr = row >> 4;
+            s_last = (uint32_t)N * sr - 8;
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
+            for (int g = 0; g < G; ++g) s_row[g] = (uint32_t)min(n0 + step * g + (lane >> 2), N - 1) * sr;
+        }
+    }
+    // Token rows: of(r) is where row r begins in x_buf.
+    template <class OF>
+    __device__ __forceinline__ void aim_tokens(int n, OF of) {
+        rows = n;
+#pragma unroll
+        for (int p = 0; p < MOST; ++p)
+            if (PER * p < n) x_off[p] = of(min(PER * p + lane / (64 / PER), n - 1));
+    }
+
+    // Eight bytes of scales: inside the array, which has eight.
+    __device__ __forceinline__ void eight(uint64_t& raw, uint32_t& early, const uint8_t* at, uint32_t want, uint32_t last) {
+        const uint32_t o = min(want, last);
+        early = want - o;
+        __builtin_memcpy(&raw, at + o, 8);
+    }
+    // Lane 4 r + j: of row r the scales of chunk j of the unit.
+    __device__ __forceinline__ void scales() {
+        if constexpr (W::MX) {
+            const uint32_t sr = row >> 4, c = min(8u * (uint32_t)(chunk0 + (lane & 3)), sr);      // behind the row's end: some bytes that are not used
+#pragma unroll
+            for (int g = 0; g < G; ++g) eight(s_raw[g], s_early[g], s_at[g], s_row[g] + c, s_last);
+            if constexpr (rows4()) {
+                const int64_t want = sx_base + sx_row + c, o = min(want, sx_end);
+                sx_early = (uint32_t)(want - o);
+                __builtin_memcpy(&sx_raw, sx_at + o, 8);
+            }
+        }
+    }
+    __device__ __forceinline__ void settle_scales() {
+        if constexpr (W::MX) {
+#pragma unroll
+            for (int g = 0; g < G; ++g) s_held[g] = s_raw[g] >> (4 * s_early[g]) >> (4 * s_early[g]);
+            if constexpr (rows4()) sx_held = sx_raw >> (4 * sx_early) >> (4 * sx_early);
+        }
+    }
+
+    // Chunk j of the unit into part b.
+    __device__ __forceinline__ void fetch(int b, int j) {
+        const uint32_t c = chunk0 + j < chunk_end ? (uint32_t)(chunk0 + j) : kNoChunk;
+        {
+            const int slots = W::ROWB / 16, slot = lane % slots;
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");             // what lay there has been read
+#pragma unroll
+            for (int p = 0; p < MOST; ++p) {
+                if (p > 0 && PER * p >= rows) break;                       // (the first one without a question: the waits below count on it)
+                const int r = PER * p + lane / slots;
+                uint32_t piece;                                            // which 16 bytes of the row slot `slot` holds (see fragment)
+                if constexpr (!W::MX) piece = slot ^ (r & 15);
+                else if constexpr (W::ROWB == 512) piece = (slot & 16) + 4 * ((slot ^ r) & 3) + (((slot ^ r) & 15) >> 2);
+                else piece = slot ^ ((r >> 1) & 7);
+                const uint32_t at = c * W::ROWB + 16 * piece;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(x_buf, (sk_lds_void*)(lds + b * half + p * 1024), 16, (int)(at < x_row ? x_off[p] + at : kBehind), 0, 0, 0);
+            }
+        }
+        const uint32_t piece = (lane >> 4) + ((lane & 8) >> 1);
 #pragma unroll
         for (int l = 0; l < W::LINES; ++l) {
-            const int64_t at = ((int64_t)c * W::LINES + l) * 128;
-            const int o1 = 128 * l + 16 * piece, o2 = 128 * l + 16 * (piece ^ 4);
-            d.v[g][2 * l] = load_piece<COLD>(r[g].first + at - (o1 < left ? 0 : o1));
-            d.v[g][2 * l + 1] = load_piece<COLD>(r[g].second + at - (o2 < left ? 0 : o2));
-        }
-        if constexpr (W::MX) {
-            const int blocks = left >> 4;
+            const uint32_t at = (c * W::LINES + l) * 128, o1 = at + 16 * piece, o2 = at + 16 * (piece ^ 4);
+            const uint32_t v1 = o1 < row ? w1 + o1 : kBehind, v2 = o2 < row ? w2 + o2 : kBehind;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                d.s[g][h] = 0;
+            for (int g = 0; g < G; ++g) {
+                v[b][g][2 * l] = __builtin_bit_cast(mx_u32x4, __builtin_amdgcn_raw_buffer_load_b128(w_buf[g], (int)(v1 + g * w_add), 0, COLD ? 2 : 0));      // 2: not kept
+                v[b][g][2 * l + 1] = __builtin_bit_cast(mx_u32x4, __builtin_amdgcn_raw_buffer_load_b128(w_buf[g], (int)(v2 + g * w_add), 0, COLD ? 2 : 0));
+            }
+        }
+    }
+
+    // Piece p of the lane's token row in part b.  Slots are permuted by the row so that the lanes that the LDS serves in a cycle (0-3, 12-15 and
+    // 20-27; 4-11, 16-19 and 28-31; and so on) meet different banks.  Lanes behind the last row read row 0.
+    __device__ __forceinline__ mx_u32x4 fragment(int b, int p, int rows_of_unit) const {
+        const int q = lane >> 4, r = (lane & 15) < rows_of_unit ? lane & 15 : 0;
+        int slot;
+        if constexpr (!W::MX) slot = (4 * p + q) ^ r;
+        else if constexpr (W::ROWB == 512) slot = 16 * (p >> 2) + ((q + 4 * (p & 3)) ^ r);
+        else slot = (4 * p + q) ^ ((r >> 1) & 7);
+        return *reinterpret_cast<const mx_u32x4*>(lds + b * half + r * W::ROWB + 16 * slot);
+    }
+    static __device__ __forceinline__ mx_f32x4 mfma(mx_u32x4 a, mx_u32x4 x, mx_f32x4 c) {
+        if constexpr (W::F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(sk_f16x8, a), __builtin_bit_cast(sk_f16x8, x), c, 0, 0, 0);
+        else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mx_bf16x8, a), __builtin_bit_cast(mx_bf16x8, x), c, 0, 0, 0);
+    }
+    // acc[g] += chunk j of the unit that began with chunk `first` and has so many rows, in part b.
+    __device__ __forceinline__ void multiply(mx_f32x4 (&acc)[G], int b, int j, int first, int rows_of_unit) {
+        // the other part's requests came later than all of this one's, those for its weights and one for a token row at least
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LATER + 1) : "memory");
+        __builtin_amdgcn_sched_barrier(0);                                 // (nothing that waits for this part moves in front of the requests)
+        if constexpr (W::MX) {
+            const int from = 16 * (lane & 15) + 4 * j, q = lane >> 4;      // bytes: lane 4 (lane & 15) + j
+            const uint32_t block = 8 * (uint32_t)(first + j) + q, blocks = row >> 4;
+            auto turn = [&](uint32_t (&d)[2], uint64_t held) {             // this lane's bytes; behind the row's end: 0
+                const uint32_t lo = (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)(uint32_t)held), hi = (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)(uint32_t)(held >> 32));
+                d[0] = block < blocks ? lo >> (8 * q) & 255u : 0u;
+                d[1] = block + 4 < blocks ? hi >> (8 * q) & 255u : 0u;
+            };
+#pragma unroll
+            for (int g = 0; g < G; ++g) turn(s[g], s_held[g]);
+            if constexpr (rows4()) turn(sx, sx_held);
+        }
+        mx_u32x4 x[W::MX && W::ROWB == 512 ? 8 : 4];
+        constexpr int P = W::MX ? (W::ROWB == 512 ? 8 : 2) : 4;
+#pragma unroll
+        for (int p = 0; p < P; ++p) x[p] = fragment(b, p, rows_of_unit);
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int l = 0; l < W::LINES; ++l) line_pieces(v[b][g][2 * l], v[b][g][2 * l + 1], v[b][g][2 * l], v[b][g][2 * l + 1]);
+#pragma unroll
+        for (int p = 0; p < 2 * W::LINES; ++p) {
+            if constexpr (!W::MX) {
+#pragma unroll
+                for (int g = 0; g < G; ++g) acc[g] = mfma(v[b][g][p], x[p], acc[g]);
+            } else if constexpr (W::ROWB == 512) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (4 * h + i < blocks) d.s[g][h] |= (uint32_t)r[g].scale[8 * (int64_t)c + 4 * h + i] << (8 * i);
-            }
-        }
-    }
-}
-// Lines -> pieces: v[g][2 l] and v[g][2 l + 1] become this lane's piece of the lower and the upper 64 bytes of line l.
-template <class W, int G>
-__device__ __forceinline__ void skinny_settle(SkinnyChunk<W, G>& d) {
 #pragma unroll
-    for (int g = 0; g < G; ++g)
-#pragma unroll
-        for (int l = 0; l < W::LINES; ++l) line_pieces(d.v[g][2 * l], d.v[g][2 * l + 1], d.v[g][2 * l], d.v[g][2 * l + 1]);
-}
-template <class W, int G>
-__device__ __forceinline__ void skinny_zero_tail(SkinnyChunk<W, G>& d, int left, int lane) {
-#pragma unroll
-    for (int g = 0; g < G; ++g)
-#pragma unroll
-        for (int p = 0; p < 2 * W::LINES; ++p)
-            if (64 * p + 16 * (lane >> 4) >= left) d.v[g][p] = mx_u32x4{0u, 0u, 0u, 0u};
-}
-
-// The scale of piece p (0: the lower 64 bytes, 1: the upper) of this lane, in the low byte.
-__device__ __forceinline__ uint32_t skinny_scale(const uint32_t (&s)[2], int p, int lane) { return s[p] >> (8 * (lane >> 4)); }
-
-// Token rows of 16 bits: x points at the lane's row; the pieces of chunk c.  k of piece p, 16-bit weights: 32 p + 8 q; MXFP4: 128 (p / 4) +
-// 32 q + 8 (p % 4), q = lane >> 4.
-template <class W>
-__device__ __forceinline__ int skinny_k(int p, int lane) {
-    return W::MX ? 128 * (p >> 2) + 32 * (lane >> 4) + 8 * (p & 3) : 32 * p + 8 * (lane >> 4);
-}
-template <class W>
-__device__ __forceinline__ void skinny_tokens(mx_u32x4 (&x)[W::FRAGS], const uint16_t* row, int c, int lane) {
-#pragma unroll
-    for (int p = 0; p < W::FRAGS; ++p) x[p] = *reinterpret_cast<const mx_u32x4*>(row + (int64_t)c * W::K + skinny_k<W>(p, lane));
-}
-// ... zeros behind the row's end (an infinity there would make a NaN of the weights' zeros).  left: values of the row that the chunk has.
-template <class W>
-__device__ __forceinline__ void skinny_tokens_tail(mx_u32x4 (&x)[W::FRAGS], const uint16_t* row, int c, int left, int lane) {
-#pragma unroll
-    for (int p = 0; p < W::FRAGS; ++p) {
-        const int k = skinny_k<W>(p, lane);
-        x[p] = mx_u32x4{0u, 0u, 0u, 0u};
-        if (k < left) x[p] = *reinterpret_cast<const mx_u32x4*>(row + (int64_t)c * W::K + k);
-    }
-}
-
-template <class W>
-__device__ __forceinline__ mx_f32x4 skinny_mfma(mx_u32x4 a, mx_u32x4 b, mx_f32x4 c) {
-    if constexpr (W::F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(sk_f16x8, a), __builtin_bit_cast(sk_f16x8, b), c, 0, 0, 0);
-    else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mx_bf16x8, a), __builtin_bit_cast(mx_bf16x8, b), c, 0, 0, 0);
-}
-// acc[g] += the chunk's weights times 16 token rows of 16 bits; d has been settled.
-template <class W, int G>
-__device__ __forceinline__ void skinny_multiply(mx_f32x4 (&acc)[G], const SkinnyChunk<W, G>& d, const mx_u32x4 (&x)[W::FRAGS], int lane) {
-#pragma unroll
-    for (int p = 0; p < 2 * W::LINES; ++p) {
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-            if constexpr (W::MX) {
-                const float s = mx_scale(skinny_scale(d.s[g], p, lane) & 255u);
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    acc[g] = skinny_mfma<W>(__builtin_bit_cast(mx_u32x4, mx_widen8(d.v[g][p][j], s)), x[4 * p + j], acc[g]);
+                    for (int g = 0; g < G; ++g) {
+                        const uint32_t codes = v[b][g][p][i];
+                        acc[g] = mfma(__builtin_bit_cast(mx_u32x4, mx_widen8(codes, mx_scale(s[g][p]))), x[4 * p + i], acc[g]);
+                    }
             } else {
-                acc[g] = skinny_mfma<W>(d.v[g][p], x[p], acc[g]);
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    // (the upper half, which 4-bit operands do not have, is left open)
+                    const mx_i32x8 av = __builtin_bit_cast(mx_i32x8, __builtin_shufflevector(v[b][g][p], v[b][g][p], 0, 1, 2, 3, -1, -1, -1, -1));
+                    const mx_i32x8 bv = __builtin_bit_cast(mx_i32x8, __builtin_shufflevector(x[p], x[p], 0, 1, 2, 3, -1, -1, -1, -1));
+                    acc[g] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, acc[g], 4 /* e2m1 */, 4, 0, (int)s[g][p], 0, (int)sx[p]);
+                }
             }
         }
     }
-}
-
-// Both operands in MXFP4: the scaled instruction over 128 values; a scale is the low byte of its register.
-__device__ __forceinline__ mx_f32x4 mx_mfma(mx_u32x4 a, uint32_t sa, mx_u32x4 b, uint32_t sb, mx_f32x4 c) {
-    // (the upper half, which 4-bit operands do not have, is left open)
-    const mx_i32x8 av = __builtin_bit_cast(mx_i32x8, __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1));
-    const mx_i32x8 bv = __builtin_bit_cast(mx_i32x8, __builtin_shufflevector(b, b, 0, 1, 2, 3, -1, -1, -1, -1));
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4 /* e2m1 */, 4, 0, (int)sa, 0, (int)sb);
-}
+    // Units 0 .. n - 1: next(u) aims at unit u (u = n: nothing, chunk_end = 0), done(u) follows the last product of unit u.
+    template <class NEXT, class DONE>
+    __device__ __forceinline__ void run(int n, mx_f32x4 (&acc)[G], NEXT next, DONE done) {
+        if (n == 0) return;
+        next(0);
+        scales();
+        fetch(0, 0);
+        fetch(1, 1);
+        for (int u = 0; u < n; ++u) {
+            const int first = chunk0, n_rows = rows;
+            settle_scales();
+            multiply(acc, 0, 0, first, n_rows);
+            fetch(0, 2);
+            multiply(acc, 1, 1, first, n_rows);
+            fetch(1, 3);
+            next(u + 1);
+            scales();
+            multiply(acc, 0, 2, first, n_rows);
+            fetch(0, 0);
+            multiply(acc, 1, 3, first, n_rows);
+            fetch(1, 1);
+            done(u);
+        }
+    }
+};
 
 // Sums of KS wavefronts that shared a contraction, through LDS, in the order of the wavefronts: returns whether this one holds them.
 // red: [KS - 1][G][64] of 16 bytes for each set of columns.  Every wavefront of the workgroup calls it.
