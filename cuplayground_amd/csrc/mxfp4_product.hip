@@ -162,6 +162,11 @@ __global__ __launch_bounds__(256) void mx_small_kernel(MxProduct p) {
     if (i >= p.M * p.N) return;
     const int64_t m = i / p.N;
     const int n = (int)(i - m * p.N);
+    int e = 0;
+    if (p.count) {
+        while (e < p.E && (m < p.offset[e] || m >= (int64_t)p.offset[e] + p.count[e])) ++e;
+        if (e == p.E) return;                     // no expert's row
+    }
     auto value = [&](const void* codes, const uint8_t* scales, int64_t row, int k) {
         const uint32_t c = static_cast<const uint8_t*>(codes)[row * (p.K >> 1) + (k >> 1)] >> (4 * (k & 1));
         return __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c & 15u, mx_scale(scales[row * (p.K >> 5) + (k >> 5)]), 0)[0];
@@ -169,22 +174,24 @@ __global__ __launch_bounds__(256) void mx_small_kernel(MxProduct p) {
     float sum = 0.0f;
     for (int k = 0; k < p.K; ++k) {
         const float a = ROWS4 ? value(p.a, p.a_scales, m, k) : bf16_bits_to_f32(static_cast<const uint16_t*>(p.a)[m * p.K + k]);
-        sum = __builtin_fmaf(a, value(p.w, p.s, n, k), sum);
+        sum = __builtin_fmaf(a, value(p.w, p.s, (int64_t)e * p.N + n, k), sum);
     }
-    if (p.bias) sum += bf16_bits_to_f32(p.bias[n]);
+    if (p.bias) sum += bf16_bits_to_f32(p.bias[(int64_t)e * p.N + n]);
     p.out[i] = (uint16_t)pack2_bf16(p.act == MOE_ACT_GELU ? gelu16(sum) : p.act == MOE_ACT_RELU && sum < 0.0f ? 0.0f : sum, 0.0f);
 }
 
 // ---- more rows: tiles ----
 //
 // RH x CW wavefronts of 16 NT rows x 16 CG columns each, KS sets of them that share the contraction.  Operands go straight into LDS a slab of
-// the contraction at a time, one slab ahead, and are read through buffers that end where they end: rows behind the block's last one,
+// the contraction at a time, AHEAD slabs ahead, and are read through buffers that end where they end: rows behind the block's last one,
 // columns behind the matrix's and what lies behind K are zeros without a branch.  Every slab takes the same path: what is requested behind
 // the last one lies behind the operands' ends, and every set runs as many slabs as the longest (of zeros).  Where paths with and without
 // requests met, every wait would be one for all of them.
-// Every request of this wavefront for the slab has landed and its reads of the other stage are done, then so have everybody's.
+// Every request of this wavefront for the slab has landed -- LATER ones that came behind may be on their way -- and its reads of the stage
+// that is filled next are done, then so have everybody's.
+template <int LATER = 0>
 __device__ __forceinline__ void mx_meet() {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LATER) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
@@ -214,10 +221,11 @@ __device__ __forceinline__ bool mx_join(mx_f32x4 (&acc)[NT][CG], int ks, int sw,
 // -- rows in bf16 --
 // A slab is 128 values: 256 bytes of a token row, 64 of a weight row, of which a lane's 16 are a whole block and, widened, four fragments
 // (skinny.hpp).  Scales go through registers: two stages of a 128 x 128 tile's operands are half of the LDS to the byte.
-template <int RH_, int NT_, int CW_, int CG_, int KS_>
+template <int RH_, int NT_, int CW_, int CG_, int KS_, int AHEAD_ = 1>
 struct MxTile {
     static constexpr bool ROWS4 = false;
-    static constexpr int RH = RH_, NT = NT_, CW = CW_, CG = CG_, KS = KS_;
+    static constexpr int RH = RH_, NT = NT_, CW = CW_, CG = CG_, KS = KS_, AHEAD = AHEAD_;      // AHEAD: slabs that are on their way while one is multiplied
+    static constexpr int STAGES = AHEAD + 1;
     static constexpr int BM = 16 * NT * RH, BN = 16 * CG * CW;
     static constexpr int SET = RH * CW;                        // wavefronts of a set
     static constexpr int THREADS = 64 * SET * KS;
@@ -225,7 +233,7 @@ struct MxTile {
     static constexpr int RB = NT % 4 == 0 ? 4 : NT % 3 == 0 ? 3 : NT;      // groups of 16 rows whose fragments are in registers at once (twice)
     static constexpr int STAGE = BM * 256 + BN * 64;
     static constexpr int SUMS = (KS - 1) * SET * NT * CG * 1024;
-    static constexpr int LDS = 2 * KS * STAGE > SUMS ? 2 * KS * STAGE : SUMS;
+    static constexpr int LDS = STAGES * KS * STAGE > SUMS ? STAGES * KS * STAGE : SUMS;
     static constexpr int BLOCKS = NT * CG >= 32 ? 1 : NT * CG >= 16 ? 2 : 160 * 1024 / LDS;      // workgroups of a compute unit
     static constexpr int WAVES_PER_SIMD = BLOCKS * THREADS / 256 < 4 ? BLOCKS * THREADS / 256 : 4;
     static_assert(SET % 4 == 0 && BM % (4 * SET) == 0 && BN % (16 * SET) == 0, "every wavefront of a set brings as many rows, in steps of 16");
@@ -246,33 +254,49 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void mx_tile_kernel(
     const uint32_t arow = 2 * (uint32_t)K, wrow = (uint32_t)K >> 1, srow = (uint32_t)K >> 5;
 
     // Rows into LDS: an instruction of a wavefront writes 1 KB of LDS in the order of its lanes, so what a slot holds is decided by the
-    // address its lane reads.  The LDS serves a 16-byte read to lanes 0-3, 12-15 and 20-27 in one cycle, to 4-11, 16-19 and 28-31 in the
-    // next: chunk 4 q + j of a row, the one that lane (row, q) reads as its j-th, lies in slot (q + 4 j) ^ row: no two of a cycle meet.
-    const int swapped = (lane & 15) ^ ((4 * sw + q) & 15);
-    const uint32_t chunk = 4 * (swapped & 3) + (swapped >> 2), a_off = (uint32_t)(4 * sw + q) * arow;
-    unsigned char* const stages = smem + ks * 2 * T::STAGE;
-    const int slabs_all = (K + 127) >> 7, slabs = (slabs_all + KS - 1) / KS;       // of a row; set ks takes ks, ks + KS, ...
-    // (a weight row's chunk c lies in slot c ^ w_turn: of rows four apart, which meet the same banks, two take chunk q and two q ^ 1)
-    auto w_turn = [](int row) { return (4 - (row >> 2)) & 3; };
+    // address its lane reads: piece j of segment q (64 bytes, block q) of a row lies in slot 4 (q ^ turn) + (j ^ row) (skinny.hpp, sk_turn).
+    const int arow_of = 4 * sw + q;               // (of 16: all that the permutation depends on)
+    const uint32_t chunk = 4 * ((idx >> 2) ^ sk_turn(arow_of)) + ((idx ^ arow_of) & 3), a_off = (uint32_t)arow_of * arow;
+    unsigned char* const stages = smem + ks * T::STAGES * T::STAGE;
+    const int slabs_all = (K + 127) >> 7, slabs = (slabs_all + KS - 1) / KS, begin = ks * slabs;       // of a row; the set's
+    // (a weight row's block lies in slot q ^ turn, for the same reason)
     const int c0 = t.n0 + 16 * CG * wn;
-    const uint32_t w_chunk = (lane & 3) ^ w_turn(lane >> 2), w_off = (uint32_t)(t.n0 + 16 * sw + (lane >> 2)) * wrow, s_off = (uint32_t)(c0 + idx) * srow + q;
-    const __amdgpu_buffer_rsrc_t a_buf = mx_buffer(t.a, (uint32_t)t.rows * arow), w_buf = mx_buffer(t.w, (uint32_t)N * wrow), s_buf = mx_buffer(t.s, (uint32_t)N * srow);
-    auto issue = [&](int s) {                     // slab number s of this set into stage s & 1
-        unsigned char* const st = stages + (s & 1) * T::STAGE;
-        const uint32_t slab = s * KS + ks, at = slab * 256 + 16 * chunk, w_at = slab * 64 + 16 * w_chunk;
+    const uint32_t w_chunk = (lane & 3) ^ sk_turn(lane >> 2), w_off = (uint32_t)(t.n0 + 16 * sw + (lane >> 2)) * wrow;
+    const __amdgpu_buffer_rsrc_t a_buf = mx_buffer(t.a, (uint32_t)t.rows * arow), w_buf = mx_buffer(t.w, (uint32_t)N * wrow);
+    constexpr int LOADS = T::LOADS_A + T::LOADS_W;
+    auto issue = [&](int s, unsigned char* st, int first, int last) {  // requests [first, last) of slab number s of this set
+        const uint32_t slab = begin + s, at = slab * 256 + 16 * chunk, w_at = slab * 64 + 16 * w_chunk;
         const uint32_t v = at < arow ? a_off + at : kBehind, vw = w_at < wrow ? w_off + w_at : kBehind;
 #pragma unroll
-        for (int i = 0; i < T::LOADS_A; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(a_buf, (mx_lds_void*)(st + (i * T::SET + sw) * 1024), 16, (int)(v + i * T::SET * 4 * arow), 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < T::LOADS_W; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(w_buf, (mx_lds_void*)(st + T::BM * 256 + (i * T::SET + sw) * 1024), 16, (int)(vw + i * T::SET * 16 * wrow), 0, 0, 0);
+        for (int l = first; l < last && l < LOADS; ++l) {
+            const int i = l - T::LOADS_W;
+            if (l < T::LOADS_W)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(w_buf, (mx_lds_void*)(st + T::BM * 256 + (l * T::SET + sw) * 1024), 16, (int)(vw + l * T::SET * 16 * wrow), 0, 0, 0);
+            else
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(a_buf, (mx_lds_void*)(st + (i * T::SET + sw) * 1024), 16, (int)(v + i * T::SET * 4 * arow), 0, 0, 0);
+        }
     };
-    uint32_t ws[CG];
-    auto load_scales = [&](int s) {
-        const uint32_t slab = s * KS + ks, v = slab * 4 + q < srow ? s_off + 4 * slab : kBehind;
+    // Scales, of UNIT slabs at a time: lane LPR r + j has eight bytes, those of slabs 2 j and 2 j + 1, of row r of the wavefront's 16 CG.
+    // (The address unit takes as long over a byte a lane as over sixteen: a fetch of single bytes for every group and slab took as many of
+    // its cycles as half of the operands.)
+    constexpr int LPR = 4 / CG, UNIT = 2 * LPR;
+    const uint32_t s_row = (uint32_t)min(c0 + lane / LPR, N - 1) * srow, s_last = (uint32_t)N * srow - 8;
+    uint64_t raw, held;
+    uint32_t early;                               // bytes that the fetch lies in front of what was wanted
+    auto fetch_scales = [&](int s) {
+        const uint32_t want = s_row + min(4 * (uint32_t)(begin + s) + 8 * (lane % LPR), srow), o = min(want, s_last);
+        early = want - o;
+        __builtin_memcpy(&raw, t.s + o, 8);
+    };
+    float scale[CG];
+    auto settle_scales = [&](int s, int u) {      // of slab s + u, the unit's u-th; behind the row's end: 0
+        const bool in = 4 * (uint32_t)(begin + s + u) + q < srow;
+        const int mine = (int)(uint32_t)(u & 1 ? held >> 32 : held);
 #pragma unroll
-        for (int g = 0; g < CG; ++g) ws[g] = __builtin_amdgcn_raw_buffer_load_b8(s_buf, (int)(v + g * 16 * srow), 0, 0);
+        for (int g = 0; g < CG; ++g) {
+            const uint32_t four = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * ((16 * g + idx) * LPR + u / 2), mine);
+            scale[g] = mx_scale(in ? four >> (8 * q) & 255u : 0u);
+        }
     };
 
     mx_f32x4 acc[NT][CG];
@@ -283,16 +307,15 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void mx_tile_kernel(
 
     // A slab, in blocks of RB groups of rows of a quarter (32 values a lane group): the next block's fragments are read, and the next quarter's
     // weights widened, under the products of the one before.
-    constexpr int NB = NT / RB, SEQ = 4 * NB;
-    float scale[CG];
-    auto slab = [&](const unsigned char* st) {
+    constexpr int NB = NT / RB, SEQ = 4 * NB, STEP = (LOADS + SEQ - 1) / SEQ;
+    auto slab = [&](const unsigned char* st, auto request) {      // request(n): in front of block n
         const unsigned char* base = st + (wm * 16 * NT + idx) * 256;
         mx_u32x4 x[2][RB], w[CG];
         mx_bf16x8 wf[2][CG];
 #pragma unroll
-        for (int g = 0; g < CG; ++g) w[g] = *reinterpret_cast<const mx_u32x4*>(st + T::BM * 256 + (wn * 16 * CG + 16 * g + idx) * 64 + ((q ^ w_turn(idx)) << 4));
+        for (int g = 0; g < CG; ++g) w[g] = *reinterpret_cast<const mx_u32x4*>(st + T::BM * 256 + (wn * 16 * CG + 16 * g + idx) * 64 + ((q ^ sk_turn(idx)) << 4));
         auto read = [&](int n) {
-            const int at = ((q + 4 * (n / NB)) ^ idx) << 4;
+            const int at = (4 * (q ^ sk_turn(idx)) + ((n / NB) ^ (idx & 3))) << 4;
 #pragma unroll
             for (int i = 0; i < RB; ++i) x[n & 1][i] = *reinterpret_cast<const mx_u32x4*>(base + (n % NB * RB + i) * 16 * 256 + at);
         };
@@ -308,6 +331,7 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void mx_tile_kernel(
 #pragma unroll
         for (int n = 0; n < SEQ; ++n) {
             const int quarter = n / NB, ib = n % NB;
+            request(n);
             if (n + 1 < SEQ) read(n + 1);
             if (ib == NB - 1 && quarter < 3) widen(quarter + 1);
 #pragma unroll
@@ -319,21 +343,32 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void mx_tile_kernel(
         }
     };
 
-    issue(0);
+    constexpr int AHEAD = T::AHEAD, REQUESTS = LOADS;
+    auto after = [&](unsigned char* st) { return st + T::STAGE == stages + T::STAGES * T::STAGE ? stages : st + T::STAGE; };
+    unsigned char* now = stages;                  // the stage of the slab that is next; the one in front of it is filled next
+    unsigned char* fill = stages + AHEAD * T::STAGE;
     if (t.rows > wm * 16 * NT) {
-        load_scales(0);
-        for (int s = 0; s < slabs; ++s) {
-            mx_meet();
+        fetch_scales(0);
 #pragma unroll
-            for (int g = 0; g < CG; ++g) scale[g] = mx_scale(ws[g]);
-            issue(s + 1);
-            load_scales(s + 1);
-            slab(stages + (s & 1) * T::STAGE);
+        for (int s = 0; s < AHEAD; ++s) issue(s, stages + s * T::STAGE, 0, LOADS);
+        for (int s = 0; s < slabs; s += UNIT) {
+#pragma unroll
+            for (int u = 0; u < UNIT; ++u) {
+                if (u > 0 && s + u >= slabs) break;
+                mx_meet<(AHEAD - 1) * REQUESTS>();
+                if (u == 0) held = raw >> (4 * early) >> (4 * early);
+                if (u == 0) fetch_scales(s + UNIT);
+                settle_scales(s, u);
+                slab(now, [&](int n) { issue(s + u + AHEAD, fill, STEP * n, STEP * (n + 1)); });
+                now = after(now), fill = after(fill);
+            }
         }
     } else {                                      // no rows for this wavefront: it brings the others theirs
+        for (int s = 0; s < AHEAD; ++s) issue(s, stages + s * T::STAGE, 0, LOADS);
         for (int s = 0; s < slabs; ++s) {
-            mx_meet();
-            issue(s + 1);
+            mx_meet<(AHEAD - 1) * REQUESTS>();
+            issue(s + AHEAD, fill, 0, LOADS);
+            fill = after(fill);
         }
     }
     if (!mx_join<KS, T::SET, NT, CG>(acc, ks, sw, smem, lane)) return;
@@ -533,24 +568,29 @@ hipError_t launch_stream_form(const MxProduct& p, int KS, bool cold, hipStream_t
     return hipGetLastError();
 }
 
+// How a streamer's launch is cut.  About eight wavefronts a compute unit keep the memory busy; more only start pipelines, each of which a
+// chunk or two do not pay for.  14336 x 4096, us, one wavefront a contraction / 2 / 4 / 8: 12.0 / 8.3 / 8.8 / 13.3; 4096 x 14336: 32.5 / 18.4 / 12.0 / 8.8.
+// Two groups of columns a wavefront halve the token rows' reads, where there are columns enough: 65536 x 4096 for 16 rows 48 -> 37.
+struct StreamCut {
+    bool wide;
+    int KS;
+    int64_t waves;
+    int chunks;                 // of a wavefront, whole units
+};
+StreamCut stream_cut(const MxProduct& p) {
+    const int64_t blocks = p.count ? std::min<int64_t>(p.E, p.M) : (p.M + 15) / 16, groups = blocks * ((p.N + 15) / 16);
+    const int chunks = (p.K + 255) / 256;
+    StreamCut c{groups >= 2048, 1, 0, 0};
+    c.waves = c.wide ? (groups + 1) / 2 : groups;
+    while (c.KS < kStreamWaves && 4 * c.KS <= chunks && c.waves * 2 <= 2048) c.KS *= 2, c.waves *= 2;
+    c.chunks = ((chunks + c.KS - 1) / c.KS + kUnit - 1) / kUnit * kUnit;
+    return c;
+}
 template <bool ROWS4>
 hipError_t launch_stream(const MxProduct& p, hipStream_t st) {
-    const int64_t blocks = p.count ? std::min<int64_t>(p.E, p.M) : (p.M + 15) / 16;
-    const int chunks = (p.K + 255) / 256;
-    const int64_t groups = blocks * ((p.N + 15) / 16);         // wavefronts if each had 16 columns and the whole contraction
-#ifdef TUNE
-    static const int t_wide = getenv("T_WIDE") ? atoi(getenv("T_WIDE")) : -1, t_ks = getenv("T_KS") ? atoi(getenv("T_KS")) : -1;
-    const bool wide = t_wide >= 0 ? t_wide : groups >= 4096;
-    int KS = 1;
-    while (KS < 8 && KS * 2 <= chunks && groups / (wide ? 2 : 1) * KS < 4096) KS *= 2;
-    if (t_ks > 0) KS = t_ks;
-#else
-    const bool wide = groups >= 4096;
-    int KS = 1;
-    while (KS < 8 && KS * 2 <= chunks && groups / (wide ? 2 : 1) * KS < 4096) KS *= 2;
-#endif
-    const bool cold = blocks * p.N * p.K / 2 > ((int64_t)256 << 20);
-    return wide ? launch_stream_form<ROWS4, 2>(p, KS, cold, st) : launch_stream_form<ROWS4, 1>(p, KS, cold, st);
+    const StreamCut c = stream_cut(p);
+    const bool cold = (p.count ? std::min<int64_t>(p.E, p.M) : 1) * p.N * p.K / 2 > ((int64_t)256 << 20);      // more than the memory-side cache holds
+    return c.wide ? launch_stream_form<ROWS4, 2>(p, c.KS, cold, st) : launch_stream_form<ROWS4, 1>(p, c.KS, cold, st);
 }
 
 template <bool ROWS4>
@@ -562,22 +602,13 @@ hipError_t launch_small(const MxProduct& p, hipStream_t st) {
 hipError_t launch_product16(const MxProduct& p, int form, hipStream_t st) {
     switch (form) {
         case 0: return launch_stream<false>(p, st);
-        case 1: return launch_tile<MxTile<1, 2, 4, 1, 2>>(p, st);     // 32 x 64
-        case 2: return launch_tile<MxTile<1, 4, 4, 1, 2>>(p, st);     // 64 x 64
-        case 3: return launch_tile<MxTile<1, 8, 4, 2, 1>>(p, st);     // 128 x 128
-#ifdef TUNE
-        case 6: return launch_tile<MxTile<1, 16, 8, 2, 1>>(p, st);
-        case 7: return launch_tile<MxTile<1, 6, 4, 2, 1>>(p, st);
-        case 8: return launch_tile<MxTile<1, 4, 4, 2, 1>>(p, st);
-        case 9: return launch_tile<MxTile<1, 4, 4, 1, 4>>(p, st);
-        case 10: return launch_tile<MxTile<1, 8, 4, 1, 1>>(p, st);
-        case 11: return launch_tile<MxTile<1, 4, 4, 2, 2>>(p, st);
-        case 12: return launch_tile<MxTile<1, 2, 4, 1, 4>>(p, st);
-        case 13: return launch_tile<MxTile<1, 2, 4, 2, 2>>(p, st);
-        case 14: return launch_tile<MxTile<1, 2, 4, 2, 1>>(p, st);
-        case 15: return launch_tile<MxTile<1, 1, 4, 1, 4>>(p, st);
-        case 16: return launch_tile<MxTile<1, 1, 4, 2, 2>>(p, st);
-#endif
+        case 1: return launch_tile<MxTile<1, 1, 4, 1, 2, 4>>(p, st);  // 16 x 64
+        case 2: return launch_tile<MxTile<1, 2, 4, 1, 2, 2>>(p, st);  // 32 x 64
+        case 3: return launch_tile<MxTile<1, 3, 4, 1, 2, 3>>(p, st);  // 48 x 64
+        case 4: return launch_tile<MxTile<1, 4, 4, 1, 2>>(p, st);     // 64 x 64
+        case 5: return launch_tile<MxTile<1, 4, 4, 2, 1>>(p, st);     // 64 x 128
+        case 6: return launch_tile<MxTile<1, 6, 4, 2, 1>>(p, st);     // 96 x 128
+        case 7: return launch_tile<MxTile<1, 8, 4, 2, 1>>(p, st);     // 128 x 128
         default: return launch_tile<MxTile<2, 8, 4, 4, 1>>(p, st);    // 256 x 256
     }
 }
@@ -585,34 +616,56 @@ hipError_t launch_product4(const MxProduct& p, int form, hipStream_t st) {
     switch (form) {
         case 0: return launch_stream<true>(p, st);
         case 1: return launch_tile<MxTile4<1, 1, 2, 1, 4>>(p, st);    // 32 x 64
-        case 2: return launch_tile<MxTile4<1, 2, 2, 1, 2>>(p, st);    // 64 x 64
-        case 3: return launch_tile<MxTile4<2, 2, 2, 2, 1>>(p, st);    // 128 x 128
-#ifdef TUNE
-        case 5: return launch_tile<MxTile4<1, 1, 2, 1, 2>>(p, st);
+        case 2: return launch_tile<MxTile4<1, 1, 2, 1, 2>>(p, st);
+        case 3: return launch_tile<MxTile4<1, 2, 2, 1, 2>>(p, st);    // 64 x 64
+        case 4: return launch_tile<MxTile4<1, 2, 4, 1, 1>>(p, st);    // 64 x 128
+        case 5: return launch_tile<MxTile4<2, 2, 2, 2, 1>>(p, st);    // 128 x 128
         case 6: return launch_tile<MxTile4<2, 2, 4, 2, 1>>(p, st);    // 128 x 256
-        case 7: return launch_tile<MxTile4<2, 1, 2, 2, 1>>(p, st);    // 64 x 128
-        case 8: return launch_tile<MxTile4<1, 2, 4, 1, 1>>(p, st);    // 64 x 128
-        case 9: return launch_tile<MxTile4<1, 2, 2, 1, 4>>(p, st);    // 64 x 64
-        case 11: return launch_tile<MxTile4<1, 2, 4, 1, 2>>(p, st);    // 64 x 128
-#endif
         default: return launch_tile<MxTile4<4, 2, 2, 4, 1>>(p, st);   // 256 x 256
     }
 }
 
+// What a tile costs, in us: a launch of its form; a slab of the contraction where a compute unit has one tile; the same for every further
+// tile of the unit.  Fitted to 1.3 to 800 us of 145 products of 17 to 3000 rows, dense and of experts, each with every form that
+// was near; the choice by these is 4 % (rows in MXFP4: 2 %) behind the best of the forms over them, 16 % (22 %) at worst.
+struct TileCost {
+    int rows, columns;
+    float launch, slab, more;
+};
+constexpr TileCost kTiles16[] = {{}, {16, 64, 3.2f, 0.158f, 0.187f}, {32, 64, 3.0f, 0.208f, 0.241f}, {48, 64, 3.3f, 0.25f, 0.409f}, {64, 64, 3.1f, 0.343f, 0.352f},
+                                 {64, 128, 3.1f, 0.621f, 0.482f}, {96, 128, 2.8f, 0.805f, 0.684f}, {128, 128, 4.4f, 0.822f, 0.836f}, {256, 256, 10.4f, 2.17f, 2.11f}};
+constexpr TileCost kTiles4[] = {{}, {32, 64, 3.9f, 0.193f, 0.501f}, {32, 64, 2.8f, 0.248f, 0.204f}, {64, 64, 2.8f, 0.303f, 0.445f}, {64, 128, 2.3f, 0.567f, 0.61f},
+                                {128, 128, 3.4f, 0.742f, 0.921f}, {128, 256, 5.5f, 0.997f, 1.852f}, {256, 256, 7.8f, 1.41f, 2.781f}};
+
+// The form that should take least; 0: the streamer.  Of experts' rows the host knows how many there are, not whose: about as many each.
 int product_form(const MxProduct& p) {
-    const int64_t rows = p.count ? (p.M + p.E - 1) / p.E : p.M;
-    if (rows <= 16) return 0;
-    if (rows <= 32) return 1;
-    if (rows <= 64) return 2;
-    const int64_t tiles = (p.count ? p.M / 256 + p.E : (p.M + 255) / 256) * ((p.N + 255) / 256);
-    return rows >= 256 && tiles >= 192 ? 4 : 3;
+    const bool rows4 = p.a_scales != nullptr;
+    const int64_t experts = p.count ? std::min<int64_t>(p.E, p.M) : 1;
+    const double each = (double)p.M / experts;
+    // (a chunk of a wavefront, with one or two groups of columns; and what its token rows add)
+    const StreamCut c = stream_cut(p);
+    const double rows = std::min(each, 16.0);
+    double best = 3.8 + (rows4 ? 0.03 : 0.2) * rows + c.chunks * std::max(1.0, c.waves / 2048.0) * ((c.wide ? 1.3 : 0.5) + (rows4 ? 0.003 : 0.017) * rows);
+    if (p.count && each > 16) best = 1e30;               // a row block an expert, at most
+    int form = 0;
+    const int forms = rows4 ? (int)(sizeof kTiles4 / sizeof kTiles4[0]) : (int)(sizeof kTiles16 / sizeof kTiles16[0]);
+    for (int f = 1; f < forms; ++f) {
+        const TileCost& t = rows4 ? kTiles4[f] : kTiles16[f];
+        const double blocks = !p.count ? (double)((p.M + t.rows - 1) / t.rows) : each > 0.75 * t.rows ? (double)p.M / t.rows + 0.5 * experts : (double)experts;
+        const double tiles = std::ceil(blocks * ((p.N + t.columns - 1) / t.columns) / 256.0);      // of the compute unit that has most
+        const int slabs = rows4 ? (p.K + 255) / 256 : (p.K + 127) / 128;
+        const double cost = t.launch + slabs * (t.slab + t.more * (tiles - 1));
+        if (cost < best) best = cost, form = f;
+    }
+    return form;
 }
 
 bool is_small(const MxProduct& p) { return (int64_t)p.N * p.K < 256 || (p.a_scales && p.M * p.K < 256); }      // eight scales are fetched at a time
 int64_t product_workgroups(const MxProduct& p, int form) {
     if (is_small(p)) return (p.M * p.N + 255) / 256;
-    constexpr int BM[] = {16, 32, 64, 128, 256}, BN[] = {16, 64, 64, 128, 256};      // (the streamer's narrowest)
-    return mx_grid(p, BM[form], BN[form]);
+    if (form == 0) return mx_grid(p, 16, 16);               // its narrowest
+    const TileCost& t = p.a_scales ? kTiles4[form] : kTiles16[form];
+    return mx_grid(p, t.rows, t.columns);
 }
 
 }  // namespace

@@ -64,6 +64,12 @@ __host__ __device__ constexpr int skinny_lds(int rows) {
     return 2 * ((rows * W::ROWB + 1023) / 1024) * 1024;
 }
 
+// Where the pieces (16 bytes) of a row's segments (64 bytes) lie in LDS.  A 16-byte read is served to lanes 0-3, 12-15 and 20-27 in a cycle, to
+// 4-11, 16-19 and 28-31 in the next, and so on.  Lane (row, q) reads piece j of segment q: with segment q in place q ^ sk_turn(row), and
+// piece j in place j ^ row of it, those of a cycle meet every bank once.  And the four lanes that fill a place read one segment: of pieces from
+// four segments the address unit makes four requests.
+__device__ __forceinline__ int sk_turn(int row) { return (4 - (row >> 2)) & 3; }
+
 // One wavefront's stream.  aim() says what the next unit is made of; scales(), fetch() and multiply() go through its chunks.
 template <class W, int G, bool COLD>
 struct Skinny {
@@ -156,7 +162,7 @@ struct Skinny {
                 const int r = PER * p + lane / slots;
                 uint32_t piece;                                            // which 16 bytes of the row slot `slot` holds (see fragment)
                 if constexpr (!W::MX) piece = slot ^ (r & 15);
-                else if constexpr (W::ROWB == 512) piece = (slot & 16) + 4 * ((slot ^ r) & 3) + (((slot ^ r) & 15) >> 2);
+                else if constexpr (W::ROWB == 512) piece = (slot & 16) + 4 * (((slot >> 2) & 3) ^ sk_turn(r)) + ((slot ^ r) & 3);
                 else piece = slot ^ ((r >> 1) & 7);
                 const uint32_t at = c * W::ROWB + 16 * piece;
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(x_buf, (sk_lds_void*)(lds + b * half + p * 1024), 16, (int)(at < x_row ? x_off[p] + at : kBehind), 0, 0, 0);
@@ -175,13 +181,12 @@ struct Skinny {
         }
     }
 
-    // Piece p of the lane's token row in part b.  Slots are permuted by the row so that the lanes that the LDS serves in a cycle (0-3, 12-15 and
-    // 20-27; 4-11, 16-19 and 28-31; and so on) meet different banks.  Lanes behind the last row read row 0.
+    // Piece p of the lane's token row in part b.  Slots are permuted by the row (sk_turn).  Lanes behind the last row read row 0.
     __device__ __forceinline__ mx_u32x4 fragment(int b, int p, int rows_of_unit) const {
         const int q = lane >> 4, r = (lane & 15) < rows_of_unit ? lane & 15 : 0;
         int slot;
         if constexpr (!W::MX) slot = (4 * p + q) ^ r;
-        else if constexpr (W::ROWB == 512) slot = 16 * (p >> 2) + ((q + 4 * (p & 3)) ^ r);
+        else if constexpr (W::ROWB == 512) slot = 16 * (p >> 2) + 4 * (q ^ sk_turn(r)) + ((p ^ r) & 3);
         else slot = (4 * p + q) ^ ((r >> 1) & 7);
         return *reinterpret_cast<const mx_u32x4*>(lds + b * half + r * W::ROWB + 16 * slot);
     }

@@ -124,6 +124,19 @@ def test_product_large(M, N, K, rows4):
 
 
 @pytest.mark.parametrize("rows4", [False, True])
+@pytest.mark.parametrize("M,N,K", [
+    (34, 8587, 32), (94, 8045, 448), (409, 6995, 160), (726, 6321, 352), (328, 8325, 544), (1358, 8901, 672), (227, 8262, 576), (584, 6660, 1056),
+    (1154, 6865, 800), (1, 33001, 1056), (13, 33010, 1056), (2, 323, 4128), (14, 186, 3936), (491, 222, 4032), (1, 3, 4032), (982, 150, 1312)])
+def test_product_at_odd_sizes_of_every_kernel(M, N, K, rows4):
+    """The sizes reach every tile and cut of the streamer, and end inside their rows, columns and slabs."""
+    g = _gen(M + N + K)
+    a, sa, av = _rows(g, M, K, rows4)
+    w, s, wv = _held(g, N, K)
+    bias = torch.randn(N, generator=g, device=DEV).bfloat16()
+    plain.product_close(moe.gemm_mxfp4(a, w, s, bias, act=api.ACT_GELU, a_scales=sa), av, wv, bias.double(), 1)
+
+
+@pytest.mark.parametrize("rows4", [False, True])
 @pytest.mark.parametrize("M", [5, 40, 200])
 def test_product_keeps_what_is_not_finite_where_it_is(M, rows4):
     """A row that holds a NaN or an infinity, a column whose scale is NaN: no other row or column sees them, at the end of a cut-off row
@@ -185,6 +198,30 @@ def test_expert_product(counts, N, K, rows4):
         if n:
             plain.product_close(out[at:at + n], av[at:at + n], wv[e], bias[e].double(), 1)
         at += n
+
+
+@pytest.mark.parametrize("rows4", [False, True])
+@pytest.mark.parametrize("A,E,N,K", [(1, 3, 1088, 64), (3, 3, 64, 64), (34, 30, 2240, 960), (726, 30, 448, 320), (422, 8, 1536, 256), (733, 30, 2176, 64),
+                                     (2132, 8, 1920, 384), (2253, 30, 832, 704), (1470, 30, 1920, 1088), (1987, 8, 1600, 640), (2428, 8, 2496, 1024)])
+def test_expert_product_of_every_kernel(A, E, N, K, rows4):
+    """As above, with as many rows an expert as chance gives it; behind a gap in front of the last expert's."""
+    g = _gen(A + N + K)
+    layer = _layer(A, 1, E, N, K)
+    a, sa, av = _rows(g, A, K, rows4)
+    w, s, wv = _held(g, E, N, K)
+    of = torch.randint(0, E + 1, (A,), generator=g, device=DEV)              # E: nobody's, the gap
+    count = torch.bincount(of, minlength=E + 1).to(torch.int32)
+    gap, count = int(count[E]), count[:E].contiguous()
+    offset = (torch.cumsum(count, 0) - count).to(torch.int32)
+    offset[E - 1] += gap
+    out = torch.full((A, N), 7.0, dtype=torch.bfloat16, device=DEV)
+    layer.expert_gemm_mxfp4(a, w, s, None, count, offset, act=api.ACT_NONE, a_scales=sa, out=out)
+    left = torch.ones(A, dtype=torch.bool, device=DEV)
+    for e, (at, n) in enumerate(zip(offset.tolist(), count.tolist())):
+        if n:
+            plain.product_close(out[at:at + n], av[at:at + n], wv[e])
+        left[at:at + n] = False
+    assert bool((out[left] == 7.0).all())
 
 
 def test_products_are_the_same_every_time_on_any_stream_and_in_a_graph():
