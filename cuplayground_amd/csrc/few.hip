@@ -19,6 +19,7 @@ namespace {
 
 constexpr int kFewThreads = 512, kFewWaves = 8;
 constexpr int kFewPairs = kFewTokens * kMaxTopK;
+static_assert(kFewPairs <= 256, "packed rows in a byte");
 
 // What every workgroup knows of the routing.
 struct FewPlan {
@@ -29,7 +30,8 @@ struct FewPlan {
     int16_t list[kFewPairs];           // experts that are hit, ascending
     float row_w[kFewPairs];            // gate weight of a packed row
     uint8_t row_t[kFewPairs];          // its token
-    int32_t hit, kept;
+    int32_t part[3][kFewWaves];        // of 64 experts each: rows, experts that are hit, rows of the one that has most
+    int32_t hit, kept, most;           // experts that are hit, rows, rows of the expert that has most
 };
 
 template <class ET>
@@ -54,15 +56,37 @@ __device__ __forceinline__ void few_logits(const uint16_t* __restrict__ x, const
     float p[TT];
 #pragma unroll
     for (int t = 0; t < TT; ++t) p[t] = 0.0f;
-    for (int k = 8 * lane; k < H; k += 512) {
-        union { mx_u32x4 v; uint16_t s[8]; } gv, xv;
-        gv.v = *reinterpret_cast<const mx_u32x4*>(g + (int64_t)e * H + k);
+    union Eight { mx_u32x4 v; uint16_t s[8]; };
+    auto load = [&](const uint16_t* row, int k) {
+        Eight r;
+        r.v = *reinterpret_cast<const mx_u32x4*>(row + k);
+        return r;
+    };
+    auto add = [&](const Eight& xv, const Eight& gv, float& sum) {
 #pragma unroll
-        for (int t = 0; t < TT; ++t) {
-            xv.v = *reinterpret_cast<const mx_u32x4*>(x + (int64_t)(t0 + min(t, n - 1)) * H + k);
+        for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(few_widen<ET>(xv.s[i]), few_widen<ET>(gv.s[i]), sum);
+    };
+    const uint16_t* const ge = g + (int64_t)e * H;
+    int k = 8 * lane;
+    constexpr int U = 4;                       // steps that are fetched together: one trip to memory for them
+    for (int k0 = 0; k0 + 512 * U <= H; k0 += 512 * U, k += 512 * U) {
+        Eight gv[U], xv[U][TT];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) p[t] = __builtin_fmaf(few_widen<ET>(xv.s[i]), few_widen<ET>(gv.s[i]), p[t]);
+        for (int u = 0; u < U; ++u) {
+            gv[u] = load(ge, k + 512 * u);
+#pragma unroll
+            for (int t = 0; t < TT; ++t) xv[u][t] = load(x + (int64_t)(t0 + min(t, n - 1)) * H, k + 512 * u);
         }
+        __builtin_amdgcn_sched_barrier(0);     // (or each would move to its use, and be waited for by itself)
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int t = 0; t < TT; ++t) add(xv[u][t], gv[u], p[t]);
+    }
+    for (; k < H; k += 512) {
+        const Eight gv = load(ge, k);
+#pragma unroll
+        for (int t = 0; t < TT; ++t) add(load(x + (int64_t)(t0 + min(t, n - 1)) * H, k), gv, p[t]);
     }
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
@@ -87,35 +111,38 @@ __global__ __launch_bounds__(256) void few_logits_kernel(FewArgs a) {
 // From the selection in p.w / p.idx (behind a barrier): masks, packed rows, the list.  Called by the whole workgroup.
 __device__ __forceinline__ void few_plan(FewPlan& p, const FewArgs& a) {
     const int tid = threadIdx.x, lane = tid & 63, P = a.S * a.k;
-    for (int e = tid; e < a.E; e += blockDim.x) p.mask[e] = 0;
+    if (tid < a.E) p.mask[tid] = 0;
     __syncthreads();
     if (tid < P && (unsigned)p.idx[tid] < (unsigned)a.E) atomicOr(&p.mask[p.idx[tid]], 1u << (tid / a.k));     // a token names an expert once
     __syncthreads();
-    if (tid < kWave) {
-        int hit = 0, rows = 0;
-        for (int c = 0; c < a.E; c += kWave) {
-            const int e = c + lane;
-            uint32_t m = e < a.E ? p.mask[e] : 0u;
-            if (a.drop)                                        // the first `capacity` tokens stay
-                while (__popc(m) > a.capacity) m &= ~(1u << (31 - __clz(m)));
-            const int n = __popc(m);
-            int inc = n;
+    static_assert(kMaxExperts <= kWave * kFewWaves, "64 experts a wavefront");
+    const int wave = tid >> 6, e = tid;
+    uint32_t m = e < a.E ? p.mask[e] : 0u;
+    if (a.drop)                                        // the first `capacity` tokens stay
+        while (__popc(m) > a.capacity) m &= ~(1u << (31 - __clz(m)));
+    const int n = __popc(m);
+    int inc = n, most = n;
 #pragma unroll
-            for (int off = 1; off < kWave; off <<= 1) {
-                const int o = __shfl_up(inc, off, kWave);
-                if (lane >= off) inc += o;
-            }
-            const unsigned long long any = __ballot(n > 0);
-            if (e < a.E) {
-                p.mask[e] = m;
-                p.base[e] = (int16_t)(rows + inc - n);
-            }
-            if (n > 0) p.list[hit + __popcll(any & ((1ull << lane) - 1ull))] = (int16_t)e;
-            hit += __popcll(any);
-            rows += __shfl(inc, kWave - 1, kWave);
-        }
-        if (lane == 0) p.hit = hit, p.kept = rows;
+    for (int off = 1; off < kWave; off <<= 1) {
+        const int o = __shfl_up(inc, off, kWave);
+        if (lane >= off) inc += o;
+        most = max(most, __shfl_xor(most, off, kWave));
     }
+    const unsigned long long any = __ballot(n > 0);
+    if (lane == kWave - 1) p.part[0][wave] = inc, p.part[1][wave] = __popcll(any), p.part[2][wave] = most;
+    __syncthreads();
+    int rows = 0, hit = 0, all_rows = 0, all_hit = 0, all_most = 0;
+#pragma unroll
+    for (int w = 0; w < kFewWaves; ++w) {
+        if (w < wave) rows += p.part[0][w], hit += p.part[1][w];
+        all_rows += p.part[0][w], all_hit += p.part[1][w], all_most = max(all_most, p.part[2][w]);
+    }
+    if (e < a.E) {
+        p.mask[e] = m;
+        p.base[e] = (int16_t)(rows + inc - n);
+    }
+    if (n > 0) p.list[hit + __popcll(any & ((1ull << lane) - 1ull))] = (int16_t)e;
+    if (tid == 0) p.hit = all_hit, p.kept = all_rows, p.most = all_most;
     __syncthreads();
     if (tid < P) {
         const int e = p.idx[tid], t = tid / a.k;
@@ -153,17 +180,21 @@ __device__ __forceinline__ void few_report(const FewPlan& p, const FewArgs& a) {
 
 // The up (and gate) projection: a task is 16 columns of both matrices of an expert, or 32 of the one, over the whole of H, by KS wavefronts.
 // With KS = 1 a wavefront goes from task to task without a pause: the next one's weights are requested under the last ones' products.
+//
+// Of LDS a wavefront has kRowLds for token rows, so that two workgroups have room on a compute unit; where an expert has more rows than that,
+// half of the wavefronts work, with the others' room.  (With KS > 1, where there is little to do, as much as S rows may take.)
+constexpr int kRowLds = 8192;
 template <class W, class ET, bool GATED, bool COLD>
-__global__ __launch_bounds__(kFewThreads, 2) void few_up_kernel(FewArgs a, int KS) {
+__global__ __launch_bounds__(kFewThreads, 4) void few_up_kernel(FewArgs a, int KS) {
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ FewPlan plan;
-    __shared__ mx_f32x4 red[(kFewWaves - 1) * 2 * 64];           // first the logits of a small router
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const float* logits = a.logits;
     if (a.fold) {
-        float* own = reinterpret_cast<float*>(red);
+        float* own = reinterpret_cast<float*>(smem);
         for (int e = wave; e < a.E; e += kFewWaves)
-            for (int t0 = 0; t0 < a.S; t0 += kLogitTokens)
+            if (a.S == 1) few_logits<ET, 1>((const uint16_t*)a.x, (const uint16_t*)a.gate_w, a.gate_bias, e, 0, 1, a.H, own + e, a.E, lane);
+            else for (int t0 = 0; t0 < a.S; t0 += kLogitTokens)
                 few_logits<ET, kLogitTokens>((const uint16_t*)a.x, (const uint16_t*)a.gate_w, a.gate_bias, e, t0, min(kLogitTokens, a.S - t0), a.H, own + e, a.E, lane);
         logits = own;
         __syncthreads();
@@ -180,16 +211,19 @@ __global__ __launch_bounds__(kFewThreads, 2) void few_up_kernel(FewArgs a, int K
     constexpr int G = 2, COLS = GATED ? 16 : 32;
     const int H = a.H, I = a.I, chunks = (H + W::K - 1) / W::K;
     const int ncol = I / COLS, tasks = plan.hit * ncol;
-    const int ks = wave % KS, first = blockIdx.x * (kFewWaves / KS) + wave / KS, stride = gridDim.x * (kFewWaves / KS);
+    const bool half = KS == 1 && skinny_lds<W>(plan.most) > kRowLds;
+    const int waves = half ? kFewWaves / 2 : kFewWaves;
+    const int ks = wave % KS, first = blockIdx.x * (waves / KS) + wave / KS, stride = gridDim.x * (waves / KS);
     const int share = (chunks + KS - 1) / KS, begin = min(ks * share, chunks), end = min(begin + share, chunks);      // chunks of a task that are this wavefront's
     const int units = (end - begin + kUnit - 1) / kUnit;
     const int idx = lane & 15, q = lane >> 4;
     const int64_t mat = W::row_bytes((int64_t)H * I), smat = (int64_t)I * (H >> 5);
 
     // (with KS > 1 the launch has a set of wavefronts for every task there can be)
-    const int mytasks = first < tasks ? (KS > 1 ? 1 : (tasks - 1 - first) / stride + 1) : 0;
+    const int mytasks = wave < waves && first < tasks ? (KS > 1 ? 1 : (tasks - 1 - first) / stride + 1) : 0;
     Skinny<W, G, COLD> st;
-    st.init(smem + wave * skinny_lds<W>(a.S), a.S, H);
+    const int lds = half ? 2 * kRowLds : KS == 1 ? min(skinny_lds<W>(a.S), kRowLds) : skinny_lds<W>(a.S);
+    st.init(smem + wave * lds, plan.most, H);
     st.x_buf = mx_buffer(a.x, (uint32_t)a.S * st.x_row);
     int task = first, unit = 0;          // the next unit to be fetched
     auto next = [&](int u) {
@@ -206,7 +240,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void few_up_kernel(FewArgs a, int K
                 if constexpr (W::MX) st.s_at[g] = (GATED && g ? a.s_gate : a.s_up) + e * smat;
             }
             st.aim_weights(n0, I, GATED ? 0 : 16);
-            st.aim_tokens(__builtin_amdgcn_readfirstlane(__popc(plan.mask[e])), [&](int r) { return (uint32_t)plan.row_t[base + r] * st.x_row; });
+            st.aim_tokens(__builtin_amdgcn_readfirstlane(__popc(plan.mask[e])), [&](int r) { return plan.row_t[base + r]; });
         }
         st.chunk0 = begin + kUnit * unit;
         st.chunk_end = end;
@@ -255,14 +289,18 @@ __global__ __launch_bounds__(kFewThreads, 2) void few_up_kernel(FewArgs a, int K
         done_unit = 0, done_task += stride;
     });
     if (KS > 1) {
-        const bool holds = skinny_join<G>(acc, ks, KS, red + wave / KS * (KS - 1) * G * 64, lane);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");           // the rows' place is the sums' now
+        __syncthreads();
+        const bool holds = skinny_join<G>(acc, ks, KS, reinterpret_cast<mx_f32x4*>(smem) + wave / KS * (KS - 1) * G * 64, lane);
         if (holds && mytasks) store(first);
     }
 }
 
-// The down projection and the combine: a workgroup owns 16 G columns of out; its wavefronts share the (expert, unit of I) pairs.
-template <class W, class ET, int G, bool COLD>
-__global__ __launch_bounds__(kFewThreads, 2) void few_down_kernel(FewArgs a) {
+// The down projection and the combine: a workgroup owns 16 columns of out; its wavefronts share the (expert, chunk of I) pairs, as many
+// each.  LDS as for the up projection: 7168 columns, 448 workgroups, are one round instead of two.
+template <class W, class ET, bool COLD>
+__global__ __launch_bounds__(kFewThreads, 4) void few_down_kernel(FewArgs a) {
+    constexpr int G = 1;
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ FewPlan plan;
     __shared__ mx_f32x4 red[(kFewWaves - 1) * G * 64];
@@ -274,50 +312,56 @@ __global__ __launch_bounds__(kFewThreads, 2) void few_down_kernel(FewArgs a) {
     __syncthreads();
     few_plan(plan, a);
 
-    const int H = a.H, I = a.I, chunks = (I + W::K - 1) / W::K, units = (chunks + kUnit - 1) / kUnit;      // of an expert
+    const int H = a.H, I = a.I, chunks = (I + W::K - 1) / W::K;      // of an expert
     const int n0 = blockIdx.x * 16 * G;
     const int idx = lane & 15, q = lane >> 4;
     const int64_t mat = W::row_bytes((int64_t)H * I), smat = (int64_t)H * (I >> 5);
-    const int all = plan.hit * units;
-    const int begin = (int)((int64_t)all * wave / kFewWaves), end = (int)((int64_t)all * (wave + 1) / kFewWaves);
+    const bool half = skinny_lds<W>(plan.most) > kRowLds;
+    const int waves = half ? kFewWaves / 2 : kFewWaves, all = plan.hit * chunks;
+    const int begin = (int)((int64_t)all * min(wave, waves) / waves), end = (int)((int64_t)all * min(wave + 1, waves) / waves);
+    int j = begin / chunks, c = begin - j * chunks, next_j = j, next_c = c;
+    // units: of the first expert's rest, of whole experts, of the last one's part
+    const int head = min(end - begin, chunks - c), rest = end - begin - head;
+    auto units_of = [](int n) { return (n + kUnit - 1) / kUnit; };
+    const int units = units_of(head) + rest / chunks * units_of(chunks) + units_of(rest % chunks);
     Skinny<W, G, COLD> st;
-    st.init(smem + wave * skinny_lds<W>(a.S), a.S, I);
+    const int own = half ? 2 * kRowLds : min(skinny_lds<W>(a.S), kRowLds);
+    st.init(smem + wave * own, plan.most, I);
     st.x_buf = mx_buffer(a.h, (uint32_t)plan.kept * st.x_row);
     st.aim_weights(n0, H, 16);
-    int j = begin / units, unit = begin - j * units;
     bool aimed = false;
     auto next = [&](int u) {
-        if (u == end - begin) {
+        if (u == units) {
             st.chunk_end = 0;
             return;
         }
-        if (!aimed || unit == 0) {
-            const int e = __builtin_amdgcn_readfirstlane(plan.list[j]), base = __builtin_amdgcn_readfirstlane(plan.base[e]);
+        if (!aimed || next_c == 0) {
+            const int e = __builtin_amdgcn_readfirstlane(plan.list[next_j]), base = __builtin_amdgcn_readfirstlane(plan.base[e]);
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 st.w_buf[g] = mx_buffer(static_cast<const char*>(a.w_down) + e * mat, (uint32_t)mat);
                 if constexpr (W::MX) st.s_at[g] = a.s_down + e * smat;
             }
-            st.aim_tokens(__builtin_amdgcn_readfirstlane(__popc(plan.mask[e])), [&](int r) { return (uint32_t)(base + r) * st.x_row; });
+            st.aim_tokens(__builtin_amdgcn_readfirstlane(__popc(plan.mask[e])), [&](int r) { return base + r; });
             aimed = true;
         }
-        st.chunk0 = kUnit * unit;
-        st.chunk_end = chunks;
-        if (++unit == units) unit = 0, ++j;
+        st.chunk0 = next_c;
+        st.chunk_end = min(chunks, end - next_j * chunks);
+        next_c += kUnit;
+        if (next_c >= chunks) next_c = 0, ++next_j;
     };
     mx_f32x4 out[1][G] = {}, acc[G] = {};
-    int done_j = j, done_unit = unit, left = end - begin;
-    bool whole = unit == 0;              // the expert's first unit is among them
-    st.run(left, acc, next, [&](int) {
-        --left;
-        if (++done_unit < units && left > 0) return;
+    bool whole = c == 0;                 // the expert's first chunk is among them
+    st.run(units, acc, next, [&](int) {
+        c += kUnit;
+        if (c < min(chunks, end - j * chunks)) return;
         // the columns are the expert's rows in order: lane (row, q) hands its sums to the lane of the row's token
-        const int e = __builtin_amdgcn_readfirstlane(plan.list[done_j]);
+        const int e = __builtin_amdgcn_readfirstlane(plan.list[j]);
         const uint32_t m = plan.mask[e];
         const bool in = (m >> idx) & 1u;
         const int r = __popc(m & ((1u << idx) - 1u)), from = 4 * ((lane & 48) + (in ? r : 0));
         const float w = in ? plan.row_w[plan.base[e] + r] : 0.0f;
-        const uint16_t* bd = a.b_down && whole ? (const uint16_t*)a.b_down + (int64_t)e * H + n0 + 4 * q : nullptr;      // the bias goes with the first unit
+        const uint16_t* bd = a.b_down && whole ? (const uint16_t*)a.b_down + (int64_t)e * H + n0 + 4 * q : nullptr;      // the bias goes with the first chunk
 #pragma unroll
         for (int g = 0; g < G; ++g)
 #pragma unroll
@@ -328,7 +372,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void few_down_kernel(FewArgs a) {
             }
 #pragma unroll
         for (int g = 0; g < G; ++g) acc[g] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
-        done_unit = 0, ++done_j, whole = true;
+        c = 0, ++j, whole = true;
     });
     if (!skinny_join<G>(out[0], wave, kFewWaves, red, lane) || idx >= a.S) return;
 #pragma unroll
@@ -343,26 +387,28 @@ template <class W, class ET, bool COLD>
 hipError_t launch_few_form(const FewArgs& a, hipStream_t st) {
     const bool gated = a.w_gate != nullptr;
     const int64_t most = std::min<int64_t>(a.E, (int64_t)a.S * a.k) * (a.I / (gated ? 16 : 32));      // tasks there can be
-    const int chunks = (a.H + W::K - 1) / W::K, lds = kFewWaves * skinny_lds<W>(a.S);
+    const int chunks = (a.H + W::K - 1) / W::K, lds = skinny_lds<W>(a.S);
     static const hipError_t ready = [] {
-        constexpr int bytes = kFewWaves * skinny_lds<W>(kFewTokens);
-        for (const void* f : {reinterpret_cast<const void*>(few_up_kernel<W, ET, true, COLD>), reinterpret_cast<const void*>(few_up_kernel<W, ET, false, COLD>),
-                              reinterpret_cast<const void*>(few_down_kernel<W, ET, 1, COLD>)}) {
-            const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        constexpr int up = kFewWaves * skinny_lds<W>(kFewTokens);
+        const void* const ups[] = {reinterpret_cast<const void*>(few_up_kernel<W, ET, true, COLD>), reinterpret_cast<const void*>(few_up_kernel<W, ET, false, COLD>)};
+        for (const void* f : ups) {
+            const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, up);
             if (e != hipSuccess) return e;
         }
-        return hipSuccess;
+        return hipFuncSetAttribute(reinterpret_cast<const void*>(few_down_kernel<W, ET, COLD>), hipFuncAttributeMaxDynamicSharedMemorySize, kFewWaves * kRowLds);
     }();
     if (ready != hipSuccess) return ready;
     int KS = 1;
     while (KS < kFewWaves && 2 * KS * kUnit <= chunks && most * KS < 1024) KS *= 2;
     const int64_t sets = (most + kFewWaves / KS - 1) / (kFewWaves / KS);
+    // (as many workgroups as there is room for at once: every one of them makes the plan)
     const unsigned grid = (unsigned)(KS > 1 ? sets : std::min<int64_t>(sets, 512));
-    if (gated) few_up_kernel<W, ET, true, COLD><<<grid, kFewThreads, lds, st>>>(a, KS);
-    else few_up_kernel<W, ET, false, COLD><<<grid, kFewThreads, lds, st>>>(a, KS);
+    const int up_lds = kFewWaves * (KS > 1 ? lds : std::min(lds, kRowLds));
+    if (gated) few_up_kernel<W, ET, true, COLD><<<grid, kFewThreads, up_lds, st>>>(a, KS);
+    else few_up_kernel<W, ET, false, COLD><<<grid, kFewThreads, up_lds, st>>>(a, KS);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    few_down_kernel<W, ET, 1, COLD><<<a.H / 16, kFewThreads, lds, st>>>(a);
+    few_down_kernel<W, ET, COLD><<<a.H / 16, kFewThreads, kFewWaves * std::min(lds, kRowLds), st>>>(a);
     return hipGetLastError();
 }
 template <class W, class ET>
@@ -375,7 +421,7 @@ hipError_t launch_few_weights(const FewArgs& a, hipStream_t st) {
 }  // namespace
 
 hipError_t launch_few(FewArgs a, bool f16, bool mxfp4, hipStream_t st) {
-    a.fold = (int64_t)a.S * a.E * a.H <= kFoldProducts && a.S * a.E <= (kFewWaves - 1) * 2 * 64 * 4;
+    a.fold = (int64_t)a.S * a.E * a.H <= kFoldProducts && a.S * a.E * (int)sizeof(float) <= kFewWaves * 2048;       // (the least LDS that the rows have)
     if (!a.fold) {
         const int waves = a.E * ((a.S + kLogitTokens - 1) / kLogitTokens);
         if (f16) few_logits_kernel<f16_s><<<(waves + 3) / 4, 256, 0, st>>>(a);

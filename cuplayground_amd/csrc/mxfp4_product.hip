@@ -140,7 +140,7 @@ __global__ __launch_bounds__(64 * kStreamWaves) void mx_stream_kernel(MxProduct 
     }
     st.x_buf = mx_buffer(t.a, (uint32_t)t.rows * st.x_row);
     st.aim_weights(n0, p.N, 16);
-    st.aim_tokens(t.rows, [&](int r) { return (uint32_t)r * st.x_row; });
+    st.aim_tokens(t.rows, [](int r) { return r; });
     if constexpr (ROWS4) {
         st.sx_at = p.a_scales;                    // (the whole array: the eight bytes at the end of a block's may lie behind it)
         st.sx_base = t.row0 * (K >> 5);

@@ -89,7 +89,8 @@ struct Skinny {
     const uint8_t* sx_at;
     uint32_t s_last;                                       // the last eight bytes of the matrix's scales
     int64_t sx_base, sx_end;                               // the token rows' scales: where row 0 begins, the array's last eight bytes
-    uint32_t w1, w2, w_add, s_row[G], x_off[MOST], sx_row, row, x_row;
+    uint32_t w1, w2, w_add, s_row[G], sx_row, row, x_row;
+    uint32_t x_of[(MOST + 3) / 4];                         // the lane's token rows' places in x_buf, a byte each
     int rows, chunk0, chunk_end;                           // token rows, chunks [chunk0, chunk_end) of the unit
     int lane;
     unsigned char* lds;
@@ -114,13 +115,15 @@ struct Skinny {
             for (int g = 0; g < G; ++g) s_row[g] = (uint32_t)min(n0 + step * g + (lane >> 2), N - 1) * sr;
         }
     }
-    // Token rows: of(r) is where row r begins in x_buf.
+    // Token rows: row r is row of(r) of x_buf.
     template <class OF>
     __device__ __forceinline__ void aim_tokens(int n, OF of) {
         rows = n;
 #pragma unroll
-        for (int p = 0; p < MOST; ++p)
-            if (PER * p < n) x_off[p] = of(min(PER * p + lane / (64 / PER), n - 1));
+        for (int p = 0; p < MOST; ++p) {
+            if (p % 4 == 0) x_of[p / 4] = 0;
+            if (PER * p < n) x_of[p / 4] |= (uint32_t)of(min(PER * p + lane / (64 / PER), n - 1)) << (8 * (p & 3));
+        }
     }
 
     // Eight bytes of scales: inside the array, which has eight.
@@ -165,7 +168,7 @@ struct Skinny {
                 else if constexpr (W::ROWB == 512) piece = (slot & 16) + 4 * (((slot >> 2) & 3) ^ sk_turn(r)) + ((slot ^ r) & 3);
                 else piece = slot ^ ((r >> 1) & 7);
                 const uint32_t at = c * W::ROWB + 16 * piece;
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(x_buf, (sk_lds_void*)(lds + b * half + p * 1024), 16, (int)(at < x_row ? x_off[p] + at : kBehind), 0, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(x_buf, (sk_lds_void*)(lds + b * half + p * 1024), 16, (int)(at < x_row ? (x_of[p / 4] >> (8 * (p & 3)) & 255u) * x_row + at : kBehind), 0, 0, 0);
             }
         }
         const uint32_t piece = (lane >> 4) + ((lane & 8) >> 1);

@@ -6,42 +6,26 @@
 
 namespace moe355 {
 
-struct Cand {
-    float v;
-    int i;
-};
-__device__ __forceinline__ bool better(const Cand& a, const Cand& b) {
-    return a.v > b.v || (a.v == b.v && a.i < b.i);
+// Logits as integers in their order: a NaN ranks as -inf (and 0 behind that is no logit's), -0 as 0.
+__device__ __forceinline__ uint32_t rank_key(float v) {
+    const uint32_t u = __float_as_uint(v != v ? -INFINITY : v + 0.0f);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-
-// The best candidate of the 64 lanes, in every lane.  `better` is a total order, so the result does not depend on the
-// order of the comparisons: lanes exchange through the cross-lane data paths of the ALU (within quads, then mirrored
-// within 8 and 16 lanes), which cost a few cycles each where a shuffle through the LDS crossbar costs a round trip,
-// and the four rows meet through scalar registers.
+// The largest of the 64 lanes' keys: lanes exchange through the cross-lane data paths of the ALU (within quads, then mirrored within 8
+// and 16 lanes), which cost a few cycles each where a shuffle through the LDS crossbar costs a round trip, and the four rows meet
+// through scalar registers.
 template <int CTRL>
-__device__ __forceinline__ Cand dpp_cand(const Cand& c) {
-    Cand o;
-    o.v = __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(c.v), CTRL, 0xF, 0xF, false));
-    o.i = __builtin_amdgcn_update_dpp(0, c.i, CTRL, 0xF, 0xF, false);
-    return o;
+__device__ __forceinline__ uint32_t dpp_max(uint32_t k) {
+    return max(k, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)k, CTRL, 0xF, 0xF, false));
 }
-__device__ __forceinline__ Cand wave_best(Cand c) {
-    Cand o = dpp_cand<0xB1>(c);            // quad_perm [1,0,3,2]: lane ^ 1
-    if (better(o, c)) c = o;
-    o = dpp_cand<0x4E>(c);                 // quad_perm [2,3,0,1]: lane ^ 2
-    if (better(o, c)) c = o;
-    o = dpp_cand<0x141>(c);                // row_half_mirror: i <-> 7 - i within 8 lanes
-    if (better(o, c)) c = o;
-    o = dpp_cand<0x140>(c);                // row_mirror: i <-> 15 - i within 16 lanes
-    if (better(o, c)) c = o;
-    Cand best{__int_as_float(__builtin_amdgcn_readlane(__float_as_int(c.v), 0)), __builtin_amdgcn_readlane(c.i, 0)};
-#pragma unroll
-    for (int row = 1; row < 4; ++row) {
-        const Cand r{__int_as_float(__builtin_amdgcn_readlane(__float_as_int(c.v), 16 * row)),
-                     __builtin_amdgcn_readlane(c.i, 16 * row)};
-        if (better(r, best)) best = r;
-    }
-    return best;
+__device__ __forceinline__ uint32_t wave_max(uint32_t k) {
+    k = dpp_max<0xB1>(k);             // quad_perm [1,0,3,2]: lane ^ 1
+    k = dpp_max<0x4E>(k);             // quad_perm [2,3,0,1]: lane ^ 2
+    k = dpp_max<0x141>(k);            // row_half_mirror: i <-> 7 - i within 8 lanes
+    k = dpp_max<0x140>(k);            // row_mirror: i <-> 15 - i within 16 lanes
+    const uint32_t a = max((uint32_t)__builtin_amdgcn_readlane((int)k, 0), (uint32_t)__builtin_amdgcn_readlane((int)k, 16));
+    const uint32_t b = max((uint32_t)__builtin_amdgcn_readlane((int)k, 32), (uint32_t)__builtin_amdgcn_readlane((int)k, 48));
+    return max(a, b);
 }
 
 // `row`: the E logits of token t (global memory, or LDS when the logits kernel selects right behind its sums).
@@ -56,40 +40,44 @@ __device__ __forceinline__ void topk_one_token(const float* __restrict__ row, in
                                                int lane) {
     static_assert(J >= 1 && J <= kMaxExperts / kWave, "slots per lane");
     float v[J];
-    unsigned avail = 0;
+    uint32_t key[J];                  // 0: no expert, or taken
+    unsigned valid = 0;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
         const int e = j * kWave + lane;
         v[j] = 0.0f;
+        key[j] = 0;
         if (e < E) {
             v[j] = row[e];
-            avail |= 1u << j;
+            key[j] = rank_key(v[j]);
+            valid |= 1u << j;
         }
     }
-    const unsigned valid = avail;
-    float my_l = 0.0f;
     int my_i = 0;
-    float top_l = 0.0f;
     for (int r = 0; r < k; ++r) {
-        Cand c{-INFINITY, 0x7FFFFFFF};
+        uint32_t most = key[0];
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-            if ((avail >> j) & 1u) {
-                Cand d{v[j] != v[j] ? -INFINITY : v[j], j * kWave + lane};
-                if (better(d, c)) c = d;
-            }
+        for (int j = 1; j < J; ++j) most = max(most, key[j]);
+        most = wave_max(most);
+        int i = 0;                    // the lowest index that has it
+#pragma unroll
+        for (int j = J - 1; j >= 0; --j) {
+            const unsigned long long m = __ballot(key[j] == most);
+            if (m) i = j * kWave + __builtin_ctzll(m);
         }
-        c = wave_best(c);
-        if ((c.i & (kWave - 1)) == lane) avail &= ~(1u << (c.i >> 6));
-        // the logit behind the winning key, as stored (a NaN ranks as -inf but stays a NaN in the weights)
-        float mine = v[0];
 #pragma unroll
-        for (int j = 1; j < J; ++j) mine = (c.i >> 6) == j ? v[j] : mine;
-        // c comes out of wave_best through scalar registers: the winner's lane is uniform, so a lane read, not a shuffle
-        const float cv = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), c.i & (kWave - 1)));
-        if (lane == r) { my_l = cv; my_i = c.i; }
-        if (r == 0) top_l = cv;
+        for (int j = 0; j < J; ++j)
+            if (j * kWave + lane == i) key[j] = 0;
+        if (lane == r) my_i = i;
     }
+    // the logits behind the keys, as stored (a NaN ranks as -inf but stays a NaN in the weights)
+    float my_l = 0.0f;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        const float l = __shfl(v[j], my_i & (kWave - 1), kWave);
+        if ((my_i >> 6) == j) my_l = l;
+    }
+    const float top_l = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(my_l), 0));
     float p = 0.0f;
     if (gate_fn == MOE_GATE_SOFTMAX) {
         float part = 0.0f;
