@@ -524,13 +524,10 @@ class MoELayer:
         s = weights.get("s_up")
         return s is not None and s.dtype == torch.uint8
 
-    def forward_few(self, x, weights: dict, out=None, routing: dict | None = None):
-        """out[S,H] = MoE(x) for at most 16 tokens of a bf16 or fp16 layer, in two launches (three with a large router).  Expert weights in
-        the layer's type, or (bf16 layers) in MXFP4: w_* from quantize_mxfp4 as uint8 [E,N,K/2], s_* as uint8 [E,N,K/32].  `routing` (from
-        new_routing()) receives the routing result when given."""
+    def _few_weights(self, weights: dict):
+        """The weights' addresses and, of MXFP4 weights, the scales' (else None); every tensor has been checked."""
         import torch
-        cfg, act = self.cfg, self.act_dtype
-        S, H, I, E = self.S, self.H, cfg.intermediate_size, self.E
+        H, I, E, act = self.H, self.cfg.intermediate_size, self.E, self.act_dtype
         mx = self._mxfp4_weights(weights)
         unknown = set(weights) - set(self.WEIGHT_KEYS)
         if unknown:
@@ -554,27 +551,38 @@ class MoELayer:
                     setattr(sc, name, t.data_ptr())
                     continue
             setattr(w, name, t.data_ptr())
+        return w, sc if mx else None
+
+    def forward_few(self, x, weights: dict, out=None, routing: dict | None = None):
+        """out[S,H] = MoE(x) for at most 16 tokens of a bf16 or fp16 layer, in two launches (three with a large router).  Expert weights in
+        the layer's type, or (bf16 layers) in MXFP4: w_* from quantize_mxfp4 as uint8 [E,N,K/2], s_* as uint8 [E,N,K/32].  `routing` (from
+        new_routing()) receives the routing result when given."""
+        import torch
+        S, H, act = self.S, self.H, self.act_dtype
+        w, sc = self._few_weights(weights)
         _device_operand("x", x, act, (S, H))
         if out is None:
             out = torch.empty(S, H, dtype=act, device=x.device)
         else:
             _device_operand("out", out, act, (S, H))
         r = None if routing is None else C.byref(_CRouting(*[routing[n].data_ptr() for n, _ in _CRouting._fields_]))
-        _check(self.L.moe_forward_few(self._h, _ptr(x), C.byref(w), C.byref(sc) if mx else None, _ptr(out), r, _ptr(self.workspace),
+        _check(self.L.moe_forward_few(self._h, _ptr(x), C.byref(w), None if sc is None else C.byref(sc), _ptr(out), r, _ptr(self.workspace),
                                       self.workspace_bytes, _stream()), "moe_forward_few")
         return out
 
     def forward_mxfp4(self, x, weights: dict):
         """out[S,H] = MoE(x) of a bf16 layer whose expert weights are in MXFP4, for any number of tokens: forward_few for a few, else the
         stages one by one, the projections by expert_gemm_mxfp4."""
-        import torch
-        if self.S <= FEW_TOKENS:
-            return self.forward_few(x, weights)
         if not self._mxfp4_weights(weights):
             raise TypeError("forward_mxfp4 takes expert weights from quantize_mxfp4")
-        cfg = self.cfg
+        if self.S <= FEW_TOKENS:
+            return self.forward_few(x, weights)
+        cfg, gated = self.cfg, self.cfg.hidden_act == ACT_SWIGLU
+        self._few_weights(weights)
         _device_operand("x", x, self.act_dtype, (self.S, self.H))
-        _device_operand("gate_w", weights["gate_w"], self.act_dtype, (self.E, self.H))
+        missing = [n for n in ("gate_w", "w_up", "w_down", "s_down") + (("w_gate", "s_gate") if gated else ()) if weights.get(n) is None]
+        if missing:
+            raise ValueError("missing tensors %s" % missing)
         idx, gate = self.gate(x, weights["gate_w"], weights.get("gate_bias"))
         r = self.route(idx)
         count, offset = r["expert_count"], r["expert_offset"]
@@ -583,7 +591,7 @@ class MoELayer:
         def project(a, name, act):
             return self.expert_gemm_mxfp4(a, weights["w_" + name], weights["s_" + name], weights.get("b_" + name), count, offset, act=act)
 
-        if cfg.hidden_act == ACT_SWIGLU:
+        if gated:
             h = self.act_forward(project(rows, "up", ACT_NONE), project(rows, "gate", ACT_NONE), count, offset)
         else:
             h = project(rows, "up", cfg.hidden_act)

@@ -388,27 +388,22 @@ hipError_t launch_few_form(const FewArgs& a, hipStream_t st) {
     const bool gated = a.w_gate != nullptr;
     const int64_t most = std::min<int64_t>(a.E, (int64_t)a.S * a.k) * (a.I / (gated ? 16 : 32));      // tasks there can be
     const int chunks = (a.H + W::K - 1) / W::K, lds = skinny_lds<W>(a.S);
-    static const hipError_t ready = [] {
-        constexpr int up = kFewWaves * skinny_lds<W>(kFewTokens);
-        const void* const ups[] = {reinterpret_cast<const void*>(few_up_kernel<W, ET, true, COLD>), reinterpret_cast<const void*>(few_up_kernel<W, ET, false, COLD>)};
-        for (const void* f : ups) {
-            const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, up);
-            if (e != hipSuccess) return e;
-        }
-        return hipFuncSetAttribute(reinterpret_cast<const void*>(few_down_kernel<W, ET, COLD>), hipFuncAttributeMaxDynamicSharedMemorySize, kFewWaves * kRowLds);
-    }();
-    if (ready != hipSuccess) return ready;
     int KS = 1;
     while (KS < kFewWaves && 2 * KS * kUnit <= chunks && most * KS < 1024) KS *= 2;
     const int64_t sets = (most + kFewWaves / KS - 1) / (kFewWaves / KS);
     // (as many workgroups as there is room for at once: every one of them makes the plan)
     const unsigned grid = (unsigned)(KS > 1 ? sets : std::min<int64_t>(sets, 512));
     const int up_lds = kFewWaves * (KS > 1 ? lds : std::min(lds, kRowLds));
+    hipError_t e = gated ? allow_lds(few_up_kernel<W, ET, true, COLD>, up_lds) : allow_lds(few_up_kernel<W, ET, false, COLD>, up_lds);
+    if (e != hipSuccess) return e;
     if (gated) few_up_kernel<W, ET, true, COLD><<<grid, kFewThreads, up_lds, st>>>(a, KS);
     else few_up_kernel<W, ET, false, COLD><<<grid, kFewThreads, up_lds, st>>>(a, KS);
-    const hipError_t e = hipGetLastError();
+    e = hipGetLastError();
     if (e != hipSuccess) return e;
-    few_down_kernel<W, ET, COLD><<<a.H / 16, kFewThreads, kFewWaves * std::min(lds, kRowLds), st>>>(a);
+    const int down_lds = kFewWaves * std::min(lds, kRowLds);
+    e = allow_lds(few_down_kernel<W, ET, COLD>, down_lds);
+    if (e != hipSuccess) return e;
+    few_down_kernel<W, ET, COLD><<<a.H / 16, kFewThreads, down_lds, st>>>(a);
     return hipGetLastError();
 }
 template <class W, class ET>

@@ -547,8 +547,8 @@ hipError_t launch_tile(const MxProduct& p, hipStream_t st) {
         if constexpr (T::ROWS4) return mx_tile4_kernel<T>;
         else return mx_tile_kernel<T>;
     }();
-    static const hipError_t ready = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
-    if (ready != hipSuccess) return ready;
+    const hipError_t e = allow_lds(kernel, T::LDS);
+    if (e != hipSuccess) return e;
     kernel<<<(unsigned)mx_grid(p, T::BM, T::BN), T::THREADS, T::LDS, st>>>(p);
     return hipGetLastError();
 }
@@ -557,12 +557,8 @@ template <bool ROWS4, int CG>
 hipError_t launch_stream_form(const MxProduct& p, int KS, bool cold, hipStream_t st) {
     const int rows = (int)(p.count ? 16 : std::min<int64_t>(p.M, 16)), lds = kStreamWaves * skinny_lds<WeightsMx<ROWS4>>(rows);
     const unsigned grid = (unsigned)mx_grid(p, 16, 16 * CG * (kStreamWaves / KS));
-    static const hipError_t ready = [] {
-        constexpr int most = kStreamWaves * skinny_lds<WeightsMx<ROWS4>>(16);
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(mx_stream_kernel<ROWS4, CG, true>), hipFuncAttributeMaxDynamicSharedMemorySize, most);
-        return e != hipSuccess ? e : hipFuncSetAttribute(reinterpret_cast<const void*>(mx_stream_kernel<ROWS4, CG, false>), hipFuncAttributeMaxDynamicSharedMemorySize, most);
-    }();
-    if (ready != hipSuccess) return ready;
+    const hipError_t e = cold ? allow_lds(mx_stream_kernel<ROWS4, CG, true>, lds) : allow_lds(mx_stream_kernel<ROWS4, CG, false>, lds);
+    if (e != hipSuccess) return e;
     if (cold) mx_stream_kernel<ROWS4, CG, true><<<grid, 64 * kStreamWaves, lds, st>>>(p, KS, rows);
     else mx_stream_kernel<ROWS4, CG, false><<<grid, 64 * kStreamWaves, lds, st>>>(p, KS, rows);
     return hipGetLastError();

@@ -56,6 +56,11 @@ struct WeightsMx {
     static __host__ __device__ __forceinline__ int64_t row_bytes(int64_t k) { return k >> 1; }
     static __device__ __forceinline__ uint32_t token_bytes(uint32_t k) { return ROWS4 ? k >> 1 : 2 * k; }
 };
+// Dynamic LDS of a launch; on every launch, for it holds for the current device.
+template <class K>
+hipError_t allow_lds(K kernel, int bytes) {
+    return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
 constexpr int kUnit = 4;                       // chunks that share a fetch of scales
 constexpr uint32_t kNoChunk = 1u << 22;        // a chunk behind every row's end
 // LDS of a wavefront: two chunks of token rows, whole instructions of them.
@@ -70,7 +75,8 @@ __host__ __device__ constexpr int skinny_lds(int rows) {
 // four segments the address unit makes four requests.
 __device__ __forceinline__ int sk_turn(int row) { return (4 - (row >> 2)) & 3; }
 
-// One wavefront's stream.  aim() says what the next unit is made of; scales(), fetch() and multiply() go through its chunks.
+// One wavefront's stream.  aim_weights() and aim_tokens() say what the next unit is made of; scales(), fetch() and multiply() go through its
+// chunks.
 template <class W, int G, bool COLD>
 struct Skinny {
     static constexpr bool rows4() { return W::MX && W::ROWB == 128; }

@@ -212,3 +212,80 @@ def test_mxfp4_layer_from_a_checkpoint_to_its_answers(tmp_path):
         assert (got.double() - want.double()).norm() <= 6 * 2.0 ** -8 * want.double().norm()
         module = torch_op.MoE355.from_packed(cfg, loaded)
         assert torch.equal(module(x), got)
+
+
+@pytest.mark.parametrize("weights", ["mxfp4", "own"])
+@pytest.mark.parametrize("S,H,I,E,k", [(16, 2048, 64, 2, 2), (16, 4096, 128, 3, 2), (13, 4096, 64, 2, 1), (16, 8192, 192, 5, 2), (16, 192, 4160, 4, 3)])
+def test_few_with_many_rows_an_expert(S, H, I, E, k, weights):
+    """Experts of nine rows and more, where wavefronts share a contraction, and where half of them work."""
+    cfg = _config(S, H, I, E, k, api.ACT_SWIGLU)
+    x, w, exact = _inputs(cfg, weights, True, seed=S + H + I)
+    layer = moe.MoELayer(cfg)
+    routing = layer.new_routing()
+    got = layer.forward_few(x, w, routing=routing)
+    torch.cuda.synchronize()
+    _close(got, x, cfg, w, exact, routing["topk_idx"].cpu(), routing["topk_w"].cpu(), routing["slot"].cpu())
+
+
+@pytest.mark.parametrize("E,k", [(8, 3), (64, 6), (200, 8), (512, 16)])
+def test_selection_among_equal_and_infinite_logits(E, k):
+    """The order of selection: the larger logit, the lower index among equal ones (0 and -0 are), a NaN like -inf; k distinct experts always."""
+    cfg = _config(3, 64, 64, E, k, api.ACT_RELU, gate=api.GATE_SIGMOID)
+    _, w, _ = _inputs(cfg, "own", False, seed=E)
+    layer = moe.MoELayer(cfg)
+    x = torch.zeros(3, 64, device=DEV, dtype=torch.bfloat16)
+    inf, nan = math.inf, math.nan
+    rows = [[0.0] * E, [-inf] * E, [nan] * E, [nan, -inf] * (E // 2), [(-1) ** e * 0.0 for e in range(E)], [float(e % 5) for e in range(E)],
+            [inf if e % 7 == 3 else nan if e % 3 == 0 else -float(e) for e in range(E)], [-inf if e < E - 2 else -3.0 for e in range(E)],
+            [-3.0e38 if e % 2 else 1e-45 for e in range(E)]]
+    for row in rows:
+        keys = [-inf if math.isnan(v) else v for v in row]
+        want = sorted(range(E), key=lambda e: (-keys[e], e))[:k]
+        w["gate_bias"] = torch.tensor(row, device=DEV)                  # the products of a row of zeros are zeros: these are the logits
+        idx, wts = layer.gate(x, w["gate_w"], w["gate_bias"])
+        routing = layer.new_routing()
+        layer.forward_few(x, w, routing=routing)
+        assert idx.tolist() == [want] * 3 and routing["topk_idx"].tolist() == [want] * 3, row[:8]
+        assert torch.equal(torch.isnan(wts), torch.isnan(routing["topk_w"]))
+        assert torch.equal(wts.nan_to_num(7.0), routing["topk_w"].nan_to_num(7.0))
+
+
+def test_layer_refusals():
+    """Operands of another kind are refused before anything is launched, for a few tokens and for many."""
+    for S in (4, 40):
+        cfg = _config(S, 64, 64, 4, 2, api.ACT_SWIGLU)
+        x, w, _ = _inputs(cfg, "mxfp4", True, seed=S)
+        layer = moe.MoELayer(cfg)
+        layer.forward_mxfp4(x, w)
+        own = _inputs(cfg, "own", True, seed=S)[1]
+        with pytest.raises(TypeError):
+            layer.forward_mxfp4(x, own)
+        with pytest.raises(TypeError):
+            layer.forward_mxfp4(x.float(), w)
+        for bad in ({"w_up": own["w_up"]}, {"gate_bias": torch.zeros(4, device=DEV, dtype=torch.bfloat16)}, {"b_down": own["b_down"].float()}):
+            with pytest.raises(TypeError):
+                layer.forward_mxfp4(x, {**w, **bad})
+        for bad in ({"extra": x}, {"s_gate": w["s_gate"][:, :32]}, {"w_down": w["w_down"].cpu()}, {"b_up": own["b_up"][:2]}):
+            with pytest.raises(ValueError):
+                layer.forward_mxfp4(x, {**w, **bad})
+        for name in ("gate_w", "w_gate", "s_down", "s_gate", "w_down"):
+            with pytest.raises((ValueError, moe.MoEError)):
+                layer.forward_mxfp4(x, {n: t for n, t in w.items() if n != name})
+    with pytest.raises(moe.MoEError):
+        layer.forward_few(x, w)                       # 40 tokens
+
+
+def test_few_beyond_4_gib_of_weights():
+    """The last of 150 experts of 29 MB a matrix; the others' weights are zeros under scales of 2^-127."""
+    E, H, I = 150, 4096, 14336
+    cfg = _config(2, H, I, E, 1, api.ACT_RELU)
+    one, w1, exact = _inputs(_config(2, H, I, 1, 1, api.ACT_RELU), "mxfp4", False, seed=3)
+    w = {"gate_w": torch.zeros(E, H, dtype=torch.bfloat16, device=DEV), "gate_bias": torch.arange(E, dtype=torch.float32, device=DEV)}
+    for n in ("w_up", "s_up", "w_down", "s_down"):
+        w[n] = torch.zeros(E, *w1[n].shape[1:], dtype=torch.uint8, device=DEV)
+        w[n][-1] = w1[n][0]
+    layer = moe.MoELayer(cfg)
+    routing = layer.new_routing()
+    got = layer.forward_few(one, w, routing=routing)
+    assert routing["topk_idx"].tolist() == [[E - 1]] * 2
+    _close(got, one, cfg, w, {m: {E - 1: exact[m][0]} for m in exact}, routing["topk_idx"].cpu(), routing["topk_w"].cpu(), routing["slot"].cpu())

@@ -250,3 +250,33 @@ def test_products_are_the_same_every_time_on_any_stream_and_in_a_graph():
         torch.cuda.synchronize()
         for a, b in zip(want, out):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("rows4", [False, True])
+def test_products_whose_offsets_pass_32_bits(rows4):
+    """More than 4 GiB of rows, of results, and of experts' weights: the last of each."""
+    g = _gen(7)
+    for M, N, K in ((560000, 32, 16384) if rows4 else (280000, 32, 8192), (160000, 14336, 64)):
+        w, s, wv = _held(g, N, K)
+        a, sa, av = _rows(g, 300, K, rows4)
+        big = torch.zeros(M, a.shape[1], dtype=a.dtype, device=DEV)
+        big[-300:] = a
+        if rows4:
+            bs = torch.full((M, K // 32), 127, dtype=torch.uint8, device=DEV)
+            bs[-300:] = sa
+        out = moe.gemm_mxfp4(big, w, s, a_scales=bs if rows4 else None)
+        plain.product_close(out[-300:], av, wv)
+        assert not out[:-300].any()
+        del out, big
+    E, H, I, n = 150, 4096, 14336, 40
+    layer = _layer(n, 1, E, I, H)
+    w1, s1, wv = _held(g, I, H)
+    w = torch.zeros(E, I, H // 2, dtype=torch.uint8, device=DEV)
+    s = torch.zeros(E, I, H // 32, dtype=torch.uint8, device=DEV)
+    w[-1], s[-1] = w1, s1
+    count = torch.zeros(E, dtype=torch.int32, device=DEV)
+    for rows in (3, n):
+        count[-1] = rows
+        a, sa, av = _rows(g, n, H, rows4)
+        out = layer.expert_gemm_mxfp4(a, w, s, None, count, torch.zeros_like(count), a_scales=sa)
+        plain.product_close(out[:rows], av[:rows], wv)
