@@ -77,7 +77,7 @@ struct Derived {
 struct WsLayout {
     size_t logits, topk_idx, topk_w, slot, pair_row, token_indices, expert_count, expert_offset, rank_local,
         block_hist, mtiles, seg0, seg1, segq, qstate, cstate, done0, done1, pair_mt, wg_clock, arrive, stats_prob, stats_cnt, h, y,
-        wide, xq, sx, hq, sh, split_cnt, split_part, x_pieces, w_pieces, total;
+        wide, xq, sx, hq, sh, split_cnt, split_part, x_pieces, w_pieces, few_part, few_arrived, total;
 };
 
 // Storage type of activations (x, biases, h, y, out): the layer's own, except that tf32 -- fp32 storage with
@@ -181,6 +181,10 @@ WsLayout layout(const Derived& d) {
     w.split_part = take(split_tiles * d.plan.ksplit * ((size_t)d.plan.block_m * bf16_block_n1(d.plan.tile)) * 4);
     w.x_pieces = take(d.f32_pieces ? (size_t)d.S * d.H * 6 : 0);
     w.w_pieces = take(d.f32_pieces ? (size_t)d.wide_mats * d.E * d.I * d.H * 6 : 0);
+    // moe_forward_few: sums of workgroups that share columns
+    const int parts = d.S <= kFewTokens && d.act_bytes == 2 ? few_parts(d.H) : 1;
+    w.few_part = take(parts > 1 ? (size_t)d.H / 16 * parts * 1024 : 0);
+    w.few_arrived = take(parts > 1 ? (size_t)d.H / 16 * 4 : 0);
     w.total = off;
     return w;
 }
@@ -995,6 +999,9 @@ int moe_forward_few(moe_handle* h, const void* x, const moe_weights* w, const mo
     a.topk_w = at<float>(workspace, h->ws.topk_w);
     a.h = at<char>(workspace, h->ws.h);
     a.out = out;
+    a.part = at<float>(workspace, h->ws.few_part);
+    a.arrived = at<int32_t>(workspace, h->ws.few_arrived);
+    a.parts = few_parts(d.H);
     if (routing) a.r = *routing;
     a.S = d.S, a.H = d.H, a.I = d.I, a.E = d.E, a.k = d.k;
     a.act = h->cfg.hidden_act, a.gate_fn = h->cfg.gate_fn, a.norm = h->cfg.norm_topk_prob;

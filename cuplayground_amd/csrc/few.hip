@@ -10,6 +10,10 @@
 //             once.  No expert's output row is ever rounded or stored.
 // Weights stream as in skinny.hpp.  The router's sums and selection are those of the general path to the bit (the fixed order of 64
 // partial sums; topk.hpp), and so are slots, drops and packed rows: the intermediate lies where that path would put it.
+//
+// Bound by memory.  us in few_logits + few_up + few_down, one token of 4096 x 14336, 8 experts, 2 chosen, SwiGLU, MXFP4 (187 MB): 30 + 17; 16 tokens
+// of 7168 x 2048, 256 experts, 8 chosen (about 2.4 GB): 9 + 290 + 154, 5.3 TB/s; 4 tokens of 2048 x 1408, 64 experts, 6 chosen, bf16 (about 0.36 GB):
+// 5 + 55 + 41.
 #include "act_deriv.hpp"
 #include "skinny.hpp"
 #include "topk.hpp"
@@ -206,7 +210,11 @@ __global__ __launch_bounds__(kFewThreads, 4) void few_up_kernel(FewArgs a, int K
     }
     __syncthreads();
     few_plan(plan, a);
-    if (blockIdx.x == 0) few_report(plan, a);
+    if (blockIdx.x == 0) {
+        few_report(plan, a);
+        if (a.parts > 1)
+            for (int i = threadIdx.x; i < a.H / 16; i += kFewThreads) a.arrived[i] = 0;      // for few_down
+    }
 
     constexpr int G = 2, COLS = GATED ? 16 : 32;
     const int H = a.H, I = a.I, chunks = (H + W::K - 1) / W::K;
@@ -313,12 +321,14 @@ __global__ __launch_bounds__(kFewThreads, 4) void few_down_kernel(FewArgs a) {
     few_plan(plan, a);
 
     const int H = a.H, I = a.I, chunks = (I + W::K - 1) / W::K;      // of an expert
-    const int n0 = blockIdx.x * 16 * G;
+    const int group = (int)blockIdx.x / a.parts, part = (int)blockIdx.x - group * a.parts, n0 = group * 16 * G;
     const int idx = lane & 15, q = lane >> 4;
     const int64_t mat = W::row_bytes((int64_t)H * I), smat = (int64_t)H * (I >> 5);
     const bool half = skinny_lds<W>(plan.most) > kRowLds;
-    const int waves = half ? kFewWaves / 2 : kFewWaves, all = plan.hit * chunks;
-    const int begin = (int)((int64_t)all * min(wave, waves) / waves), end = (int)((int64_t)all * min(wave + 1, waves) / waves);
+    const int waves = half ? kFewWaves / 2 : kFewWaves;
+    const int64_t all = (int64_t)plan.hit * chunks;
+    const int64_t shares = (int64_t)waves * a.parts;
+    const int first = part * waves + min(wave, waves), begin = (int)(all * first / shares), end = wave < waves ? (int)(all * (first + 1) / shares) : begin;
     int j = begin / chunks, c = begin - j * chunks, next_j = j, next_c = c;
     // units: of the first expert's rest, of whole experts, of the last one's part
     const int head = min(end - begin, chunks - c), rest = end - begin - head;
@@ -374,22 +384,52 @@ __global__ __launch_bounds__(kFewThreads, 4) void few_down_kernel(FewArgs a) {
         for (int g = 0; g < G; ++g) acc[g] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
         c = 0, ++j, whole = true;
     });
-    if (!skinny_join<G>(out[0], wave, kFewWaves, red, lane) || idx >= a.S) return;
+    if (!skinny_join<G>(out[0], wave, kFewWaves, red, lane)) return;
+    if (a.parts > 1) {
+        // The sums of workgroups that share these columns, wherever they run: written through, counted, and added up in their order by the
+        // last that comes.
+        static_assert(G == 1, "a part is 16 columns of 16 tokens");
+        uint64_t* const parts = reinterpret_cast<uint64_t*>(a.part) + ((int64_t)group * a.parts * 64 + lane) * 2;
+        union { mx_f32x4 v; uint64_t w[2]; } s;
+        s.v = out[0][0];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) __hip_atomic_store(parts + part * 128 + i, s.w[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        int before = 0;
+        if (lane == 0) before = __hip_atomic_fetch_add(a.arrived + group, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (__builtin_amdgcn_readfirstlane(before) != a.parts - 1) return;
+        asm volatile("" ::: "memory");
+        out[0][0] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int z = 0; z < a.parts; ++z) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) s.w[i] = __hip_atomic_load(parts + z * 128 + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            out[0][0] += s.v;
+        }
+    }
+    if (idx >= a.S) return;
 #pragma unroll
     for (int g = 0; g < G; ++g)
         *reinterpret_cast<uint2*>((uint16_t*)a.out + (int64_t)idx * H + n0 + 16 * g + 4 * q) = uint2{few_pack<ET>(out[0][g][0], out[0][g][1]), few_pack<ET>(out[0][g][2], out[0][g][3])};
 }
 
-// Router products up to which every workgroup makes the logits itself instead of a launch in front.
-constexpr int64_t kFoldProducts = 1 << 18;
+// Bytes of weights for 16 columns from which workgroups share them, where few_parts() has more than one: each streams some 36 KB a us, and the
+// sums' way through memory costs 2 us.  The whole call, us, by one / shared: 4 tokens, 24 of 64 experts of 2048 x 1408, bf16 86.7 / 77.9; 1 token,
+// 6 of them (0.26 MB) 42.3 / 40.6, in MXFP4 (0.07 MB) 25.8 / 27.2; 16 tokens, 32 experts of 1024 x 512, bf16, by four 42.2 / 35.4.
+constexpr int64_t kShareBytes = 192 << 10;
+// Router products up to which every workgroup makes the logits itself instead of a launch in front: an expert a wavefront, about.  One token, the
+// whole call in us, launch in front / not: 8 experts, H 4096, 51.2 / 48.3; 64 experts, H 2048, 25.8 / 28.3; 256, H 7168, 67.7 / 159.
+constexpr int64_t kFoldProducts = 1 << 16;
 
 template <class W, class ET, bool COLD>
 hipError_t launch_few_form(const FewArgs& a, hipStream_t st) {
     const bool gated = a.w_gate != nullptr;
     const int64_t most = std::min<int64_t>(a.E, (int64_t)a.S * a.k) * (a.I / (gated ? 16 : 32));      // tasks there can be
     const int chunks = (a.H + W::K - 1) / W::K, lds = skinny_lds<W>(a.S);
+    // Wavefronts of a task: until there are more than a thousand, and no less than a unit of chunks for each.  The whole call for one token, in us,
+    // with 1 / 2 / 4 / 8: 528 tasks (64 experts of 1408 x 2048, 6 chosen) MXFP4 31.6 / 28.3 / 32.1 / 42.8, bf16 58 / 45 / 48 / 58; 1024 tasks of 28
+    // chunks 67.6 / 57.4 / 56.5 / 61.5; 256 tasks of 16 chunks 33 / 26 / 22 / 22.
     int KS = 1;
-    while (KS < kFewWaves && 2 * KS * kUnit <= chunks && most * KS < 1024) KS *= 2;
+    while (KS < kFewWaves && 2 * KS * kUnit <= chunks && most * KS <= 1024) KS *= 2;
     const int64_t sets = (most + kFewWaves / KS - 1) / (kFewWaves / KS);
     // (as many workgroups as there is room for at once: every one of them makes the plan)
     const unsigned grid = (unsigned)(KS > 1 ? sets : std::min<int64_t>(sets, 512));
@@ -403,7 +443,7 @@ hipError_t launch_few_form(const FewArgs& a, hipStream_t st) {
     const int down_lds = kFewWaves * std::min(lds, kRowLds);
     e = allow_lds(few_down_kernel<W, ET, COLD>, down_lds);
     if (e != hipSuccess) return e;
-    few_down_kernel<W, ET, COLD><<<a.H / 16, kFewThreads, down_lds, st>>>(a);
+    few_down_kernel<W, ET, COLD><<<a.H / 16 * a.parts, kFewThreads, down_lds, st>>>(a);
     return hipGetLastError();
 }
 template <class W, class ET>
@@ -417,6 +457,7 @@ hipError_t launch_few_weights(const FewArgs& a, hipStream_t st) {
 
 hipError_t launch_few(FewArgs a, bool f16, bool mxfp4, hipStream_t st) {
     a.fold = (int64_t)a.S * a.E * a.H <= kFoldProducts && a.S * a.E * (int)sizeof(float) <= kFewWaves * 2048;       // (the least LDS that the rows have)
+    if (std::min<int64_t>(a.E, (int64_t)a.S * a.k) * 16 * (mxfp4 ? a.I / 2 : 2 * (int64_t)a.I) < kShareBytes) a.parts = 1;
     if (!a.fold) {
         const int waves = a.E * ((a.S + kLogitTokens - 1) / kLogitTokens);
         if (f16) few_logits_kernel<f16_s><<<(waves + 3) / 4, 256, 0, st>>>(a);

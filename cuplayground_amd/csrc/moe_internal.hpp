@@ -258,9 +258,13 @@ struct FewArgs {
     float* topk_w;
     void* h;                    // [S k, I] in the workspace
     void* out;                  // [S, H]
+    float* part;                // [H / 16][parts][256] sums of workgroups that share columns, and how many of each have arrived
+    int32_t* arrived;           // [H / 16]
     moe_routing_out r;          // the caller's copies (members may be null)
-    int32_t S, H, I, E, k, act, gate_fn, norm, drop, capacity, fold;
+    int32_t S, H, I, E, k, act, gate_fn, norm, drop, capacity, fold, parts;
 };
+// Workgroups that may share 16 columns of the down projection, where the columns are too few for all compute units.
+inline int few_parts(int H) { return H <= 1024 ? 4 : H <= 2048 ? 2 : 1; }
 hipError_t launch_few(FewArgs a, bool f16, bool mxfp4, hipStream_t st);
 
 // ---- backward building blocks (csrc/backward.hip) ----

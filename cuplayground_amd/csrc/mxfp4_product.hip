@@ -1,5 +1,8 @@
 // Products whose weights are MXFP4 (mxfp4.hpp): out = act(a . w^T + bias), w [N][K] codes with a scale for 32 values of a row, the rows a
 // in bf16 or in MXFP4 too; one matrix, or a matrix per expert over packed rows.  Sums in fp32, rounded once on store.
+//
+// Three kinds of kernel: a weight streamer for up to 16 rows a block; tiles for bf16 rows, on the bf16 instructions, the weights widened between
+// LDS and them; tiles for MXFP4 rows, on the scaled instructions.  product_form() takes the one whose fitted cost is least.
 #include "act_deriv.hpp"
 #include "grouped_task.hpp"
 #include "skinny.hpp"
@@ -7,7 +10,6 @@
 namespace moe355 {
 namespace {
 
-typedef __attribute__((address_space(1))) void mx_gbl_void;
 typedef __attribute__((address_space(3))) void mx_lds_void;
 
 struct MxTask {
@@ -121,6 +123,7 @@ __device__ __forceinline__ void mx_store_tile(const MxProduct& p, const MxTask& 
 constexpr int kStreamWaves = 8;
 
 // KS wavefronts share a contraction, a share in a row each, 8 / KS sets of 16 CG columns a workgroup.  rows_most: token rows that LDS is there for.
+// Bound by memory (skinny.hpp).  One row times 4096 x 14336: 8.9 us, 2.4 of them the launch; 16 rows 13.7.
 template <bool ROWS4, int CG, bool COLD>
 __global__ __launch_bounds__(64 * kStreamWaves) void mx_stream_kernel(MxProduct p, int KS, int rows_most) {
     typedef WeightsMx<ROWS4> W;
@@ -221,6 +224,11 @@ __device__ __forceinline__ bool mx_join(mx_f32x4 (&acc)[NT][CG], int ks, int sw,
 // -- rows in bf16 --
 // A slab is 128 values: 256 bytes of a token row, 64 of a weight row, of which a lane's 16 are a whole block and, widened, four fragments
 // (skinny.hpp).  Scales go through registers: two stages of a 128 x 128 tile's operands are half of the LDS to the byte.
+// What bounds it: on large products the matrix instructions, 8192 x 14336 x 4096 by 256 x 256 in 670 to 690 us, 1.4 PFLOP/s (a product of bf16
+// by the library: 1.45; widening costs an eighth of the products' issue and hides behind the other wavefront of the SIMD).  On few rows, LDS: every
+// wavefront reads all rows of the block, 48 x 14336 x 4096 13.5 us.  On experts of some ninety rows, weights that come from memory for one
+// row block each: 6016 rows, 64 experts of 1408 x 2048, 55 us; 45 with the weights in the memory-side cache.  Neither a third stage, nor twice
+// the wavefronts, nor one that asks for weight lines ahead of the others shortens that.
 template <int RH_, int NT_, int CW_, int CG_, int KS_, int AHEAD_ = 1>
 struct MxTile {
     static constexpr bool ROWS4 = false;
@@ -379,6 +387,9 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void mx_tile_kernel(
 // A slab is 256 values, 128 bytes of every row, both operands in LDS.  Products are 32 x 32 over 64 values: the scaled instruction of that
 // shape takes 33 cycles, that of 16 x 16 over 128 values, half as much work, 31 (measured).  A lane's 16 bytes are the block of its
 // row that it multiplies.  NT, CG: 32-row and 32-column blocks of a wavefront.
+// 8192 x 14336 x 4096 by 256 x 256: 303 us, 3.2 PFLOP/s; about 8 of a tile's 43 us are its first slab's way and its stores, so that
+// 8192 x 8192 x 16384 runs at 3.9.  (A workgroup that goes from tile to tile, the next one's first slab requested under the last products of
+// the one before, took 292, but other shapes and the bf16 tiles lost: stores are waited for in the order of the requests.)
 template <int RH_, int NT_, int CW_, int CG_, int KS_>
 struct MxTile4 {
     static constexpr bool ROWS4 = true;

@@ -8,6 +8,7 @@
 // Blocks follow each other in memory as rows do, so the pass knows no rows: a flat array of 32-value blocks.  Bound by memory: four lanes
 // share a block, 16 bytes of 16-bit values each, so that loads and stores are whole lines; a wavefront takes four times 512 values
 // at once to have that many loads in flight, and its lanes keep one scale each of the 64 for a single store of a whole piece.
+// 114688 x 4096 bf16 values: 215 to 235 us to codes (5.3 TB/s read and written), 185 back (6.4); 64 x 7168, 2.8 and 2.6, a launch.
 #include "mxfp4.hpp"
 
 namespace moe355 {

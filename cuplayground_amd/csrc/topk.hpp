@@ -1,5 +1,8 @@
 // Top-k selection and gate weights of one token by one wavefront; shared by the stand-alone top-k kernel and by the
 // single-workgroup router of decode-sized layers.
+//
+// Bound by its own steps, k times a search for the largest: on integer keys a step is a maximum a lane, four across lanes and a ballot a
+// slot; comparing (value, index) pairs through every exchange took four times as long (two tokens of 256 experts, 8 of them: 8 us, now 2).
 #pragma once
 
 #include "moe_internal.hpp"

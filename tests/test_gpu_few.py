@@ -215,9 +215,9 @@ def test_mxfp4_layer_from_a_checkpoint_to_its_answers(tmp_path):
 
 
 @pytest.mark.parametrize("weights", ["mxfp4", "own"])
-@pytest.mark.parametrize("S,H,I,E,k", [(16, 2048, 64, 2, 2), (16, 4096, 128, 3, 2), (13, 4096, 64, 2, 1), (16, 8192, 192, 5, 2), (16, 192, 4160, 4, 3)])
+@pytest.mark.parametrize("S,H,I,E,k", [(16, 2048, 64, 2, 2), (16, 4096, 128, 3, 2), (13, 4096, 64, 2, 1), (16, 8192, 192, 5, 2), (16, 192, 4160, 4, 3), (8, 2048, 832, 64, 8)])
 def test_few_with_many_rows_an_expert(S, H, I, E, k, weights):
-    """Experts of nine rows and more, where wavefronts share a contraction, and where half of them work."""
+    """Experts of nine rows and more, where wavefronts share a contraction, and where half of them work; workgroups that share columns."""
     cfg = _config(S, H, I, E, k, api.ACT_SWIGLU)
     x, w, exact = _inputs(cfg, weights, True, seed=S + H + I)
     layer = moe.MoELayer(cfg)
