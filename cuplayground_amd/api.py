@@ -285,7 +285,8 @@ def _device_operand(name, t, dtype, shape):
 
 def _on_current_device(name, t):
     import torch
-    if not t.is_cuda or t.get_device() != torch.cuda.current_device():
+    current = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)      # (a tensor on a GPU: the runtime is up)
+    if not t.is_cuda or t.get_device() != current():
         raise ValueError("%s lies on %s: expected the current GPU" % (name, t.device))
 
 
@@ -601,6 +602,8 @@ class MoELayer:
         """expert_gemm on weights in MXFP4: w uint8 [E,N,K/2], w_scales uint8 [E,N,K/32]; a_rows bf16 [S k,K], or uint8 [S k,K/2] with
         a_scales uint8 [S k,K/32].  Rows of no expert are not written."""
         import torch
+        if w.dim() != 3:
+            raise ValueError("expert_gemm_mxfp4 takes a matrix for every expert")
         N, K, A = w.shape[1], 2 * w.shape[2], self.S * self.k
         _device_operand("w", w, torch.uint8, (self.E, N, K // 2))
         _device_operand("w_scales", w_scales, torch.uint8, (self.E, N, K // 32))

@@ -273,6 +273,14 @@ def test_layer_refusals():
                 layer.forward_mxfp4(x, {n: t for n, t in w.items() if n != name})
     with pytest.raises(moe.MoEError):
         layer.forward_few(x, w)                       # 40 tokens
+    count = torch.full((4,), 20, dtype=torch.int32, device=DEV)
+    offset = (torch.cumsum(count, 0) - count).int()
+    rows = torch.zeros(80, 64, dtype=torch.bfloat16, device=DEV)
+    for bad in ((rows, w["w_up"][0], w["s_up"]), (rows[:79], w["w_up"], w["s_up"]), (rows, w["w_up"], w["s_up"][:, :, :1])):
+        with pytest.raises(ValueError):
+            layer.expert_gemm_mxfp4(*bad, None, count, offset)
+    with pytest.raises(moe.MoEError):
+        layer.expert_gemm_mxfp4(rows, w["w_up"], w["s_up"], None, count, offset, act=api.ACT_SWIGLU)
 
 
 def test_few_beyond_4_gib_of_weights():
