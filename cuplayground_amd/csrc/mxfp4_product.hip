@@ -119,6 +119,41 @@ __device__ __forceinline__ void mx_store_tile(const MxProduct& p, const MxTask& 
     else all(std::integral_constant<int, MOE_ACT_NONE>{}, Whole{});
 }
 
+// mx_store_tile through LDS of the wavefront's own (mx_rows_lds bytes, where nothing else is read or written any more), for N of a multiple
+// of 8: as the instructions leave them, a store writes 16 or 32 bytes of 32 or 16 rows; this way it writes 64 to 256 bytes of a row.  Both rows in
+// MXFP4, us, without / with: 8192 x 14336 x 4096 305 / 275, 1777 x 2752 x 1344 14.0 / 11.4; rows in bf16 672 / 657, 19.7 / 17.8.
+template <int NT, int CG, int ROWS, int COLS>
+__device__ __host__ constexpr int mx_rows_lds() { return ROWS * NT * (2 * COLS * CG + 16); }
+template <int NT, int CG, int ROWS, int COLS>
+__device__ __forceinline__ void mx_store_rows(const MxProduct& p, const MxTask& t, unsigned char* own, int lane, int row, int col, int row0, int col0, const mx_f32x4 (&acc)[NT][CG]) {
+    constexpr int PITCH = 2 * COLS * CG + 16, LANES = COLS * CG / 8;      // LANES of 16 bytes to a row
+    auto all = [&](auto act_c) {
+        constexpr int ACT = decltype(act_c)::value;
+#pragma unroll
+        for (int g = 0; g < CG; ++g) {
+            const mx_f32x4 b = mx_bias4(p, t, col0 + COLS * g + col);
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                const mx_f32x4 u = acc[i][g] + b;
+                float v[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[r] = ACT == MOE_ACT_GELU ? gelu16(u[r]) : ACT == MOE_ACT_RELU && u[r] < 0.0f ? 0.0f : u[r];      // a NaN stays a NaN
+                *reinterpret_cast<uint2*>(own + (ROWS * i + row) * PITCH + 2 * (COLS * g + col)) = uint2{pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3])};
+            }
+        }
+    };
+    if (p.act == MOE_ACT_GELU) all(std::integral_constant<int, MOE_ACT_GELU>{});
+    else if (p.act == MOE_ACT_RELU) all(std::integral_constant<int, MOE_ACT_RELU>{});
+    else all(std::integral_constant<int, MOE_ACT_NONE>{});
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    const int at = lane / LANES, piece = lane % LANES, c = col0 + 8 * piece;
+#pragma unroll
+    for (int r = 0; r < ROWS * NT; r += 64 / LANES) {
+        const mx_u32x4 v = *reinterpret_cast<const mx_u32x4*>(own + (r + at) * PITCH + 16 * piece);
+        if (row0 + r + at < t.rows && c < p.N) *reinterpret_cast<mx_u32x4*>(t.out + (int64_t)(row0 + r + at) * p.N + c) = v;
+    }
+}
+
 // ---- up to 16 rows a block: a weight streamer ----
 constexpr int kStreamWaves = 8;
 
@@ -224,10 +259,10 @@ __device__ __forceinline__ bool mx_join(mx_f32x4 (&acc)[NT][CG], int ks, int sw,
 // -- rows in bf16 --
 // A slab is 128 values: 256 bytes of a token row, 64 of a weight row, of which a lane's 16 are a whole block and, widened, four fragments
 // (skinny.hpp).  Scales go through registers: two stages of a 128 x 128 tile's operands are half of the LDS to the byte.
-// What bounds it: on large products the matrix instructions, 8192 x 14336 x 4096 by 256 x 256 in 670 to 690 us, 1.4 PFLOP/s (a product of bf16
+// What bounds it: on large products the matrix instructions, 8192 x 14336 x 4096 by 256 x 256 in 657 us, 1.46 PFLOP/s (a product of bf16
 // by the library: 1.45; widening costs an eighth of the products' issue and hides behind the other wavefront of the SIMD).  On few rows, LDS: every
 // wavefront reads all rows of the block, 48 x 14336 x 4096 13.5 us.  On experts of some ninety rows, weights that come from memory for one
-// row block each: 6016 rows, 64 experts of 1408 x 2048, 55 us; 45 with the weights in the memory-side cache.  Neither a third stage, nor twice
+// row block each: 6016 rows, 64 experts of 1408 x 2048, 54 us; some ten less with the weights in the memory-side cache.  Neither a third stage, nor twice
 // the wavefronts, nor one that asks for weight lines ahead of the others shortens that.
 template <int RH_, int NT_, int CW_, int CG_, int KS_, int AHEAD_ = 1>
 struct MxTile {
@@ -380,6 +415,15 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void mx_tile_kernel(
         }
     }
     if (!mx_join<KS, T::SET, NT, CG>(acc, ks, sw, smem, lane)) return;
+    if constexpr (KS == 1) {
+        constexpr int OWN = mx_rows_lds<NT, CG, 16, 16>();
+        static_assert(T::SET * OWN <= T::LDS, "a place for every wavefront");
+        if (!(N & 7)) {
+            mx_meet();
+            mx_store_rows<NT, CG, 16, 16>(p, t, smem + sw * OWN, lane, idx, 4 * q, 16 * wm * NT, c0, acc);
+            return;
+        }
+    }
     mx_store_tile<NT, CG>(p, t, 16 * wm * NT + idx, c0 + 4 * q, acc);
 }
 
@@ -387,9 +431,7 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void mx_tile_kernel(
 // A slab is 256 values, 128 bytes of every row, both operands in LDS.  Products are 32 x 32 over 64 values: the scaled instruction of that
 // shape takes 33 cycles, that of 16 x 16 over 128 values, half as much work, 31 (measured).  A lane's 16 bytes are the block of its
 // row that it multiplies.  NT, CG: 32-row and 32-column blocks of a wavefront.
-// 8192 x 14336 x 4096 by 256 x 256: 303 us, 3.2 PFLOP/s; about 8 of a tile's 43 us are its first slab's way and its stores, so that
-// 8192 x 8192 x 16384 runs at 3.9.  (A workgroup that goes from tile to tile, the next one's first slab requested under the last products of
-// the one before, took 292, but other shapes and the bf16 tiles lost: stores are waited for in the order of the requests.)
+// 8192 x 14336 x 4096 by 256 x 256: 275 us, 3.5 PFLOP/s; between tiles there is the way of the first slab and of the results.
 template <int RH_, int NT_, int CW_, int CG_, int KS_>
 struct MxTile4 {
     static constexpr bool ROWS4 = true;
@@ -543,6 +585,15 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void mx_tile4_kernel
 #pragma unroll
         for (int g = 0; g < 4 * CG; ++g) sum[i][g] = mx_f32x4{acc[i][g / 4][4 * (g % 4)], acc[i][g / 4][4 * (g % 4) + 1], acc[i][g / 4][4 * (g % 4) + 2], acc[i][g / 4][4 * (g % 4) + 3]};
     if (!mx_join<KS, SET, NT, 4 * CG>(sum, ks, sw, smem, lane)) return;
+    if constexpr (KS == 1) {
+        constexpr int OWN = mx_rows_lds<NT, 4 * CG, 32, 8>();
+        static_assert(SET * OWN <= T::LDS, "a place for every wavefront");
+        if (!(N & 7)) {
+            mx_meet();
+            mx_store_rows<NT, 4 * CG, 32, 8>(p, t, smem + sw * OWN, lane, r32, 4 * b, wm * 32 * NT, t.n0 + wn * 32 * CG, sum);
+            return;
+        }
+    }
     mx_store_tile<NT, 4 * CG, 32, 8>(p, t, wm * 32 * NT + r32, t.n0 + wn * 32 * CG + 4 * b, sum);
 }
 
@@ -633,16 +684,16 @@ hipError_t launch_product4(const MxProduct& p, int form, hipStream_t st) {
 }
 
 // What a tile costs, in us: a launch of its form; a slab of the contraction where a compute unit has one tile; the same for every further
-// tile of the unit.  Fitted to 1.3 to 800 us of 145 products of 17 to 3000 rows, dense and of experts, each with every form that
-// was near; the choice by these is 4 % (rows in MXFP4: 2 %) behind the best of the forms over them, 16 % (22 %) at worst.
+// tile of the unit.  Fitted to products of 17 to 6000 rows, 5 to 800 us, dense and of experts, each with every form that was near: over 246 of
+// them the choice by these is 1.4 % behind the best of the forms on average, 38 % at worst (one of 35 rows for each of 8 experts).
 struct TileCost {
     int rows, columns;
     float launch, slab, more;
 };
 constexpr TileCost kTiles16[] = {{}, {16, 64, 3.2f, 0.158f, 0.187f}, {32, 64, 3.0f, 0.208f, 0.241f}, {48, 64, 3.3f, 0.25f, 0.409f}, {64, 64, 3.1f, 0.343f, 0.352f},
                                  {64, 128, 3.1f, 0.621f, 0.482f}, {96, 128, 2.8f, 0.805f, 0.684f}, {128, 128, 4.4f, 0.822f, 0.836f}, {256, 256, 10.4f, 2.17f, 2.11f}};
-constexpr TileCost kTiles4[] = {{}, {32, 64, 3.9f, 0.193f, 0.501f}, {32, 64, 2.8f, 0.248f, 0.204f}, {64, 64, 2.8f, 0.303f, 0.445f}, {64, 128, 2.3f, 0.567f, 0.61f},
-                                {128, 128, 3.4f, 0.742f, 0.921f}, {128, 256, 5.5f, 0.997f, 1.852f}, {256, 256, 7.8f, 1.41f, 2.781f}};
+constexpr TileCost kTiles4[] = {{}, {32, 64, 4.3f, 0.179f, 0.524f}, {32, 64, 3.2f, 0.231f, 0.281f}, {64, 64, 3.3f, 0.284f, 0.449f}, {64, 128, 2.6f, 0.538f, 0.559f},
+                                {128, 128, 3.3f, 0.682f, 0.862f}, {128, 256, 3.8f, 0.963f, 1.70f}, {256, 256, 4.9f, 1.39f, 2.58f}};
 
 // The form that should take least; 0: the streamer.  Of experts' rows the host knows how many there are, not whose: about as many each.
 int product_form(const MxProduct& p) {
