@@ -985,6 +985,8 @@ int moe_forward_few(moe_handle* h, const void* x, const moe_weights* w, const mo
     if (mx && (!mx->s_up || !mx->s_down || sw != (mx->s_gate != nullptr))) return MOE_ERR_BAD_ARGUMENT;
     for (const void* p : {x, w->gate_w, w->w_up, w->w_gate, w->w_down, (const void*)out})
         if ((uintptr_t)p % 16) return MOE_ERR_BAD_ARGUMENT;       // the kernels read and write 16 and 8 bytes at a time
+    for (const void* p : {w->b_up, w->b_gate, w->b_down})
+        if ((uintptr_t)p % 8) return MOE_ERR_BAD_ARGUMENT;
     // 32-bit offsets: a matrix, the intermediate rows
     if ((int64_t)d.H * d.I * (mx ? 1 : 4) / 2 >= ((int64_t)3 << 30) || (int64_t)d.S * d.k * d.I * 2 >= ((int64_t)3 << 30)) return MOE_ERR_UNSUPPORTED;
     const int rc = check_ws(h, workspace, workspace_bytes);

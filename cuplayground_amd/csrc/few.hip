@@ -53,6 +53,32 @@ __device__ __forceinline__ uint32_t few_pack(float lo, float hi) {
     }
 }
 
+// Four neighbouring values of a bias, or zeros; one load.
+template <class ET>
+__device__ __forceinline__ mx_f32x4 few_bias(const uint16_t* b, int col) {
+    uint16_t raw[4] = {0, 0, 0, 0};
+    if (b) __builtin_memcpy(raw, b + col, 8);
+    return mx_f32x4{few_widen<ET>(raw[0]), few_widen<ET>(raw[1]), few_widen<ET>(raw[2]), few_widen<ET>(raw[3])};
+}
+// Four neighbouring values of an expert's bias for the unit that is multiplied, fetched with the unit's scales: a load where the sums are done
+// would be waited for behind all weights that are on their way by then.  A bias that is not there is a buffer of no bytes: zeros.
+template <class ET>
+struct FewBias {
+    typedef uint32_t Pair __attribute__((ext_vector_type(2)));
+    Pair now, then;
+    __amdgpu_buffer_rsrc_t buf;
+    __device__ __forceinline__ void aim(const void* b, int64_t at, int n) {
+        buf = mx_buffer(b ? static_cast<const uint16_t*>(b) + at : nullptr, b ? 2u * (uint32_t)n : 0u);
+    }
+    __device__ __forceinline__ void next(int col) {
+        now = then;
+        then = __builtin_bit_cast(Pair, __builtin_amdgcn_raw_buffer_load_b64(buf, 2 * col, 0, 0));
+    }
+    __device__ __forceinline__ mx_f32x4 get() const {
+        return mx_f32x4{few_widen<ET>((uint16_t)now[0]), few_widen<ET>((uint16_t)(now[0] >> 16)), few_widen<ET>((uint16_t)now[1]), few_widen<ET>((uint16_t)(now[1] >> 16))};
+    }
+};
+
 // Logits of one expert for tokens t0 .. t0 + n - 1 (n <= TT) by a wavefront: lane p adds up, in ascending k, the products of every k with
 // (k / 8) % 64 == p, one multiply-add each; the partial sums are folded pairwise.  logits[t] at out[t * stride].
 template <class ET, int TT>
@@ -260,6 +286,7 @@ __global__ __launch_bounds__(kFewThreads, 4) void few_up_kernel(FewArgs a, int K
         const int e = __builtin_amdgcn_readfirstlane(plan.list[j]);
         if (idx >= __popc(plan.mask[e])) return;
         uint16_t* h = (uint16_t*)a.h + (int64_t)(plan.base[e] + idx) * I;
+        // (fetched here: kept from the task's beginning they would cost the registers of a second workgroup)
         const uint16_t* bu = a.b_up ? (const uint16_t*)a.b_up + (int64_t)e * I : nullptr;
         const uint16_t* bg = a.b_gate ? (const uint16_t*)a.b_gate + (int64_t)e * I : nullptr;
         auto put = [&](int col, float (&v)[4]) {
@@ -267,23 +294,19 @@ __global__ __launch_bounds__(kFewThreads, 4) void few_up_kernel(FewArgs a, int K
         };
         if constexpr (GATED) {
             const int col = n0 + 4 * q;
+            const mx_f32x4 up = acc[0] + few_bias<ET>(bu, col), gate = acc[1] + few_bias<ET>(bg, col);
             float v[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float up = acc[0][r] + (bu ? few_widen<ET>(bu[col + r]) : 0.0f), gate = acc[1][r] + (bg ? few_widen<ET>(bg[col + r]) : 0.0f);
-                v[r] = silu16(gate) * up;
-            }
+            for (int r = 0; r < 4; ++r) v[r] = silu16(gate[r]) * up[r];
             put(col, v);
         } else {
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 const int col = n0 + 16 * g + 4 * q;
+                const mx_f32x4 up = acc[g] + few_bias<ET>(bu, col);
                 float v[4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float up = acc[g][r] + (bu ? few_widen<ET>(bu[col + r]) : 0.0f);
-                    v[r] = a.act == MOE_ACT_GELU ? gelu16(up) : (up < 0.0f ? 0.0f : up);
-                }
+                for (int r = 0; r < 4; ++r) v[r] = a.act == MOE_ACT_GELU ? gelu16(up[r]) : (up[r] < 0.0f ? 0.0f : up[r]);
                 put(col, v);
             }
         }
@@ -340,25 +363,26 @@ __global__ __launch_bounds__(kFewThreads, 4) void few_down_kernel(FewArgs a) {
     st.x_buf = mx_buffer(a.h, (uint32_t)plan.kept * st.x_row);
     st.aim_weights(n0, H, 16);
     bool aimed = false;
+    FewBias<ET> bias[G] = {};
     auto next = [&](int u) {
-        if (u == units) {
-            st.chunk_end = 0;
-            return;
-        }
-        if (!aimed || next_c == 0) {
+        const bool live = u < units;
+        if (live && (!aimed || next_c == 0)) {
             const int e = __builtin_amdgcn_readfirstlane(plan.list[next_j]), base = __builtin_amdgcn_readfirstlane(plan.base[e]);
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 st.w_buf[g] = mx_buffer(static_cast<const char*>(a.w_down) + e * mat, (uint32_t)mat);
                 if constexpr (W::MX) st.s_at[g] = a.s_down + e * smat;
+                bias[g].aim(a.b_down, (int64_t)e * H, H);
             }
             st.aim_tokens(__builtin_amdgcn_readfirstlane(__popc(plan.mask[e])), [&](int r) { return base + r; });
             aimed = true;
         }
         st.chunk0 = next_c;
-        st.chunk_end = min(chunks, end - next_j * chunks);
+        st.chunk_end = live ? min(chunks, end - next_j * chunks) : 0;
         next_c += kUnit;
         if (next_c >= chunks) next_c = 0, ++next_j;
+#pragma unroll
+        for (int g = 0; g < G; ++g) bias[g].next(n0 + 16 * g + 4 * q);
     };
     mx_f32x4 out[1][G] = {}, acc[G] = {};
     bool whole = c == 0;                 // the expert's first chunk is among them
@@ -371,15 +395,15 @@ __global__ __launch_bounds__(kFewThreads, 4) void few_down_kernel(FewArgs a) {
         const bool in = (m >> idx) & 1u;
         const int r = __popc(m & ((1u << idx) - 1u)), from = 4 * ((lane & 48) + (in ? r : 0));
         const float w = in ? plan.row_w[plan.base[e] + r] : 0.0f;
-        const uint16_t* bd = a.b_down && whole ? (const uint16_t*)a.b_down + (int64_t)e * H + n0 + 4 * q : nullptr;      // the bias goes with the first chunk
 #pragma unroll
-        for (int g = 0; g < G; ++g)
+        for (int g = 0; g < G; ++g) {
+            const mx_f32x4 first = whole ? bias[g].get() : mx_f32x4{0.f, 0.f, 0.f, 0.f};      // the bias goes with the first chunk
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                float y = __uint_as_float(__builtin_amdgcn_ds_bpermute(from, (int)__float_as_uint(acc[g][i])));
-                if (bd) y += few_widen<ET>(bd[16 * g + i]);
+                const float y = __uint_as_float(__builtin_amdgcn_ds_bpermute(from, (int)__float_as_uint(acc[g][i]))) + first[i];
                 if (in) out[0][g][i] = __builtin_fmaf(w, y, out[0][g][i]);      // a token that is not the expert's: not even a NaN of it
             }
+        }
 #pragma unroll
         for (int g = 0; g < G; ++g) acc[g] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
         c = 0, ++j, whole = true;

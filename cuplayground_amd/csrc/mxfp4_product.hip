@@ -66,15 +66,27 @@ __device__ __forceinline__ bool mx_task(const MxProduct& p, int BN, MxTask& t) {
     return true;
 }
 
-// The bias of four neighbouring columns.
-__device__ __forceinline__ mx_f32x4 mx_bias4(const MxProduct& p, const MxTask& t, int col) {
-    mx_f32x4 b = {0.f, 0.f, 0.f, 0.f};
-    if (t.bias) {
+// The bias of CG groups of four neighbouring columns, COLS apart; of columns behind the last some bias.  All loads at once and without a
+// question: one trip to memory.
+template <int CG, int COLS>
+__device__ __forceinline__ void mx_bias(const MxProduct& p, const MxTask& t, int col0, mx_f32x4 (&b)[CG]) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (col + r < p.N) b[r] = bf16_bits_to_f32(t.bias[col + r]);
+    for (int g = 0; g < CG; ++g) b[g] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
+    if (!t.bias) return;
+    uint16_t raw[CG][4];
+    if (p.N & 3) {
+#pragma unroll
+        for (int g = 0; g < CG; ++g)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) raw[g][r] = t.bias[min(col0 + COLS * g + r, p.N - 1)];
+    } else {
+#pragma unroll
+        for (int g = 0; g < CG; ++g) __builtin_memcpy(raw[g], t.bias + min(col0 + COLS * g, p.N - 4), 8);
     }
-    return b;
+#pragma unroll
+    for (int g = 0; g < CG; ++g)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) b[g][r] = bf16_bits_to_f32(raw[g][r]);
 }
 // Four neighbouring columns of a token row, as the matrix instructions leave them in a lane.  whole: N is a multiple of 4.
 template <int ACT>
@@ -98,8 +110,7 @@ template <int NT, int CG, int ROWS = 16, int COLS = 16>
 __device__ __forceinline__ void mx_store_tile(const MxProduct& p, const MxTask& t, int row0, int col0, const mx_f32x4 (&acc)[NT][CG]) {
     const int N = p.N;
     mx_f32x4 b[CG];
-#pragma unroll
-    for (int g = 0; g < CG; ++g) b[g] = mx_bias4(p, t, col0 + COLS * g);
+    mx_bias<CG, COLS>(p, t, col0, b);
     auto all = [&](auto act_c, auto whole_c) {
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
@@ -127,14 +138,15 @@ __device__ __host__ constexpr int mx_rows_lds() { return ROWS * NT * (2 * COLS *
 template <int NT, int CG, int ROWS, int COLS>
 __device__ __forceinline__ void mx_store_rows(const MxProduct& p, const MxTask& t, unsigned char* own, int lane, int row, int col, int row0, int col0, const mx_f32x4 (&acc)[NT][CG]) {
     constexpr int PITCH = 2 * COLS * CG + 16, LANES = COLS * CG / 8;      // LANES of 16 bytes to a row
+    mx_f32x4 b[CG];
+    mx_bias<CG, COLS>(p, t, col0 + col, b);
     auto all = [&](auto act_c) {
         constexpr int ACT = decltype(act_c)::value;
 #pragma unroll
         for (int g = 0; g < CG; ++g) {
-            const mx_f32x4 b = mx_bias4(p, t, col0 + COLS * g + col);
 #pragma unroll
             for (int i = 0; i < NT; ++i) {
-                const mx_f32x4 u = acc[i][g] + b;
+                const mx_f32x4 u = acc[i][g] + b[g];
                 float v[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) v[r] = ACT == MOE_ACT_GELU ? gelu16(u[r]) : ACT == MOE_ACT_RELU && u[r] < 0.0f ? 0.0f : u[r];      // a NaN stays a NaN

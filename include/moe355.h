@@ -432,7 +432,8 @@ int moe_expert_gemm_mxfp4(moe_handle* h, const void* a_rows, const uint8_t* a_sc
  * w_down of *w are codes and *mx has their scales (s_* of *w stay NULL); the router and the biases keep the activations' type.  The routing
  * is moe_forward's to the bit, and so are capacity, drops and what `routing` receives.  Sums in fp32; the intermediate rows are rounded to the
  * activations' type, an expert's output rows are not rounded before the combine, so `out` differs from moe_forward's by that rounding.
- * The workspace is the handle's; one call at a time per workspace.  MOE_ERR_UNSUPPORTED: more tokens, another type of layer, a matrix of
+ * Tensors are 16-byte aligned, biases 8-byte (gate_bias and scales as they come).  The workspace is the handle's; one call at a time per
+ * workspace.  MOE_ERR_UNSUPPORTED: more tokens, another type of layer, a matrix of
  * 3 GiB and more. */
 typedef struct moe_mxfp4_scales {
     const uint8_t* s_up;      /* [E, I, H / 32] */

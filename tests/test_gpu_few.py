@@ -273,6 +273,10 @@ def test_layer_refusals():
                 layer.forward_mxfp4(x, {n: t for n, t in w.items() if n != name})
     with pytest.raises(moe.MoEError):
         layer.forward_few(x, w)                       # 40 tokens
+    few = moe.MoELayer(_config(4, 64, 64, 4, 2, api.ACT_SWIGLU))
+    odd = torch.zeros(4 * 64 + 1, dtype=torch.bfloat16, device=DEV)[1:].view(4, 64)
+    with pytest.raises(moe.MoEError):
+        few.forward_few(x[:4].contiguous(), {**w, "b_down": odd})          # a bias that is not 8-byte aligned
     count = torch.full((4,), 20, dtype=torch.int32, device=DEV)
     offset = (torch.cumsum(count, 0) - count).int()
     rows = torch.zeros(80, 64, dtype=torch.bfloat16, device=DEV)
