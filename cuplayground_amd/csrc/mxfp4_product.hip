@@ -697,7 +697,8 @@ hipError_t launch_product4(const MxProduct& p, int form, hipStream_t st) {
 
 // What a tile costs, in us: a launch of its form; a slab of the contraction where a compute unit has one tile; the same for every further
 // tile of the unit.  Fitted to products of 17 to 6000 rows, 5 to 800 us, dense and of experts, each with every form that was near: over 246 of
-// them the choice by these is 1.4 % behind the best of the forms on average, 38 % at worst (one of 35 rows for each of 8 experts).
+// them the choice by these is 1.4 % behind the best of the forms on average, over 73 more of experts with 20 to 130 rows each, evenly and not,
+// 3.3 %; 38 % at worst (35 rows for each of 8 experts).
 struct TileCost {
     int rows, columns;
     float launch, slab, more;
@@ -707,7 +708,8 @@ constexpr TileCost kTiles16[] = {{}, {16, 64, 3.2f, 0.158f, 0.187f}, {32, 64, 3.
 constexpr TileCost kTiles4[] = {{}, {32, 64, 4.3f, 0.179f, 0.524f}, {32, 64, 3.2f, 0.231f, 0.281f}, {64, 64, 3.3f, 0.284f, 0.449f}, {64, 128, 2.6f, 0.538f, 0.559f},
                                 {128, 128, 3.3f, 0.682f, 0.862f}, {128, 256, 3.8f, 0.963f, 1.70f}, {256, 256, 4.9f, 1.39f, 2.58f}};
 
-// The form that should take least; 0: the streamer.  Of experts' rows the host knows how many there are, not whose: about as many each.
+// The form that should take least; 0: the streamer.  Of experts' rows the host knows how many there are, not whose: a block an expert where the
+// mean is small for it, else half a block more than the mean fills.
 int product_form(const MxProduct& p) {
     const bool rows4 = p.a_scales != nullptr;
     const int64_t experts = p.count ? std::min<int64_t>(p.E, p.M) : 1;
@@ -715,16 +717,19 @@ int product_form(const MxProduct& p) {
     // (a chunk of a wavefront, with one or two groups of columns; and what its token rows add)
     const StreamCut c = stream_cut(p);
     const double rows = std::min(each, 16.0);
-    double best = 3.8 + (rows4 ? 0.03 : 0.2) * rows + c.chunks * std::max(1.0, c.waves / 2048.0) * ((c.wide ? 1.3 : 0.5) + (rows4 ? 0.003 : 0.017) * rows);
+    auto row_blocks = [&](int rows) { return !p.count ? (double)((p.M + rows - 1) / rows) : each > 0.6 * rows ? (double)p.M / rows + 0.5 * experts : (double)experts; };
+    const double rounds = std::max(1.0, c.waves / 2048.0) * (p.count ? row_blocks(16) / experts : 1.0);
+    double best = 3.8 + (rows4 ? 0.03 : 0.2) * rows + c.chunks * rounds * ((c.wide ? 1.3 : 0.5) + (rows4 ? 0.003 : 0.017) * rows);
     if (p.count && each > 16) best = 1e30;               // a row block an expert, at most
     int form = 0;
+    const bool cold = experts * p.N * p.K / 2 > ((int64_t)96 << 20);
     const int forms = rows4 ? (int)(sizeof kTiles4 / sizeof kTiles4[0]) : (int)(sizeof kTiles16 / sizeof kTiles16[0]);
     for (int f = 1; f < forms; ++f) {
         const TileCost& t = rows4 ? kTiles4[f] : kTiles16[f];
-        const double blocks = !p.count ? (double)((p.M + t.rows - 1) / t.rows) : each > 0.75 * t.rows ? (double)p.M / t.rows + 0.5 * experts : (double)experts;
-        const double tiles = std::ceil(blocks * ((p.N + t.columns - 1) / t.columns) / 256.0);      // of the compute unit that has most
+        const double tiles = std::ceil(row_blocks(t.rows) * ((p.N + t.columns - 1) / t.columns) / 256.0);      // of the compute unit that has most
         const int slabs = rows4 ? (p.K + 255) / 256 : (p.K + 127) / 128;
-        const double cost = t.launch + slabs * (t.slab + t.more * (tiles - 1));
+        // (and of weights that no cache holds a compute unit is brought some 24 KB a us)
+        const double cost = std::max(t.launch + slabs * (t.slab + t.more * (tiles - 1)), cold ? 2.4 + tiles * t.columns * (p.K * 17.0 / 32) / 24e3 : 0.0);
         if (cost < best) best = cost, form = f;
     }
     return form;
