@@ -696,8 +696,8 @@ hipError_t launch_product4(const MxProduct& p, int form, hipStream_t st) {
 }
 
 // What a tile costs, in us: a launch of its form; a slab of the contraction where a compute unit has one tile; the same for every further
-// tile of the unit.  Fitted to products of 17 to 6000 rows, 5 to 800 us, dense and of experts, each with every form that was near: over 246 of
-// them the choice by these is 1.4 % behind the best of the forms on average, over 73 more of experts with 20 to 130 rows each, evenly and not,
+// tile of the unit.  Fitted to products of 17 to 6000 rows, 5 to 800 us, dense and of experts, each with every form that was near: over 240 of
+// them the choice by these is 1.2 % behind the best of the forms on average, over 68 more of experts with 20 to 130 rows each, evenly and not,
 // 3.3 %; 38 % at worst (35 rows for each of 8 experts).
 struct TileCost {
     int rows, columns;

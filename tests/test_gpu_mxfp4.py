@@ -127,7 +127,7 @@ def test_product_large(M, N, K, rows4):
 @pytest.mark.parametrize("M,N,K", [
     (34, 8587, 32), (94, 8045, 448), (409, 6995, 160), (726, 6321, 352), (328, 8325, 544), (1358, 8901, 672), (227, 8262, 576), (584, 6660, 1056),
     (1154, 6865, 800), (1, 33001, 1056), (13, 33010, 1056), (2, 323, 4128), (14, 186, 3936), (491, 222, 4032), (1, 3, 4032), (982, 150, 1312),
-    (1358, 8904, 672), (1154, 6872, 800), (1, 33001, 8192)])
+    (1358, 8904, 672), (1154, 6872, 800), (1, 33001, 8192), (3, 65540, 4096)])
 def test_product_at_odd_sizes_of_every_kernel(M, N, K, rows4):
     """The sizes reach every tile and cut of the streamer, and end inside their rows, columns and slabs."""
     g = _gen(M + N + K)
