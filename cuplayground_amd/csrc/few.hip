@@ -13,7 +13,7 @@
 //
 // Bound by memory.  us in few_logits + few_up + few_down, one token of 4096 x 14336, 8 experts, 2 chosen, SwiGLU, MXFP4 (187 MB): 30 + 17; 16 tokens
 // of 7168 x 2048, 256 experts, 8 chosen (about 2.4 GB): 9 + 290 + 154, 5.3 TB/s; 4 tokens of 2048 x 1408, 64 experts, 6 chosen, bf16 (about 0.36 GB):
-// 5 + 55 + 41.
+// 5 + 57 + 27.
 #include "act_deriv.hpp"
 #include "skinny.hpp"
 #include "topk.hpp"
