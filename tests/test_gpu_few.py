@@ -301,3 +301,30 @@ def test_few_beyond_4_gib_of_weights():
     got = layer.forward_few(one, w, routing=routing)
     assert routing["topk_idx"].tolist() == [[E - 1]] * 2
     _close(got, one, cfg, w, {m: {E - 1: exact[m][0]} for m in exact}, routing["topk_idx"].cpu(), routing["topk_w"].cpu(), routing["slot"].cpu())
+
+
+@pytest.mark.parametrize("act,gate,norm,capacity", [(api.ACT_GELU, api.GATE_SIGMOID, 1, 1.0), (api.ACT_SWIGLU, api.GATE_SOFTMAX, 0, 0.75), (api.ACT_RELU, api.GATE_SOFTMAX, 1, 0.0)])
+@pytest.mark.parametrize("S", [11, 17, 130])
+def test_mxfp4_layer_with_drops_and_biases(S, act, gate, norm, capacity):
+    """forward_mxfp4 on both sides of the few tokens, against the layer in 64 bits with the routing of the general path: its bf16 rows, and the
+    stages' roundings of projections and experts' rows, are at most five of half a unit each, weighted as the sums weight them."""
+    F = torch.nn.functional
+    cfg = _config(S, 320, 448, 12, 3, act, gate=gate, norm=norm, capacity=capacity)
+    x, w, exact = _inputs(cfg, "mxfp4", True, seed=S + act, gate_bias=True)
+    layer = moe.MoELayer(cfg)
+    got = layer.forward_mxfp4(x, w)
+    idx, wts = layer.gate(x, w["gate_w"], w["gate_bias"])
+    slot = layer.route(idx)["slot"]
+    if capacity:
+        assert int((slot < 0).sum()) > 0
+    want = torch.zeros(S, 320, dtype=torch.float64, device=DEV)
+    for t in range(S):
+        for r in range(3):
+            if slot[t, r] >= 0:
+                e = int(idx[t, r])
+                u = exact["up"][e] @ x[t].double() + w["b_up"][e].double()
+                h = F.silu(exact["gate"][e] @ x[t].double() + w["b_gate"][e].double()) * u if act == api.ACT_SWIGLU else plain.activate(u, act)
+                want[t] += wts[t, r].double() * (exact["down"][e] @ h + w["b_down"][e].double())
+    assert (got.double() - want).norm() <= 5 * 2.0 ** -8 * want.norm()
+    lost = (slot < 0).all(1)
+    assert not got[lost].any()
