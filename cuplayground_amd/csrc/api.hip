@@ -70,6 +70,7 @@ struct Derived {
     FfnPlan plan;
     int nblk;          // workgroups of the slot-assignment kernels
     bool f32_pieces;   // fp32 layer that runs on bf16 pieces
+    int few_parts;     // workgroups that may share 16 columns in moe_forward_few; 0: not a layer that it takes
     int wide_mats;     // weight matrices per expert (3 with SwiGLU, else 2)
     int max_mtiles;
 };
@@ -77,7 +78,7 @@ struct Derived {
 struct WsLayout {
     size_t logits, topk_idx, topk_w, slot, pair_row, token_indices, expert_count, expert_offset, rank_local,
         block_hist, mtiles, seg0, seg1, segq, qstate, cstate, done0, done1, pair_mt, wg_clock, arrive, stats_prob, stats_cnt, h, y,
-        wide, xq, sx, hq, sh, split_cnt, split_part, x_pieces, w_pieces, few_part, few_arrived, total;
+        wide, xq, sx, hq, sh, split_cnt, split_part, x_pieces, w_pieces, few_arrived, total;
 };
 
 // Storage type of activations (x, biases, h, y, out): the layer's own, except that tf32 -- fp32 storage with
@@ -97,6 +98,17 @@ int check_supported(const moe_config& c) {
 }
 
 WsLayout layout(const Derived& d);
+
+// moe_forward_few's sums of workgroups that share columns, and how many of each have arrived.
+size_t few_sum_bytes(int H, int parts) { return parts > 1 ? (size_t)H / 16 * parts * 1024 : 0; }
+size_t few_shared_bytes(int H, int parts) { return parts > 1 ? few_sum_bytes(H, parts) + (size_t)H / 16 * 4 : 0; }
+int few_parts_of(const Derived& d, int torch_dtype) {
+    if (d.S > kFewTokens || (torch_dtype != MOE_DTYPE_BF16 && torch_dtype != MOE_DTYPE_FP16)) return 0;
+    // what moe_forward_static took without them it takes still
+    Derived with = d;
+    with.few_parts = few_parts(d.H);
+    return layout(d).total <= MOE355_STATIC_WORKSPACE_BYTES && layout(with).total > MOE355_STATIC_WORKSPACE_BYTES ? 1 : with.few_parts;
+}
 
 // An fp32 layer on the 128 x 128 matrix-core tile runs on bf16 pieces instead (ffn_f32_pieces.hip) from this many rows per expert on,
 // where f32_pieces_choice.hpp expects that to be faster and its workspace may grow so far.
@@ -133,8 +145,9 @@ int derive(const moe_config& c, const moe_options& o, Derived* d) {
     d->wide_in_workspace = d->plan.widen && o.prepared_weights != 1;
     d->nblk = ceil_div(d->A, kRouteBlock);
     d->max_mtiles = ceil_div(d->A, d->plan.block_m) + d->E;
-    d->f32_pieces = false;
+    d->f32_pieces = false, d->few_parts = 0;
     d->f32_pieces = f32_pieces_ok(*d, o, c.drop_tokens != 0);
+    d->few_parts = few_parts_of(*d, c.torch_dtype);
     return MOE_OK;
 }
 
@@ -166,7 +179,9 @@ WsLayout layout(const Derived& d) {
     w.stats_prob = take((size_t)kStatsBlocks * d.E * 8);
     w.stats_cnt = take((size_t)kStatsBlocks * d.E * 4);
     w.h = take((size_t)d.A * d.I * (d.f32_pieces ? 6 : d.act_bytes));      // in fp32 or as pieces
-    w.y = take((size_t)d.A * d.H * d.act_bytes);
+    // (moe_forward_few stores no expert's output row: its shared sums lie there, and only where y is smaller than they are it grows)
+    w.y = take(std::max((size_t)d.A * d.H * d.act_bytes, few_shared_bytes(d.H, d.few_parts)));
+    w.few_arrived = w.y + few_sum_bytes(d.H, d.few_parts);
     // bf16 copies of an e4m3 layer's expert weights (up, down, gate), rewritten by every call of such a plan
     w.wide = take(d.wide_in_workspace ? (size_t)d.wide_mats * d.E * d.I * d.H * 2 : 0);
     // e4m3 x e4m3 plan: token rows and intermediate rows as e4m3 codes + one fp32 scale per (row, 128 columns)
@@ -181,10 +196,6 @@ WsLayout layout(const Derived& d) {
     w.split_part = take(split_tiles * d.plan.ksplit * ((size_t)d.plan.block_m * bf16_block_n1(d.plan.tile)) * 4);
     w.x_pieces = take(d.f32_pieces ? (size_t)d.S * d.H * 6 : 0);
     w.w_pieces = take(d.f32_pieces ? (size_t)d.wide_mats * d.E * d.I * d.H * 6 : 0);
-    // moe_forward_few: sums of workgroups that share columns
-    const int parts = d.S <= kFewTokens && d.act_bytes == 2 ? few_parts(d.H) : 1;
-    w.few_part = take(parts > 1 ? (size_t)d.H / 16 * parts * 1024 : 0);
-    w.few_arrived = take(parts > 1 ? (size_t)d.H / 16 * 4 : 0);
     w.total = off;
     return w;
 }
@@ -979,7 +990,7 @@ int moe_forward_few(moe_handle* h, const void* x, const moe_weights* w, const mo
     if (hipGetDevice(&dev) != hipSuccess || dev != h->arch.device) return MOE_ERR_BAD_ARGUMENT;
     const Derived& d = h->d;
     const bool sw = h->cfg.hidden_act == MOE_ACT_SWIGLU, f16 = d.act_dtype == MOE_DTYPE_FP16;
-    if (d.act_dtype == MOE_DTYPE_F32 || h->cfg.torch_dtype == MOE_DTYPE_FP8_E4M3_B128 || d.S > kFewTokens || (mx && f16)) return MOE_ERR_UNSUPPORTED;
+    if (!d.few_parts || (mx && f16)) return MOE_ERR_UNSUPPORTED;
     if (!w->gate_w || !w->w_up || !w->w_down || sw != (w->w_gate != nullptr) || (!sw && w->b_gate)) return MOE_ERR_BAD_ARGUMENT;
     if (w->s_up || w->s_down || w->s_gate || w->prepared) return MOE_ERR_BAD_ARGUMENT;
     if (mx && (!mx->s_up || !mx->s_down || sw != (mx->s_gate != nullptr))) return MOE_ERR_BAD_ARGUMENT;
@@ -1001,9 +1012,9 @@ int moe_forward_few(moe_handle* h, const void* x, const moe_weights* w, const mo
     a.topk_w = at<float>(workspace, h->ws.topk_w);
     a.h = at<char>(workspace, h->ws.h);
     a.out = out;
-    a.part = at<float>(workspace, h->ws.few_part);
+    a.part = at<float>(workspace, h->ws.y);
     a.arrived = at<int32_t>(workspace, h->ws.few_arrived);
-    a.parts = few_parts(d.H);
+    a.parts = d.few_parts;
     if (routing) a.r = *routing;
     a.S = d.S, a.H = d.H, a.I = d.I, a.E = d.E, a.k = d.k;
     a.act = h->cfg.hidden_act, a.gate_fn = h->cfg.gate_fn, a.norm = h->cfg.norm_topk_prob;
