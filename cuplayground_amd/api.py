@@ -576,14 +576,18 @@ class MoELayer:
         stages one by one, the projections by expert_gemm_mxfp4."""
         if not self._mxfp4_weights(weights):
             raise TypeError("forward_mxfp4 takes expert weights from quantize_mxfp4")
+        cfg, gated = self.cfg, self.cfg.hidden_act == ACT_SWIGLU
+        needed = {"gate_w", "w_up", "w_down", "s_up", "s_down"} | ({"w_gate", "s_gate"} if gated else set())
+        given = {n for n, t in weights.items() if t is not None}
+        if needed - given:
+            raise ValueError("missing tensors %s" % sorted(needed - given))
+        others = given - needed - {"gate_bias", "b_up", "b_down"} - ({"b_gate"} if gated else set())
+        if others:
+            raise ValueError("tensors %s do not belong to this layer" % sorted(others))
         if self.S <= FEW_TOKENS:
             return self.forward_few(x, weights)
-        cfg, gated = self.cfg, self.cfg.hidden_act == ACT_SWIGLU
         self._few_weights(weights)
         _device_operand("x", x, self.act_dtype, (self.S, self.H))
-        missing = [n for n in ("gate_w", "w_up", "w_down", "s_down") + (("w_gate", "s_gate") if gated else ()) if weights.get(n) is None]
-        if missing:
-            raise ValueError("missing tensors %s" % missing)
         idx, gate = self.gate(x, weights["gate_w"], weights.get("gate_bias"))
         r = self.route(idx)
         count, offset = r["expert_count"], r["expert_offset"]

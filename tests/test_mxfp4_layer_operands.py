@@ -1,0 +1,70 @@
+"""What the MXFP4 layer looks at before its first launch, alike for a few tokens and for many: on the CPU, with entry points that fail
+when they are reached."""
+import pytest
+import torch
+
+import cuplayground_amd as moe
+from cuplayground_amd import api
+
+SIDES = pytest.mark.parametrize("S", [11, 40])
+E, H, I = 4, 64, 96
+
+
+class _Launched(Exception):
+    pass
+
+
+def _layer(monkeypatch, S, act=api.ACT_SWIGLU, dtype=api.DTYPE_BF16):
+    """A layer without a handle; _Launched says that a call got as far as an entry point of the library."""
+    layer = api.MoELayer.__new__(api.MoELayer)
+    layer.cfg = moe.MoEConfig(expert_top_k=2, hidden_act=act, hidden_size=H, intermediate_size=I, micro_batch=1, num_experts=E, sequence_len=S, torch_dtype=dtype)
+    layer.S, layer.k, layer.E, layer.H, layer.act_dtype = S, 2, E, H, api._torch_act_dtype(dtype)
+    layer._h = layer.workspace = None
+    layer.workspace_bytes = 0
+
+    def launched(*a):
+        raise _Launched
+    layer.L = type("L", (), dict.fromkeys([n for n in api.EXPORTS if n != "moe_destroy"], staticmethod(launched)))
+    monkeypatch.setattr(api, "_stream", lambda: None)
+    monkeypatch.setattr(api, "_on_current_device", lambda name, t: None)
+    return layer
+
+
+def _set(act=api.ACT_SWIGLU, dtype=torch.bfloat16):
+    w = {"gate_w": torch.zeros(E, H, dtype=dtype), "gate_bias": torch.zeros(E)}
+    for m in ("up", "down", "gate")[:3 if act == api.ACT_SWIGLU else 2]:
+        N, K = (H, I) if m == "down" else (I, H)
+        w["w_" + m], w["s_" + m] = torch.zeros(E, N, K // 2, dtype=torch.uint8), torch.zeros(E, N, K // 32, dtype=torch.uint8)
+        w["b_" + m] = torch.zeros(E, N, dtype=dtype)
+    return w
+
+
+def _x(S, dtype=torch.bfloat16):
+    return torch.zeros(S, H, dtype=dtype)
+
+
+@SIDES
+@pytest.mark.parametrize("act", [api.ACT_RELU, api.ACT_GELU, api.ACT_SWIGLU])
+def test_a_whole_set_reaches_the_launches(monkeypatch, S, act):
+    layer, w = _layer(monkeypatch, S, act), _set(act)
+    for gone in ((), ("gate_bias", "b_up"), ("b_down",)):
+        for as_none in (False, True):
+            given = {n: None if n in gone else t for n, t in w.items() if as_none or n not in gone}
+            with pytest.raises(_Launched):
+                layer.forward_mxfp4(_x(S), given)
+
+
+@SIDES
+def test_tensors_that_are_not_the_layers_are_refused(monkeypatch, S):
+    """A gate's tensors where the activation has none, prepared operands, unknown names; and missing ones."""
+    layer, w, gated = _layer(monkeypatch, S, api.ACT_GELU), _set(api.ACT_GELU), _set()
+    for name in ("w_gate", "s_gate", "b_gate"):
+        with pytest.raises(ValueError, match=name):
+            layer.forward_mxfp4(_x(S), {**w, name: gated[name]})
+    for name in ("prepared", "extra"):
+        with pytest.raises(ValueError, match=name):
+            layer.forward_mxfp4(_x(S), {**w, name: torch.zeros(16, dtype=torch.uint8)})
+    layer = _layer(monkeypatch, S)
+    for name in ("gate_w", "w_up", "w_gate", "w_down", "s_gate", "s_down"):
+        with pytest.raises(ValueError, match=name):
+            layer.forward_mxfp4(_x(S), {n: t for n, t in gated.items() if n != name})
