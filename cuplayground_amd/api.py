@@ -17,6 +17,7 @@ _LIB_PATH = os.path.join(_HERE, "libmoe355.so")
 DTYPE_F32, DTYPE_TF32, DTYPE_BF16, DTYPE_FP16, DTYPE_FP8 = 0, 1, 2, 3, 4
 DTYPE_MXFP4 = 16               # operands of the MXFP4 entry points (no layer's torch_dtype)
 FEW_TOKENS = 16                # tokens that MoELayer.forward_few takes at most
+_UNSUPPORTED, _BAD_ARGUMENT = 2, 4      # of moe_status, for what is refused in front of a call
 ACT_RELU, ACT_GELU, ACT_SWIGLU, ACT_NONE = 0, 1, 2, 3
 GATE_SOFTMAX, GATE_SIGMOID = 0, 1
 FFN_AUTO, FFN_TILED, FFN_PERSISTENT = 0, 1, 2
@@ -283,6 +284,12 @@ def _device_operand(name, t, dtype, shape):
     _on_current_device(name, t)
 
 
+def _on_16_bytes(name, t):
+    """Operands that are read 16 bytes at a time: refused by name, and before the first of several launches."""
+    if t.data_ptr() % 16:
+        raise MoEError(_BAD_ARGUMENT, "%s does not lie on 16 bytes" % name)
+
+
 def _on_current_device(name, t):
     import torch
     current = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)      # (a tensor on a GPU: the runtime is up)
@@ -539,6 +546,7 @@ class MoELayer:
                 continue
             if name == "gate_w":
                 _device_operand(name, t, act, (E, H))
+                _on_16_bytes(name, t)
             elif name == "gate_bias":
                 _device_operand(name, t, torch.float32, (E,))
             else:
@@ -547,6 +555,7 @@ class MoELayer:
                     _device_operand(name, t, act, (E, N))
                 elif name[0] == "w":
                     _device_operand(name, t, torch.uint8 if mx else act, (E, N, K // 2 if mx else K))
+                    _on_16_bytes(name, t)
                 elif mx and name[:2] == "s_":
                     _device_operand(name, t, torch.uint8, (E, N, K // 32))
                     setattr(sc, name, t.data_ptr())
@@ -562,10 +571,12 @@ class MoELayer:
         S, H, act = self.S, self.H, self.act_dtype
         w, sc = self._few_weights(weights)
         _device_operand("x", x, act, (S, H))
+        _on_16_bytes("x", x)
         if out is None:
             out = torch.empty(S, H, dtype=act, device=x.device)
         else:
             _device_operand("out", out, act, (S, H))
+            _on_16_bytes("out", out)
         r = None if routing is None else C.byref(_CRouting(*[routing[n].data_ptr() for n, _ in _CRouting._fields_]))
         _check(self.L.moe_forward_few(self._h, _ptr(x), C.byref(w), None if sc is None else C.byref(sc), _ptr(out), r, _ptr(self.workspace),
                                       self.workspace_bytes, _stream()), "moe_forward_few")
@@ -576,6 +587,8 @@ class MoELayer:
         stages one by one, the projections by expert_gemm_mxfp4."""
         if not self._mxfp4_weights(weights):
             raise TypeError("forward_mxfp4 takes expert weights from quantize_mxfp4")
+        if self.cfg.torch_dtype != DTYPE_BF16:
+            raise MoEError(_UNSUPPORTED, "expert weights in MXFP4 go with bf16 layers")
         cfg, gated = self.cfg, self.cfg.hidden_act == ACT_SWIGLU
         needed = {"gate_w", "w_up", "w_down", "s_up", "s_down"} | ({"w_gate", "s_gate"} if gated else set())
         given = {n for n, t in weights.items() if t is not None}
@@ -588,6 +601,7 @@ class MoELayer:
             return self.forward_few(x, weights)
         self._few_weights(weights)
         _device_operand("x", x, self.act_dtype, (self.S, self.H))
+        _on_16_bytes("x", x)
         idx, gate = self.gate(x, weights["gate_w"], weights.get("gate_bias"))
         r = self.route(idx)
         count, offset = r["expert_count"], r["expert_offset"]

@@ -68,3 +68,34 @@ def test_tensors_that_are_not_the_layers_are_refused(monkeypatch, S):
     for name in ("gate_w", "w_up", "w_gate", "w_down", "s_gate", "s_down"):
         with pytest.raises(ValueError, match=name):
             layer.forward_mxfp4(_x(S), {n: t for n, t in gated.items() if n != name})
+
+
+def _odd(t):
+    """The same values one element further on than 16 bytes."""
+    flat = torch.zeros(t.numel() + 16, dtype=t.dtype)
+    skip = next(i for i in range(1, 17) if flat[i:].data_ptr() % 16)
+    return flat[skip:skip + t.numel()].view(t.shape)
+
+
+@SIDES
+def test_operands_that_do_not_lie_on_16_bytes_are_refused_by_name(monkeypatch, S):
+    layer, w = _layer(monkeypatch, S), _set()
+    for name in ("gate_w", "w_up", "w_gate", "w_down"):
+        with pytest.raises(moe.MoEError, match=name) as e:
+            layer.forward_mxfp4(_x(S), {**w, name: _odd(w[name])})
+        assert e.value.status == 4
+    with pytest.raises(moe.MoEError, match="x does"):
+        layer.forward_mxfp4(_odd(_x(S)), w)
+    with pytest.raises(_Launched):                   # scales are read byte by byte
+        layer.forward_mxfp4(_x(S), {**w, "s_up": _odd(w["s_up"])})
+    if S <= api.FEW_TOKENS:
+        with pytest.raises(moe.MoEError, match="out does"):
+            layer.forward_few(_x(S), w, out=_odd(_x(S)))
+
+
+@SIDES
+@pytest.mark.parametrize("dtype,act_dtype", [(api.DTYPE_FP16, torch.float16), (api.DTYPE_F32, torch.float32), (api.DTYPE_FP8, torch.bfloat16)])
+def test_layers_of_another_type_are_refused(monkeypatch, S, dtype, act_dtype):
+    with pytest.raises(moe.MoEError) as e:
+        _layer(monkeypatch, S, dtype=dtype).forward_mxfp4(_x(S, act_dtype), _set(dtype=act_dtype))
+    assert e.value.status == 2
