@@ -468,6 +468,8 @@ class MoELayer:
         return out
 
     def _weights(self, weights: dict) -> _CWeights:
+        if self._mxfp4_weights(weights):          # an eighth to a half of the bytes that this layer's kernels would read
+            raise TypeError("expert weights in MXFP4: forward_mxfp4 (or forward_few) takes them")
         w = _CWeights()
         for n in self.WEIGHT_KEYS:
             t = weights.get(n)

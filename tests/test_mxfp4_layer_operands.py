@@ -99,3 +99,15 @@ def test_layers_of_another_type_are_refused(monkeypatch, S, dtype, act_dtype):
     with pytest.raises(moe.MoEError) as e:
         _layer(monkeypatch, S, dtype=dtype).forward_mxfp4(_x(S, act_dtype), _set(dtype=act_dtype))
     assert e.value.status == 2
+
+
+@SIDES
+@pytest.mark.parametrize("dtype", [api.DTYPE_BF16, api.DTYPE_FP8])
+def test_layers_of_wider_weights_refuse_a_set_in_4_bits(monkeypatch, S, dtype):
+    """An e4m3 layer has scales too, and codes of twice the size: it would read past these."""
+    layer, w = _layer(monkeypatch, S, dtype=dtype), _set()
+    layer.L.moe_prepared_bytes = staticmethod(lambda h, n: setattr(n._obj, "value", 256) or 0)
+    for call in (lambda: layer.forward(_x(S), w), lambda: layer.forward(_x(S), w, static_workspace=True),
+                 lambda: layer.prepare_weights(w, out=torch.zeros(256, dtype=torch.uint8))):
+        with pytest.raises(TypeError, match="forward_mxfp4"):
+            call()
