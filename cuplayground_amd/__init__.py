@@ -21,6 +21,7 @@ from .api import (  # noqa: F401
     quantize_mxfp4,
     dequantize_mxfp4,
     gemm_mxfp4,
+    gemm_mxfp4_plan,
     transpose,
 )
 from . import api  # noqa: F401

@@ -32,7 +32,7 @@ EXPORTS = (
     "moe_set_ffn_mode", "moe_get_ffn_mode", "moe_forward", "moe_forward_static", "moe_set_spin_limit", "moe_clear_stall", "moe_gate", "moe_router_stats", "moe_route", "moe_gemm_bias_act", "moe_combine",
     "moe_set_stage_timing", "moe_get_stage_ms", "moe_get_stage_samples", "moe_get_task_counts", "moe_get_queue_balance", "moe_task_trace_bytes", "moe_set_task_trace", "moe_get_task_trace", "moe_measure_mfma_tflops",
     "moe_measure_hbm_read_gbs", "moe_quant_block128", "moe_dequant_block128", "moe_backward_scratch_bytes", "moe_transpose", "moe_expert_gemm",
-    "moe_expert_gemm_act_backward", "moe_expert_gemm_act_backward_supported", "moe_expert_gemm_kn", "moe_expert_gemm_kn_supported", "moe_expert_gemm_pair", "moe_expert_gemm_kn_pair", "moe_expert_wgrads", "moe_expert_wgrad", "moe_act_backward", "moe_bias_grad", "moe_combine_backward", "moe_dispatch_rows", "moe_act_forward", "moe_dispatch_backward", "moe_router_grad_bytes", "moe_combine_router_backward", "moe_dispatch_router_backward", "moe_gate_wgrad", "moe_gate_wgrad_rows", "moe_quant_mxfp4", "moe_dequant_mxfp4", "moe_gemm_mxfp4", "moe_expert_gemm_mxfp4", "moe_forward_few", "moe_last_hip_error", "moe_status_string",
+    "moe_expert_gemm_act_backward", "moe_expert_gemm_act_backward_supported", "moe_expert_gemm_kn", "moe_expert_gemm_kn_supported", "moe_expert_gemm_pair", "moe_expert_gemm_kn_pair", "moe_expert_wgrads", "moe_expert_wgrad", "moe_act_backward", "moe_bias_grad", "moe_combine_backward", "moe_dispatch_rows", "moe_act_forward", "moe_dispatch_backward", "moe_router_grad_bytes", "moe_combine_router_backward", "moe_dispatch_router_backward", "moe_gate_wgrad", "moe_gate_wgrad_rows", "moe_quant_mxfp4", "moe_dequant_mxfp4", "moe_gemm_mxfp4", "moe_gemm_mxfp4_plan", "moe_expert_gemm_mxfp4", "moe_forward_few", "moe_last_hip_error", "moe_status_string",
     "moe_version",
 )
 
@@ -184,6 +184,7 @@ def load_library():
     L.moe_quant_mxfp4.argtypes = [vp, i32, i64, i64, vp, vp, vp]
     L.moe_dequant_mxfp4.argtypes = [vp, vp, i64, i64, i32, vp, vp]
     L.moe_gemm_mxfp4.argtypes = [vp, vp, i32, vp, vp, vp, vp, i64, i64, i64, i32, vp]
+    L.moe_gemm_mxfp4_plan.argtypes = [i64, i64, i64, i32, i32] + [C.POINTER(i32)] * 3
     L.moe_expert_gemm_mxfp4.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, vp, vp]
     L.moe_forward_few.argtypes = [vp, vp, C.POINTER(_CWeights), C.POINTER(_CMxfp4Scales), vp, C.POINTER(_CRouting), vp, C.c_size_t, vp]
     L.moe_last_hip_error.argtypes = [vp]
@@ -1070,6 +1071,15 @@ def gemm_mxfp4(A, w, w_scales, bias=None, act: int = ACT_NONE, a_scales=None):
     _check(load_library().moe_gemm_mxfp4(_ptr(A), _ptr(a_scales), DTYPE_BF16 if a_scales is None else DTYPE_MXFP4, _ptr(w), _ptr(w_scales), _ptr(bias),
                                          _ptr(out), M, N, K, act, _stream()), "moe_gemm_mxfp4")
     return out
+
+
+def gemm_mxfp4_plan(M: int, N: int, K: int, experts: int = 0, rows4: bool = False) -> dict:
+    """Which kernel gemm_mxfp4 takes for these sizes, or (experts > 0) expert_gemm_mxfp4 for M rows on so many experts: rows x columns of a
+    workgroup's tile and the parts of the contraction that its wavefronts share; 16 x 16 or 16 x 32 is the weight streamer, 1 x 1 the kernel
+    of the smallest matrices."""
+    out = [C.c_int32(0) for _ in range(3)]
+    _check(load_library().moe_gemm_mxfp4_plan(M, N, K, experts, DTYPE_MXFP4 if rows4 else DTYPE_BF16, *[C.byref(v) for v in out]), "moe_gemm_mxfp4_plan")
+    return dict(zip(("rows", "columns", "parts"), (v.value for v in out)))
 
 
 def gemm_bias_act(A, B, bias, act: int, tile: int = OPT_AUTO):

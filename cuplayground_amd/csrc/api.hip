@@ -999,7 +999,7 @@ int moe_forward_few(moe_handle* h, const void* x, const moe_weights* w, const mo
     for (const void* p : {w->b_up, w->b_gate, w->b_down})
         if ((uintptr_t)p % 8) return MOE_ERR_BAD_ARGUMENT;
     // 32-bit offsets: a matrix, the intermediate rows
-    if ((int64_t)d.H * d.I * (mx ? 1 : 4) / 2 >= ((int64_t)3 << 30) || (int64_t)d.S * d.k * d.I * 2 >= ((int64_t)3 << 30)) return MOE_ERR_UNSUPPORTED;
+    if ((int64_t)d.H * d.I * (mx ? 1 : 4) / 2 >= kBufferBytes || (int64_t)d.S * d.k * d.I * 2 >= kBufferBytes) return MOE_ERR_UNSUPPORTED;
     const int rc = check_ws(h, workspace, workspace_bytes);
     if (rc) return rc;
     FewArgs a{};
@@ -1247,9 +1247,10 @@ int moe_expert_gemm_mxfp4(moe_handle* h, const void* a_rows, const uint8_t* a_sc
     if (h->cfg.torch_dtype != MOE_DTYPE_BF16) return MOE_ERR_UNSUPPORTED;
     if (!((N == h->d.H && K == h->d.I) || (N == h->d.I && K == h->d.H))) return MOE_ERR_BAD_ARGUMENT;
     const MxProduct p{a_rows, a_scales, w, w_scales, (const uint16_t*)bias, expert_count, expert_offset, (uint16_t*)out_rows, h->d.A, N, K, h->d.E, act};
-    const int rc = check_product_mxfp4(p, a_scales ? MOE_DTYPE_MXFP4 : MOE_DTYPE_BF16);
+    int form;
+    const int rc = check_product_mxfp4(p, a_scales ? MOE_DTYPE_MXFP4 : MOE_DTYPE_BF16, &form);
     if (rc) return rc;
-    const hipError_t e = launch_product_mxfp4(p, MOE_OPT_AUTO, (hipStream_t)stream);
+    const hipError_t e = launch_product_mxfp4(p, form, (hipStream_t)stream);
     return e == hipSuccess ? MOE_OK : hip_fail(h, e);
 }
 

@@ -223,6 +223,7 @@ hipError_t launch_ffn_persistent(const FfnArgs& a, int dtype, const FfnPlan& p, 
 int ffn_persistent_blocks(int dtype, int tile, int compute_units);
 
 // ---- MXFP4 (csrc/mxfp4_quant.hip, csrc/mxfp4_product.hip) and the layer for a few tokens (csrc/few.hip) ----
+constexpr int64_t kBufferBytes = (int64_t)3 << 30;      // a matrix read through one buffer has less: offsets are 32 bits, and some lie behind its end
 hipError_t launch_quant_mxfp4(const void* x, int dtype, int64_t values, void* codes, uint8_t* scales, hipStream_t st);
 hipError_t launch_dequant_mxfp4(const void* codes, const uint8_t* scales, int64_t values, int dtype, void* out, hipStream_t st);
 struct MxProduct {              // out = act(a . w^T + bias), one matrix or (count, offset) one an expert over packed rows
@@ -237,7 +238,7 @@ struct MxProduct {              // out = act(a . w^T + bias), one matrix or (cou
     int64_t M;
     int N, K, E, act;
 };
-int check_product_mxfp4(const MxProduct& p, int a_dtype);       // moe_status
+int check_product_mxfp4(const MxProduct& p, int a_dtype, int* form);      // moe_status; form: which kernel, for the launch
 hipError_t launch_product_mxfp4(const MxProduct& p, int form, hipStream_t st);
 constexpr int kFewTokens = 16;  // tokens a call of the layer for a few tokens takes: columns of a matrix instruction
 struct FewArgs {

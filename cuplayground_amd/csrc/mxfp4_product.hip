@@ -669,29 +669,29 @@ hipError_t launch_small(const MxProduct& p, hipStream_t st) {
     return hipGetLastError();
 }
 
-hipError_t launch_product16(const MxProduct& p, int form, hipStream_t st) {
-    switch (form) {
-        case 0: return launch_stream<false>(p, st);
-        case 1: return launch_tile<MxTile<1, 1, 4, 1, 2, 4>>(p, st);  // 16 x 64
-        case 2: return launch_tile<MxTile<1, 2, 4, 1, 2, 2>>(p, st);  // 32 x 64
-        case 3: return launch_tile<MxTile<1, 3, 4, 1, 2, 3>>(p, st);  // 48 x 64
-        case 4: return launch_tile<MxTile<1, 4, 4, 1, 2>>(p, st);     // 64 x 64
-        case 5: return launch_tile<MxTile<1, 4, 4, 2, 1>>(p, st);     // 64 x 128
-        case 6: return launch_tile<MxTile<1, 6, 4, 2, 1>>(p, st);     // 96 x 128
-        case 7: return launch_tile<MxTile<1, 8, 4, 2, 1>>(p, st);     // 128 x 128
-        default: return launch_tile<MxTile<2, 8, 4, 4, 1>>(p, st);    // 256 x 256
+// Forms: 0 the streamer, from 1 on the tiles of the tables below.  f(the tile's type, as a pointer to nothing).
+template <class F>
+auto with_tile(bool rows4, int form, F f) {
+    if (rows4) {
+        switch (form) {
+            case 1: return f((MxTile4<1, 1, 2, 1, 4>*)nullptr);     // 32 x 64
+            case 2: return f((MxTile4<1, 1, 2, 1, 2>*)nullptr);
+            case 3: return f((MxTile4<1, 2, 2, 1, 2>*)nullptr);     // 64 x 64
+            case 4: return f((MxTile4<1, 2, 4, 1, 1>*)nullptr);     // 64 x 128
+            case 5: return f((MxTile4<2, 2, 2, 2, 1>*)nullptr);     // 128 x 128
+            case 6: return f((MxTile4<2, 2, 4, 2, 1>*)nullptr);     // 128 x 256
+            default: return f((MxTile4<4, 2, 2, 4, 1>*)nullptr);    // 256 x 256
+        }
     }
-}
-hipError_t launch_product4(const MxProduct& p, int form, hipStream_t st) {
     switch (form) {
-        case 0: return launch_stream<true>(p, st);
-        case 1: return launch_tile<MxTile4<1, 1, 2, 1, 4>>(p, st);    // 32 x 64
-        case 2: return launch_tile<MxTile4<1, 1, 2, 1, 2>>(p, st);
-        case 3: return launch_tile<MxTile4<1, 2, 2, 1, 2>>(p, st);    // 64 x 64
-        case 4: return launch_tile<MxTile4<1, 2, 4, 1, 1>>(p, st);    // 64 x 128
-        case 5: return launch_tile<MxTile4<2, 2, 2, 2, 1>>(p, st);    // 128 x 128
-        case 6: return launch_tile<MxTile4<2, 2, 4, 2, 1>>(p, st);    // 128 x 256
-        default: return launch_tile<MxTile4<4, 2, 2, 4, 1>>(p, st);   // 256 x 256
+        case 1: return f((MxTile<1, 1, 4, 1, 2, 4>*)nullptr);       // 16 x 64
+        case 2: return f((MxTile<1, 2, 4, 1, 2, 2>*)nullptr);       // 32 x 64
+        case 3: return f((MxTile<1, 3, 4, 1, 2, 3>*)nullptr);       // 48 x 64
+        case 4: return f((MxTile<1, 4, 4, 1, 2>*)nullptr);          // 64 x 64
+        case 5: return f((MxTile<1, 4, 4, 2, 1>*)nullptr);          // 64 x 128
+        case 6: return f((MxTile<1, 6, 4, 2, 1>*)nullptr);          // 96 x 128
+        case 7: return f((MxTile<1, 8, 4, 2, 1>*)nullptr);          // 128 x 128
+        default: return f((MxTile<2, 8, 4, 4, 1>*)nullptr);         // 256 x 256
     }
 }
 
@@ -735,9 +735,10 @@ int product_form(const MxProduct& p) {
     return form;
 }
 
+constexpr int kSmallForm = -1;
 bool is_small(const MxProduct& p) { return (int64_t)p.N * p.K < 256 || (p.a_scales && p.M * p.K < 256); }      // eight scales are fetched at a time
 int64_t product_workgroups(const MxProduct& p, int form) {
-    if (is_small(p)) return (p.M * p.N + 255) / 256;
+    if (form == kSmallForm) return (p.M * p.N + 255) / 256;
     if (form == 0) return mx_grid(p, 16, 16);               // its narrowest
     const TileCost& t = p.a_scales ? kTiles4[form] : kTiles16[form];
     return mx_grid(p, t.rows, t.columns);
@@ -745,24 +746,25 @@ int64_t product_workgroups(const MxProduct& p, int form) {
 
 }  // namespace
 
-// form: MOE_OPT_AUTO, or the kernel asked for
 hipError_t launch_product_mxfp4(const MxProduct& p, int form, hipStream_t st) {
     if (p.M == 0) return hipSuccess;
-    if (is_small(p)) return p.a_scales ? launch_small<true>(p, st) : launch_small<false>(p, st);
-    if (form < 0) form = product_form(p);
-    return p.a_scales ? launch_product4(p, form, st) : launch_product16(p, form, st);
+    const bool rows4 = p.a_scales != nullptr;
+    if (form == kSmallForm) return rows4 ? launch_small<true>(p, st) : launch_small<false>(p, st);
+    if (form == 0) return rows4 ? launch_stream<true>(p, st) : launch_stream<false>(p, st);
+    return with_tile(rows4, form, [&](auto* t) { return launch_tile<std::remove_pointer_t<decltype(t)>>(p, st); });
 }
 
-// What the kernels read and write at a time, their 32-bit offsets and the launches' sizes.
-int check_product_mxfp4(const MxProduct& p, int a_dtype) {
+// What the kernels read and write at a time, their 32-bit offsets and the launches' sizes; and the kernel that the product takes.
+int check_product_mxfp4(const MxProduct& p, int a_dtype, int* form) {
     auto aligned = [](const void* a) { return (uintptr_t)a % 16 == 0; };
     if (p.M < 0 || p.N < 1 || p.K < kMxBlock || p.K % kMxBlock || !p.w || !p.s) return MOE_ERR_BAD_ARGUMENT;
     if (p.act != MOE_ACT_RELU && p.act != MOE_ACT_GELU && p.act != MOE_ACT_NONE) return MOE_ERR_BAD_ARGUMENT;
     if (a_dtype != MOE_DTYPE_BF16 && a_dtype != MOE_DTYPE_MXFP4) return MOE_ERR_UNSUPPORTED;
     if (p.M > 0 && (!p.a || !p.out || (a_dtype == MOE_DTYPE_MXFP4) != (p.a_scales != nullptr))) return MOE_ERR_BAD_ARGUMENT;
     if (!aligned(p.a) || !aligned(p.w) || !aligned(p.out) || (uintptr_t)p.bias % 2) return MOE_ERR_BAD_ARGUMENT;
-    if (p.K > (1 << 20) || (int64_t)p.N * (p.K / 2) >= ((int64_t)3 << 30) || p.M > INT32_MAX) return MOE_ERR_UNSUPPORTED;
-    return product_workgroups(p, product_form(p)) < ((int64_t)1 << 22) ? MOE_OK : MOE_ERR_UNSUPPORTED;      // 1024 threads each: 2^32
+    if (p.K > (1 << 20) || (int64_t)p.N * (p.K / 2) >= kBufferBytes || p.M > INT32_MAX) return MOE_ERR_UNSUPPORTED;
+    *form = is_small(p) ? kSmallForm : product_form(p);
+    return product_workgroups(p, *form) < ((int64_t)1 << 22) ? MOE_OK : MOE_ERR_UNSUPPORTED;      // 1024 threads each: 2^32
 }
 
 }  // namespace moe355
@@ -774,7 +776,33 @@ extern "C" int moe_gemm_mxfp4(const void* a, const uint8_t* a_scales, int32_t a_
     if (M < 0 || N < 1 || K < 1) return MOE_ERR_BAD_ARGUMENT;
     if (N > INT32_MAX / 2 || K > INT32_MAX / 2) return MOE_ERR_UNSUPPORTED;
     const MxProduct p{a, a_scales, w, w_scales, (const uint16_t*)bias, nullptr, nullptr, (uint16_t*)out, M, (int)N, (int)K, 1, act};
-    const int rc = check_product_mxfp4(p, a_dtype);
+    int form;
+    const int rc = check_product_mxfp4(p, a_dtype, &form);
     if (rc) return rc;
-    return launch_product_mxfp4(p, MOE_OPT_AUTO, (hipStream_t)stream) == hipSuccess ? MOE_OK : MOE_ERR_HIP;
+    return launch_product_mxfp4(p, form, (hipStream_t)stream) == hipSuccess ? MOE_OK : MOE_ERR_HIP;
+}
+
+extern "C" int moe_gemm_mxfp4_plan(int64_t M, int64_t N, int64_t K, int32_t experts, int32_t a_dtype, int32_t* rows, int32_t* columns, int32_t* parts) {
+    if (M < 1 || N < 1 || K < 1 || experts < 0 || experts > kMaxExperts || !rows || !columns || !parts) return MOE_ERR_BAD_ARGUMENT;
+    if (N > INT32_MAX / 2 || K > INT32_MAX / 2) return MOE_ERR_UNSUPPORTED;
+    // an operand that is there, as far as the choice looks at it
+    alignas(16) static const uint8_t some[16] = {};
+    alignas(16) static uint16_t result[8];
+    const int32_t* const table = experts ? reinterpret_cast<const int32_t*>(some) : nullptr;
+    const MxProduct p{some, a_dtype == MOE_DTYPE_MXFP4 ? some : nullptr, some, some, nullptr, table, table, result, M, (int)N, (int)K, experts ? experts : 1, MOE_ACT_NONE};
+    int form;
+    const int rc = check_product_mxfp4(p, a_dtype, &form);
+    if (rc) return rc;
+    if (form == kSmallForm) {
+        *rows = *columns = *parts = 1;
+    } else if (form == 0) {
+        const StreamCut c = stream_cut(p);
+        *rows = 16, *columns = c.wide ? 32 : 16, *parts = c.KS;
+    } else {
+        with_tile(a_dtype == MOE_DTYPE_MXFP4, form, [&](auto* t) {
+            typedef std::remove_pointer_t<decltype(t)> T;
+            *rows = T::BM, *columns = T::BN, *parts = T::KS;
+        });
+    }
+    return MOE_OK;
 }

@@ -30,7 +30,6 @@ typedef __attribute__((address_space(3))) void sk_lds_void;
 constexpr uint32_t kBehind = 0xD0000000u;      // an offset behind the end of every buffer here, also with a tile's rows added to it (offsets
                                                // are whole in the vector register: the range check is against what a scalar offset leaves of the
                                                // buffer, and that may be less than nothing)
-constexpr int64_t kBufferBytes = (int64_t)3 << 30;      // what a buffer may have at most
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_buffer(const void* p, uint32_t bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00020000);
 }

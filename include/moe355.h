@@ -418,10 +418,15 @@ int moe_quant_mxfp4(const void* x, int32_t src_dtype, int64_t rows, int64_t K, v
 int moe_dequant_mxfp4(const void* codes, const uint8_t* scales, int64_t rows, int64_t K, int32_t dst_dtype, void* out, void* stream);
 /* moe_gemm_bias_act on such a matrix: out [M, N] (bf16) = act(a . w^T + bias), w [N, K] in MXFP4, bias [N] bf16 or null, act RELU, GELU or
  * NONE.  a [M, K]: bf16 (a_dtype = MOE_DTYPE_BF16, a_scales null; the weights are widened exactly, the products are bf16's) or MXFP4
- * (a_dtype = MOE_DTYPE_MXFP4, codes with a_scales).  Sums in fp32, rounded once.  a, w and out 16-byte aligned; any M (0: nothing is done)
- * and N, K a multiple of 32.  MOE_ERR_UNSUPPORTED: other types, a matrix of 3 GiB and more. */
+ * (a_dtype = MOE_DTYPE_MXFP4, codes with a_scales).  Sums in fp32, rounded once.  a, w and out 16-byte aligned; any N, any M
+ * below 2^31 (0: nothing is done), K a multiple of 32 up to 2^20.  MOE_ERR_UNSUPPORTED: other types, codes of a matrix of 3 GiB and more,
+ * more workgroups than a launch takes (2^22; with 256 x 256 tiles that is 2.7e11 results). */
 int moe_gemm_mxfp4(const void* a, const uint8_t* a_scales, int32_t a_dtype, const void* w, const uint8_t* w_scales, const void* bias, void* out,
                    int64_t M, int64_t N, int64_t K, int32_t act, void* stream);
+/* Which kernel a product of these sizes takes: moe_gemm_mxfp4's (experts = 0), or moe_expert_gemm_mxfp4's of M rows on so many experts.
+ * *rows x *columns of a workgroup's tile and the *parts of the contraction that its wavefronts share; 16 x 16 or 16 x 32 columns of a
+ * wavefront: the weight streamer; 1 x 1: matrices too small for either.  What the product would be refused for is returned.  Host only. */
+int moe_gemm_mxfp4_plan(int64_t M, int64_t N, int64_t K, int32_t experts, int32_t a_dtype, int32_t* rows, int32_t* columns, int32_t* parts);
 /* moe_expert_gemm (below) on such weights: the rows of every expert of a bf16 layer through its matrix, w [E, N, K] in MXFP4, bias [E, N] or
  * null, rows as above (a_scales null: bf16, else MXFP4).  (N, K) is (H, I) or (I, H).  Rows of no expert are neither read nor written.  No
  * scratch. */
