@@ -569,7 +569,8 @@ class MoELayer:
     def forward_few(self, x, weights: dict, out=None, routing: dict | None = None):
         """out[S,H] = MoE(x) for at most 16 tokens of a bf16 or fp16 layer, in two launches (three with a large router).  Expert weights in
         the layer's type, or (bf16 layers) in MXFP4: w_* from quantize_mxfp4 as uint8 [E,N,K/2], s_* as uint8 [E,N,K/32].  `routing` (from
-        new_routing()) receives the routing result when given."""
+        new_routing()) receives the routing result when given.  Against forward() on 16-bit weights: 162 -> 116 us for 1 token of 8 experts of
+        4096 x 14336, 51 -> 38 of 64 of 2048 x 1408; with 16 tokens 480 -> 489 and 173 -> 168."""
         import torch
         S, H, act = self.S, self.H, self.act_dtype
         w, sc = self._few_weights(weights)
@@ -587,7 +588,8 @@ class MoELayer:
 
     def forward_mxfp4(self, x, weights: dict):
         """out[S,H] = MoE(x) of a bf16 layer whose expert weights are in MXFP4, for any number of tokens: forward_few for a few, else the
-        stages one by one, the projections by expert_gemm_mxfp4."""
+        stages one by one, the projections by expert_gemm_mxfp4.  The stages store what they hand on in bf16: above 16 tokens a SwiGLU
+        layer's two projections and the experts' rows are rounded too, and a token's answer is 0.0039 from 64 bits instead of 0.0024."""
         if not self._mxfp4_weights(weights):
             raise TypeError("forward_mxfp4 takes expert weights from quantize_mxfp4")
         if self.cfg.torch_dtype != DTYPE_BF16:

@@ -7,7 +7,9 @@
 //             few_logits has left them), the selection a token a wavefront, a mask of tokens an expert -- and streams gate and up rows;
 //   few_down  a workgroup owns 16 output columns and goes through all experts that are hit: with the tokens as the columns of the matrix
 //             instruction's result, an expert's share of the combine is a multiply-add on the accumulators, in fp32, and out is written
-//             once.  No expert's output row is ever rounded or stored.
+//             once.  No expert's output row is ever rounded or stored.  The intermediate is rounded to the activations' 16 bits, for it is
+//             an operand of 16-bit matrix instructions: distance from 64 bits 0.0024 in bf16, 0.0017 of it the output's own rounding (0.0029 on
+//             the general path, which rounds the experts' rows too).
 // Weights stream as in skinny.hpp.  The router's sums and selection are those of the general path to the bit (the fixed order of 64
 // partial sums; topk.hpp), and so are slots, drops and packed rows: the intermediate lies where that path would put it.
 //

@@ -272,8 +272,9 @@ __device__ __forceinline__ bool mx_join(mx_f32x4 (&acc)[NT][CG], int ks, int sw,
 // A slab is 128 values: 256 bytes of a token row, 64 of a weight row, of which a lane's 16 are a whole block and, widened, four fragments
 // (skinny.hpp).  Scales go through registers: two stages of a 128 x 128 tile's operands are half of the LDS to the byte.
 // What bounds it: on large products the matrix instructions, 8192 x 14336 x 4096 by 256 x 256 in 657 us, 1.46 PFLOP/s (a product of bf16
-// by the library: 1.45; widening costs an eighth of the products' issue and hides behind the other wavefront of the SIMD).  On few rows, LDS: every
-// wavefront reads all rows of the block, 48 x 14336 x 4096 13.5 us.  On experts of some ninety rows, weights that come from memory for one
+// by the library: 1.45; widening costs an eighth of the products' issue and hides behind the other wavefront of the SIMD).  On few rows, the way
+// of a slab from memory, with one workgroup a compute unit to wait for it: 48 x 14336 x 4096 13.5 us, in which the matrix units and LDS are busy a
+// fifth of the cycles each and wavefronts wait for half of theirs.  On experts of some ninety rows, weights that come from memory for one
 // row block each: 6016 rows, 64 experts of 1408 x 2048, 54 us; some ten less with the weights in the memory-side cache.  Neither a third stage, nor twice
 // the wavefronts, nor one that asks for weight lines ahead of the others shortens that.
 template <int RH_, int NT_, int CW_, int CG_, int KS_, int AHEAD_ = 1>
@@ -443,7 +444,10 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void mx_tile_kernel(
 // A slab is 256 values, 128 bytes of every row, both operands in LDS.  Products are 32 x 32 over 64 values: the scaled instruction of that
 // shape takes 33 cycles, that of 16 x 16 over 128 values, half as much work, 31 (measured).  A lane's 16 bytes are the block of its
 // row that it multiplies.  NT, CG: 32-row and 32-column blocks of a wavefront.
-// 8192 x 14336 x 4096 by 256 x 256: 275 us, 3.5 PFLOP/s; between tiles there is the way of the first slab and of the results.
+// 8192 x 14336 x 4096 by 256 x 256: 275 us, 3.5 PFLOP/s, where the instruction's own rate is 10 at 2.4 GHz (7.6 at the 1.8 GHz that this runs at).
+// No unit bounds it: the matrix units are busy 45 % of the cycles, LDS a quarter, and wavefronts wait for 30 % of theirs -- every slab of 256 values
+// ends in a wait for all requests and a meeting, with one slab under way and two wavefronts a SIMD; the way of a tile's first slab and of its results
+// is a small part (workgroups that went from tile to tile gained 4 %).
 template <int RH_, int NT_, int CW_, int CG_, int KS_>
 struct MxTile4 {
     static constexpr bool ROWS4 = true;
@@ -722,6 +726,10 @@ int product_form(const MxProduct& p) {
     double best = 3.8 + (rows4 ? 0.03 : 0.2) * rows + c.chunks * rounds * ((c.wide ? 1.3 : 0.5) + (rows4 ? 0.003 : 0.017) * rows);
     if (p.count && each > 16) best = 1e30;               // a row block an expert, at most
     int form = 0;
+    // (whose cost below is memory's.  Rows in MXFP4, without / with it, us, weights of several calls in turn: 64 experts of 1408 x 2048, 88 MiB, one row
+    // each 21.9 / 27.9, 40 rows 24.8 / 31.8; 4 of 4096 x 14336, 112 MiB, one row 27.9 / 25.3; 64 of 2048 x 2048, 128 MiB, 34.7 / 31.0, 80 rows 50.9 / 40.5; 16 of
+    // 4096 x 4096 35.1 / 29.0; 8 of 4096 x 14336, 224 MiB, 45.9 / 47.7, 80 rows 91.5 / 83.9; 64 of 2048 x 7168, 448 MiB, 104.9 / 82.1, 80 rows 157.6 / 143.1.
+    // Rows in bf16 hardly ever get another form by it.)
     const bool cold = experts * p.N * p.K / 2 > ((int64_t)96 << 20);
     const int forms = rows4 ? (int)(sizeof kTiles4 / sizeof kTiles4[0]) : (int)(sizeof kTiles16 / sizeof kTiles16[0]);
     for (int f = 1; f < forms; ++f) {

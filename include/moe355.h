@@ -437,6 +437,8 @@ int moe_expert_gemm_mxfp4(moe_handle* h, const void* a_rows, const uint8_t* a_sc
  * w_down of *w are codes and *mx has their scales (s_* of *w stay NULL); the router and the biases keep the activations' type.  The routing
  * is moe_forward's to the bit, and so are capacity, drops and what `routing` receives.  Sums in fp32; the intermediate rows are rounded to the
  * activations' type, an expert's output rows are not rounded before the combine, so `out` differs from moe_forward's by that rounding.
+ * On 16-bit weights it takes less time than moe_forward up to 4 tokens (1 token: 9 to 44 % less); with 8 to 16 tokens 3 to 14 % less on experts
+ * of 2048 x 1408, and 2 to 4 % more on experts of 4096 x 14336 or 7168 x 2048.
  * Tensors are 16-byte aligned, biases 8-byte (gate_bias and scales as they come).  The workspace is the handle's; one call at a time per
  * workspace.  MOE_ERR_UNSUPPORTED: more tokens, another type of layer, a matrix of
  * 3 GiB and more. */
