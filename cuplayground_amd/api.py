@@ -285,10 +285,10 @@ def _device_operand(name, t, dtype, shape):
     _on_current_device(name, t)
 
 
-def _on_16_bytes(name, t):
-    """Operands that are read 16 bytes at a time: refused by name, and before the first of several launches."""
-    if t.data_ptr() % 16:
-        raise MoEError(_BAD_ARGUMENT, "%s does not lie on 16 bytes" % name)
+def _on_16_bytes(name, t, n=16):
+    """Operands that are read 16 (n) bytes at a time: refused by name, and before the first of several launches."""
+    if t.data_ptr() % n:
+        raise MoEError(_BAD_ARGUMENT, "%s does not lie on %d bytes" % (name, n))
 
 
 def _on_current_device(name, t):
@@ -574,6 +574,9 @@ class MoELayer:
         import torch
         S, H, act = self.S, self.H, self.act_dtype
         w, sc = self._few_weights(weights)
+        for name in ("b_up", "b_gate", "b_down"):
+            if weights.get(name) is not None:
+                _on_16_bytes(name, weights[name], 8)
         _device_operand("x", x, act, (S, H))
         _on_16_bytes("x", x)
         if out is None:
@@ -629,6 +632,8 @@ class MoELayer:
             raise ValueError("expert_gemm_mxfp4 takes a matrix for every expert")
         N, K, A = w.shape[1], 2 * w.shape[2], self.S * self.k
         _device_operand("w", w, torch.uint8, (self.E, N, K // 2))
+        for name, t in (("w", w), ("a_rows", a_rows)) + (() if out is None else (("out", out),)):
+            _on_16_bytes(name, t)
         _device_operand("w_scales", w_scales, torch.uint8, (self.E, N, K // 32))
         if a_scales is None:
             _device_operand("a_rows", a_rows, torch.bfloat16, (A, K))
@@ -1069,6 +1074,8 @@ def gemm_mxfp4(A, w, w_scales, bias=None, act: int = ACT_NONE, a_scales=None):
         _device_operand("a_scales", a_scales, torch.uint8, (M, K // 32))
     if bias is not None:
         _device_operand("bias", bias, torch.bfloat16, (N,))
+    _on_16_bytes("A", A)
+    _on_16_bytes("w", w)
     out = torch.empty(M, N, dtype=torch.bfloat16, device=A.device)
     _check(load_library().moe_gemm_mxfp4(_ptr(A), _ptr(a_scales), DTYPE_BF16 if a_scales is None else DTYPE_MXFP4, _ptr(w), _ptr(w_scales), _ptr(bias),
                                          _ptr(out), M, N, K, act, _stream()), "moe_gemm_mxfp4")

@@ -111,3 +111,30 @@ def test_layers_of_wider_weights_refuse_a_set_in_4_bits(monkeypatch, S, dtype):
                  lambda: layer.prepare_weights(w, out=torch.zeros(256, dtype=torch.uint8))):
         with pytest.raises(TypeError, match="forward_mxfp4"):
             call()
+
+
+def test_products_and_few_tokens_name_what_does_not_lie_right(monkeypatch):
+    """... and a bias of the layer for a few tokens that does not lie on 8 bytes; above them any bias will do."""
+    for S in (11, 40):
+        layer, w = _layer(monkeypatch, S), _set()
+        for name in ("b_up", "b_gate", "b_down"):
+            shifted = torch.zeros(w[name].numel() + 1, dtype=torch.bfloat16)[1:].view(w[name].shape)
+            assert shifted.data_ptr() % 8
+            with pytest.raises(moe.MoEError if S <= api.FEW_TOKENS else _Launched, match=name if S <= api.FEW_TOKENS else None):
+                layer.forward_mxfp4(_x(S), {**w, name: shifted})
+    layer, w = _layer(monkeypatch, 11), _set()
+    rows, out, table = torch.zeros(22, H, dtype=torch.bfloat16), torch.zeros(22, I, dtype=torch.bfloat16), torch.zeros(E, dtype=torch.int32)
+
+    def product(a=rows, w=w["w_up"], out=out):
+        return layer.expert_gemm_mxfp4(a, w, _set()["s_up"], None, table, table, out=out)
+
+    with pytest.raises(_Launched):
+        product()
+    for name, kw in (("w", dict(w=_odd(w["w_up"]))), ("a_rows", dict(a=_odd(rows))), ("out", dict(out=_odd(out)))):
+        with pytest.raises(moe.MoEError, match=name + " does") as e:
+            product(**kw)
+        assert e.value.status == 4
+    one, scales = w["w_up"][0], w["s_up"][0]
+    for name, a, m in (("A", _odd(rows), one), ("w", rows, _odd(one))):
+        with pytest.raises(moe.MoEError, match=name + " does"):
+            moe.gemm_mxfp4(a, m, scales)
