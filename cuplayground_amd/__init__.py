@@ -22,6 +22,10 @@ from .api import (  # noqa: F401
     dequantize_mxfp4,
     gemm_mxfp4,
     gemm_mxfp4_plan,
+    rms_norm,
+    rms_norm_backward,
+    rms_norm_rows128,
+    act_rows128,
     transpose,
 )
 from . import api  # noqa: F401

@@ -32,7 +32,7 @@ EXPORTS = (
     "moe_set_ffn_mode", "moe_get_ffn_mode", "moe_forward", "moe_forward_static", "moe_set_spin_limit", "moe_clear_stall", "moe_gate", "moe_router_stats", "moe_route", "moe_gemm_bias_act", "moe_combine",
     "moe_set_stage_timing", "moe_get_stage_ms", "moe_get_stage_samples", "moe_get_task_counts", "moe_get_queue_balance", "moe_task_trace_bytes", "moe_set_task_trace", "moe_get_task_trace", "moe_measure_mfma_tflops",
     "moe_measure_hbm_read_gbs", "moe_quant_block128", "moe_dequant_block128", "moe_backward_scratch_bytes", "moe_transpose", "moe_expert_gemm",
-    "moe_expert_gemm_act_backward", "moe_expert_gemm_act_backward_supported", "moe_expert_gemm_kn", "moe_expert_gemm_kn_supported", "moe_expert_gemm_pair", "moe_expert_gemm_kn_pair", "moe_expert_wgrads", "moe_expert_wgrad", "moe_act_backward", "moe_bias_grad", "moe_combine_backward", "moe_dispatch_rows", "moe_act_forward", "moe_dispatch_backward", "moe_router_grad_bytes", "moe_combine_router_backward", "moe_dispatch_router_backward", "moe_gate_wgrad", "moe_gate_wgrad_rows", "moe_quant_mxfp4", "moe_dequant_mxfp4", "moe_gemm_mxfp4", "moe_gemm_mxfp4_plan", "moe_expert_gemm_mxfp4", "moe_forward_few", "moe_last_hip_error", "moe_status_string",
+    "moe_expert_gemm_act_backward", "moe_expert_gemm_act_backward_supported", "moe_expert_gemm_kn", "moe_expert_gemm_kn_supported", "moe_expert_gemm_pair", "moe_expert_gemm_kn_pair", "moe_expert_wgrads", "moe_expert_wgrad", "moe_act_backward", "moe_bias_grad", "moe_combine_backward", "moe_dispatch_rows", "moe_act_forward", "moe_dispatch_backward", "moe_router_grad_bytes", "moe_combine_router_backward", "moe_dispatch_router_backward", "moe_gate_wgrad", "moe_gate_wgrad_rows", "moe_quant_mxfp4", "moe_dequant_mxfp4", "moe_gemm_mxfp4", "moe_gemm_mxfp4_plan", "moe_expert_gemm_mxfp4", "moe_forward_few", "moe_rms_norm", "moe_rms_norm_scratch_bytes", "moe_rms_norm_backward", "moe_act_rows128", "moe_last_hip_error", "moe_status_string",
     "moe_version",
 )
 
@@ -187,6 +187,10 @@ def load_library():
     L.moe_gemm_mxfp4_plan.argtypes = [i64, i64, i64, i32, i32] + [C.POINTER(i32)] * 3
     L.moe_expert_gemm_mxfp4.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, vp, vp]
     L.moe_forward_few.argtypes = [vp, vp, C.POINTER(_CWeights), C.POINTER(_CMxfp4Scales), vp, C.POINTER(_CRouting), vp, C.c_size_t, vp]
+    L.moe_rms_norm.argtypes = [vp, vp, vp, i64, i32, C.c_float, i32, i32, vp, vp, vp, vp, vp]
+    L.moe_rms_norm_scratch_bytes.argtypes = [i64, i32, C.POINTER(C.c_size_t)]
+    L.moe_rms_norm_backward.argtypes = [vp, vp, vp, vp, i64, i32, C.c_float, i32, i32, vp, vp, vp, C.c_size_t, vp]
+    L.moe_act_rows128.argtypes = [vp, vp, i64, i32, i32, vp, vp, i32, vp, vp, vp]
     L.moe_last_hip_error.argtypes = [vp]
     L.moe_status_string.argtypes = [C.c_int]; L.moe_status_string.restype = C.c_char_p
     L.moe_version.restype = C.c_int
@@ -1089,6 +1093,97 @@ def gemm_mxfp4_plan(M: int, N: int, K: int, experts: int = 0, rows4: bool = Fals
     out = [C.c_int32(0) for _ in range(3)]
     _check(load_library().moe_gemm_mxfp4_plan(M, N, K, experts, DTYPE_MXFP4 if rows4 else DTYPE_BF16, *[C.byref(v) for v in out]), "moe_gemm_mxfp4_plan")
     return dict(zip(("rows", "columns", "parts"), (v.value for v in out)))
+
+
+def _norm_operands(x, weight, **others):
+    """(rows, H, the rows' type, the weight's); every operand lies on the current GPU, in one piece and in the shape of x."""
+    import torch
+    known = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_FP16}
+    if x.dtype not in known:
+        raise TypeError("rows of %s: the norm takes fp32, bf16 and fp16" % x.dtype)
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError("the norm takes rows of at least one value")
+    H = x.shape[-1]
+    if weight.dtype != torch.float32:
+        _device_operand("weight", weight, x.dtype, (H,))
+    else:
+        _device_operand("weight", weight, torch.float32, (H,))
+    for name, t in dict(others, x=x).items():
+        if t is not None:
+            _device_operand(name, t, x.dtype, x.shape)
+    return x.numel() // H, H, known[x.dtype], known[weight.dtype]
+
+
+def rms_norm(x, weight, eps: float = 1e-6, residual=None):
+    """y = h * weight / sqrt(mean of h^2 + eps) over the last dimension, h = x + residual rounded to x's type: y, or (y, h) with a residual.
+    fp32, bf16 or fp16 of any shape [.., H], H up to 16384; weight [H] in that type or in fp32."""
+    import torch
+    rows, H, dtype, wdtype = _norm_operands(x, weight, residual=residual)
+    out = torch.empty_like(x)
+    h = None if residual is None else torch.empty_like(x)
+    _check(load_library().moe_rms_norm(_ptr(x), _ptr(residual), _ptr(weight), rows, H, eps, dtype, wdtype, _ptr(h), _ptr(out), None, None, _stream()),
+           "moe_rms_norm")
+    return out if residual is None else (out, h)
+
+
+def rms_norm_backward(dout, h, weight, eps: float = 1e-6, dsum=None):
+    """(dx, dweight) of rms_norm: h is what was normalised (x, or the sum with the residual), dsum the gradient that h has from elsewhere
+    (None: none).  dx is the gradient of x and of the residual alike; dweight has the weight's type."""
+    import torch
+    rows, H, dtype, wdtype = _norm_operands(h, weight, dout=dout, dsum=dsum)
+    L = load_library()
+    n = C.c_size_t(0)
+    _check(L.moe_rms_norm_scratch_bytes(rows, H, C.byref(n)), "moe_rms_norm_scratch_bytes")
+    scratch = torch.empty(n.value, dtype=torch.uint8, device=h.device)
+    dx, dweight = torch.empty_like(h), torch.empty_like(weight)
+    _check(L.moe_rms_norm_backward(_ptr(dout), _ptr(h), _ptr(weight), _ptr(dsum), rows, H, eps, dtype, wdtype, _ptr(dx), _ptr(dweight), _ptr(scratch),
+                                   n.value, _stream()), "moe_rms_norm_backward")
+    return dx, dweight
+
+
+def rms_norm_rows128(x, weight, eps: float = 1e-6, residual=None, want_rows: bool = False):
+    """rms_norm with its result in e4m3, one scale for 128 values of a row (the format of quantize_rows128, from the fp32 values): (uint8 codes
+    [.., H], fp32 scales [.., H/128], the rows in x's type or None, h or None).  H a multiple of 128.  One pass where rms_norm and
+    quantize_rows128 are two."""
+    import torch
+    rows, H, dtype, wdtype = _norm_operands(x, weight, residual=residual)
+    if H % 128:
+        raise ValueError("rows of %d values: rows in e4m3 hold a multiple of 128" % H)
+    for name, t in (("x", x), ("weight", weight), ("residual", residual)):
+        if t is not None:
+            _on_16_bytes(name, t)
+    q = torch.empty(x.shape, dtype=torch.uint8, device=x.device)
+    s = torch.empty(*x.shape[:-1], H // 128, dtype=torch.float32, device=x.device)
+    out = torch.empty_like(x) if want_rows else None
+    h = None if residual is None else torch.empty_like(x)
+    _check(load_library().moe_rms_norm(_ptr(x), _ptr(residual), _ptr(weight), rows, H, eps, dtype, wdtype, _ptr(h), _ptr(out), _ptr(q), _ptr(s), _stream()),
+           "moe_rms_norm")
+    return q, s, out, h
+
+
+def act_rows128(u_rows, g_rows, act: int, expert_count=None, expert_offset=None):
+    """silu(g) * u (ACT_SWIGLU), gelu(u) or relu(u) (g_rows None) of bf16 rows [R, I], I a multiple of 128, in e4m3 with one scale for 128 values of
+    a row: (uint8 codes [R, I], fp32 scales [R, I/128]), rows of gemm_block128.  With a route's expert_count and expert_offset the rows of no
+    expert are neither read nor written."""
+    import torch
+    if u_rows.dim() != 2 or u_rows.shape[1] % 128 or u_rows.shape[1] == 0:
+        raise ValueError("u_rows has shape %s: expected rows of a multiple of 128 values" % (tuple(u_rows.shape),))
+    for name, t in (("u_rows", u_rows), ("g_rows", g_rows)):
+        if t is not None:
+            _device_operand(name, t, torch.bfloat16, u_rows.shape)
+            _on_16_bytes(name, t)
+    R, I = u_rows.shape
+    if (expert_count is None) != (expert_offset is None):
+        raise ValueError("expert_count and expert_offset go together")
+    E = 0 if expert_count is None else expert_count.numel()
+    for name, t in (("expert_count", expert_count), ("expert_offset", expert_offset)):
+        if t is not None:
+            _device_operand(name, t, torch.int32, (E,))
+    q = torch.empty(R, I, dtype=torch.uint8, device=u_rows.device)
+    s = torch.empty(R, I // 128, dtype=torch.float32, device=u_rows.device)
+    _check(load_library().moe_act_rows128(_ptr(u_rows), _ptr(g_rows), R, I, act, _ptr(expert_count), _ptr(expert_offset), E, _ptr(q), _ptr(s), _stream()),
+           "moe_act_rows128")
+    return q, s
 
 
 def gemm_bias_act(A, B, bias, act: int, tile: int = OPT_AUTO):

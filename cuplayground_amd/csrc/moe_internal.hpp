@@ -268,6 +268,36 @@ struct FewArgs {
 inline int few_parts(int H) { return H <= 1024 ? 4 : H <= 2048 ? 2 : 1; }
 hipError_t launch_few(FewArgs a, bool f16, bool mxfp4, hipStream_t st);
 
+// ---- the norm in front of a layer, forth and back (csrc/norm.hip) ----
+constexpr int kNormMost = 16384;                        // values of a row: a layer's widest
+constexpr int64_t kNormRows = ((int64_t)1 << 22) - 1;   // rows of a call: a workgroup of 1024 threads each, and a launch has less than 2^32 threads
+struct NormArgs {
+    const void* x;              // [rows, H]
+    const void* residual;       // [rows, H] or null
+    const void* weight;         // [H] in the rows' type or in fp32
+    void* sum;                  // [rows, H]: x + residual; null without one
+    void* out;                  // [rows, H] or null
+    uint8_t* q;                 // [rows, H] e4m3 codes, or null
+    float* scales;              // [rows, H / 128]
+    int64_t rows;
+    int H;
+    float eps;
+    bool weight_f32;
+};
+struct NormBackwardArgs {
+    const void* dy;             // [rows, H]
+    const void* h;              // [rows, H] what was normalised
+    const void* weight;
+    const void* dsum;           // [rows, H] or null: the gradient of h that comes from elsewhere
+    void* dx;                   // [rows, H]
+    void* dw;                   // [H] in the weight's type
+    float* part;                // scratch: [norm_parts(rows)][H]
+    int64_t rows;
+    int H;
+    float eps;
+    bool weight_f32;
+};
+
 // ---- backward building blocks (csrc/backward.hip) ----
 size_t backward_scratch_bytes(int64_t A, int E, int H, int I, int elem_bytes);
 hipError_t launch_transpose(const void* src, void* dst, int64_t batch, int64_t rows, int64_t cols, int elem_bytes,

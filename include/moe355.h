@@ -450,6 +450,31 @@ typedef struct moe_mxfp4_scales {
 int moe_forward_few(moe_handle* h, const void* x, const moe_weights* w, const moe_mxfp4_scales* mx, void* out, const moe_routing_out* routing,
                     void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- The norm in front of a layer -------------------------------------------------------------------------------------
+ * The reference has no norm; a layer of experts stands behind one, in a residual stream.  Asynchronous on `stream`, nothing is allocated,
+ * everything can be captured into a graph.
+ *
+ * moe_rms_norm: h = x + residual, rounded to the rows' type and stored in `sum` (residual = sum = NULL: h = x); y = h * weight / sqrt(mean of
+ *   the row's h^2 + eps), in fp32.  x, residual, sum and out are [rows, H] in `dtype` (fp32, bf16, fp16), weight [H] in that type or in fp32
+ *   (weight_dtype).  y goes to `out`, rounded once, and / or to q [rows, H] and scales [rows, H / 128] in e4m3 with a scale for 128 values, the
+ *   format of moe_quant_rows128, from the fp32 values (scale = amax / 448, not below 2^-126): rows of a product with block scales.  Either may
+ *   be NULL, not both.  sum may be x or residual; else nothing overlaps.  The squares' mean has to be a number of fp32.  H up to 16384; with q
+ *   a multiple of 128, and x, residual, weight, sum and out 16-byte aligned (else elements may lie anywhere that whole ones can), q 8-byte.
+ *   rows < 2^22; 0: nothing is done.  MOE_ERR_UNSUPPORTED: other types, longer rows, more of them.
+ * moe_rms_norm_backward: from dout = dL/dout, h (what was normalised: x, or `sum`) and, where h goes on to elsewhere, dsum = dL/dh from there
+ *   (or NULL): dx [rows, H] = dL/dx (= dL/dresidual), rounded once, and dweight [H] in the weight's type.  Sums in fp32, in a fixed
+ *   order: the same inputs give the same bits.  scratch: moe_rms_norm_scratch_bytes, 4-byte aligned, overwritten.  rows = 0: dweight = 0.
+ * moe_act_rows128: the experts' activation with its result in that format: silu(g) * u (act SWIGLU), gelu(u) or relu(u) (g = NULL) of bf16
+ *   rows [rows, I], I a multiple of 128, u and g 16-byte aligned.  With expert_count / expert_offset [E] (of moe_route) only the packed rows
+ *   that belong to an expert are read and written; NULL: all.  MOE_ERR_UNSUPPORTED: 2^24 * 2048 values and more. */
+int moe_rms_norm(const void* x, const void* residual, const void* weight, int64_t rows, int32_t H, float eps, int32_t dtype, int32_t weight_dtype,
+                 void* sum, void* out, void* q, float* scales, void* stream);
+int moe_rms_norm_scratch_bytes(int64_t rows, int32_t H, size_t* bytes);
+int moe_rms_norm_backward(const void* dout, const void* h, const void* weight, const void* dsum, int64_t rows, int32_t H, float eps, int32_t dtype,
+                          int32_t weight_dtype, void* dx, void* dweight, void* scratch, size_t scratch_bytes, void* stream);
+int moe_act_rows128(const void* u, const void* g, int64_t rows, int32_t I, int32_t act, const int32_t* expert_count, const int32_t* expert_offset,
+                    int32_t E, void* q, float* scales, void* stream);
+
 /* ---- Backward building blocks (fp32, tf32, bf16 and fp16 layers; e4m3 layers: MOE_ERR_UNSUPPORTED) ------------------
  * The reference declares a training knob (is_training, aristos_config.schema.json:20-23) that none of its code reads
  * and has no backward pass; these entry points are what a training step needs beyond the forward stages above.  All
