@@ -22,6 +22,8 @@ from .api import (  # noqa: F401
     dequantize_mxfp4,
     gemm_mxfp4,
     gemm_mxfp4_plan,
+    gemm_block128,
+    gemm_block128_plan,
     rms_norm,
     rms_norm_backward,
     rms_norm_rows128,

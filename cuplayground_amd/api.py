@@ -32,7 +32,7 @@ EXPORTS = (
     "moe_set_ffn_mode", "moe_get_ffn_mode", "moe_forward", "moe_forward_static", "moe_set_spin_limit", "moe_clear_stall", "moe_gate", "moe_router_stats", "moe_route", "moe_gemm_bias_act", "moe_combine",
     "moe_set_stage_timing", "moe_get_stage_ms", "moe_get_stage_samples", "moe_get_task_counts", "moe_get_queue_balance", "moe_task_trace_bytes", "moe_set_task_trace", "moe_get_task_trace", "moe_measure_mfma_tflops",
     "moe_measure_hbm_read_gbs", "moe_quant_block128", "moe_dequant_block128", "moe_backward_scratch_bytes", "moe_transpose", "moe_expert_gemm",
-    "moe_expert_gemm_act_backward", "moe_expert_gemm_act_backward_supported", "moe_expert_gemm_kn", "moe_expert_gemm_kn_supported", "moe_expert_gemm_pair", "moe_expert_gemm_kn_pair", "moe_expert_wgrads", "moe_expert_wgrad", "moe_act_backward", "moe_bias_grad", "moe_combine_backward", "moe_dispatch_rows", "moe_act_forward", "moe_dispatch_backward", "moe_router_grad_bytes", "moe_combine_router_backward", "moe_dispatch_router_backward", "moe_gate_wgrad", "moe_gate_wgrad_rows", "moe_quant_mxfp4", "moe_dequant_mxfp4", "moe_gemm_mxfp4", "moe_gemm_mxfp4_plan", "moe_expert_gemm_mxfp4", "moe_forward_few", "moe_rms_norm", "moe_rms_norm_scratch_bytes", "moe_rms_norm_backward", "moe_act_rows128", "moe_last_hip_error", "moe_status_string",
+    "moe_expert_gemm_act_backward", "moe_expert_gemm_act_backward_supported", "moe_expert_gemm_kn", "moe_expert_gemm_kn_supported", "moe_expert_gemm_pair", "moe_expert_gemm_kn_pair", "moe_expert_wgrads", "moe_expert_wgrad", "moe_act_backward", "moe_bias_grad", "moe_combine_backward", "moe_dispatch_rows", "moe_act_forward", "moe_dispatch_backward", "moe_router_grad_bytes", "moe_combine_router_backward", "moe_dispatch_router_backward", "moe_gate_wgrad", "moe_gate_wgrad_rows", "moe_quant_mxfp4", "moe_dequant_mxfp4", "moe_gemm_mxfp4", "moe_gemm_mxfp4_plan", "moe_expert_gemm_mxfp4", "moe_forward_few", "moe_gemm_block128", "moe_gemm_block128_plan", "moe_expert_gemm_block128", "moe_rms_norm", "moe_rms_norm_scratch_bytes", "moe_rms_norm_backward", "moe_act_rows128", "moe_last_hip_error", "moe_status_string",
     "moe_version",
 )
 
@@ -187,6 +187,9 @@ def load_library():
     L.moe_gemm_mxfp4_plan.argtypes = [i64, i64, i64, i32, i32] + [C.POINTER(i32)] * 3
     L.moe_expert_gemm_mxfp4.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, vp, vp]
     L.moe_forward_few.argtypes = [vp, vp, C.POINTER(_CWeights), C.POINTER(_CMxfp4Scales), vp, C.POINTER(_CRouting), vp, C.c_size_t, vp]
+    L.moe_gemm_block128.argtypes = [vp, vp, vp, vp, vp, vp, i64, i64, i64, i32, vp]
+    L.moe_gemm_block128_plan.argtypes = [i64, i64, i64, i32] + [C.POINTER(i32)] * 3
+    L.moe_expert_gemm_block128.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, vp, vp]
     L.moe_rms_norm.argtypes = [vp, vp, vp, i64, i32, C.c_float, i32, i32, vp, vp, vp, vp, vp]
     L.moe_rms_norm_scratch_bytes.argtypes = [i64, i32, C.POINTER(C.c_size_t)]
     L.moe_rms_norm_backward.argtypes = [vp, vp, vp, vp, i64, i32, C.c_float, i32, i32, vp, vp, vp, C.c_size_t, vp]
@@ -293,6 +296,12 @@ def _on_16_bytes(name, t, n=16):
     """Operands that are read 16 (n) bytes at a time: refused by name, and before the first of several launches."""
     if t.data_ptr() % n:
         raise MoEError(_BAD_ARGUMENT, "%s does not lie on %d bytes" % (name, n))
+
+
+def _codes(name, t, shape):
+    """_device_operand of e4m3 codes, as bytes or as float8 values."""
+    import torch
+    _device_operand(name, t, t.dtype if t.dtype == torch.float8_e4m3fn else torch.uint8, shape)
 
 
 def _on_current_device(name, t):
@@ -654,6 +663,35 @@ class MoELayer:
             _device_operand("out", out, torch.bfloat16, (A, N))
         _check(self.L.moe_expert_gemm_mxfp4(self._h, _ptr(a_rows), _ptr(a_scales), _ptr(w), _ptr(w_scales), _ptr(bias), _ptr(expert_count),
                                             _ptr(expert_offset), N, K, act, _ptr(out), _stream()), "moe_expert_gemm_mxfp4")
+        return out
+
+    def expert_gemm_block128(self, a_rows, a_scales, w, w_scales, bias, expert_count, expert_offset, act: int = ACT_NONE, token_indices=None, out=None):
+        """expert_gemm of an e4m3 layer on rows in e4m3: w [E,N,K] codes with w_scales fp32 [E,N/128,K/128]; a_rows codes [S k,K] with a_scales fp32
+        [S k,K/128], the packed rows, or with token_indices (of route()) the tokens' rows [S,K], from which they are fetched.  bf16 rows out;
+        rows of no expert are not written."""
+        import torch
+        if w.dim() != 3:
+            raise ValueError("expert_gemm_block128 takes a matrix for every expert")
+        (_, N, K), A = w.shape, self.S * self.k
+        rows = A if token_indices is None else self.S
+        _codes("w", w, (self.E, N, K))
+        _codes("a_rows", a_rows, (rows, K))
+        _device_operand("w_scales", w_scales, torch.float32, (self.E, (N + 127) // 128, K // 128))
+        _device_operand("a_scales", a_scales, torch.float32, (rows, K // 128))
+        for name, t in (("w", w), ("a_rows", a_rows)) + (() if out is None else (("out", out),)):
+            _on_16_bytes(name, t)
+        if bias is not None:
+            _device_operand("bias", bias, torch.bfloat16, (self.E, N))
+        for name, t in (("expert_count", expert_count), ("expert_offset", expert_offset)):
+            _device_operand(name, t, torch.int32, (self.E,))
+        if token_indices is not None:
+            _device_operand("token_indices", token_indices, torch.int32, (A,))
+        if out is None:
+            out = torch.empty(A, N, dtype=torch.bfloat16, device=w.device)
+        else:
+            _device_operand("out", out, torch.bfloat16, (A, N))
+        _check(self.L.moe_expert_gemm_block128(self._h, _ptr(a_rows), _ptr(a_scales), _ptr(token_indices), _ptr(w), _ptr(w_scales), _ptr(bias),
+                                               _ptr(expert_count), _ptr(expert_offset), N, K, act, _ptr(out), _stream()), "moe_expert_gemm_block128")
         return out
 
     def set_spin_limit(self, polls: int):
@@ -1092,6 +1130,35 @@ def gemm_mxfp4_plan(M: int, N: int, K: int, experts: int = 0, rows4: bool = Fals
     of the smallest matrices."""
     out = [C.c_int32(0) for _ in range(3)]
     _check(load_library().moe_gemm_mxfp4_plan(M, N, K, experts, DTYPE_MXFP4 if rows4 else DTYPE_BF16, *[C.byref(v) for v in out]), "moe_gemm_mxfp4_plan")
+    return dict(zip(("rows", "columns", "parts"), (v.value for v in out)))
+
+
+def gemm_block128(A, a_scales, w, w_scales, bias=None, act: int = ACT_NONE):
+    """C [M,N] (bf16) = act(A.W^T + bias), both in e4m3 (uint8 codes or float8 values): A [M,K] with a scale for 128 values of a row, a_scales fp32
+    [M,K/128]; W [N,K] with one for each block of 128 x 128, w_scales fp32 [ceil(N/128),K/128]."""
+    import torch
+    if w.dim() != 2 or A.dim() != 2:
+        raise ValueError("gemm_block128 takes matrices")
+    M, (N, K) = A.shape[0], w.shape
+    _codes("w", w, (N, K))
+    _codes("A", A, (M, K))
+    _device_operand("w_scales", w_scales, torch.float32, ((N + 127) // 128, K // 128))
+    _device_operand("a_scales", a_scales, torch.float32, (M, K // 128))
+    if bias is not None:
+        _device_operand("bias", bias, torch.bfloat16, (N,))
+    _on_16_bytes("A", A)
+    _on_16_bytes("w", w)
+    out = torch.empty(M, N, dtype=torch.bfloat16, device=A.device)
+    _check(load_library().moe_gemm_block128(_ptr(A), _ptr(a_scales), _ptr(w), _ptr(w_scales), _ptr(bias), _ptr(out), M, N, K, act, _stream()),
+           "moe_gemm_block128")
+    return out
+
+
+def gemm_block128_plan(M: int, N: int, K: int, experts: int = 0) -> dict:
+    """Which kernel gemm_block128 takes for these sizes, or (experts > 0) expert_gemm_block128 for M rows on so many experts: rows x columns of a
+    workgroup's tile and the parts of the contraction that its wavefronts share; 16 x 16 or 16 x 32 is the weight streamer."""
+    out = [C.c_int32(0) for _ in range(3)]
+    _check(load_library().moe_gemm_block128_plan(M, N, K, experts, *[C.byref(v) for v in out]), "moe_gemm_block128_plan")
     return dict(zip(("rows", "columns", "parts"), (v.value for v in out)))
 
 

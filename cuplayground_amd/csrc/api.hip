@@ -1254,6 +1254,23 @@ int moe_expert_gemm_mxfp4(moe_handle* h, const void* a_rows, const uint8_t* a_sc
     return e == hipSuccess ? MOE_OK : hip_fail(h, e);
 }
 
+int moe_expert_gemm_block128(moe_handle* h, const void* a_rows, const float* a_scales, const int32_t* token_indices, const void* w, const float* w_scales,
+                             const void* bias, const int32_t* expert_count, const int32_t* expert_offset, int32_t N, int32_t K, int32_t act, void* out_rows,
+                             void* stream) {
+    if (!h || !expert_count || !expert_offset) return MOE_ERR_BAD_ARGUMENT;
+    int dev = -1;
+    if (hipGetDevice(&dev) != hipSuccess || dev != h->arch.device) return MOE_ERR_BAD_ARGUMENT;
+    if (h->cfg.torch_dtype != MOE_DTYPE_FP8_E4M3_B128) return MOE_ERR_UNSUPPORTED;
+    if (!((N == h->d.H && K == h->d.I) || (N == h->d.I && K == h->d.H))) return MOE_ERR_BAD_ARGUMENT;
+    const RowsProduct p{(const uint8_t*)a_rows, a_scales, (const uint8_t*)w, w_scales, (const uint16_t*)bias, expert_count, expert_offset, token_indices,
+                        (uint16_t*)out_rows, h->d.A, token_indices ? h->d.S : h->d.A, N, K, h->d.E, act};
+    int form;
+    const int rc = check_product_block128(p, &form);
+    if (rc) return rc;
+    const hipError_t e = launch_product_block128(p, form, (hipStream_t)stream);
+    return e == hipSuccess ? MOE_OK : hip_fail(h, e);
+}
+
 int moe_expert_gemm_act_backward(moe_handle* h, const void* dy_rows, const void* w, const void* u_rows, const void* g_rows,
                                  const int32_t* expert_count, const int32_t* expert_offset, int32_t N, int32_t K,
                                  void* du_rows, void* dg_rows, void* scratch, size_t scratch_bytes, void* stream) {

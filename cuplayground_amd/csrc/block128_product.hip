@@ -1,0 +1,446 @@
+// Products of rows in e4m3 (rows8.hpp: a scale for 128 values of a row) with weights in e4m3 that have a scale for each block of 128 x 128:
+//
+//   out[m, n] = act(sum over blocks b of K:  s_a[m, b] s_w[n / 128, b]  (sum over k in b of a[m, k] w[n, k])  + bias[n])
+//
+// One matrix, or a matrix per expert over packed rows, which may be fetched from the tokens' rows by their indices.  The inner sums are one 16 x 16 x
+// 128 matrix instruction each, exact products in fp32; the vector ALU folds them into the accumulators with the product of the two scales, which is
+// one number a lane where the token rows are the instruction's columns.  Sums in fp32, rounded once on store -- but for what the instruction itself does:
+// it adds eight neighbouring products at a time, cut off below 2^-13 of the power of two that the largest begins with (measured).  Against
+// the sum in 64 bits that is 1e-4 of the result's mean square, a tenth of what its rounding to bf16 is.
+//
+// Two kinds of kernel: a weight streamer for up to 16 rows a block, and tiles.  block_form() takes the one whose fitted cost is least.
+#include "grouped_task.hpp"
+#include "product_rows.hpp"
+
+namespace moe355 {
+namespace {
+
+struct RowsTask {
+    const uint8_t* a;         // the block's first row (rows fetched by index: row 0 of all)
+    const float* a_scales;
+    const uint8_t* w;         // the expert's matrix
+    const float* s;
+    const uint16_t* bias;     // of the expert, or null
+    const int32_t* token;     // of the block's rows, or null
+    uint16_t* out;            // at the block's first row
+    int rows, n0;
+};
+
+// Which block of BM rows and which BN columns a workgroup takes.
+template <int BM>
+__device__ __forceinline__ bool rows_task(const RowsProduct& p, int BN, RowsTask& t) {
+    const int ncol = (p.N + BN - 1) / BN;
+    int expert = 0, ctile, rows;
+    int64_t row0;
+    if (p.count) {
+        GroupedTask g;
+        if (!grouped_task<BM>(p.count, p.offset, p.E, ncol, (int)blockIdx.x, g)) return false;
+        expert = g.expert, ctile = g.ctile, row0 = g.row0, rows = g.rows;
+        if (row0 < 0 || row0 + rows > p.M) return false;          // tables that are not this layer's: nothing behind the buffers is touched
+    } else {
+        // an eighth of the tiles in a row for each XCD, kRowChunk row blocks at a time, as for the experts
+        const int blocks = (int)((p.M + BM - 1) / BM);
+        const int64_t total = (int64_t)blocks * ncol, share = (total + 7) / 8;
+        const int64_t id = (int64_t)(blockIdx.x & 7) * share + (blockIdx.x >> 3);
+        if ((int64_t)(blockIdx.x >> 3) >= share || id >= total) return false;
+        int rb = (int)(id / ((int64_t)kRowChunk * ncol)) * kRowChunk;
+        const int width = min(kRowChunk, blocks - rb), local = (int)(id - (int64_t)rb * ncol);
+        ctile = local / width;
+        rb += local - ctile * width;
+        row0 = (int64_t)rb * BM;
+        rows = (int)min((int64_t)BM, p.M - row0);
+    }
+    // the same in every lane, and said so
+    row0 = mx_uniform(row0), expert = __builtin_amdgcn_readfirstlane(expert), ctile = __builtin_amdgcn_readfirstlane(ctile), rows = __builtin_amdgcn_readfirstlane(rows);
+    const int KB = p.K >> 7;
+    const int64_t first = p.token ? 0 : row0;
+    t.a = p.a + first * p.K;
+    t.a_scales = p.a_scales + first * KB;
+    t.w = p.w + (int64_t)expert * p.N * p.K;
+    t.s = p.s + (int64_t)expert * ((p.N + 127) >> 7) * KB;
+    t.bias = p.bias ? p.bias + (int64_t)expert * p.N : nullptr;
+    t.token = p.token ? p.token + row0 : nullptr;
+    t.out = p.out + row0 * p.N;
+    t.rows = rows;
+    t.n0 = ctile * BN;
+    return true;
+}
+// Row r of the block as the buffers below count rows; kNoRow where there is none (an index that is no token's is none).
+constexpr uint32_t kNoRow = 0xFFFFFFFFu;
+__device__ __forceinline__ uint32_t rows_source(const RowsProduct& p, const RowsTask& t, int r) {
+    if (r >= t.rows) return kNoRow;
+    if (!t.token) return (uint32_t)r;
+    const uint32_t i = (uint32_t)t.token[r];
+    return i < (uint32_t)p.tokens ? i : kNoRow;
+}
+// The scales of a call are read-only: through scalar loads.
+typedef const __attribute__((address_space(4))) float rows_cfloat;
+
+__device__ __forceinline__ mx_f32x4 rows_mfma(const mx_i32x8& w, const mx_i32x8& x) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, mx_f32x4{0.f, 0.f, 0.f, 0.f}, 0 /* e4m3 */, 0, 0, 0, 0, 0);
+}
+__device__ __forceinline__ mx_i32x8 rows_operand(const mx_u32x4& lower, const mx_u32x4& upper) {
+    return __builtin_bit_cast(mx_i32x8, __builtin_shufflevector(lower, upper, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// ---- up to 16 rows a block: a weight streamer ----
+//
+// A wavefront owns G groups of 16 columns over its share of the contraction; weights come whole 128-byte lines of eight rows at a time
+// (stream_lines.hpp), which is a block of K, and stay in registers with the token rows' pieces, kDepth blocks on their way.
+constexpr int kRowsWaves = 8, kDepth = 4;
+
+template <int G, bool COLD>
+__global__ __launch_bounds__(64 * kRowsWaves) void rows_stream_kernel(RowsProduct p, int KS) {
+    __shared__ mx_f32x4 red[(kRowsWaves - 1) * G * 64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int ks = wave % KS, set = wave / KS;
+    RowsTask t;
+    if (!rows_task<16>(p, 16 * G * (kRowsWaves / KS), t)) return;
+    const int n0 = t.n0 + 16 * G * set, KB = p.K >> 7;
+    const uint32_t K = (uint32_t)p.K;
+    const int64_t rows_all = p.token ? p.tokens : t.rows;
+    const __amdgpu_buffer_rsrc_t x_buf = mx_buffer(t.a, (uint32_t)(rows_all * K)), w_buf = mx_buffer(t.w, (uint32_t)p.N * K),
+                                 s_buf = mx_buffer(t.a_scales, (uint32_t)(rows_all * KB * 4));
+    const int q = lane >> 4;
+    // (lanes behind the last row: the block's first one again, whose lines are on their way anyway)
+    uint32_t src = rows_source(p, t, (lane & 15) < t.rows ? lane & 15 : 0);
+    const uint32_t x_at = src == kNoRow ? kBehind : src * K + 16 * q, s_at = src == kNoRow ? kBehind : src * (uint32_t)KB * 4;
+    const uint32_t piece = q + ((lane & 8) >> 1);
+    const uint32_t w1 = (uint32_t)(n0 + (lane & 7)) * K + 16 * piece, w2 = (uint32_t)(n0 + 8 + (lane & 7)) * K + 16 * (piece ^ 4);
+    rows_cfloat* const sw = (rows_cfloat*)(uintptr_t)(t.s + (int64_t)min(n0 >> 7, (p.N - 1) >> 7) * KB);
+
+    const int share = (KB + KS - 1) / KS, begin = min(ks * share, KB), end = min(begin + share, KB);
+    mx_u32x4 w[kDepth][G][2], x[kDepth][2];
+    float sa[kDepth];
+    auto fetch = [&](int slot, int c) {            // what lies behind the share's end: zeros
+        const bool in = c < end;
+        const uint32_t at = 128u * (uint32_t)c;
+        x[slot][0] = __builtin_bit_cast(mx_u32x4, __builtin_amdgcn_raw_buffer_load_b128(x_buf, (int)(in ? x_at + at : kBehind), 0, 0));
+        x[slot][1] = __builtin_bit_cast(mx_u32x4, __builtin_amdgcn_raw_buffer_load_b128(x_buf, (int)(in ? x_at + at + 64 : kBehind), 0, 0));
+        sa[slot] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(s_buf, (int)(in ? s_at + 4u * (uint32_t)c : kBehind), 0, 0));
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            w[slot][g][0] = __builtin_bit_cast(mx_u32x4, __builtin_amdgcn_raw_buffer_load_b128(w_buf, (int)(in ? w1 + at + g * 16 * K : kBehind), 0, COLD ? 2 : 0));      // 2: not kept
+            w[slot][g][1] = __builtin_bit_cast(mx_u32x4, __builtin_amdgcn_raw_buffer_load_b128(w_buf, (int)(in ? w2 + at + g * 16 * K : kBehind), 0, COLD ? 2 : 0));
+        }
+    };
+    mx_f32x4 acc[1][G] = {};
+    if (begin < end) {
+#pragma unroll
+        for (int d = 0; d < kDepth; ++d) fetch(d, begin + d);
+        for (int c = begin; c < end; c += kDepth) {
+#pragma unroll
+            for (int d = 0; d < kDepth; ++d) {
+                const float s = sa[d] * (c + d < end ? sw[c + d] : 0.0f);
+                const mx_i32x8 xv = rows_operand(x[d][0], x[d][1]);
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    mx_u32x4 lower, upper;
+                    line_pieces(w[d][g][0], w[d][g][1], lower, upper);
+                    const mx_f32x4 part = rows_mfma(rows_operand(lower, upper), xv);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[0][g][r] = __builtin_fmaf(part[r], s, acc[0][g][r]);
+                }
+                fetch(d, c + d + kDepth);
+            }
+        }
+    }
+    if (!skinny_join<G>(acc[0], ks, KS, red + set * (KS - 1) * G * 64, lane)) return;
+    mx_store_tile<1, G>(p, t, lane & 15, n0 + 4 * q, acc);
+}
+
+// ---- more rows: tiles ----
+//
+// RH x CW wavefronts of 16 NT rows x 16 CG columns each, KS sets of them that share the contraction.  A slab is a block of K: 128 bytes of every row
+// of either operand, straight into LDS AHEAD slabs ahead, and 4 bytes of every token row, its scale.  Everything is read through buffers that end
+// where the operands do: rows behind the block's last one, columns behind the matrix's and what lies behind K are zeros without a branch.
+template <int RH_, int NT_, int CW_, int CG_, int KS_, int AHEAD_>
+struct RowsTile {
+    static constexpr int RH = RH_, NT = NT_, CW = CW_, CG = CG_, KS = KS_, AHEAD = AHEAD_;
+    static constexpr int STAGES = AHEAD + 1;
+    static constexpr int BM = 16 * NT * RH, BN = 16 * CG * CW;
+    static constexpr int SET = RH * CW;
+    static constexpr int THREADS = 64 * SET * KS;
+    static constexpr int LOADS_A = BM / 8 / SET, LOADS_W = BN / 8 / SET;      // an instruction of a wavefront brings 8 rows
+    static constexpr int SCALERS = (BM + 63) / 64;                            // wavefronts of a set that bring scales
+    static constexpr int STAGE = (BM + BN) * 128 + SCALERS * 256;
+    static constexpr int SUMS = (KS - 1) * SET * NT * CG * 1024;
+    static constexpr int OUT = KS == 1 ? SET * mx_rows_lds<NT, CG, 16, 16>() : 0;
+    static constexpr int LDS = std::max(std::max(STAGES * KS * STAGE, SUMS), OUT);
+    static constexpr int BLOCKS = std::min(160 * 1024 / LDS, NT * CG >= 32 ? 8 / (SET * KS) : 16 / (SET * KS));      // workgroups of a compute unit
+    static constexpr int WAVES_PER_SIMD = std::max(1, BLOCKS * THREADS / 256);
+    static_assert(BM % (8 * SET) == 0 && BN % (8 * SET) == 0 && SCALERS <= SET, "every wavefront of a set brings as many rows");
+    static_assert(128 % (16 * CG) == 0, "a wavefront's columns have one scale");
+    static_assert(LDS <= 160 * 1024, "LDS of a compute unit");
+};
+
+template <class T>
+__global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_tile_kernel(RowsProduct p) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    constexpr int NT = T::NT, CG = T::CG, KS = T::KS, SET = T::SET, BM = T::BM, BN = T::BN, AHEAD = T::AHEAD;
+    RowsTask t;
+    if (!rows_task<BM>(p, BN, t)) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int ks = wave / SET, sw = wave % SET;
+    const int wm = sw / T::CW, wn = sw % T::CW;
+    const int idx = lane & 15, q = lane >> 4;
+    const int N = p.N, KB = p.K >> 7;
+    const uint32_t K = (uint32_t)p.K;
+
+    // Rows into LDS: an instruction writes 1 KB of LDS in the order of its lanes.  Piece c (16 bytes) of a row lies in slot c ^ (row / 2): the reads
+    // below meet no bank twice in a cycle.
+    const int lrow = lane >> 3;
+    const uint32_t chunk = (lane & 7) ^ (((8 * sw + lrow) >> 1) & 7);         // (the rows of a wavefront's further instructions are a multiple of 16 on)
+    static_assert(SET % 2 == 0, "rows of a wavefront's instructions lie a multiple of 16 apart");
+    const int64_t rows_all = p.token ? p.tokens : t.rows;
+    const __amdgpu_buffer_rsrc_t a_buf = mx_buffer(t.a, (uint32_t)(rows_all * K)), w_buf = mx_buffer(t.w, (uint32_t)N * K),
+                                 s_buf = mx_buffer(t.a_scales, (uint32_t)(rows_all * KB * 4));
+    uint32_t a_off[T::LOADS_A];
+#pragma unroll
+    for (int i = 0; i < T::LOADS_A; ++i) {
+        const uint32_t src = rows_source(p, t, 8 * (i * SET + sw) + lrow);
+        a_off[i] = src == kNoRow ? kBehind : src * K + 16 * chunk;
+    }
+    const uint32_t w_off = (uint32_t)(t.n0 + 8 * sw + lrow) * K + 16 * chunk;
+    const bool scaler = sw < T::SCALERS;
+    uint32_t s_off = kBehind;
+    if (scaler) {
+        const uint32_t src = rows_source(p, t, 64 * sw + lane);
+        s_off = src == kNoRow ? kBehind : src * (uint32_t)KB * 4;
+    }
+    unsigned char* const stages = smem + ks * T::STAGES * T::STAGE;
+    const int slabs = (KB + KS - 1) / KS, begin = ks * slabs, end = min(begin + slabs, KB);      // of the set; all run as many
+    constexpr int LOADS = T::LOADS_A + T::LOADS_W;
+    auto issue = [&](int s, unsigned char* st, int first, int last) {         // requests [first, last) of slab number s of this set
+        const int k = begin + s;
+        const bool in = k < end;
+        const uint32_t at = 128u * (uint32_t)k;
+#pragma unroll
+        for (int l = first; l < last && l < LOADS; ++l) {
+            const int i = l - T::LOADS_W;
+            if (l < T::LOADS_W)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(w_buf, (mx_lds_void*)(st + BM * 128 + (l * SET + sw) * 1024), 16, (int)(in ? w_off + at + l * SET * 8 * K : kBehind), 0, 0, 0);
+            else
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(a_buf, (mx_lds_void*)(st + (i * SET + sw) * 1024), 16, (int)(in ? a_off[i] + at : kBehind), 0, 0, 0);
+        }
+        if (first == 0 && scaler)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(s_buf, (mx_lds_void*)(st + (BM + BN) * 128 + sw * 256), 4, (int)(in ? s_off + 4u * (uint32_t)k : kBehind), 0, 0, 0);
+    };
+    const int c0 = t.n0 + 16 * CG * wn;
+    rows_cfloat* const ws = (rows_cfloat*)(uintptr_t)(t.s + (int64_t)min(c0 >> 7, (N - 1) >> 7) * KB);
+
+    mx_f32x4 acc[NT][CG];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int g = 0; g < CG; ++g) acc[i][g] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
+
+    // A slab, a group of 16 columns at a time: the next group's fragments are read, and the last one's products folded, under this one's.
+    auto slab = [&](const unsigned char* st, float s_w, auto request) {       // request(g): in front of group g
+        const unsigned char* xb = st + (wm * 16 * NT + idx) * 128;
+        const unsigned char* wb = st + (BM + wn * 16 * CG + idx) * 128;
+        const float* sb = reinterpret_cast<const float*>(st + (BM + BN) * 128) + wm * 16 * NT + idx;
+        const int at0 = (q ^ (idx >> 1)) << 4, at1 = ((4 + q) ^ (idx >> 1)) << 4;
+        mx_i32x8 x[NT], w[2];
+        float sc[NT];
+        mx_f32x4 part[2][NT];
+        auto read = [&](const unsigned char* b, int i) {
+            return rows_operand(*reinterpret_cast<const mx_u32x4*>(b + i * 16 * 128 + at0), *reinterpret_cast<const mx_u32x4*>(b + i * 16 * 128 + at1));
+        };
+        w[0] = read(wb, 0);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) x[i] = read(xb, i);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) sc[i] = sb[16 * i] * s_w;
+#pragma unroll
+        for (int g = 0; g <= CG; ++g) {
+            if (g < CG) request(g);
+            if (g + 1 < CG) w[(g + 1) & 1] = read(wb, g + 1);
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                if (g < CG) part[g & 1][i] = rows_mfma(w[g & 1], x[i]);
+                if (g > 0) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[i][g - 1][r] = __builtin_fmaf(part[(g - 1) & 1][i][r], sc[i], acc[i][g - 1][r]);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    auto after = [&](unsigned char* st) { return st + T::STAGE == stages + T::STAGES * T::STAGE ? stages : st + T::STAGE; };
+    auto meet = [&] {                             // (a slab's requests are LOADS, and one more of the wavefronts that bring scales)
+        if (AHEAD > 1 && scaler) mx_meet<(AHEAD - 1) * (LOADS + 1)>();
+        else mx_meet<(AHEAD - 1) * LOADS>();
+    };
+    unsigned char* now = stages;                  // the stage of the slab that is next; the one in front of it is filled next
+    unsigned char* fill = stages + AHEAD * T::STAGE;
+#pragma unroll
+    for (int s = 0; s < AHEAD; ++s) issue(s, stages + s * T::STAGE, 0, LOADS);
+    constexpr int PER = (LOADS + CG - 1) / CG;
+    if (t.rows > wm * 16 * NT) {
+        for (int s = 0; s < slabs; ++s) {
+            const float s_w = begin + s < end ? ws[begin + s] : 0.0f;
+            meet();
+            slab(now, s_w, [&](int g) { issue(s + AHEAD, fill, g * PER, g * PER + PER); });
+            now = after(now), fill = after(fill);
+        }
+    } else {                                      // no rows for this wavefront: it brings the others theirs
+        for (int s = 0; s < slabs; ++s) {
+            meet();
+            issue(s + AHEAD, fill, 0, LOADS);
+            fill = after(fill);
+        }
+    }
+    if (!mx_join<KS, SET, NT, CG>(acc, ks, sw, smem, lane)) return;
+    if constexpr (KS == 1) {
+        mx_meet();                                // (requests for slabs behind the last one: zeros, but they write to LDS)
+        if (!(N & 7)) {
+            mx_store_rows<NT, CG, 16, 16>(p, t, smem + sw * mx_rows_lds<NT, CG, 16, 16>(), lane, idx, 4 * q, 16 * wm * NT, c0, acc);
+            return;
+        }
+    }
+    mx_store_tile<NT, CG>(p, t, 16 * wm * NT + idx, c0 + 4 * q, acc);
+}
+
+// ---- launches ----
+
+// Workgroups of a launch: blocks of BM rows (an expert's last one is its own) times column tiles, in eight equal shares.
+int64_t rows_grid(const RowsProduct& p, int BM, int BN) {
+    const int64_t ncol = (p.N + BN - 1) / BN, blocks = p.count ? p.M / BM + p.E : (p.M + BM - 1) / BM;
+    return (blocks * ncol + 7) / 8 * 8 + (p.count ? 16 : 0);
+}
+
+struct RowsCut {
+    bool wide;
+    int KS;
+    int64_t waves;
+    int chunks;                 // of a wavefront, whole turns
+};
+RowsCut rows_cut(const RowsProduct& p) {
+    const int64_t blocks = p.count ? std::min<int64_t>(p.E, p.M) : (p.M + 15) / 16, groups = blocks * ((p.N + 15) / 16);
+    const int chunks = p.K / 128;
+    RowsCut c{groups >= 4096, 1, 0, 0};
+    c.waves = c.wide ? (groups + 1) / 2 : groups;
+    while (c.KS < kRowsWaves && 2 * kDepth * c.KS <= chunks && c.waves * 2 <= 4096) c.KS *= 2, c.waves *= 2;
+    c.chunks = ((chunks + c.KS - 1) / c.KS + kDepth - 1) / kDepth * kDepth;
+    return c;
+}
+hipError_t launch_rows_stream(const RowsProduct& p, hipStream_t st) {
+    const RowsCut c = rows_cut(p);
+    const bool cold = (p.count ? std::min<int64_t>(p.E, p.M) : 1) * p.N * p.K > ((int64_t)256 << 20);      // more than the memory-side cache holds
+    const unsigned grid = (unsigned)rows_grid(p, 16, 16 * (c.wide ? 2 : 1) * (kRowsWaves / c.KS));
+    auto launch = [&](auto kernel) {
+        kernel<<<grid, 64 * kRowsWaves, 0, st>>>(p, c.KS);
+        return hipGetLastError();
+    };
+    if (c.wide) return cold ? launch(rows_stream_kernel<2, true>) : launch(rows_stream_kernel<2, false>);
+    return cold ? launch(rows_stream_kernel<1, true>) : launch(rows_stream_kernel<1, false>);
+}
+template <class T>
+hipError_t launch_rows_tile(const RowsProduct& p, hipStream_t st) {
+    const hipError_t e = allow_lds(rows_tile_kernel<T>, T::LDS);
+    if (e != hipSuccess) return e;
+    rows_tile_kernel<T><<<(unsigned)rows_grid(p, T::BM, T::BN), T::THREADS, T::LDS, st>>>(p);
+    return hipGetLastError();
+}
+
+// Forms: 0 the streamer, from 1 on these tiles.  f(the tile's type, as a pointer to nothing).
+template <class F>
+auto with_rows_tile(int form, F f) {
+    switch (form) {
+        case 1: return f((RowsTile<1, 2, 4, 1, 2, 3>*)nullptr);      // 32 x 64
+        case 2: return f((RowsTile<1, 4, 4, 1, 2, 2>*)nullptr);      // 64 x 64
+        case 3: return f((RowsTile<1, 4, 4, 2, 1, 2>*)nullptr);      // 64 x 128
+        case 4: return f((RowsTile<2, 4, 2, 4, 1, 1>*)nullptr);      // 128 x 128
+        case 5: return f((RowsTile<2, 4, 2, 8, 1, 2>*)nullptr);      // 128 x 256
+        default: return f((RowsTile<4, 4, 2, 8, 1, 1>*)nullptr);     // 256 x 256
+    }
+}
+struct RowsCost {
+    int rows, columns;
+    float launch, slab, more;
+};
+constexpr RowsCost kRowsTiles[] = {{}, {32, 64, 3.5f, 0.20f, 0.25f}, {64, 64, 3.5f, 0.25f, 0.35f}, {64, 128, 3.5f, 0.4f, 0.4f}, {128, 128, 3.5f, 0.7f, 0.7f},
+                                   {128, 256, 4.5f, 1.0f, 1.0f}, {256, 256, 6.0f, 1.6f, 1.6f}};
+
+// The form that should take least; 0: the streamer.
+int block_form(const RowsProduct& p) {
+    const int64_t experts = p.count ? std::min<int64_t>(p.E, p.M) : 1;
+    const double each = (double)p.M / experts;
+    const RowsCut c = rows_cut(p);
+    auto row_blocks = [&](int rows) { return !p.count ? (double)((p.M + rows - 1) / rows) : each > 0.6 * rows ? (double)p.M / rows + 0.5 * experts : (double)experts; };
+    const double rounds = std::max(1.0, c.waves / 2048.0) * (p.count ? row_blocks(16) / experts : 1.0);
+    double best = 4.0 + c.chunks * rounds * (c.wide ? 0.7 : 0.35);
+    if (each > 16) best = 1e30;
+    int form = 0;
+    for (int f = 1; f < (int)(sizeof kRowsTiles / sizeof kRowsTiles[0]); ++f) {
+        const RowsCost& t = kRowsTiles[f];
+        const double tiles = std::ceil(row_blocks(t.rows) * ((p.N + t.columns - 1) / t.columns) / 256.0);      // of the compute unit that has most
+        const double cost = t.launch + p.K / 128 * (t.slab + t.more * (tiles - 1));
+        if (cost < best) best = cost, form = f;
+    }
+    return form;
+}
+int64_t block_workgroups(const RowsProduct& p, int form) {
+    return form == 0 ? rows_grid(p, 16, 16) : rows_grid(p, kRowsTiles[form].rows, kRowsTiles[form].columns);
+}
+
+}  // namespace
+
+// What the kernels read and write at a time, their 32-bit offsets and the launches' sizes; and the kernel that the product takes.
+int check_product_block128(const RowsProduct& p, int* form) {
+    auto off = [](const void* a, uintptr_t n) { return (uintptr_t)a % n != 0; };
+    if (p.M < 0 || p.tokens < 0 || p.N < 1 || p.K < 128 || p.K % 128 || !p.w || !p.s) return MOE_ERR_BAD_ARGUMENT;
+    if (p.act != MOE_ACT_RELU && p.act != MOE_ACT_GELU && p.act != MOE_ACT_NONE) return MOE_ERR_BAD_ARGUMENT;
+    if (p.M > 0 && (!p.a || !p.a_scales || !p.out)) return MOE_ERR_BAD_ARGUMENT;
+    if (off(p.a, 16) || off(p.w, 16) || off(p.out, 16) || off(p.a_scales, 4) || off(p.s, 4) || off(p.bias, 2) || off(p.token, 4)) return MOE_ERR_BAD_ARGUMENT;
+    if (p.K > (1 << 20) || (int64_t)p.N * p.K >= kBufferBytes || p.M > INT32_MAX) return MOE_ERR_UNSUPPORTED;
+    if (p.token && (p.tokens > INT32_MAX || p.tokens * p.K >= kBufferBytes)) return MOE_ERR_UNSUPPORTED;
+    *form = block_form(p);
+    return block_workgroups(p, *form) < ((int64_t)1 << 22) ? MOE_OK : MOE_ERR_UNSUPPORTED;      // 512 threads each: 2^31
+}
+
+hipError_t launch_product_block128(const RowsProduct& p, int form, hipStream_t st) {
+    if (p.M == 0) return hipSuccess;
+    if (form == 0) return launch_rows_stream(p, st);
+    return with_rows_tile(form, [&](auto* t) { return launch_rows_tile<std::remove_pointer_t<decltype(t)>>(p, st); });
+}
+
+}  // namespace moe355
+
+using namespace moe355;
+
+extern "C" int moe_gemm_block128(const void* a, const float* a_scales, const void* w, const float* w_scales, const void* bias, void* out, int64_t M, int64_t N,
+                                 int64_t K, int32_t act, void* stream) {
+    if (M < 0 || N < 1 || K < 1) return MOE_ERR_BAD_ARGUMENT;
+    if (N > INT32_MAX / 2 || K > INT32_MAX / 2) return MOE_ERR_UNSUPPORTED;
+    const RowsProduct p{(const uint8_t*)a, a_scales, (const uint8_t*)w, w_scales, (const uint16_t*)bias, nullptr, nullptr, nullptr, (uint16_t*)out, M, M, (int)N, (int)K, 1, act};
+    int form;
+    const int rc = check_product_block128(p, &form);
+    if (rc) return rc;
+    return launch_product_block128(p, form, (hipStream_t)stream) == hipSuccess ? MOE_OK : MOE_ERR_HIP;
+}
+
+extern "C" int moe_gemm_block128_plan(int64_t M, int64_t N, int64_t K, int32_t experts, int32_t* rows, int32_t* columns, int32_t* parts) {
+    if (M < 1 || N < 1 || K < 1 || experts < 0 || experts > kMaxExperts || !rows || !columns || !parts) return MOE_ERR_BAD_ARGUMENT;
+    if (N > INT32_MAX / 2 || K > INT32_MAX / 2) return MOE_ERR_UNSUPPORTED;
+    // an operand that is there, as far as the choice looks at it
+    alignas(16) static const uint8_t some[16] = {};
+    alignas(16) static uint16_t result[8];
+    const int32_t* const table = experts ? reinterpret_cast<const int32_t*>(some) : nullptr;
+    const float* const scales = reinterpret_cast<const float*>(some);
+    const RowsProduct p{some, scales, some, scales, nullptr, table, table, nullptr, result, M, M, (int)N, (int)K, experts ? experts : 1, MOE_ACT_NONE};
+    int form;
+    const int rc = check_product_block128(p, &form);
+    if (rc) return rc;
+    if (form == 0) {
+        const RowsCut c = rows_cut(p);
+        *rows = 16, *columns = c.wide ? 32 : 16, *parts = c.KS;
+    } else {
+        with_rows_tile(form, [&](auto* t) {
+            typedef std::remove_pointer_t<decltype(t)> T;
+            *rows = T::BM, *columns = T::BN, *parts = T::KS;
+        });
+    }
+    return MOE_OK;
+}

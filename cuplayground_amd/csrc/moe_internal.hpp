@@ -268,6 +268,23 @@ struct FewArgs {
 inline int few_parts(int H) { return H <= 1024 ? 4 : H <= 2048 ? 2 : 1; }
 hipError_t launch_few(FewArgs a, bool f16, bool mxfp4, hipStream_t st);
 
+// ---- products of e4m3 rows with e4m3 weights in blocks (csrc/block128_product.hip) ----
+struct RowsProduct {            // out = act(a . w^T + bias), one matrix or (count, offset) one an expert over packed rows
+    const uint8_t* a;           // [M, K] codes, or (token) [tokens, K]
+    const float* a_scales;      // [M or tokens, K / 128]
+    const uint8_t* w;           // [E, N, K] codes
+    const float* s;             // [E, ceil(N / 128), K / 128]
+    const uint16_t* bias;       // [E, N] bf16, or null
+    const int32_t* count;       // [E] rows of every expert, or null: one matrix, M rows
+    const int32_t* offset;
+    const int32_t* token;       // [M] which row of a is a packed row, or null: the packed row itself
+    uint16_t* out;              // [M, N]
+    int64_t M, tokens;
+    int N, K, E, act;
+};
+int check_product_block128(const RowsProduct& p, int* form);      // moe_status; form: which kernel, for the launch
+hipError_t launch_product_block128(const RowsProduct& p, int form, hipStream_t st);
+
 // ---- the norm in front of a layer, forth and back (csrc/norm.hip) ----
 constexpr int kNormMost = 16384;                        // values of a row: a layer's widest
 constexpr int64_t kNormRows = ((int64_t)1 << 22) - 1;   // rows of a call: a workgroup of 1024 threads each, and a launch has less than 2^32 threads

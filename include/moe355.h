@@ -450,6 +450,27 @@ typedef struct moe_mxfp4_scales {
 int moe_forward_few(moe_handle* h, const void* x, const moe_weights* w, const moe_mxfp4_scales* mx, void* out, const moe_routing_out* routing,
                     void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- Products of rows and weights that are both in e4m3 -------------------------------------------------------------
+ * Rows a with a scale for 128 values (moe_quant_rows128, moe_rms_norm, moe_act_rows128), weights w with one for each block of 128 x 128
+ * (moe_quant_block128).  No counterpart in the reference, whose dtypes stop at fp16.  Asynchronous on `stream`, no scratch, can be captured.
+ *
+ * moe_gemm_block128: out [M, N] (bf16) = act(a . w^T + bias), a [M, K] codes with a_scales [M, K / 128] fp32, w [N, K] codes with w_scales
+ *   [ceil(N / 128), K / 128] fp32, bias [N] bf16 or NULL, act RELU, GELU or NONE.  Products and their sums in fp32, rounded once.  K a multiple
+ *   of 128 up to 2^20, any N (a last block of fewer rows has scales too), any M below 2^31 (0: nothing is done); a, w and out 16-byte
+ *   aligned.  MOE_ERR_UNSUPPORTED: a matrix of 3 GiB and more, more workgroups than a launch takes (2^22).
+ * moe_gemm_block128_plan: which kernel a product of these sizes takes, as moe_gemm_mxfp4_plan says it (16 x 16 or 16 x 32: the weight streamer).
+ *   Host only.
+ * moe_expert_gemm_block128: the rows of every expert of an e4m3 layer through its matrix, w [E, N, K], w_scales [E, N / 128, K / 128], bias [E, N]
+ *   or NULL.  (N, K) is (H, I) or (I, H).  a_rows are the packed rows [S k, K], or, with token_indices [S k] (of moe_route), the tokens' rows
+ *   [S, K] (below 3 GiB), from which every packed row is fetched: no dispatch in front; an index that is no token's stands for a row of
+ *   zeros.  Rows of no expert are neither read nor written.  e4m3 layers only (else MOE_ERR_UNSUPPORTED). */
+int moe_gemm_block128(const void* a, const float* a_scales, const void* w, const float* w_scales, const void* bias, void* out, int64_t M, int64_t N,
+                      int64_t K, int32_t act, void* stream);
+int moe_gemm_block128_plan(int64_t M, int64_t N, int64_t K, int32_t experts, int32_t* rows, int32_t* columns, int32_t* parts);
+int moe_expert_gemm_block128(moe_handle* h, const void* a_rows, const float* a_scales, const int32_t* token_indices, const void* w, const float* w_scales,
+                             const void* bias, const int32_t* expert_count, const int32_t* expert_offset, int32_t N, int32_t K, int32_t act, void* out_rows,
+                             void* stream);
+
 /* ---- The norm in front of a layer -------------------------------------------------------------------------------------
  * The reference has no norm; a layer of experts stands behind one, in a residual stream.  Asynchronous on `stream`, nothing is allocated,
  * everything can be captured into a graph.
