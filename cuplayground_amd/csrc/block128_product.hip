@@ -226,8 +226,16 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_tile_kerne
         if (first == 0 && scaler)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(s_buf, (mx_lds_void*)(st + (BM + BN) * 128 + sw * 256), 4, (int)(in ? s_off + 4u * (uint32_t)k : kBehind), 0, 0, 0);
     };
+    // The weights' scales: one a slab, 64 slabs of them in the lanes of a register.  (As scalar loads they would share their counter with the reads of
+    // LDS, and return out of order: every wait for a fragment would be one for all.)
     const int c0 = t.n0 + 16 * CG * wn;
-    rows_cfloat* const ws = (rows_cfloat*)(uintptr_t)(t.s + (int64_t)min(c0 >> 7, (N - 1) >> 7) * KB);
+    const float* const ws = t.s + (int64_t)min(c0 >> 7, (N - 1) >> 7) * KB;
+    float held = 0.0f;
+    auto weight_scale = [&](int s) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, held), s & 63)); };
+    auto hold = [&](int s) {
+        held = begin + s + lane < end ? ws[begin + s + lane] : 0.0f;
+        asm volatile("" : "+v"(held));            // (the wait for it is here, not in every slab)
+    };
 
     mx_f32x4 acc[NT][CG];
 #pragma unroll
@@ -279,7 +287,8 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_tile_kerne
     constexpr int PER = (LOADS + CG - 1) / CG;
     if (t.rows > wm * 16 * NT) {
         for (int s = 0; s < slabs; ++s) {
-            const float s_w = begin + s < end ? ws[begin + s] : 0.0f;
+            if ((s & 63) == 0) hold(s);
+            const float s_w = weight_scale(s);
             meet();
             slab(now, s_w, [&](int g) { issue(s + AHEAD, fill, g * PER, g * PER + PER); });
             now = after(now), fill = after(fill);
@@ -300,6 +309,190 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_tile_kerne
         }
     }
     mx_store_tile<NT, CG>(p, t, 16 * wm * NT + idx, c0 + 4 * q, acc);
+}
+
+// -- large tiles: halves of a slab --
+//
+// What bounded the tiles above at these sizes were their loads: two stages are all that LDS has room for, a stage could be filled again once the whole
+// slab in it was multiplied, and a slab ended in a wait for the slowest of its lines (8192 x 14336 x 14336 by 256 x 256: 1457 us; without the loads 928,
+// without the products 1374).  Here a slab is consumed in halves -- all token rows and the first half of every wavefront's columns, then the second half
+// -- with a meeting in front of each, and what a half leaves is filled for the slab after the next at once: requests are a slab and a half
+// ahead instead of three quarters.  The last group's products wait for the next slab's meeting and run under its first reads.
+template <int RH_, int NT_, int CW_, int CG_>
+struct RowsDeep {
+    static constexpr int RH = RH_, NT = NT_, CW = CW_, CG = CG_, KS = 1;
+    static constexpr int BM = 16 * NT * RH, BN = 16 * CG * CW;
+    static constexpr int SET = RH * CW, THREADS = 64 * SET;
+    static constexpr int HALF = CG / 2;
+    static constexpr int LOADS_A = BM / 8 / SET;               // an instruction of a wavefront brings 8 rows; of a half of the columns: CW of them
+    static constexpr int STAGE = (BM + BN) * 128 + SET * 256;  // (a place for scales for every wavefront, so that all of them make as many requests)
+    static constexpr int LDS = std::max(2 * STAGE, SET * mx_rows_lds<NT, CG, 16, 16>());
+    static constexpr int BLOCKS = std::min(160 * 1024 / LDS, 8 / SET);
+    static constexpr int WAVES_PER_SIMD = BLOCKS * THREADS / 256;
+    static_assert(SET == CG && CG % 2 == 0 && SET % 2 == 0 && BM % (8 * SET) == 0 && BM <= 64 * SET && NT == 4, "a half of a wavefront's columns is an instruction of every wavefront");
+    static_assert(128 % (16 * CG) == 0 && LDS <= 160 * 1024, "columns of one scale; LDS of a compute unit");
+};
+
+template <class T>
+__global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_deep_kernel(RowsProduct p) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    constexpr int NT = T::NT, CG = T::CG, SET = T::SET, BM = T::BM, BN = T::BN, HALF = T::HALF;
+    RowsTask t;
+    if (!rows_task<BM>(p, BN, t)) return;
+    const int lane = threadIdx.x & 63, sw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = sw / T::CW, wn = sw % T::CW;
+    const int idx = lane & 15, q = lane >> 4;
+    const int N = p.N, KB = p.K >> 7;
+    const uint32_t K = (uint32_t)p.K;
+
+    const int lrow = lane >> 3;
+    const uint32_t chunk = (lane & 7) ^ (((8 * sw + lrow) >> 1) & 7);         // (rows_tile_kernel)
+    const int64_t rows_all = p.token ? p.tokens : t.rows;
+    const __amdgpu_buffer_rsrc_t a_buf = mx_buffer(t.a, (uint32_t)(rows_all * K)), w_buf = mx_buffer(t.w, (uint32_t)N * K),
+                                 s_buf = mx_buffer(t.a_scales, (uint32_t)(rows_all * KB * 4));
+    uint32_t a_off[T::LOADS_A];
+#pragma unroll
+    for (int i = 0; i < T::LOADS_A; ++i) {
+        const uint32_t src = rows_source(p, t, 8 * (i * SET + sw) + lrow);
+        a_off[i] = src == kNoRow ? kBehind : src * K + 16 * chunk;
+    }
+    const uint32_t s_src = rows_source(p, t, 64 * sw + lane), s_off = s_src == kNoRow ? kBehind : s_src * (uint32_t)KB * 4;
+    // A half of the columns is an instruction for every wavefront column l.
+    uint32_t w_off[2][T::CW];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int l = 0; l < T::CW; ++l) w_off[h][l] = (uint32_t)(t.n0 + 16 * CG * l + 16 * HALF * h + 8 * sw + lrow) * K + 16 * chunk;
+    // Where a slab lies in the rows is a scalar offset (below K, which no buffer is shorter than: the range check compares with what it leaves of the
+    // buffer).  Behind the last slab: the last one again, which nobody reads.
+    auto issue_columns = [&](int s, int h, int l) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(w_buf, (mx_lds_void*)(smem + (s & 1) * T::STAGE + (BM + 16 * CG * l + 16 * HALF * h + 8 * sw) * 128), 16, (int)w_off[h][l], 128 * min(s, KB - 1), 0, 0);
+    };
+    auto issue_rows = [&](int s, int i) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(a_buf, (mx_lds_void*)(smem + (s & 1) * T::STAGE + (i * SET + sw) * 1024), 16, (int)a_off[i], 128 * min(s, KB - 1), 0, 0);
+        if (i == 0)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(s_buf, (mx_lds_void*)(smem + (s & 1) * T::STAGE + (BM + BN) * 128 + sw * 256), 4, (int)s_off, 4 * min(s, KB - 1), 0, 0);
+    };
+    // Requests are one to a group of products: a wavefront whose requests queue at the address unit issues nothing else.  Slab s in its order:
+    // the first half of the columns of slab s + 1 behind the first meeting, then the second half of it, and behind the second meeting the
+    // rows of slab s + 2.  So behind what the first meeting waits for came a half of columns and a slab's rows, behind the second one's as
+    // much and two halves of columns.
+    constexpr int ROWS_IN_ALL = T::LOADS_A + 1;
+    auto meet_first = [] { mx_meet<T::CW + ROWS_IN_ALL>(); };
+    auto meet_second = [] { mx_meet<2 * T::CW + ROWS_IN_ALL>(); };
+    const int c0 = t.n0 + 16 * CG * wn;
+    const float* const ws = t.s + (int64_t)min(c0 >> 7, (N - 1) >> 7) * KB;
+    float held = 0.0f;                            // the weights' scales of 64 slabs (rows_tile_kernel)
+    auto hold = [&](int s) {
+        held = s + lane < KB ? ws[s + lane] : 0.0f;
+        asm volatile("" : "+v"(held));            // (the wait for it is here, not in every slab)
+    };
+
+    mx_f32x4 acc[NT][CG];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int g = 0; g < CG; ++g) acc[i][g] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
+
+    auto request = [&](int s, int g) {            // in front of group g of slab s (group CG - 1: that of the slab before, behind the first meeting)
+        // order: CG - 1, 0, .. HALF - 2 | HALF - 1, .. CG - 2
+        const int n = g == CG - 1 ? 0 : g + 1;
+        if (n < HALF) {
+#pragma unroll
+            for (int j = 2 * T::CW * n / HALF; j < 2 * T::CW * (n + 1) / HALF; ++j) issue_columns(s + 1, j / T::CW, j % T::CW);
+        } else {
+#pragma unroll
+            for (int j = T::LOADS_A * (n - HALF) / HALF; j < T::LOADS_A * (n - HALF + 1) / HALF; ++j) issue_rows(s + 2, j);
+        }
+    };
+    // what slabs -1 and -2 would have asked for
+#pragma unroll
+    for (int i = 0; i < T::LOADS_A; ++i) issue_rows(0, i);
+#pragma unroll
+    for (int j = 0; j < 2 * T::CW; ++j) issue_columns(0, j / T::CW, j % T::CW);
+#pragma unroll
+    for (int i = 0; i < T::LOADS_A; ++i) issue_rows(1, i);
+    if (t.rows > wm * 16 * NT) {
+        mx_i32x8 x[NT], w[2];
+        float sc[NT], sc_next[NT];
+        mx_f32x4 part[NT];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            x[i] = mx_i32x8{};
+            sc[i] = 0.0f;
+            part[i] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        w[0] = w[1] = mx_i32x8{};
+        const int at0 = (q ^ (idx >> 1)) << 4, at1 = ((4 + q) ^ (idx >> 1)) << 4;
+        auto read = [&](const unsigned char* b, int i) {
+            return rows_operand(*reinterpret_cast<const mx_u32x4*>(b + i * 16 * 128 + at0), *reinterpret_cast<const mx_u32x4*>(b + i * 16 * 128 + at1));
+        };
+        // Products of group g.  A product is folded three instructions later, so the first three here fold what is left of group `last`.
+        auto fold = [&](int i, int g, float scale) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[i][g][r] = __builtin_fmaf(part[i][r], scale, acc[i][g][r]);
+        };
+        auto group = [&](int g, int last, const float (&last_scale)[NT], const float (&scale)[NT]) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                part[i] = rows_mfma(w[g & 1], x[i]);
+                if (i + 1 < NT) fold(i + 1, last, last_scale[i + 1]);
+                else fold(0, g, scale[0]);
+            }
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);      // a matrix instruction,
+                __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);      // four of the vector ALU
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        for (int s = 0; s < KB; ++s) {
+            if ((s & 63) == 0) hold(s);
+            const float s_w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, held), s & 63));
+            const unsigned char* st = smem + (s & 1) * T::STAGE;
+            const unsigned char* xb = st + (wm * 16 * NT + idx) * 128;
+            const unsigned char* wb = st + (BM + wn * 16 * CG + idx) * 128;
+            const float* sb = reinterpret_cast<const float*>(st + (BM + BN) * 128) + wm * 16 * NT + idx;
+            meet_first();
+            w[0] = read(wb, 0);
+            request(s, CG - 1);
+            __builtin_amdgcn_sched_barrier(0);
+            group(CG - 1, CG - 2, sc, sc);        // of the slab before
+#pragma unroll
+            for (int i = 0; i < NT; ++i) x[i] = read(xb, i);
+#pragma unroll
+            for (int i = 0; i < NT; ++i) sc_next[i] = sb[16 * i] * s_w;
+            w[1] = read(wb, 1);
+            request(s, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            group(0, CG - 1, sc, sc_next);
+#pragma unroll
+            for (int i = 0; i < NT; ++i) sc[i] = sc_next[i];
+#pragma unroll
+            for (int g = 1; g < CG - 1; ++g) {
+                if (g == HALF - 1) meet_second();
+                w[(g + 1) & 1] = read(wb, g + 1);
+                request(s, g);
+                __builtin_amdgcn_sched_barrier(0);
+                group(g, g - 1, sc, sc);
+            }
+        }
+        group(CG - 1, CG - 2, sc, sc);
+#pragma unroll
+        for (int i = 1; i < NT; ++i) fold(i, CG - 1, sc[i]);
+    } else {                                      // no rows for this wavefront: it brings the others theirs
+        for (int s = 0; s < KB; ++s) {
+            meet_first();
+#pragma unroll
+            for (int n = 0; n < CG; ++n) {
+                if (n == HALF) meet_second();
+                request(s, n == 0 ? CG - 1 : n - 1);
+            }
+        }
+    }
+    mx_meet();                                    // (the requests behind the last slab write to LDS)
+    if (!(N & 7)) mx_store_rows<NT, CG, 16, 16>(p, t, smem + sw * mx_rows_lds<NT, CG, 16, 16>(), lane, idx, 4 * q, 16 * wm * NT, c0, acc);
+    else mx_store_tile<NT, CG>(p, t, 16 * wm * NT + idx, c0 + 4 * q, acc);
 }
 
 // ---- launches ----
@@ -337,10 +530,14 @@ hipError_t launch_rows_stream(const RowsProduct& p, hipStream_t st) {
     return cold ? launch(rows_stream_kernel<1, true>) : launch(rows_stream_kernel<1, false>);
 }
 template <class T>
+struct RowsKernel { static constexpr void (*kernel)(RowsProduct) = rows_tile_kernel<T>; };
+template <int RH, int NT, int CW, int CG>
+struct RowsKernel<RowsDeep<RH, NT, CW, CG>> { static constexpr void (*kernel)(RowsProduct) = rows_deep_kernel<RowsDeep<RH, NT, CW, CG>>; };
+template <class T>
 hipError_t launch_rows_tile(const RowsProduct& p, hipStream_t st) {
-    const hipError_t e = allow_lds(rows_tile_kernel<T>, T::LDS);
+    const hipError_t e = allow_lds(RowsKernel<T>::kernel, T::LDS);
     if (e != hipSuccess) return e;
-    rows_tile_kernel<T><<<(unsigned)rows_grid(p, T::BM, T::BN), T::THREADS, T::LDS, st>>>(p);
+    RowsKernel<T>::kernel<<<(unsigned)rows_grid(p, T::BM, T::BN), T::THREADS, T::LDS, st>>>(p);
     return hipGetLastError();
 }
 
@@ -351,9 +548,9 @@ auto with_rows_tile(int form, F f) {
         case 1: return f((RowsTile<1, 2, 4, 1, 2, 3>*)nullptr);      // 32 x 64
         case 2: return f((RowsTile<1, 4, 4, 1, 2, 2>*)nullptr);      // 64 x 64
         case 3: return f((RowsTile<1, 4, 4, 2, 1, 2>*)nullptr);      // 64 x 128
-        case 4: return f((RowsTile<2, 4, 2, 4, 1, 1>*)nullptr);      // 128 x 128
+        case 4: return f((RowsDeep<2, 4, 2, 4>*)nullptr);            // 128 x 128
         case 5: return f((RowsTile<2, 4, 2, 8, 1, 2>*)nullptr);      // 128 x 256
-        default: return f((RowsTile<4, 4, 2, 8, 1, 1>*)nullptr);     // 256 x 256
+        default: return f((RowsDeep<4, 4, 2, 8>*)nullptr);           // 256 x 256
     }
 }
 struct RowsCost {
