@@ -73,9 +73,6 @@ __device__ __forceinline__ uint32_t rows_source(const RowsProduct& p, const Rows
     const uint32_t i = (uint32_t)t.token[r];
     return i < (uint32_t)p.tokens ? i : kNoRow;
 }
-// The scales of a call are read-only: through scalar loads.
-typedef const __attribute__((address_space(4))) float rows_cfloat;
-
 __device__ __forceinline__ mx_f32x4 rows_mfma(const mx_i32x8& w, const mx_i32x8& x) {
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, mx_f32x4{0.f, 0.f, 0.f, 0.f}, 0 /* e4m3 */, 0, 0, 0, 0, 0);
 }
@@ -86,10 +83,12 @@ __device__ __forceinline__ mx_i32x8 rows_operand(const mx_u32x4& lower, const mx
 // ---- up to 16 rows a block: a weight streamer ----
 //
 // A wavefront owns G groups of 16 columns over its share of the contraction; weights come whole 128-byte lines of eight rows at a time
-// (stream_lines.hpp), which is a block of K, and stay in registers with the token rows' pieces, kDepth blocks on their way.
-constexpr int kRowsWaves = 8, kDepth = 4;
+// (stream_lines.hpp), which is a block of K, and stay in registers, kDepth blocks on their way.  Token rows come the same way (of up to eight rows,
+// without MORE, one instruction), and the token rows' scales four blocks of 16 rows an instruction: the address unit takes as long over a
+// request in pieces as over whole lines.
+constexpr int kRowsWaves = 8, kDepth = 4;      // (four: the blocks of K that an instruction brings the scales of)
 
-template <int G, bool COLD>
+template <int G, bool MORE, bool COLD>
 __global__ __launch_bounds__(64 * kRowsWaves) void rows_stream_kernel(RowsProduct p, int KS) {
     __shared__ mx_f32x4 red[(kRowsWaves - 1) * G * 64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -102,40 +101,61 @@ __global__ __launch_bounds__(64 * kRowsWaves) void rows_stream_kernel(RowsProduc
     const __amdgpu_buffer_rsrc_t x_buf = mx_buffer(t.a, (uint32_t)(rows_all * K)), w_buf = mx_buffer(t.w, (uint32_t)p.N * K),
                                  s_buf = mx_buffer(t.a_scales, (uint32_t)(rows_all * KB * 4));
     const int q = lane >> 4;
-    // (lanes behind the last row: the block's first one again, whose lines are on their way anyway)
-    uint32_t src = rows_source(p, t, (lane & 15) < t.rows ? lane & 15 : 0);
-    const uint32_t x_at = src == kNoRow ? kBehind : src * K + 16 * q, s_at = src == kNoRow ? kBehind : src * (uint32_t)KB * 4;
     const uint32_t piece = q + ((lane & 8) >> 1);
     const uint32_t w1 = (uint32_t)(n0 + (lane & 7)) * K + 16 * piece, w2 = (uint32_t)(n0 + 8 + (lane & 7)) * K + 16 * (piece ^ 4);
-    rows_cfloat* const sw = (rows_cfloat*)(uintptr_t)(t.s + (int64_t)min(n0 >> 7, (p.N - 1) >> 7) * KB);
+    auto row_at = [&](int r, uint32_t bytes, uint32_t more) {
+        const uint32_t src = rows_source(p, t, r);
+        return src == kNoRow ? kBehind : src * bytes + more;
+    };
+    const uint32_t x1 = row_at(lane & 7, K, 16 * piece), x2 = row_at(8 + (lane & 7), K, 16 * (piece ^ 4));
+    const uint32_t s_at = row_at(lane & 15, (uint32_t)KB * 4, 4 * q);
+    const float* const ws = t.s + (int64_t)min(n0 >> 7, (p.N - 1) >> 7) * KB;
 
     const int share = (KB + KS - 1) / KS, begin = min(ks * share, KB), end = min(begin + share, KB);
     mx_u32x4 w[kDepth][G][2], x[kDepth][2];
-    float sa[kDepth];
-    auto fetch = [&](int slot, int c) {            // what lies behind the share's end: zeros
+    float raw;                                     // lane 16 q + r: the scale of row r in block q of a turn
+    // What lies behind the share's end: zeros.
+    auto fetch = [&](int slot, int c) {
         const bool in = c < end;
         const uint32_t at = 128u * (uint32_t)c;
-        x[slot][0] = __builtin_bit_cast(mx_u32x4, __builtin_amdgcn_raw_buffer_load_b128(x_buf, (int)(in ? x_at + at : kBehind), 0, 0));
-        x[slot][1] = __builtin_bit_cast(mx_u32x4, __builtin_amdgcn_raw_buffer_load_b128(x_buf, (int)(in ? x_at + at + 64 : kBehind), 0, 0));
-        sa[slot] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(s_buf, (int)(in ? s_at + 4u * (uint32_t)c : kBehind), 0, 0));
+        x[slot][0] = __builtin_bit_cast(mx_u32x4, __builtin_amdgcn_raw_buffer_load_b128(x_buf, (int)(in ? x1 + at : kBehind), 0, 0));
+        if (MORE) x[slot][1] = __builtin_bit_cast(mx_u32x4, __builtin_amdgcn_raw_buffer_load_b128(x_buf, (int)(in ? x2 + at : kBehind), 0, 0));
 #pragma unroll
         for (int g = 0; g < G; ++g) {
             w[slot][g][0] = __builtin_bit_cast(mx_u32x4, __builtin_amdgcn_raw_buffer_load_b128(w_buf, (int)(in ? w1 + at + g * 16 * K : kBehind), 0, COLD ? 2 : 0));      // 2: not kept
             w[slot][g][1] = __builtin_bit_cast(mx_u32x4, __builtin_amdgcn_raw_buffer_load_b128(w_buf, (int)(in ? w2 + at + g * 16 * K : kBehind), 0, COLD ? 2 : 0));
         }
     };
+    auto fetch_scales = [&](int c) { raw = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(s_buf, (int)(c + q < end ? s_at + 4u * (uint32_t)c : kBehind), 0, 0)); };
     mx_f32x4 acc[1][G] = {};
     if (begin < end) {
+        // The weights' scales: one a block of K, 64 of them in the lanes of a register.
+        float held = begin + lane < end ? ws[begin + lane] : 0.0f;
+        fetch_scales(begin);
 #pragma unroll
         for (int d = 0; d < kDepth; ++d) fetch(d, begin + d);
         for (int c = begin; c < end; c += kDepth) {
+            if (c > begin && ((c - begin) & 63) == 0) {
+                held = c + lane < end ? ws[c + lane] : 0.0f;
+                asm volatile("" : "+v"(held));    // (the wait for it is here, not in every turn)
+            }
+            const int sa = __builtin_bit_cast(int, raw);
+            fetch_scales(c + kDepth);
 #pragma unroll
             for (int d = 0; d < kDepth; ++d) {
-                const float s = sa[d] * (c + d < end ? sw[c + d] : 0.0f);
-                const mx_i32x8 xv = rows_operand(x[d][0], x[d][1]);
+                const float s = __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(4 * ((lane & 15) + 16 * d), sa)) *
+                                __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, held), (c - begin + d) & 63));
+                mx_u32x4 lower, upper;
+                if (MORE) {
+                    line_pieces(x[d][0], x[d][1], lower, upper);
+                } else {
+                    lower = x[d][0];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) upper[i] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x[d][0][i], 0x128, 0xF, 0xF, false);      // row_ror:8
+                }
+                const mx_i32x8 xv = rows_operand(lower, upper);
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
-                    mx_u32x4 lower, upper;
                     line_pieces(w[d][g][0], w[d][g][1], lower, upper);
                     const mx_f32x4 part = rows_mfma(rows_operand(lower, upper), xv);
 #pragma unroll
@@ -324,12 +344,12 @@ struct RowsDeep {
     static constexpr int BM = 16 * NT * RH, BN = 16 * CG * CW;
     static constexpr int SET = RH * CW, THREADS = 64 * SET;
     static constexpr int HALF = CG / 2;
-    static constexpr int LOADS_A = BM / 8 / SET;               // an instruction of a wavefront brings 8 rows; of a half of the columns: CW of them
+    static constexpr int LOADS_A = BM / 8 / SET, LOADS_H = BN / 16 / SET;      // an instruction of a wavefront brings 8 rows, or 8 columns of a half
     static constexpr int STAGE = (BM + BN) * 128 + SET * 256;  // (a place for scales for every wavefront, so that all of them make as many requests)
     static constexpr int LDS = std::max(2 * STAGE, SET * mx_rows_lds<NT, CG, 16, 16>());
     static constexpr int BLOCKS = std::min(160 * 1024 / LDS, 8 / SET);
     static constexpr int WAVES_PER_SIMD = BLOCKS * THREADS / 256;
-    static_assert(SET == CG && CG % 2 == 0 && SET % 2 == 0 && BM % (8 * SET) == 0 && BM <= 64 * SET && NT == 4, "a half of a wavefront's columns is an instruction of every wavefront");
+    static_assert(CG % 2 == 0 && SET % 2 == 0 && BM % (8 * SET) == 0 && BN % (16 * SET) == 0 && BM <= 64 * SET && NT == 4, "every wavefront brings as many rows and columns");
     static_assert(128 % (16 * CG) == 0 && LDS <= 160 * 1024, "columns of one scale; LDS of a compute unit");
 };
 
@@ -357,16 +377,20 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_deep_kerne
         a_off[i] = src == kNoRow ? kBehind : src * K + 16 * chunk;
     }
     const uint32_t s_src = rows_source(p, t, 64 * sw + lane), s_off = s_src == kNoRow ? kBehind : s_src * (uint32_t)KB * 4;
-    // A half of the columns is an instruction for every wavefront column l.
-    uint32_t w_off[2][T::CW];
+    // Columns: half h of every wavefront column, eight at a time; in_tile: the first of the eight that instruction l of this wavefront brings.
+    auto in_tile = [&](int h, int l) {
+        const int j = l * SET + sw;
+        return 16 * CG * (j / (2 * HALF)) + 16 * HALF * h + 8 * (j % (2 * HALF));
+    };
+    uint32_t w_off[2][T::LOADS_H];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int l = 0; l < T::CW; ++l) w_off[h][l] = (uint32_t)(t.n0 + 16 * CG * l + 16 * HALF * h + 8 * sw + lrow) * K + 16 * chunk;
+        for (int l = 0; l < T::LOADS_H; ++l) w_off[h][l] = (uint32_t)(t.n0 + in_tile(h, l) + lrow) * K + 16 * chunk;
     // Where a slab lies in the rows is a scalar offset (below K, which no buffer is shorter than: the range check compares with what it leaves of the
     // buffer).  Behind the last slab: the last one again, which nobody reads.
     auto issue_columns = [&](int s, int h, int l) {
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(w_buf, (mx_lds_void*)(smem + (s & 1) * T::STAGE + (BM + 16 * CG * l + 16 * HALF * h + 8 * sw) * 128), 16, (int)w_off[h][l], 128 * min(s, KB - 1), 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(w_buf, (mx_lds_void*)(smem + (s & 1) * T::STAGE + (BM + in_tile(h, l)) * 128), 16, (int)w_off[h][l], 128 * min(s, KB - 1), 0, 0);
     };
     auto issue_rows = [&](int s, int i) {
         __builtin_amdgcn_raw_ptr_buffer_load_lds(a_buf, (mx_lds_void*)(smem + (s & 1) * T::STAGE + (i * SET + sw) * 1024), 16, (int)a_off[i], 128 * min(s, KB - 1), 0, 0);
@@ -378,8 +402,8 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_deep_kerne
     // rows of slab s + 2.  So behind what the first meeting waits for came a half of columns and a slab's rows, behind the second one's as
     // much and two halves of columns.
     constexpr int ROWS_IN_ALL = T::LOADS_A + 1;
-    auto meet_first = [] { mx_meet<T::CW + ROWS_IN_ALL>(); };
-    auto meet_second = [] { mx_meet<2 * T::CW + ROWS_IN_ALL>(); };
+    auto meet_first = [] { mx_meet<T::LOADS_H + ROWS_IN_ALL>(); };
+    auto meet_second = [] { mx_meet<2 * T::LOADS_H + ROWS_IN_ALL>(); };
     const int c0 = t.n0 + 16 * CG * wn;
     const float* const ws = t.s + (int64_t)min(c0 >> 7, (N - 1) >> 7) * KB;
     float held = 0.0f;                            // the weights' scales of 64 slabs (rows_tile_kernel)
@@ -399,7 +423,7 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_deep_kerne
         const int n = g == CG - 1 ? 0 : g + 1;
         if (n < HALF) {
 #pragma unroll
-            for (int j = 2 * T::CW * n / HALF; j < 2 * T::CW * (n + 1) / HALF; ++j) issue_columns(s + 1, j / T::CW, j % T::CW);
+            for (int j = 2 * T::LOADS_H * n / HALF; j < 2 * T::LOADS_H * (n + 1) / HALF; ++j) issue_columns(s + 1, j / T::LOADS_H, j % T::LOADS_H);
         } else {
 #pragma unroll
             for (int j = T::LOADS_A * (n - HALF) / HALF; j < T::LOADS_A * (n - HALF + 1) / HALF; ++j) issue_rows(s + 2, j);
@@ -409,7 +433,7 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_deep_kerne
 #pragma unroll
     for (int i = 0; i < T::LOADS_A; ++i) issue_rows(0, i);
 #pragma unroll
-    for (int j = 0; j < 2 * T::CW; ++j) issue_columns(0, j / T::CW, j % T::CW);
+    for (int j = 0; j < 2 * T::LOADS_H; ++j) issue_columns(0, j / T::LOADS_H, j % T::LOADS_H);
 #pragma unroll
     for (int i = 0; i < T::LOADS_A; ++i) issue_rows(1, i);
     if (t.rows > wm * 16 * NT) {
@@ -497,9 +521,10 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_deep_kerne
 
 // ---- launches ----
 
-// Workgroups of a launch: blocks of BM rows (an expert's last one is its own) times column tiles, in eight equal shares.
+// Workgroups of a launch: blocks of BM rows times column tiles, in eight equal shares.  Experts' blocks are counted on the device; M rows on n experts
+// that have any fill (M + n (BM - 1)) / BM of them at most.
 int64_t rows_grid(const RowsProduct& p, int BM, int BN) {
-    const int64_t ncol = (p.N + BN - 1) / BN, blocks = p.count ? p.M / BM + p.E : (p.M + BM - 1) / BM;
+    const int64_t ncol = (p.N + BN - 1) / BN, n = p.count ? std::min<int64_t>(p.E, p.M) : 1, blocks = (p.M + n * (BM - 1)) / BM;
     return (blocks * ncol + 7) / 8 * 8 + (p.count ? 16 : 0);
 }
 
@@ -512,7 +537,7 @@ struct RowsCut {
 RowsCut rows_cut(const RowsProduct& p) {
     const int64_t blocks = p.count ? std::min<int64_t>(p.E, p.M) : (p.M + 15) / 16, groups = blocks * ((p.N + 15) / 16);
     const int chunks = p.K / 128;
-    RowsCut c{groups >= 4096, 1, 0, 0};
+    RowsCut c{groups >= 512, 1, 0, 0};
     c.waves = c.wide ? (groups + 1) / 2 : groups;
     while (c.KS < kRowsWaves && 2 * kDepth * c.KS <= chunks && c.waves * 2 <= 4096) c.KS *= 2, c.waves *= 2;
     c.chunks = ((chunks + c.KS - 1) / c.KS + kDepth - 1) / kDepth * kDepth;
@@ -526,8 +551,10 @@ hipError_t launch_rows_stream(const RowsProduct& p, hipStream_t st) {
         kernel<<<grid, 64 * kRowsWaves, 0, st>>>(p, c.KS);
         return hipGetLastError();
     };
-    if (c.wide) return cold ? launch(rows_stream_kernel<2, true>) : launch(rows_stream_kernel<2, false>);
-    return cold ? launch(rows_stream_kernel<1, true>) : launch(rows_stream_kernel<1, false>);
+    const bool more = p.count || p.M > 8;
+    auto rows = [&](auto g, auto m) { return cold ? launch(rows_stream_kernel<decltype(g)::value, decltype(m)::value, true>) : launch(rows_stream_kernel<decltype(g)::value, decltype(m)::value, false>); };
+    auto columns = [&](auto g) { return more ? rows(g, std::true_type{}) : rows(g, std::false_type{}); };
+    return c.wide ? columns(std::integral_constant<int, 2>{}) : columns(std::integral_constant<int, 1>{});
 }
 template <class T>
 struct RowsKernel { static constexpr void (*kernel)(RowsProduct) = rows_tile_kernel<T>; };
@@ -545,30 +572,35 @@ hipError_t launch_rows_tile(const RowsProduct& p, hipStream_t st) {
 template <class F>
 auto with_rows_tile(int form, F f) {
     switch (form) {
-        case 1: return f((RowsTile<1, 2, 4, 1, 2, 3>*)nullptr);      // 32 x 64
-        case 2: return f((RowsTile<1, 4, 4, 1, 2, 2>*)nullptr);      // 64 x 64
-        case 3: return f((RowsTile<1, 4, 4, 2, 1, 2>*)nullptr);      // 64 x 128
-        case 4: return f((RowsDeep<2, 4, 2, 4>*)nullptr);            // 128 x 128
-        case 5: return f((RowsTile<2, 4, 2, 8, 1, 2>*)nullptr);      // 128 x 256
+        case 1: return f((RowsTile<1, 1, 2, 2, 4, 2>*)nullptr);      // 16 x 64
+        case 2: return f((RowsTile<1, 2, 4, 1, 2, 3>*)nullptr);      // 32 x 64
+        case 3: return f((RowsTile<1, 4, 4, 1, 2, 2>*)nullptr);      // 64 x 64
+        case 4: return f((RowsTile<1, 4, 4, 2, 1, 2>*)nullptr);      // 64 x 128
+        case 5: return f((RowsDeep<2, 4, 2, 4>*)nullptr);            // 128 x 128
+        case 6: return f((RowsDeep<2, 4, 4, 4>*)nullptr);            // 128 x 256
         default: return f((RowsDeep<4, 4, 2, 8>*)nullptr);           // 256 x 256
     }
 }
+
+// What a tile costs, in us: a launch of its form; a slab of the contraction where a compute unit has one tile; the same for every further tile of the
+// unit.  Fitted to 270 products of 1 to 6000 rows, 4 to 1000 us, dense and of experts, evenly and not, each with every form: the choice by
+// these is 0.8 % behind the best of the forms on average, 34 % at worst (90 to 240 rows for each of 8 experts with a long contraction).
 struct RowsCost {
     int rows, columns;
     float launch, slab, more;
 };
-constexpr RowsCost kRowsTiles[] = {{}, {32, 64, 3.5f, 0.20f, 0.25f}, {64, 64, 3.5f, 0.25f, 0.35f}, {64, 128, 3.5f, 0.4f, 0.4f}, {128, 128, 3.5f, 0.7f, 0.7f},
-                                   {128, 256, 4.5f, 1.0f, 1.0f}, {256, 256, 6.0f, 1.6f, 1.6f}};
+constexpr RowsCost kRowsTiles[] = {{}, {16, 64, 3.9f, 0.142f, 0.466f}, {32, 64, 3.75f, 0.203f, 1.0f}, {64, 64, 4.26f, 0.25f, 0.683f}, {64, 128, 4.0f, 0.305f, 0.72f},
+                                   {128, 128, 4.36f, 0.847f, 0.643f}, {128, 256, 6.37f, 0.968f, 1.89f}, {256, 256, 6.77f, 1.373f, 2.07f}};
 
-// The form that should take least; 0: the streamer.
+// The form that should take least; 0: the streamer.  Of experts' rows the host knows how many there are, not whose: a block an expert where the
+// mean is small for it, else half a block more than the mean fills.
 int block_form(const RowsProduct& p) {
     const int64_t experts = p.count ? std::min<int64_t>(p.E, p.M) : 1;
     const double each = (double)p.M / experts;
     const RowsCut c = rows_cut(p);
     auto row_blocks = [&](int rows) { return !p.count ? (double)((p.M + rows - 1) / rows) : each > 0.6 * rows ? (double)p.M / rows + 0.5 * experts : (double)experts; };
     const double rounds = std::max(1.0, c.waves / 2048.0) * (p.count ? row_blocks(16) / experts : 1.0);
-    double best = 4.0 + c.chunks * rounds * (c.wide ? 0.7 : 0.35);
-    if (each > 16) best = 1e30;
+    double best = each > 16 ? 1e30 : 1.9 + 0.036 * each + c.chunks * rounds * ((c.wide ? 2.29 : 1.03) + 0.055 * each);
     int form = 0;
     for (int f = 1; f < (int)(sizeof kRowsTiles / sizeof kRowsTiles[0]); ++f) {
         const RowsCost& t = kRowsTiles[f];
