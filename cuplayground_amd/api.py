@@ -304,10 +304,30 @@ def _codes(name, t, shape):
     _device_operand(name, t, t.dtype if t.dtype == torch.float8_e4m3fn else torch.uint8, shape)
 
 
-def _on_current_device(name, t):
+def _right(operands) -> bool:
+    """Whether every (tensor or None, type -- 1: codes of a byte --, shape) lies as the kernels read it, on the current GPU: one look for the calls of a
+    decoding step.  Where it says no, the operand is looked for by name."""
     import torch
-    current = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)      # (a tensor on a GPU: the runtime is up)
-    if not t.is_cuda or t.get_device() != current():
+    device = operands[0][0].get_device()
+    if device < 0 or device != _current_device():
+        return False
+    for t, dtype, shape in operands:
+        if t is None:
+            continue
+        has = t.dtype
+        if not ((has == dtype or (dtype == 1 and (has == torch.uint8 or has == torch.float8_e4m3fn))) and t.shape == shape and t.get_device() == device
+                and t.is_contiguous()):
+            return False
+    return True
+
+
+def _current_device() -> int:
+    import torch
+    return getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)()      # (asked with a tensor on a GPU: the runtime is up)
+
+
+def _on_current_device(name, t):
+    if not t.is_cuda or t.get_device() != _current_device():
         raise ValueError("%s lies on %s: expected the current GPU" % (name, t.device))
 
 
@@ -674,22 +694,19 @@ class MoELayer:
             raise ValueError("expert_gemm_block128 takes a matrix for every expert")
         (_, N, K), A = w.shape, self.S * self.k
         rows = A if token_indices is None else self.S
-        _codes("w", w, (self.E, N, K))
-        _codes("a_rows", a_rows, (rows, K))
-        _device_operand("w_scales", w_scales, torch.float32, (self.E, (N + 127) // 128, K // 128))
-        _device_operand("a_scales", a_scales, torch.float32, (rows, K // 128))
-        for name, t in (("w", w), ("a_rows", a_rows)) + (() if out is None else (("out", out),)):
-            _on_16_bytes(name, t)
-        if bias is not None:
-            _device_operand("bias", bias, torch.bfloat16, (self.E, N))
-        for name, t in (("expert_count", expert_count), ("expert_offset", expert_offset)):
-            _device_operand(name, t, torch.int32, (self.E,))
-        if token_indices is not None:
-            _device_operand("token_indices", token_indices, torch.int32, (A,))
+        operands = (("w", w, 1, (self.E, N, K)), ("a_rows", a_rows, 1, (rows, K)), ("w_scales", w_scales, torch.float32, (self.E, (N + 127) // 128, K // 128)),
+                    ("a_scales", a_scales, torch.float32, (rows, K // 128)), ("bias", bias, torch.bfloat16, (self.E, N)),
+                    ("expert_count", expert_count, torch.int32, (self.E,)), ("expert_offset", expert_offset, torch.int32, (self.E,)),
+                    ("token_indices", token_indices, torch.int32, (A,)), ("out", out, torch.bfloat16, (A, N)))
+        if not _right([o[1:] for o in operands]):
+            for name, t, dtype, shape in operands:
+                if t is not None:
+                    _codes(name, t, shape) if dtype == 1 else _device_operand(name, t, dtype, shape)
+        for name, t in (("w", w), ("a_rows", a_rows), ("out", out)):
+            if t is not None:
+                _on_16_bytes(name, t)
         if out is None:
-            out = torch.empty(A, N, dtype=torch.bfloat16, device=w.device)
-        else:
-            _device_operand("out", out, torch.bfloat16, (A, N))
+            out = torch.empty((A, N), dtype=torch.bfloat16, device=w.device)
         _check(self.L.moe_expert_gemm_block128(self._h, _ptr(a_rows), _ptr(a_scales), _ptr(token_indices), _ptr(w), _ptr(w_scales), _ptr(bias),
                                                _ptr(expert_count), _ptr(expert_offset), N, K, act, _ptr(out), _stream()), "moe_expert_gemm_block128")
         return out
@@ -1140,17 +1157,21 @@ def gemm_block128(A, a_scales, w, w_scales, bias=None, act: int = ACT_NONE):
     if w.dim() != 2 or A.dim() != 2:
         raise ValueError("gemm_block128 takes matrices")
     M, (N, K) = A.shape[0], w.shape
-    _codes("w", w, (N, K))
-    _codes("A", A, (M, K))
-    _device_operand("w_scales", w_scales, torch.float32, ((N + 127) // 128, K // 128))
-    _device_operand("a_scales", a_scales, torch.float32, (M, K // 128))
-    if bias is not None:
-        _device_operand("bias", bias, torch.bfloat16, (N,))
+    if not _right(((A, 1, (M, K)), (a_scales, torch.float32, (M, K // 128)), (w, 1, (N, K)), (w_scales, torch.float32, ((N + 127) // 128, K // 128)),
+                   (bias, torch.bfloat16, (N,)))):
+        _codes("w", w, (N, K))
+        _codes("A", A, (M, K))
+        _device_operand("w_scales", w_scales, torch.float32, ((N + 127) // 128, K // 128))
+        _device_operand("a_scales", a_scales, torch.float32, (M, K // 128))
+        if bias is not None:
+            _device_operand("bias", bias, torch.bfloat16, (N,))
     _on_16_bytes("A", A)
     _on_16_bytes("w", w)
-    out = torch.empty(M, N, dtype=torch.bfloat16, device=A.device)
-    _check(load_library().moe_gemm_block128(_ptr(A), _ptr(a_scales), _ptr(w), _ptr(w_scales), _ptr(bias), _ptr(out), M, N, K, act, _stream()),
-           "moe_gemm_block128")
+    out = torch.empty((M, N), dtype=torch.bfloat16, device=A.device)
+    rc = load_library().moe_gemm_block128(A.data_ptr(), a_scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(), None if bias is None else bias.data_ptr(),
+                                          out.data_ptr(), M, N, K, act, _stream())
+    if rc:
+        raise MoEError(rc, "moe_gemm_block128")
     return out
 
 
@@ -1162,34 +1183,49 @@ def gemm_block128_plan(M: int, N: int, K: int, experts: int = 0) -> dict:
     return dict(zip(("rows", "columns", "parts"), (v.value for v in out)))
 
 
-def _norm_operands(x, weight, **others):
-    """(rows, H, the rows' type, the weight's); every operand lies on the current GPU, in one piece and in the shape of x."""
+_float_kinds: dict = {}      # torch's type -> the library's, of rows that a norm takes
+
+
+def _norm_operands(x, weight, *others):
+    """(rows, H, the rows' type, the weight's); every operand lies on the current GPU, in one piece and in the shape of x.  others: (name,
+    tensor or None).  One look at what is right; what is wrong is then looked for by name (a decoding step waits for this: 5 us by name)."""
     import torch
-    known = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_FP16}
-    if x.dtype not in known:
-        raise TypeError("rows of %s: the norm takes fp32, bf16 and fp16" % x.dtype)
-    if x.dim() == 0 or x.shape[-1] == 0:
-        raise ValueError("the norm takes rows of at least one value")
-    H = x.shape[-1]
-    if weight.dtype != torch.float32:
-        _device_operand("weight", weight, x.dtype, (H,))
-    else:
-        _device_operand("weight", weight, torch.float32, (H,))
-    for name, t in dict(others, x=x).items():
-        if t is not None:
-            _device_operand(name, t, x.dtype, x.shape)
-    return x.numel() // H, H, known[x.dtype], known[weight.dtype]
+    if not _float_kinds:
+        _float_kinds.update({torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_FP16})
+    dtype, shape, wdtype = x.dtype, x.shape, weight.dtype
+    kind = _float_kinds.get(dtype)
+    H = shape[-1] if shape else 0
+    device = x.get_device()
+    right = (kind is not None and H > 0 and device >= 0 and device == _current_device() and x.is_contiguous()
+             and (wdtype == dtype or wdtype == torch.float32) and weight.shape == (H,) and weight.is_contiguous() and weight.get_device() == device)
+    for name, t in others:
+        right = right and (t is None or (t.dtype == dtype and t.shape == shape and t.is_contiguous() and t.get_device() == device))
+    if not right:
+        if kind is None:
+            raise TypeError("rows of %s: the norm takes fp32, bf16 and fp16" % dtype)
+        if H == 0:
+            raise ValueError("the norm takes rows of at least one value")
+        _device_operand("weight", weight, torch.float32 if wdtype == torch.float32 else dtype, (H,))
+        for name, t in others + (("x", x),):
+            if t is not None:
+                _device_operand(name, t, dtype, shape)
+    return x.numel() // H, H, kind, _float_kinds[wdtype]
 
 
 def rms_norm(x, weight, eps: float = 1e-6, residual=None):
     """y = h * weight / sqrt(mean of h^2 + eps) over the last dimension, h = x + residual rounded to x's type: y, or (y, h) with a residual.
     fp32, bf16 or fp16 of any shape [.., H], H up to 16384; weight [H] in that type or in fp32."""
     import torch
-    rows, H, dtype, wdtype = _norm_operands(x, weight, residual=residual)
+    rows, H, dtype, wdtype = _norm_operands(x, weight, ("residual", residual))
     out = torch.empty_like(x)
-    h = None if residual is None else torch.empty_like(x)
-    _check(load_library().moe_rms_norm(_ptr(x), _ptr(residual), _ptr(weight), rows, H, eps, dtype, wdtype, _ptr(h), _ptr(out), None, None, _stream()),
-           "moe_rms_norm")
+    if residual is None:
+        h, res, total = None, None, None
+    else:
+        h = torch.empty_like(x)
+        res, total = residual.data_ptr(), h.data_ptr()
+    rc = load_library().moe_rms_norm(x.data_ptr(), res, weight.data_ptr(), rows, H, eps, dtype, wdtype, total, out.data_ptr(), None, None, _stream())
+    if rc:
+        raise MoEError(rc, "moe_rms_norm")
     return out if residual is None else (out, h)
 
 
@@ -1197,14 +1233,16 @@ def rms_norm_backward(dout, h, weight, eps: float = 1e-6, dsum=None):
     """(dx, dweight) of rms_norm: h is what was normalised (x, or the sum with the residual), dsum the gradient that h has from elsewhere
     (None: none).  dx is the gradient of x and of the residual alike; dweight has the weight's type."""
     import torch
-    rows, H, dtype, wdtype = _norm_operands(h, weight, dout=dout, dsum=dsum)
+    rows, H, dtype, wdtype = _norm_operands(h, weight, ("dout", dout), ("dsum", dsum))
     L = load_library()
     n = C.c_size_t(0)
     _check(L.moe_rms_norm_scratch_bytes(rows, H, C.byref(n)), "moe_rms_norm_scratch_bytes")
     scratch = torch.empty(n.value, dtype=torch.uint8, device=h.device)
     dx, dweight = torch.empty_like(h), torch.empty_like(weight)
-    _check(L.moe_rms_norm_backward(_ptr(dout), _ptr(h), _ptr(weight), _ptr(dsum), rows, H, eps, dtype, wdtype, _ptr(dx), _ptr(dweight), _ptr(scratch),
-                                   n.value, _stream()), "moe_rms_norm_backward")
+    rc = L.moe_rms_norm_backward(dout.data_ptr(), h.data_ptr(), weight.data_ptr(), None if dsum is None else dsum.data_ptr(), rows, H, eps, dtype, wdtype,
+                                 dx.data_ptr(), dweight.data_ptr(), scratch.data_ptr(), n.value, _stream())
+    if rc:
+        raise MoEError(rc, "moe_rms_norm_backward")
     return dx, dweight
 
 
@@ -1213,18 +1251,21 @@ def rms_norm_rows128(x, weight, eps: float = 1e-6, residual=None, want_rows: boo
     [.., H], fp32 scales [.., H/128], the rows in x's type or None, h or None).  H a multiple of 128.  One pass where rms_norm and
     quantize_rows128 are two."""
     import torch
-    rows, H, dtype, wdtype = _norm_operands(x, weight, residual=residual)
+    rows, H, dtype, wdtype = _norm_operands(x, weight, ("residual", residual))
     if H % 128:
         raise ValueError("rows of %d values: rows in e4m3 hold a multiple of 128" % H)
     for name, t in (("x", x), ("weight", weight), ("residual", residual)):
         if t is not None:
             _on_16_bytes(name, t)
-    q = torch.empty(x.shape, dtype=torch.uint8, device=x.device)
-    s = torch.empty(*x.shape[:-1], H // 128, dtype=torch.float32, device=x.device)
+    shape, device = x.shape, x.device
+    q = torch.empty(shape, dtype=torch.uint8, device=device)
+    s = torch.empty((*shape[:-1], H // 128), dtype=torch.float32, device=device)
     out = torch.empty_like(x) if want_rows else None
     h = None if residual is None else torch.empty_like(x)
-    _check(load_library().moe_rms_norm(_ptr(x), _ptr(residual), _ptr(weight), rows, H, eps, dtype, wdtype, _ptr(h), _ptr(out), _ptr(q), _ptr(s), _stream()),
-           "moe_rms_norm")
+    rc = load_library().moe_rms_norm(x.data_ptr(), None if residual is None else residual.data_ptr(), weight.data_ptr(), rows, H, eps, dtype, wdtype,
+                                     None if h is None else h.data_ptr(), None if out is None else out.data_ptr(), q.data_ptr(), s.data_ptr(), _stream())
+    if rc:
+        raise MoEError(rc, "moe_rms_norm")
     return q, s, out, h
 
 
@@ -1233,23 +1274,29 @@ def act_rows128(u_rows, g_rows, act: int, expert_count=None, expert_offset=None)
     a row: (uint8 codes [R, I], fp32 scales [R, I/128]), rows of gemm_block128.  With a route's expert_count and expert_offset the rows of no
     expert are neither read nor written."""
     import torch
-    if u_rows.dim() != 2 or u_rows.shape[1] % 128 or u_rows.shape[1] == 0:
-        raise ValueError("u_rows has shape %s: expected rows of a multiple of 128 values" % (tuple(u_rows.shape),))
+    shape = u_rows.shape
+    if len(shape) != 2 or shape[1] % 128 or shape[1] == 0:
+        raise ValueError("u_rows has shape %s: expected rows of a multiple of 128 values" % (tuple(shape),))
+    looked = _right(((u_rows, torch.bfloat16, shape), (g_rows, torch.bfloat16, shape)))
     for name, t in (("u_rows", u_rows), ("g_rows", g_rows)):
         if t is not None:
-            _device_operand(name, t, torch.bfloat16, u_rows.shape)
+            if not looked:
+                _device_operand(name, t, torch.bfloat16, shape)
             _on_16_bytes(name, t)
-    R, I = u_rows.shape
+    R, I = shape
     if (expert_count is None) != (expert_offset is None):
         raise ValueError("expert_count and expert_offset go together")
     E = 0 if expert_count is None else expert_count.numel()
     for name, t in (("expert_count", expert_count), ("expert_offset", expert_offset)):
         if t is not None:
             _device_operand(name, t, torch.int32, (E,))
-    q = torch.empty(R, I, dtype=torch.uint8, device=u_rows.device)
-    s = torch.empty(R, I // 128, dtype=torch.float32, device=u_rows.device)
-    _check(load_library().moe_act_rows128(_ptr(u_rows), _ptr(g_rows), R, I, act, _ptr(expert_count), _ptr(expert_offset), E, _ptr(q), _ptr(s), _stream()),
-           "moe_act_rows128")
+    device = u_rows.device
+    q = torch.empty((R, I), dtype=torch.uint8, device=device)
+    s = torch.empty((R, I // 128), dtype=torch.float32, device=device)
+    rc = load_library().moe_act_rows128(u_rows.data_ptr(), None if g_rows is None else g_rows.data_ptr(), R, I, act, _ptr(expert_count), _ptr(expert_offset), E,
+                                        q.data_ptr(), s.data_ptr(), _stream())
+    if rc:
+        raise MoEError(rc, "moe_act_rows128")
     return q, s
 
 
