@@ -711,6 +711,61 @@ class MoELayer:
                                                _ptr(expert_count), _ptr(expert_offset), N, K, act, _ptr(out), _stream()), "moe_expert_gemm_block128")
         return out
 
+    def forward_block128(self, x, weights: dict, norm_weight=None, eps: float = 1e-6, residual=None):
+        """out[S,H] = MoE(x) of an e4m3 layer with the rows in e4m3 too, as rms_norm_rows128 and act_rows128 make them: for any number of tokens, the
+        stages one by one, the projections by expert_gemm_block128, which fetches its rows from the tokens'.  With norm_weight [H] (bf16 or fp32) the
+        layer stands behind that norm, MoE(rms_norm(x)), its router on the bf16 rows of it; with a residual besides: (out, x + residual).
+        Rows in e4m3 carry three bits where forward()'s bf16 rows carry seven: a token's answer is some 4 % from 64 bits instead of 0.3 %."""
+        import torch
+        cfg, gated = self.cfg, self.cfg.hidden_act == ACT_SWIGLU
+        if cfg.torch_dtype != DTYPE_FP8:
+            raise MoEError(_UNSUPPORTED, "rows in e4m3 go with e4m3 layers")
+        if residual is not None and norm_weight is None:
+            raise ValueError("the residual is added in front of the norm: norm_weight is missing")
+        H, I, E = self.H, cfg.intermediate_size, self.E
+        needed = {"gate_w", "w_up", "w_down", "s_up", "s_down"} | ({"w_gate", "s_gate"} if gated else set())
+        given = {n for n, t in weights.items() if t is not None}
+        if needed - given:
+            raise ValueError("missing tensors %s" % sorted(needed - given))
+        others = given - needed - {"gate_bias", "b_up", "b_down"} - ({"b_gate"} if gated else set())
+        if others:
+            raise ValueError("tensors %s do not belong to this layer" % sorted(others))
+        # every operand before the first launch
+        for name in sorted(given):
+            t = weights[name]
+            N, K = (H, I) if name.endswith("down") else (I, H)
+            if name == "gate_w":
+                _device_operand(name, t, torch.bfloat16, (E, H))
+            elif name == "gate_bias":
+                _device_operand(name, t, torch.float32, (E,))
+            elif name[0] == "w":
+                _codes(name, t, (E, N, K))
+            elif name[0] == "s":
+                _device_operand(name, t, torch.float32, (E, N // 128, K // 128))
+            else:
+                _device_operand(name, t, torch.bfloat16, (E, N))
+            if name[0] == "w" or name == "gate_w":
+                _on_16_bytes(name, t)
+        _device_operand("x", x, torch.bfloat16, (self.S, H))
+        _on_16_bytes("x", x)
+        h = None
+        if norm_weight is None:
+            rows, (q, s) = x, quantize_rows128(x)
+        else:
+            q, s, rows, h = rms_norm_rows128(x, norm_weight, eps, residual=residual, want_rows=True)
+        idx, gate = self.gate(rows, weights["gate_w"], weights.get("gate_bias"))
+        r = self.route(idx)
+        count, offset = r["expert_count"], r["expert_offset"]
+
+        def project(a, scales, name, token_indices=None):
+            return self.expert_gemm_block128(a, scales, weights["w_" + name], weights["s_" + name], weights.get("b_" + name), count, offset,
+                                             token_indices=token_indices)
+
+        u = project(q, s, "up", r["token_indices"])
+        g = project(q, s, "gate", r["token_indices"]) if gated else None
+        out = combine(project(*act_rows128(u, g, cfg.hidden_act, count, offset), "down"), r["pair_row"], gate)
+        return out if h is None else (out, h)
+
     def set_spin_limit(self, polls: int):
         """Polls before a dependency wait of the queue kernel gives up (0: default; negative: every wait expires)."""
         _check(self.L.moe_set_spin_limit(self._h, polls))

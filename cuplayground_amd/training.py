@@ -11,7 +11,8 @@ Everything else -- dispatch, projections, activation, combine -- is one autograd
 router) whose backward runs the library's adjoints; the data gradient of the down projection
 carries the activation's derivative in its epilogue (either product; `moe_expert_gemm_act_backward`) where the layer has that kernel,
 else `moe_expert_gemm` is followed by `moe_act_backward`.  `expert_linear` and `act_down` are the projections as nodes
-of their own, for layers composed in torch.  There is no CPU path: every tensor lives on the GPU.
+of their own, for layers composed in torch.  `rms_norm` is the norm in front of such a layer as a node, `MoE355TrainBlock` the layer behind it in
+its residual stream.  There is no CPU path: every tensor lives on the GPU.
 """
 from __future__ import annotations
 
@@ -249,6 +250,39 @@ class _RoutedExperts(torch.autograd.Function):
         return dx, dup, dgate, ddown, dgate_w, None, None
 
 
+class _RMSNorm(torch.autograd.Function):
+    """(x, residual or None, weight [H]) -> (rms_norm(x + residual), x + residual), or (rms_norm(x), None).  What is kept is what was normalised; the
+    backward makes the row's sums again from it instead of keeping them."""
+
+    @staticmethod
+    def forward(ctx, x, residual, weight, eps):
+        x, weight = x.contiguous(), weight.contiguous()
+        if residual is None:
+            out, h = api.rms_norm(x, weight, eps), x
+        else:
+            out, h = api.rms_norm(x, weight, eps, residual=residual.contiguous())
+        ctx.save_for_backward(h, weight)
+        ctx.eps = eps
+        ctx.set_materialize_grads(False)
+        return out, None if residual is None else h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, dsum):
+        h, weight = (t.contiguous() for t in ctx.saved_tensors)
+        dsum = None if dsum is None else dsum.contiguous()
+        if dout is None:                          # the normalised rows went nowhere
+            return dsum, dsum, None, None
+        dx, dweight = api.rms_norm_backward(dout.contiguous(), h, weight, ctx.eps, dsum=dsum)
+        return dx, dx if ctx.needs_input_grad[1] else None, dweight if ctx.needs_input_grad[2] else None, None
+
+
+def rms_norm(x, weight, eps: float = 1e-6, residual=None):
+    """api.rms_norm with gradients for x, residual and weight: y, or (y, x + residual) with a residual."""
+    out, h = _RMSNorm.apply(x, residual, weight, eps)
+    return out if residual is None else (out, h)
+
+
 class MoE355Train(torch.nn.Module):
     """forward(x [S,H]) -> [S,H] with gradients for x, gate_w, w_up, w_gate and w_down."""
 
@@ -305,6 +339,23 @@ class MoE355Train(torch.nn.Module):
         rows = x if x.shape[0] == c.tokens else x[:c.tokens]      # rows behind the layer's tokens: zero gradients
         return _Experts.apply(rows, self.w_up, self.w_gate, self.w_down, w, self.layer, r["token_indices"], r["pair_row"],
                               count, offset)
+
+
+class MoE355TrainBlock(torch.nn.Module):
+    """A trainable layer of experts in a residual stream, behind its norm: forward(x [S,H]) -> x + MoE(rms_norm(x)), or, where the last block's
+    output has not been added to the stream yet, forward(x, residual) -> (MoE(rms_norm(h)), h) with h = x + residual for the next one's addition."""
+
+    def __init__(self, cfg: api.MoEConfig, eps: float = 1e-6, init_std: float = 0.02, seed: int = 0):
+        super().__init__()
+        self.moe = MoE355Train(cfg, init_std=init_std, seed=seed)
+        self.norm_w = torch.nn.Parameter(torch.ones(cfg.hidden_size, dtype=self.moe.layer.act_dtype, device="cuda"))
+        self.eps = eps
+
+    def forward(self, x, residual=None):
+        if residual is None:
+            return x + self.moe(rms_norm(x, self.norm_w, self.eps))
+        rows, h = rms_norm(x, self.norm_w, self.eps, residual=residual)
+        return self.moe(rows), h
 
 
 _ROUTE, _GATE_WEIGHTS = MoE355Train.route, MoE355Train.gate_weights

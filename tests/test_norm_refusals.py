@@ -92,3 +92,39 @@ def test_python_refuses_what_it_can_see():
         moe.act_rows128(x, None, api.ACT_RELU)
     with pytest.raises(ValueError, match="current GPU"):
         moe.act_rows128(x.bfloat16(), None, api.ACT_RELU)
+
+
+def test_product_arguments():
+    L = moe.load_library()
+
+    def g(a=P, sa=P, w=P, s=P, bias=None, out=P, M=4, N=64, K=256, act=api.ACT_NONE):
+        return L.moe_gemm_block128(a, sa, w, s, bias, out, M, N, K, act, None)
+
+    for kw in (dict(M=-1), dict(N=0), dict(K=0), dict(K=64), dict(K=192), dict(a=None), dict(sa=None), dict(w=None), dict(s=None), dict(out=None), dict(act=api.ACT_SWIGLU),
+               dict(act=7), dict(a=OFF8), dict(w=OFF8), dict(out=OFF8), dict(sa=OFF2), dict(s=OFF2), dict(bias=OFF1)):
+        assert g(**kw) == BAD, kw
+    for kw in (dict(N=1 << 22, K=1024), dict(K=1 << 21, N=1), dict(M=1 << 32), dict(M=(1 << 31) - 1, N=1 << 20), dict(N=1 << 40), dict(K=1 << 40)):
+        assert g(**kw) == UNSUPPORTED, kw
+    assert g(M=0) == OK and g(M=0, a=None, sa=None, out=None) == OK
+    n = [C.c_int32(0) for _ in range(3)]
+    plan = lambda M, N, K, E: L.moe_gemm_block128_plan(M, N, K, E, *[C.byref(v) for v in n])     # noqa: E731
+    assert plan(4, 64, 256, 0) == OK and plan(4, 64, 256, 8) == OK
+    assert plan(0, 64, 256, 0) == BAD and plan(4, 64, 200, 0) == BAD and plan(4, 64, 256, -1) == BAD and plan(4, 64, 256, 1000) == BAD
+    assert plan(4, 1 << 22, 1024, 0) == UNSUPPORTED and L.moe_gemm_block128_plan(4, 64, 256, 0, None, None, None) == BAD
+    assert L.moe_expert_gemm_block128(None, P, P, None, P, P, None, P, P, 128, 128, api.ACT_NONE, P, None) == BAD
+
+
+def test_python_refuses_products_that_it_can_see():
+    a, s = torch.zeros(4, 256, dtype=torch.uint8), torch.ones(4, 2)
+    w, ws = torch.zeros(130, 256, dtype=torch.uint8), torch.ones(2, 2)
+    with pytest.raises(ValueError, match="matrices"):
+        moe.gemm_block128(a[0], s, w, ws)
+    for bad in ((a, s[:, :1], w, ws), (a, s, w, ws[:1]), (torch.zeros(256, 4, dtype=torch.uint8).t(), s, w, ws), (a, s, w, ws, torch.zeros(128, dtype=torch.bfloat16))):
+        with pytest.raises(ValueError):
+            moe.gemm_block128(*bad)
+    with pytest.raises(TypeError):
+        moe.gemm_block128(a, s, w.float(), ws)
+    with pytest.raises(ValueError, match="contiguous"):
+        moe.gemm_block128(a, s, torch.zeros(256, 130, dtype=torch.uint8).t(), ws)
+    with pytest.raises(ValueError, match="current GPU"):
+        moe.gemm_block128(a, s, w, ws)
