@@ -7,6 +7,7 @@
 // Memory bounds all of it: every array passes once.  A row stays in the registers of the threads that fetched it, 16 bytes of every operand a
 // thread and step, from the sum of its squares to its results.
 #include "ffn_common.hpp"
+#include "mxfp4.hpp"
 #include "rows8.hpp"
 
 namespace moe355 {
@@ -25,25 +26,57 @@ template <> __device__ __forceinline__ float narrow<f32_e>(float v) { return v; 
 template <> __device__ __forceinline__ uint16_t narrow<bf16_e>(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }
 template <> __device__ __forceinline__ uint16_t narrow<f16_e>(float v) { return __builtin_bit_cast(uint16_t, (_Float16)v); }
 
-// VEC neighbouring elements, fetched and stored as one.
-template <class RAW, int VEC>
-struct alignas(sizeof(RAW) * VEC) Piece { RAW e[VEC]; };
-template <class T, int VEC>
-__device__ __forceinline__ Piece<typename T::raw, VEC> load(const void* p, int64_t element) {
-    return *reinterpret_cast<const Piece<typename T::raw, VEC>*>(static_cast<const typename T::raw*>(p) + element);
+// 16 bytes of neighbouring elements, fetched and stored as one.  WHOLE: rows begin on 16 bytes and end with a piece; else a piece lies anywhere that an
+// element can (memory takes 16 bytes from any address), and the last of a row may have fewer elements: those behind the row's end are zeros,
+// and are not stored.
+template <class T> constexpr int kNormVec = 16 / (int)sizeof(typename T::raw);
+template <class RAW>
+struct alignas(16) Piece { RAW e[16 / sizeof(RAW)]; };
+template <class T, bool WHOLE>
+__device__ __forceinline__ Piece<typename T::raw> load(const void* p, int64_t element, int left) {
+    typedef typename T::raw RAW;
+    const RAW* at = static_cast<const RAW*>(p) + element;
+    if constexpr (WHOLE) {
+        return *reinterpret_cast<const Piece<RAW>*>(at);
+    } else {
+        Piece<RAW> v = {};
+        if (left >= kNormVec<T>) {
+            __builtin_memcpy(&v, at, 16);
+        } else {
+#pragma unroll
+            for (int k = 0; k < kNormVec<T>; ++k)
+                if (k < left) v.e[k] = at[k];
+        }
+        return v;
+    }
 }
-template <class T, int VEC>
-__device__ __forceinline__ void store(void* p, int64_t element, const Piece<typename T::raw, VEC>& v) {
-    *reinterpret_cast<Piece<typename T::raw, VEC>*>(static_cast<typename T::raw*>(p) + element) = v;
+template <class T, bool WHOLE>
+__device__ __forceinline__ void store(void* p, int64_t element, int left, const Piece<typename T::raw>& v) {
+    typedef typename T::raw RAW;
+    RAW* at = static_cast<RAW*>(p) + element;
+    if constexpr (WHOLE) {
+        *reinterpret_cast<Piece<RAW>*>(at) = v;
+    } else if (left >= kNormVec<T>) {
+        __builtin_memcpy(at, &v, 16);
+    } else {
+#pragma unroll
+        for (int k = 0; k < kNormVec<T>; ++k)
+            if (k < left) at[k] = v.e[k];
+    }
 }
 // Of the norm's weights, in the rows' type or in fp32.
-template <class T, int VEC>
-__device__ __forceinline__ void load_weights(float (&w)[VEC], const void* p, bool f32, int c) {
+template <class T, bool WHOLE>
+__device__ __forceinline__ void load_weights(float (&w)[kNormVec<T>], const void* p, bool f32, int c, int left) {
+    constexpr int VEC = kNormVec<T>;
     if (f32) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) w[i] = static_cast<const float*>(p)[c + i];
+        for (int i = 0; i < VEC; i += 4) {
+            const auto v = load<f32_e, WHOLE>(p, c + i, left - i);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[i + k] = v.e[k];
+        }
     } else {
-        const auto v = load<T, VEC>(p, c);
+        const auto v = load<T, WHOLE>(p, c, left);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) w[i] = widen<T>(v.e[i]);
     }
@@ -51,9 +84,16 @@ __device__ __forceinline__ void load_weights(float (&w)[VEC], const void* p, boo
 
 // ---- sums over the threads of a row, in a fixed order, in all of them ----
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int off = 1; off < kWave; off <<= 1) v += __shfl_xor(v, off, kWave);
-    return v;
+    v += row_turned<8>(v);
+    v += row_turned<4>(v);
+    v += row_turned<2>(v);
+    v += row_turned<1>(v);
+    // of both rows of either half, then of both halves: what a swap leaves in its two results
+    const uint32_t r = __float_as_uint(v);
+    const auto rows = __builtin_amdgcn_permlane16_swap(r, r, false, false);
+    const uint32_t h = __float_as_uint(__uint_as_float(rows[0]) + __uint_as_float(rows[1]));
+    const auto halves = __builtin_amdgcn_permlane32_swap(h, h, false, false);
+    return __uint_as_float(halves[0]) + __uint_as_float(halves[1]);
 }
 // N sums at once; part: [N][waves of the row], of this row alone.
 template <int THREADS, int N>
@@ -77,13 +117,13 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float* part) {
     }
 }
 
-// THREADS threads to a row, NV pieces of VEC columns each; narrow rows share a workgroup of 256.
-template <int THREADS> constexpr int kNormBlock = THREADS < 256 ? 256 : THREADS;
+// THREADS threads to a row, NV pieces each; of rows that a wavefront holds, four share a workgroup.
+template <int THREADS> constexpr int kNormBlock = THREADS == kWave ? 4 * kWave : THREADS;
 
-template <class T, int VEC, int NV, int THREADS, bool Q8>
+template <class T, int NV, int THREADS, bool WHOLE, bool Q8>
 __global__ __launch_bounds__(kNormBlock<THREADS>) void norm_rows_kernel(NormArgs a) {
-    constexpr int ROWS = kNormBlock<THREADS> / THREADS;
-    typedef Piece<typename T::raw, VEC> P;
+    constexpr int ROWS = kNormBlock<THREADS> / THREADS, VEC = kNormVec<T>;
+    typedef Piece<typename T::raw> P;
     __shared__ float part[THREADS / kWave];
     const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / THREADS;
     const int t = threadIdx.x % THREADS;
@@ -94,19 +134,19 @@ __global__ __launch_bounds__(kNormBlock<THREADS>) void norm_rows_kernel(NormArgs
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (t + THREADS * i) * VEC;
-        if (c < a.H) x[i] = load<T, VEC>(a.x, at + c);
+        if (c < a.H) x[i] = load<T, WHOLE>(a.x, at + c, a.H - c);
     }
     if (a.residual) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (t + THREADS * i) * VEC;
-            if (c < a.H) res[i] = load<T, VEC>(a.residual, at + c);
+            if (c < a.H) res[i] = load<T, WHOLE>(a.residual, at + c, a.H - c);
         }
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (t + THREADS * i) * VEC;
-        if (c < a.H) load_weights<T, VEC>(w[i], a.weight, a.weight_f32, c);
+        if (c < a.H) load_weights<T, WHOLE>(w[i], a.weight, a.weight_f32, c, a.H - c);
     }
     float sum[1] = {0.0f};
 #pragma unroll
@@ -116,7 +156,7 @@ __global__ __launch_bounds__(kNormBlock<THREADS>) void norm_rows_kernel(NormArgs
         if (a.residual) {
 #pragma unroll
             for (int k = 0; k < VEC; ++k) x[i].e[k] = narrow<T>(widen<T>(x[i].e[k]) + widen<T>(res[i].e[k]));
-            store<T, VEC>(a.sum, at + c, x[i]);
+            store<T, WHOLE>(a.sum, at + c, a.H - c, x[i]);
         }
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
@@ -137,30 +177,30 @@ __global__ __launch_bounds__(kNormBlock<THREADS>) void norm_rows_kernel(NormArgs
             P o;
 #pragma unroll
             for (int k = 0; k < VEC; ++k) o.e[k] = narrow<T>(y[k]);
-            store<T, VEC>(a.out, at + c, o);
+            store<T, WHOLE>(a.out, at + c, a.H - c, o);
         }
         if constexpr (Q8) {
             constexpr int LANES = kRows8Piece / VEC;
+            struct alignas(VEC) Codes { uint32_t e[VEC / 4]; } q;
             float amax = 0.0f;
 #pragma unroll
             for (int k = 0; k < VEC; ++k) amax = fmaxf(amax, fabsf(y[k]));
             const float s = rows8_scale(rows8_max<LANES>(amax)), inverse = 1.0f / s;
             if (t % LANES == 0) a.scales[row * (a.H / kRows8Piece) + c / kRows8Piece] = s;
-            Piece<uint32_t, VEC / 4> q;
 #pragma unroll
             for (int k = 0; k < VEC; k += 4) q.e[k / 4] = rows8_codes(y[k], y[k + 1], y[k + 2], y[k + 3], s, inverse);
-            *reinterpret_cast<Piece<uint32_t, VEC / 4>*>(a.q + at + c) = q;
+            *reinterpret_cast<Codes*>(a.q + at + c) = q;
         }
     }
 }
 
 // The gradients.  A workgroup takes every gridDim.x-th row (ROWS of them at a time) and keeps its threads' columns of dw in registers; what it has of dw
 // at the end is a row of `part`, and norm_weight_grad_kernel adds those up in their order: no atomics, the same bits every time.  The next
-// row's operands are on their way while a row's sums are made.
-template <class T, int VEC, int NV, int THREADS>
+// row's operands are on their way while a row's sums are made, where a thread's share of a row is small.
+template <class T, int NV, int THREADS, bool WHOLE>
 __global__ __launch_bounds__(kNormBlock<THREADS>) void norm_backward_kernel(NormBackwardArgs a) {
-    constexpr int ROWS = kNormBlock<THREADS> / THREADS;
-    typedef Piece<typename T::raw, VEC> P;
+    constexpr int ROWS = kNormBlock<THREADS> / THREADS, VEC = kNormVec<T>;
+    typedef Piece<typename T::raw> P;
     __shared__ float part[2][2 * (THREADS / kWave)];
     const int t = threadIdx.x % THREADS;
     const int64_t step = (int64_t)gridDim.x * ROWS;
@@ -170,7 +210,7 @@ __global__ __launch_bounds__(kNormBlock<THREADS>) void norm_backward_kernel(Norm
         const int c = (t + THREADS * i) * VEC;
 #pragma unroll
         for (int k = 0; k < VEC; ++k) w[i][k] = dw[i][k] = 0.0f;
-        if (c < a.H) load_weights<T, VEC>(w[i], a.weight, a.weight_f32, c);
+        if (c < a.H) load_weights<T, WHOLE>(w[i], a.weight, a.weight_f32, c, a.H - c);
     }
     P h[NV], dy[NV], ds[NV];
     auto fetch = [&](int64_t row) {
@@ -179,71 +219,75 @@ __global__ __launch_bounds__(kNormBlock<THREADS>) void norm_backward_kernel(Norm
         for (int i = 0; i < NV; ++i) {
             const int c = (t + THREADS * i) * VEC;
             if (c >= a.H) continue;
-            h[i] = load<T, VEC>(a.h, row * a.H + c);
-            dy[i] = load<T, VEC>(a.dy, row * a.H + c);
-            if (a.dsum) ds[i] = load<T, VEC>(a.dsum, row * a.H + c);
+            h[i] = load<T, WHOLE>(a.h, row * a.H + c, a.H - c);
+            dy[i] = load<T, WHOLE>(a.dy, row * a.H + c, a.H - c);
+            if (a.dsum) ds[i] = load<T, WHOLE>(a.dsum, row * a.H + c, a.H - c);
         }
     };
+    constexpr bool AHEAD = NV == 1;               // (wider rows: the registers do not hold two rows' operands)
     int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / THREADS;
-    fetch(row);
+    if (AHEAD) fetch(row);
     for (int turn = 0; row < a.rows; row += step, turn ^= 1) {
         const int64_t at = row * a.H;
-        float hv[NV][VEC], dn[NV][VEC], sums[2] = {0.0f, 0.0f};
-        P ds_now[NV];
+        if (!AHEAD) fetch(row);
+        float sums[2] = {0.0f, 0.0f};
+        P h_now[NV], dy_now[NV], ds_now[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             if ((t + THREADS * i) * VEC >= a.H) continue;
-            ds_now[i] = ds[i];
+            h_now[i] = h[i], dy_now[i] = dy[i], ds_now[i] = ds[i];
 #pragma unroll
             for (int k = 0; k < VEC; ++k) {
-                hv[i][k] = widen<T>(h[i].e[k]);
-                dn[i][k] = widen<T>(dy[i].e[k]);
-                sums[0] = __builtin_fmaf(hv[i][k], hv[i][k], sums[0]);
-                sums[1] = __builtin_fmaf(dn[i][k] * w[i][k], hv[i][k], sums[1]);
+                const float hv = widen<T>(h[i].e[k]);
+                sums[0] = __builtin_fmaf(hv, hv, sums[0]);
+                sums[1] = __builtin_fmaf(widen<T>(dy[i].e[k]) * w[i][k], hv, sums[1]);
             }
         }
-        fetch(row + step);
+        if (AHEAD) fetch(row + step);
         row_sums<THREADS, 2>(sums, part[turn]);
         const float r = 1.0f / sqrtf(sums[0] / (float)a.H + a.eps), along = sums[1] * r / (float)a.H;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (t + THREADS * i) * VEC;
             if (c >= a.H) continue;
+            if (!AHEAD) {                         // as fetched, and not widened since: of several pieces the registers do not hold both
+                asm volatile("" : "+v"(*reinterpret_cast<mx_u32x4*>(&h_now[i])));
+                asm volatile("" : "+v"(*reinterpret_cast<mx_u32x4*>(&dy_now[i])));
+            }
             P o;
 #pragma unroll
             for (int k = 0; k < VEC; ++k) {
-                const float n = hv[i][k] * r;
-                dw[i][k] = __builtin_fmaf(dn[i][k], n, dw[i][k]);
-                float d = r * (dn[i][k] * w[i][k] - n * along);
-                if (a.dsum) d += widen<T>(ds_now[i].e[k]);
-                o.e[k] = narrow<T>(d);
+                const float n = widen<T>(h_now[i].e[k]) * r, d = widen<T>(dy_now[i].e[k]);
+                dw[i][k] = __builtin_fmaf(d, n, dw[i][k]);
+                float v = r * (d * w[i][k] - n * along);
+                if (a.dsum) v += widen<T>(ds_now[i].e[k]);
+                o.e[k] = narrow<T>(v);
             }
-            store<T, VEC>(a.dx, at + c, o);
+            store<T, WHOLE>(a.dx, at + c, a.H - c, o);
         }
     }
     if constexpr (ROWS > 1) {                      // the rows of a workgroup share a row of partial sums
-        extern __shared__ float shared[];          // [ROWS][H]
+        __shared__ float shared[ROWS][THREADS * NV * VEC];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (t + THREADS * i) * VEC;
-            if (c >= a.H) continue;
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) shared[(threadIdx.x / THREADS) * a.H + c + k] = dw[i][k];
+            for (int k = 0; k < VEC; ++k) shared[threadIdx.x / THREADS][c + k] = dw[i][k];
         }
         __syncthreads();
         for (int c = threadIdx.x; c < a.H; c += kNormBlock<THREADS>) {
-            float s = shared[c];
+            float s = shared[0][c];
 #pragma unroll
-            for (int g = 1; g < ROWS; ++g) s += shared[g * a.H + c];
+            for (int g = 1; g < ROWS; ++g) s += shared[g][c];
             a.part[(int64_t)blockIdx.x * a.H + c] = s;
         }
     } else {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (t + THREADS * i) * VEC;
-            if (c >= a.H) continue;
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) a.part[(int64_t)blockIdx.x * a.H + c + k] = dw[i][k];
+            for (int k = 0; k < VEC; ++k)
+                if (c + k < a.H) a.part[(int64_t)blockIdx.x * a.H + c + k] = dw[i][k];
         }
     }
 }
@@ -271,29 +315,29 @@ __global__ __launch_bounds__(1024) void norm_weight_grad_kernel(const float* __r
 
 // ---- the experts' activation ----
 //
-// silu(g) u, gelu(u) or relu(u) of bf16 rows, to e4m3.  The exponential of an argument in two parts and a reciprocal with one Newton step: what
-// is rounded to four bits next is then as good as with the library's expf and a division, and its code as seldom the neighbour of the exact one's.
-__device__ __forceinline__ float silu_to8(float g) {
-    constexpr float kLog2e = 1.44269504088896340736f, kLog2eRest = 1.92596299e-8f;      // log2(e) = the sum
-    const float hi = fminf(fmaxf(g * -kLog2e, -200.0f), 126.0f);
-    const float lo = fmaxf(__builtin_fmaf(g, -kLog2e, -hi) - g * kLog2eRest, -1.0f);      // (2^-16 at most, but where hi was cut)
-    const float e = __builtin_amdgcn_exp2f(hi);
-    const float d = 1.0f + __builtin_fmaf(e, lo * 0.693147180559945309417f, e);
-    const float r = __builtin_amdgcn_rcpf(d);
-    return g * (hi < 126.0f ? __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r) : 0.0f);      // further out the result is below 2^-119: 0 (of -infinity: NaN)
-}
+// silu(g) u, gelu(u) or relu(u) of bf16 rows, to e4m3.  Hardware exp2 and reciprocal (1 ulp each): the result is off by about as much as with the
+// library's expf and a division -- the argument's rounding is ln 2 |g| 2^-24 of the exponential -- and four bits see neither.  What it saves is time:
+// the vector ALU, not memory, bounded the kernel with an exponential of an argument in two parts, a Newton step and clamps: 16384 x 14336
+// SwiGLU 234 us.  Out of range everything falls into place: exp2 gives infinity and the reciprocal 0 for far negative g, and NaN for -infinity.
+__device__ __forceinline__ float silu_to8(float g) { return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.4426950408889634f)); }
 
-template <int ACT>
+// COLD: more rows than the memory-side cache holds, read past it (16384 x 14336 SwiGLU 196 -> 175 to 186 us; 6000 x 1408, which the products in front have
+// left there, 9.0 -> 9.8).
+template <int ACT, bool COLD>
 __global__ __launch_bounds__(256) void act_rows128_kernel(const uint16_t* __restrict__ u, const uint16_t* __restrict__ g, const int32_t* __restrict__ count,
                                                           const int32_t* __restrict__ offset, int E, int64_t rows, int I, uint8_t* __restrict__ q,
                                                           float* __restrict__ scales) {
     const int64_t kept = count ? min((int64_t)offset[E - 1] + count[E - 1], rows) : rows;
     const int64_t chunk = (int64_t)blockIdx.x * 256 + threadIdx.x;      // 8 values; 16 lanes share a piece
     if (chunk >= kept * (I / 8)) return;
-    const auto uu = load<bf16_e, 8>(u, chunk * 8);
+    auto fetch = [&](const uint16_t* p) {
+        if constexpr (COLD) return __builtin_bit_cast(Piece<uint16_t>, __builtin_nontemporal_load(reinterpret_cast<const mx_u32x4*>(p + chunk * 8)));
+        else return load<bf16_e, true>(p, chunk * 8, 8);
+    };
+    const auto uu = fetch(u);
     float v[8], amax = 0.0f;
     if constexpr (ACT == MOE_ACT_SWIGLU) {
-        const auto gg = load<bf16_e, 8>(g, chunk * 8);
+        const auto gg = fetch(g);
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = silu_to8(widen<bf16_e>(gg.e[k])) * widen<bf16_e>(uu.e[k]);
     } else {
@@ -309,64 +353,55 @@ __global__ __launch_bounds__(256) void act_rows128_kernel(const uint16_t* __rest
 
 // ---- launches ----
 
-template <class T> constexpr int kNormVec = 16 / (int)sizeof(typename T::raw);
-
-// f(threads, pieces a thread, columns a piece), as types: the fewest threads that hold a row in four pieces each, or, where the rows are few and
-// nothing but latency counts, in one.  Columns one by one where rows do not begin on 16 bytes.
+// f(threads, pieces a thread), as types: one piece a thread, and as few wavefronts as that takes, up to 16; then two or four.  8192 rows in bf16, us, 256
+// threads of several pieces / this: norm of 4096 values 49 / 44, of 7168 97 / 88, to e4m3 56 / 51, gradients 64 / 47; 64 rows of 7168 5.0 / 3.6.
+// (BACKWARD: for wide rows eight wavefronts, which have twice the registers each that sixteen have.)
 template <class T, bool BACKWARD, class F>
-hipError_t with_norm_shape(int H, int64_t rows, bool whole, F f) {
-    constexpr int V = kNormVec<T>;
-    auto go = [&](auto threads, auto nv, auto vec) { return f(threads, nv, vec); };
-#define NORM_SHAPE(TH, NV, VEC) go(std::integral_constant<int, TH>{}, std::integral_constant<int, NV>{}, std::integral_constant<int, VEC>{})
-    if (!whole) {
-        if (!BACKWARD && H <= 1024) return NORM_SHAPE(64, 16, 1);
-        if (H <= 4096) return NORM_SHAPE(256, 16, 1);
-        return NORM_SHAPE(1024, 16, 1);
+hipError_t with_norm_shape(int H, F f) {
+    const int pieces = (H + kNormVec<T> - 1) / kNormVec<T>;
+    auto go = [&](auto threads, auto nv) { return f(threads, nv); };
+    typedef std::integral_constant<int, 1> One;
+    if (pieces <= 64) return go(std::integral_constant<int, 64>{}, One{});
+    if (pieces <= 128) return go(std::integral_constant<int, 128>{}, One{});
+    if (pieces <= 256) return go(std::integral_constant<int, 256>{}, One{});
+    if (pieces <= 512) return go(std::integral_constant<int, 512>{}, One{});
+    if (pieces <= 1024) return go(std::integral_constant<int, 1024>{}, One{});
+    constexpr int WIDE = BACKWARD ? 512 : 1024;
+    if constexpr (sizeof(typename T::raw) == 4) {
+        if (pieces > 2048) return go(std::integral_constant<int, 1024>{}, std::integral_constant<int, 4>{});
     }
-    const int pieces = (H + V - 1) / V;
-    if (pieces <= 64) return NORM_SHAPE(64, 1, V);
-    if (!BACKWARD && rows >= 4096 && pieces <= 128) return NORM_SHAPE(64, 2, V);
-    if (pieces <= 256) return NORM_SHAPE(256, 1, V);
-    if (pieces <= 512) return NORM_SHAPE(256, 2, V);
-    if (pieces <= 1024) return NORM_SHAPE(256, 4, V);
-    if (pieces <= 2048) return NORM_SHAPE(1024, 2, V);
-    return NORM_SHAPE(1024, 4, V);
-#undef NORM_SHAPE
+    return go(std::integral_constant<int, WIDE>{}, std::integral_constant<int, 2048 / WIDE>{});
 }
 
-template <class T, bool Q8>
-hipError_t launch_norm_of(const NormArgs& a, bool whole, hipStream_t st) {
-    return with_norm_shape<T, false>(a.H, a.rows, whole, [&](auto threads, auto nv, auto vec) {
-        constexpr int TH = decltype(threads)::value, NV = decltype(nv)::value, V = decltype(vec)::value, ROWS = kNormBlock<TH> / TH;
-        if constexpr (Q8 && V == 1) {
-            return hipErrorInvalidValue;          // (rows of e4m3 are whole pieces of 128)
-        } else {
-            norm_rows_kernel<T, V, NV, TH, Q8><<<(unsigned)((a.rows + ROWS - 1) / ROWS), kNormBlock<TH>, 0, st>>>(a);
-            return hipGetLastError();
-        }
-    });
-}
 template <class T>
 hipError_t launch_norm_type(const NormArgs& a, hipStream_t st) {
-    constexpr int V = kNormVec<T>;
     auto off = [](const void* p) { return (uintptr_t)p % 16 != 0; };
-    const bool whole = a.H % V == 0 && !off(a.x) && !off(a.residual) && !off(a.weight) && !off(a.sum) && !off(a.out);
-    return a.q ? launch_norm_of<T, true>(a, whole, st) : launch_norm_of<T, false>(a, whole, st);
+    const bool whole = a.H % kNormVec<T> == 0 && !off(a.x) && !off(a.residual) && !off(a.weight) && !off(a.sum) && !off(a.out);
+    return with_norm_shape<T, false>(a.H, [&](auto threads, auto nv) {
+        constexpr int TH = decltype(threads)::value, NV = decltype(nv)::value, ROWS = kNormBlock<TH> / TH;
+        const dim3 grid((unsigned)((a.rows + ROWS - 1) / ROWS));
+        if (a.q) norm_rows_kernel<T, NV, TH, true, true><<<grid, kNormBlock<TH>, 0, st>>>(a);
+        else if (whole) norm_rows_kernel<T, NV, TH, true, false><<<grid, kNormBlock<TH>, 0, st>>>(a);
+        else norm_rows_kernel<T, NV, TH, false, false><<<grid, kNormBlock<TH>, 0, st>>>(a);
+        return hipGetLastError();
+    });
 }
 
-// Rows of partial sums of dw: as many workgroups as keep four on a compute unit busy, and not more than a quarter of the rows beyond one each.
-int64_t norm_parts(int64_t rows) { return std::min<int64_t>(rows, std::min<int64_t>(1024, std::max<int64_t>(256, rows / 4))); }
+// Rows of partial sums of dw, 1024 at most: workgroups of 4096 wavefronts in all (16 a compute unit: 8192 rows of 4096 47 us, 52 with twice as many, 62
+// with half), but not more than a quarter of the rows beyond one for each compute unit.
+int64_t norm_parts(int64_t rows, int threads) { return std::min<int64_t>(rows, std::min<int64_t>(4096 * 64 / std::max(threads, 256), std::max<int64_t>(256, rows / 4))); }
 
 template <class T>
 hipError_t launch_norm_backward_type(const NormBackwardArgs& a, hipStream_t st) {
-    constexpr int V = kNormVec<T>;
     auto off = [](const void* p) { return (uintptr_t)p % 16 != 0; };
-    const bool whole = a.H % V == 0 && !off(a.h) && !off(a.dy) && !off(a.dsum) && !off(a.weight) && !off(a.dx);
-    const int64_t parts = norm_parts(a.rows);
+    const bool whole = a.H % kNormVec<T> == 0 && !off(a.h) && !off(a.dy) && !off(a.dsum) && !off(a.weight) && !off(a.dx);
+    int64_t parts = 0;
     if (a.rows > 0) {
-        const hipError_t e = with_norm_shape<T, true>(a.H, a.rows, whole, [&](auto threads, auto nv, auto vec) {
-            constexpr int TH = decltype(threads)::value, NV = decltype(nv)::value, VE = decltype(vec)::value, ROWS = kNormBlock<TH> / TH;
-            norm_backward_kernel<T, VE, NV, TH><<<(unsigned)parts, kNormBlock<TH>, ROWS > 1 ? ROWS * a.H * 4 : 0, st>>>(a);
+        const hipError_t e = with_norm_shape<T, true>(a.H, [&](auto threads, auto nv) {
+            constexpr int TH = decltype(threads)::value, NV = decltype(nv)::value;
+            parts = norm_parts(a.rows, TH);
+            if (whole) norm_backward_kernel<T, NV, TH, true><<<(unsigned)parts, kNormBlock<TH>, 0, st>>>(a);
+            else norm_backward_kernel<T, NV, TH, false><<<(unsigned)parts, kNormBlock<TH>, 0, st>>>(a);
             return hipGetLastError();
         });
         if (e != hipSuccess) return e;
@@ -408,7 +443,7 @@ extern "C" int moe_rms_norm(const void* x, const void* residual, const void* wei
 extern "C" int moe_rms_norm_scratch_bytes(int64_t rows, int32_t H, size_t* bytes) {
     if (rows < 0 || H < 1 || !bytes) return MOE_ERR_BAD_ARGUMENT;
     if (H > kNormMost || rows > kNormRows) return MOE_ERR_UNSUPPORTED;
-    *bytes = (size_t)norm_parts(rows) * H * sizeof(float);
+    *bytes = (size_t)norm_parts(rows, 0) * H * sizeof(float);
     return MOE_OK;
 }
 
@@ -420,7 +455,7 @@ extern "C" int moe_rms_norm_backward(const void* dout, const void* h, const void
     for (const void* p : {dout, h, dsum, (const void*)dx})
         if (!norm_element(p, dtype)) return MOE_ERR_BAD_ARGUMENT;
     if (!norm_element(weight, weight_dtype) || !norm_element(dweight, weight_dtype)) return MOE_ERR_BAD_ARGUMENT;
-    if (rows > 0 && (!scratch || (uintptr_t)scratch % 4 || scratch_bytes < (size_t)norm_parts(rows) * H * sizeof(float))) return MOE_ERR_WORKSPACE;
+    if (rows > 0 && (!scratch || (uintptr_t)scratch % 4 || scratch_bytes < (size_t)norm_parts(rows, 0) * H * sizeof(float))) return MOE_ERR_WORKSPACE;
     const NormBackwardArgs a{dout, h, weight, dsum, dx, dweight, (float*)scratch, rows, H, eps, weight_dtype == MOE_DTYPE_F32};
     hipStream_t st = (hipStream_t)stream;
     const hipError_t e = dtype == MOE_DTYPE_F32 ? launch_norm_backward_type<f32_e>(a, st) : dtype == MOE_DTYPE_BF16 ? launch_norm_backward_type<bf16_e>(a, st) : launch_norm_backward_type<f16_e>(a, st);
@@ -443,7 +478,9 @@ extern "C" int moe_act_rows128(const void* u, const void* g, int64_t rows, int32
         kernel<<<grid, 256, 0, st>>>((const uint16_t*)u, (const uint16_t*)g, expert_count, expert_offset, E, rows, I, (uint8_t*)q, scales);
         return hipGetLastError() == hipSuccess ? MOE_OK : MOE_ERR_HIP;
     };
-    if (act == MOE_ACT_SWIGLU) return launch(act_rows128_kernel<MOE_ACT_SWIGLU>);
-    if (act == MOE_ACT_GELU) return launch(act_rows128_kernel<MOE_ACT_GELU>);
-    return launch(act_rows128_kernel<MOE_ACT_RELU>);
+    const bool cold = rows * I * (g ? 4 : 2) > ((int64_t)256 << 20);
+    auto of = [&](auto a) { return cold ? launch(act_rows128_kernel<decltype(a)::value, true>) : launch(act_rows128_kernel<decltype(a)::value, false>); };
+    if (act == MOE_ACT_SWIGLU) return of(std::integral_constant<int, MOE_ACT_SWIGLU>{});
+    if (act == MOE_ACT_GELU) return of(std::integral_constant<int, MOE_ACT_GELU>{});
+    return of(std::integral_constant<int, MOE_ACT_RELU>{});
 }

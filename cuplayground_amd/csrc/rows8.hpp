@@ -10,11 +10,20 @@ namespace {
 
 constexpr int kRows8Piece = 128;      // values that share a scale
 
-// The maximum over neighbouring lanes, LANES a power of two up to 32, in all of them.  (fmaxf passes over a NaN.)
+// Lanes of a row of 16, turned by N places: a DPP move, which the operation that takes it does on its way.
+template <int N>
+__device__ __forceinline__ float row_turned(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x120 + N, 0xF, 0xF, true));
+}
+// The maximum over 16 or 32 neighbouring lanes, in all of them.  (fmaxf passes over a NaN.)
 template <int LANES>
 __device__ __forceinline__ float rows8_max(float v) {
-#pragma unroll
-    for (int off = LANES / 2; off; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, kWave));
+    static_assert(LANES == 16 || LANES == 32, "rows of lanes");
+    v = fmaxf(v, row_turned<8>(v));
+    v = fmaxf(v, row_turned<4>(v));
+    v = fmaxf(v, row_turned<2>(v));
+    v = fmaxf(v, row_turned<1>(v));
+    if constexpr (LANES == 32) v = fmaxf(v, __shfl_xor(v, 16, kWave));
     return v;
 }
 __device__ __forceinline__ float rows8_scale(float amax) { return amax > 0.0f ? fmaxf(amax / 448.0f, 0x1p-126f) : 1.0f; }
