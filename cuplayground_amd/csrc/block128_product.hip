@@ -194,7 +194,7 @@ struct RowsTile {
     static_assert(LDS <= 160 * 1024, "LDS of a compute unit");
 };
 
-template <class T>
+template <class T, bool COLD>
 __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_tile_kernel(RowsProduct p) {
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr int NT = T::NT, CG = T::CG, KS = T::KS, SET = T::SET, BM = T::BM, BN = T::BN, AHEAD = T::AHEAD;
@@ -239,7 +239,7 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_tile_kerne
         for (int l = first; l < last && l < LOADS; ++l) {
             const int i = l - T::LOADS_W;
             if (l < T::LOADS_W)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(w_buf, (mx_lds_void*)(st + BM * 128 + (l * SET + sw) * 1024), 16, (int)(in ? w_off + at + l * SET * 8 * K : kBehind), 0, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(w_buf, (mx_lds_void*)(st + BM * 128 + (l * SET + sw) * 1024), 16, (int)(in ? w_off + at + l * SET * 8 * K : kBehind), 0, 0, COLD ? 2 : 0);
             else
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(a_buf, (mx_lds_void*)(st + (i * SET + sw) * 1024), 16, (int)(in ? a_off[i] + at : kBehind), 0, 0, 0);
         }
@@ -353,7 +353,7 @@ struct RowsDeep {
     static_assert(128 % (16 * CG) == 0 && LDS <= 160 * 1024, "columns of one scale; LDS of a compute unit");
 };
 
-template <class T>
+template <class T, bool COLD>
 __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_deep_kernel(RowsProduct p) {
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr int NT = T::NT, CG = T::CG, SET = T::SET, BM = T::BM, BN = T::BN, HALF = T::HALF;
@@ -390,7 +390,7 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_deep_kerne
     // Where a slab lies in the rows is a scalar offset (below K, which no buffer is shorter than: the range check compares with what it leaves of the
     // buffer).  Behind the last slab: the last one again, which nobody reads.
     auto issue_columns = [&](int s, int h, int l) {
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(w_buf, (mx_lds_void*)(smem + (s & 1) * T::STAGE + (BM + in_tile(h, l)) * 128), 16, (int)w_off[h][l], 128 * min(s, KB - 1), 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(w_buf, (mx_lds_void*)(smem + (s & 1) * T::STAGE + (BM + in_tile(h, l)) * 128), 16, (int)w_off[h][l], 128 * min(s, KB - 1), 0, COLD ? 2 : 0);
     };
     auto issue_rows = [&](int s, int i) {
         __builtin_amdgcn_raw_ptr_buffer_load_lds(a_buf, (mx_lds_void*)(smem + (s & 1) * T::STAGE + (i * SET + sw) * 1024), 16, (int)a_off[i], 128 * min(s, KB - 1), 0, 0);
@@ -528,6 +528,14 @@ int64_t rows_grid(const RowsProduct& p, int BM, int BN) {
     return (blocks * ncol + 7) / 8 * 8 + (p.count ? 16 : 0);
 }
 
+// Weights that are not kept behind their one reading: more than the memory-side cache would hold for the next call, and about one block of
+// rows for each.  Kept / not, us: 65536 x 4096 for one row 51.5 / 46.4; 256 experts of 2048 x 7168, 128 rows 303 / 277, 512 rows 624 / 563; 8 of 14336 x
+// 4096, 128 rows 98 / 86 -- but 14336 x 4096 for 48 rows, which the cache holds, 12.4 / 15.3, and many rows on 8 of 4096 x 14336 1225 / 1640.
+bool rows_cold(const RowsProduct& p, int block_rows) {
+    const int64_t experts = p.count ? std::min<int64_t>(p.E, p.M) : 1;
+    return p.M <= experts * block_rows && experts * p.N * p.K > ((int64_t)256 << 20);
+}
+
 struct RowsCut {
     bool wide;
     int KS;
@@ -545,7 +553,7 @@ RowsCut rows_cut(const RowsProduct& p) {
 }
 hipError_t launch_rows_stream(const RowsProduct& p, hipStream_t st) {
     const RowsCut c = rows_cut(p);
-    const bool cold = (p.count ? std::min<int64_t>(p.E, p.M) : 1) * p.N * p.K > ((int64_t)256 << 20);      // more than the memory-side cache holds
+    const bool cold = rows_cold(p, 16);
     const unsigned grid = (unsigned)rows_grid(p, 16, 16 * (c.wide ? 2 : 1) * (kRowsWaves / c.KS));
     auto launch = [&](auto kernel) {
         kernel<<<grid, 64 * kRowsWaves, 0, st>>>(p, c.KS);
@@ -556,15 +564,15 @@ hipError_t launch_rows_stream(const RowsProduct& p, hipStream_t st) {
     auto columns = [&](auto g) { return more ? rows(g, std::true_type{}) : rows(g, std::false_type{}); };
     return c.wide ? columns(std::integral_constant<int, 2>{}) : columns(std::integral_constant<int, 1>{});
 }
-template <class T>
-struct RowsKernel { static constexpr void (*kernel)(RowsProduct) = rows_tile_kernel<T>; };
-template <int RH, int NT, int CW, int CG>
-struct RowsKernel<RowsDeep<RH, NT, CW, CG>> { static constexpr void (*kernel)(RowsProduct) = rows_deep_kernel<RowsDeep<RH, NT, CW, CG>>; };
-template <class T>
+template <class T, bool COLD>
+struct RowsKernel { static constexpr void (*kernel)(RowsProduct) = rows_tile_kernel<T, COLD>; };
+template <int RH, int NT, int CW, int CG, bool COLD>
+struct RowsKernel<RowsDeep<RH, NT, CW, CG>, COLD> { static constexpr void (*kernel)(RowsProduct) = rows_deep_kernel<RowsDeep<RH, NT, CW, CG>, COLD>; };
+template <class T, bool COLD>
 hipError_t launch_rows_tile(const RowsProduct& p, hipStream_t st) {
-    const hipError_t e = allow_lds(RowsKernel<T>::kernel, T::LDS);
+    const hipError_t e = allow_lds(RowsKernel<T, COLD>::kernel, T::LDS);
     if (e != hipSuccess) return e;
-    RowsKernel<T>::kernel<<<(unsigned)rows_grid(p, T::BM, T::BN), T::THREADS, T::LDS, st>>>(p);
+    RowsKernel<T, COLD>::kernel<<<(unsigned)rows_grid(p, T::BM, T::BN), T::THREADS, T::LDS, st>>>(p);
     return hipGetLastError();
 }
 
@@ -583,14 +591,14 @@ auto with_rows_tile(int form, F f) {
 }
 
 // What a tile costs, in us: a launch of its form; a slab of the contraction where a compute unit has one tile; the same for every further tile of the
-// unit.  Fitted to 270 products of 1 to 6000 rows, 4 to 1000 us, dense and of experts, evenly and not, each with every form: the choice by
-// these is 0.8 % behind the best of the forms on average, 34 % at worst (90 to 240 rows for each of 8 experts with a long contraction).
+// unit.  Fitted to 575 products of 1 to 6000 rows, 4 to 1000 us, dense and of experts, evenly and not, each with every form: the choice by
+// these is 1.0 % behind the best of the forms on average, 35 % at worst (one row times 4352 x 6400).
 struct RowsCost {
     int rows, columns;
     float launch, slab, more;
 };
-constexpr RowsCost kRowsTiles[] = {{}, {16, 64, 3.9f, 0.142f, 0.466f}, {32, 64, 3.75f, 0.203f, 1.0f}, {64, 64, 4.26f, 0.25f, 0.683f}, {64, 128, 4.0f, 0.305f, 0.72f},
-                                   {128, 128, 4.36f, 0.847f, 0.643f}, {128, 256, 6.37f, 0.968f, 1.89f}, {256, 256, 6.77f, 1.373f, 2.07f}};
+constexpr RowsCost kRowsTiles[] = {{}, {16, 64, 3.88f, 0.153f, 0.458f}, {32, 64, 3.63f, 0.252f, 0.493f}, {64, 64, 4.54f, 0.25f, 0.969f}, {64, 128, 3.92f, 0.37f, 0.483f},
+                                   {128, 128, 5.16f, 0.754f, 0.553f}, {128, 256, 4.3f, 0.866f, 1.41f}, {256, 256, 6.36f, 1.467f, 1.478f}};
 
 // The form that should take least; 0: the streamer.  Of experts' rows the host knows how many there are, not whose: a block an expert where the
 // mean is small for it, else half a block more than the mean fills.
@@ -600,7 +608,7 @@ int block_form(const RowsProduct& p) {
     const RowsCut c = rows_cut(p);
     auto row_blocks = [&](int rows) { return !p.count ? (double)((p.M + rows - 1) / rows) : each > 0.6 * rows ? (double)p.M / rows + 0.5 * experts : (double)experts; };
     const double rounds = std::max(1.0, c.waves / 2048.0) * (p.count ? row_blocks(16) / experts : 1.0);
-    double best = each > 16 ? 1e30 : 1.9 + 0.036 * each + c.chunks * rounds * ((c.wide ? 2.29 : 1.03) + 0.055 * each);
+    double best = each > 16 ? 1e30 : 2.83 + 0.0545 * each + c.chunks * rounds * ((c.wide ? 1.565 : 0.868) + 0.0135 * each);
     int form = 0;
     for (int f = 1; f < (int)(sizeof kRowsTiles / sizeof kRowsTiles[0]); ++f) {
         const RowsCost& t = kRowsTiles[f];
@@ -632,7 +640,10 @@ int check_product_block128(const RowsProduct& p, int* form) {
 hipError_t launch_product_block128(const RowsProduct& p, int form, hipStream_t st) {
     if (p.M == 0) return hipSuccess;
     if (form == 0) return launch_rows_stream(p, st);
-    return with_rows_tile(form, [&](auto* t) { return launch_rows_tile<std::remove_pointer_t<decltype(t)>>(p, st); });
+    return with_rows_tile(form, [&](auto* t) {
+        typedef std::remove_pointer_t<decltype(t)> T;
+        return rows_cold(p, T::BM) ? launch_rows_tile<T, true>(p, st) : launch_rows_tile<T, false>(p, st);
+    });
 }
 
 }  // namespace moe355
