@@ -127,6 +127,8 @@ __global__ __launch_bounds__(64 * kRowsWaves) void rows_stream_kernel(RowsProduc
         }
     };
     auto fetch_scales = [&](int c) { raw = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(s_buf, (int)(c + q < end ? s_at + 4u * (uint32_t)c : kBehind), 0, 0)); };
+    MxBias<G, 16> bias;
+    bias.fetch(p, t, n0 + 4 * q);
     mx_f32x4 acc[1][G] = {};
     if (begin < end) {
         // The weights' scales: one a block of K, 64 of them in the lanes of a register.
@@ -166,7 +168,7 @@ __global__ __launch_bounds__(64 * kRowsWaves) void rows_stream_kernel(RowsProduc
         }
     }
     if (!skinny_join<G>(acc[0], ks, KS, red + set * (KS - 1) * G * 64, lane)) return;
-    mx_store_tile<1, G>(p, t, lane & 15, n0 + 4 * q, acc);
+    mx_store_tile<1, G>(p, t, lane & 15, n0 + 4 * q, acc, &bias);
 }
 
 // ---- more rows: tiles ----
@@ -250,7 +252,9 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_tile_kerne
     // LDS, and return out of order: every wait for a fragment would be one for all.)
     const int c0 = t.n0 + 16 * CG * wn;
     const float* const ws = t.s + (int64_t)min(c0 >> 7, (N - 1) >> 7) * KB;
-    float held = 0.0f;
+    float held = begin + lane < end ? ws[begin + lane] : 0.0f;      // (the first ones: in front of all requests)
+    MxBias<CG, 16> bias;
+    bias.fetch(p, t, c0 + 4 * q);
     auto weight_scale = [&](int s) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, held), s & 63)); };
     auto hold = [&](int s) {
         held = begin + s + lane < end ? ws[begin + s + lane] : 0.0f;
@@ -305,9 +309,10 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_tile_kerne
 #pragma unroll
     for (int s = 0; s < AHEAD; ++s) issue(s, stages + s * T::STAGE, 0, LOADS);
     constexpr int PER = (LOADS + CG - 1) / CG;
+    asm volatile("" : "+v"(held));
     if (t.rows > wm * 16 * NT) {
         for (int s = 0; s < slabs; ++s) {
-            if ((s & 63) == 0) hold(s);
+            if ((s & 63) == 0 && s > 0) hold(s);
             const float s_w = weight_scale(s);
             meet();
             slab(now, s_w, [&](int g) { issue(s + AHEAD, fill, g * PER, g * PER + PER); });
@@ -324,11 +329,11 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_tile_kerne
     if constexpr (KS == 1) {
         mx_meet();                                // (requests for slabs behind the last one: zeros, but they write to LDS)
         if (!(N & 7)) {
-            mx_store_rows<NT, CG, 16, 16>(p, t, smem + sw * mx_rows_lds<NT, CG, 16, 16>(), lane, idx, 4 * q, 16 * wm * NT, c0, acc);
+            mx_store_rows<NT, CG, 16, 16>(p, t, smem + sw * mx_rows_lds<NT, CG, 16, 16>(), lane, idx, 4 * q, 16 * wm * NT, c0, acc, &bias);
             return;
         }
     }
-    mx_store_tile<NT, CG>(p, t, 16 * wm * NT + idx, c0 + 4 * q, acc);
+    mx_store_tile<NT, CG>(p, t, 16 * wm * NT + idx, c0 + 4 * q, acc, &bias);
 }
 
 // -- large tiles: halves of a slab --
@@ -406,7 +411,10 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_deep_kerne
     auto meet_second = [] { mx_meet<2 * T::LOADS_H + ROWS_IN_ALL>(); };
     const int c0 = t.n0 + 16 * CG * wn;
     const float* const ws = t.s + (int64_t)min(c0 >> 7, (N - 1) >> 7) * KB;
-    float held = 0.0f;                            // the weights' scales of 64 slabs (rows_tile_kernel)
+    float held = lane < KB ? ws[lane] : 0.0f;     // the weights' scales of 64 slabs (rows_tile_kernel)
+    constexpr bool EARLY = CG <= 4;               // (the widest tile has no registers for its bias)
+    MxBias<CG, 16> bias;
+    if (EARLY) bias.fetch(p, t, c0 + 4 * q);
     auto hold = [&](int s) {
         held = s + lane < KB ? ws[s + lane] : 0.0f;
         asm volatile("" : "+v"(held));            // (the wait for it is here, not in every slab)
@@ -436,6 +444,7 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_deep_kerne
     for (int j = 0; j < 2 * T::LOADS_H; ++j) issue_columns(0, j / T::LOADS_H, j % T::LOADS_H);
 #pragma unroll
     for (int i = 0; i < T::LOADS_A; ++i) issue_rows(1, i);
+    asm volatile("" : "+v"(held));
     if (t.rows > wm * 16 * NT) {
         mx_i32x8 x[NT], w[2];
         float sc[NT], sc_next[NT];
@@ -471,7 +480,7 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_deep_kerne
             __builtin_amdgcn_sched_barrier(0);
         };
         for (int s = 0; s < KB; ++s) {
-            if ((s & 63) == 0) hold(s);
+            if ((s & 63) == 0 && s > 0) hold(s);
             const float s_w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, held), s & 63));
             const unsigned char* st = smem + (s & 1) * T::STAGE;
             const unsigned char* xb = st + (wm * 16 * NT + idx) * 128;
@@ -515,8 +524,8 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_deep_kerne
         }
     }
     mx_meet();                                    // (the requests behind the last slab write to LDS)
-    if (!(N & 7)) mx_store_rows<NT, CG, 16, 16>(p, t, smem + sw * mx_rows_lds<NT, CG, 16, 16>(), lane, idx, 4 * q, 16 * wm * NT, c0, acc);
-    else mx_store_tile<NT, CG>(p, t, 16 * wm * NT + idx, c0 + 4 * q, acc);
+    if (!(N & 7)) mx_store_rows<NT, CG, 16, 16>(p, t, smem + sw * mx_rows_lds<NT, CG, 16, 16>(), lane, idx, 4 * q, 16 * wm * NT, c0, acc, EARLY ? &bias : nullptr);
+    else mx_store_tile<NT, CG>(p, t, 16 * wm * NT + idx, c0 + 4 * q, acc, EARLY ? &bias : nullptr);
 }
 
 // ---- launches ----

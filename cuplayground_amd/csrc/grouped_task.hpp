@@ -30,7 +30,10 @@ template <int BIG>
 __device__ __forceinline__ bool grouped_task(const int32_t* __restrict__ count, const int32_t* __restrict__ offset, int E, int ncol, int id, GroupedTask& t) {
     constexpr int LEFT = BIG == 256 ? 128 : 0;          // rows up to which what is left of an expert is a block of its own kind
     const int lane = threadIdx.x & 63;
-    auto rows_of = [&](int c) { return c + lane < E ? max(count[c + lane], 0) : 0; };
+    // (the first 64 experts' counts and offsets in one trip to memory)
+    const int first_rows = lane < E ? max(count[lane], 0) : 0, first_offset = lane < E ? offset[lane] : 0;
+    auto rows_of = [&](int c) { return c == 0 ? first_rows : c + lane < E ? max(count[c + lane], 0) : 0; };
+    auto offset_of = [&](int c) { return c == 0 ? first_offset : c + lane < E ? offset[c + lane] : 0; };
     auto big_of = [&](int n) { return (n + BIG - 1 - LEFT) / BIG; };
     int big_sum = 0, left_sum = 0;         // full row blocks and remainders of all experts
     for (int c = 0; c < E; c += kWave) {
@@ -56,7 +59,7 @@ __device__ __forceinline__ bool grouped_task(const int32_t* __restrict__ count, 
     }
     int base = 0;                          // full row blocks of the experts in front
     for (int c = 0; c < E; c += kWave) {
-        const int n = rows_of(c), big = big_of(n);
+        const int n = rows_of(c), o = offset_of(c), big = big_of(n);
         int inc = big;
 #pragma unroll
         for (int off = 1; off < kWave; off <<= 1) {
@@ -77,7 +80,7 @@ __device__ __forceinline__ bool grouped_task(const int32_t* __restrict__ count, 
             rb += local - t.ctile * width;
             t.expert = c + l;
             t.rows = min(BIG, __builtin_amdgcn_readlane(n, l) - rb * BIG);
-            t.row0 = offset[t.expert] + rb * BIG;
+            t.row0 = __builtin_amdgcn_readlane(o, l) + rb * BIG;
             return true;
         }
         base += total;
@@ -86,7 +89,7 @@ __device__ __forceinline__ bool grouped_task(const int32_t* __restrict__ count, 
         int before = (id - base * ncol) / ncol;      // remainders in front of this one
         t.ctile = (id - base * ncol) - before * ncol;
         for (int c = 0; c < E; c += kWave) {
-            const int n = rows_of(c), left = max(n - big_of(n) * BIG, 0);
+            const int n = rows_of(c), o = offset_of(c), left = max(n - big_of(n) * BIG, 0);
             const unsigned long long m = __ballot(left > 0);
             const int here = __popcll(m);
             if (before < here) {
@@ -94,7 +97,7 @@ __device__ __forceinline__ bool grouped_task(const int32_t* __restrict__ count, 
                 const int l = __builtin_ctzll(__ballot(((m >> lane) & 1) && rank == before));
                 t.expert = c + l;
                 t.rows = __builtin_amdgcn_readlane(left, l);
-                t.row0 = offset[t.expert] + (__builtin_amdgcn_readlane(n, l) - t.rows);
+                t.row0 = __builtin_amdgcn_readlane(o, l) + (__builtin_amdgcn_readlane(n, l) - t.rows);
                 return true;
             }
             before -= here;

@@ -15,26 +15,40 @@ __device__ __forceinline__ int64_t mx_uniform(int64_t v) {
 }
 
 // The bias of CG groups of four neighbouring columns, COLS apart; of columns behind the last some bias.  All loads at once and without a
-// question: one trip to memory.
-template <int CG, int COLS, class PRODUCT, class TASK>
-__device__ __forceinline__ void mx_bias(const PRODUCT& p, const TASK& t, int col0, mx_f32x4 (&b)[CG]) {
-#pragma unroll
-    for (int g = 0; g < CG; ++g) b[g] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
-    if (!t.bias) return;
+// question: one trip to memory -- and, where a kernel holds them as they come (fetch()) from its start on, one that nothing waits for.
+template <int CG, int COLS>
+struct MxBias {
     uint16_t raw[CG][4];
-    if (p.N & 3) {
+    bool any;
+    template <class PRODUCT, class TASK>
+    __device__ __forceinline__ void fetch(const PRODUCT& p, const TASK& t, int col0) {
+        any = t.bias != nullptr;
+        if (!any) return;
+        if (p.N & 3) {
+#pragma unroll
+            for (int g = 0; g < CG; ++g)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) raw[g][r] = t.bias[min(col0 + COLS * g + r, p.N - 1)];
+        } else {
+#pragma unroll
+            for (int g = 0; g < CG; ++g) __builtin_memcpy(raw[g], t.bias + min(col0 + COLS * g, p.N - 4), 8);
+        }
+    }
+    __device__ __forceinline__ void widen(mx_f32x4 (&b)[CG]) const {
+#pragma unroll
+        for (int g = 0; g < CG; ++g) b[g] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
+        if (!any) return;
 #pragma unroll
         for (int g = 0; g < CG; ++g)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) raw[g][r] = t.bias[min(col0 + COLS * g + r, p.N - 1)];
-    } else {
-#pragma unroll
-        for (int g = 0; g < CG; ++g) __builtin_memcpy(raw[g], t.bias + min(col0 + COLS * g, p.N - 4), 8);
+            for (int r = 0; r < 4; ++r) b[g][r] = bf16_bits_to_f32(raw[g][r]);
     }
-#pragma unroll
-    for (int g = 0; g < CG; ++g)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) b[g][r] = bf16_bits_to_f32(raw[g][r]);
+};
+template <int CG, int COLS, class PRODUCT, class TASK>
+__device__ __forceinline__ void mx_bias(const PRODUCT& p, const TASK& t, int col0, mx_f32x4 (&b)[CG]) {
+    MxBias<CG, COLS> raw;
+    raw.fetch(p, t, col0);
+    raw.widen(b);
 }
 // Four neighbouring columns of a token row, as the matrix instructions leave them in a lane.  whole: N is a multiple of 4.
 template <int ACT, class TASK>
@@ -55,10 +69,11 @@ __device__ __forceinline__ void mx_store4(const TASK& t, int N, bool whole, int 
 }
 // ... for NT x CG of them: rows row0 + ROWS i, columns col0 + COLS g.  One activation for all: a switch at every value costs more than the values.
 template <int NT, int CG, int ROWS = 16, int COLS = 16, class PRODUCT, class TASK>
-__device__ __forceinline__ void mx_store_tile(const PRODUCT& p, const TASK& t, int row0, int col0, const mx_f32x4 (&acc)[NT][CG]) {
+__device__ __forceinline__ void mx_store_tile(const PRODUCT& p, const TASK& t, int row0, int col0, const mx_f32x4 (&acc)[NT][CG], const MxBias<CG, COLS>* held = nullptr) {
     const int N = p.N;
     mx_f32x4 b[CG];
-    mx_bias<CG, COLS>(p, t, col0, b);
+    if (held) held->widen(b);
+    else mx_bias<CG, COLS>(p, t, col0, b);
     auto all = [&](auto act_c, auto whole_c) {
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
@@ -84,10 +99,11 @@ __device__ __forceinline__ void mx_store_tile(const PRODUCT& p, const TASK& t, i
 template <int NT, int CG, int ROWS, int COLS>
 __device__ __host__ constexpr int mx_rows_lds() { return ROWS * NT * (2 * COLS * CG + 16); }
 template <int NT, int CG, int ROWS, int COLS, class PRODUCT, class TASK>
-__device__ __forceinline__ void mx_store_rows(const PRODUCT& p, const TASK& t, unsigned char* own, int lane, int row, int col, int row0, int col0, const mx_f32x4 (&acc)[NT][CG]) {
+__device__ __forceinline__ void mx_store_rows(const PRODUCT& p, const TASK& t, unsigned char* own, int lane, int row, int col, int row0, int col0, const mx_f32x4 (&acc)[NT][CG], const MxBias<CG, COLS>* held = nullptr) {
     constexpr int PITCH = 2 * COLS * CG + 16, LANES = COLS * CG / 8;      // LANES of 16 bytes to a row
     mx_f32x4 b[CG];
-    mx_bias<CG, COLS>(p, t, col0 + col, b);
+    if (held) held->widen(b);
+    else mx_bias<CG, COLS>(p, t, col0 + col, b);
     auto all = [&](auto act_c) {
         constexpr int ACT = decltype(act_c)::value;
 #pragma unroll
