@@ -217,19 +217,9 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_tile_kerne
     const int64_t rows_all = p.token ? p.tokens : t.rows;
     const __amdgpu_buffer_rsrc_t a_buf = mx_buffer(t.a, (uint32_t)(rows_all * K)), w_buf = mx_buffer(t.w, (uint32_t)N * K),
                                  s_buf = mx_buffer(t.a_scales, (uint32_t)(rows_all * KB * 4));
-    uint32_t a_off[T::LOADS_A];
-#pragma unroll
-    for (int i = 0; i < T::LOADS_A; ++i) {
-        const uint32_t src = rows_source(p, t, 8 * (i * SET + sw) + lrow);
-        a_off[i] = src == kNoRow ? kBehind : src * K + 16 * chunk;
-    }
+    uint32_t a_off[T::LOADS_A], s_off = kBehind;
     const uint32_t w_off = (uint32_t)(t.n0 + 8 * sw + lrow) * K + 16 * chunk;
     const bool scaler = sw < T::SCALERS;
-    uint32_t s_off = kBehind;
-    if (scaler) {
-        const uint32_t src = rows_source(p, t, 64 * sw + lane);
-        s_off = src == kNoRow ? kBehind : src * (uint32_t)KB * 4;
-    }
     unsigned char* const stages = smem + ks * T::STAGES * T::STAGE;
     const int slabs = (KB + KS - 1) / KS, begin = ks * slabs, end = min(begin + slabs, KB);      // of the set; all run as many
     constexpr int LOADS = T::LOADS_A + T::LOADS_W;
@@ -245,7 +235,7 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_tile_kerne
             else
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(a_buf, (mx_lds_void*)(st + (i * SET + sw) * 1024), 16, (int)(in ? a_off[i] + at : kBehind), 0, 0, 0);
         }
-        if (first == 0 && scaler)
+        if (first <= T::LOADS_W && T::LOADS_W < last && scaler)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(s_buf, (mx_lds_void*)(st + (BM + BN) * 128 + sw * 256), 4, (int)(in ? s_off + 4u * (uint32_t)k : kBehind), 0, 0, 0);
     };
     // The weights' scales: one a slab, 64 slabs of them in the lanes of a register.  (As scalar loads they would share their counter with the reads of
@@ -306,8 +296,20 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_tile_kerne
     };
     unsigned char* now = stages;                  // the stage of the slab that is next; the one in front of it is filled next
     unsigned char* fill = stages + AHEAD * T::STAGE;
+    // (columns first: of rows that are fetched by index the indices have to come before)
+    issue(0, stages, 0, T::LOADS_W);
 #pragma unroll
-    for (int s = 0; s < AHEAD; ++s) issue(s, stages + s * T::STAGE, 0, LOADS);
+    for (int i = 0; i < T::LOADS_A; ++i) {
+        const uint32_t src = rows_source(p, t, 8 * (i * SET + sw) + lrow);
+        a_off[i] = src == kNoRow ? kBehind : src * K + 16 * chunk;
+    }
+    if (scaler) {
+        const uint32_t src = rows_source(p, t, 64 * sw + lane);
+        s_off = src == kNoRow ? kBehind : src * (uint32_t)KB * 4;
+    }
+    issue(0, stages, T::LOADS_W, LOADS);
+#pragma unroll
+    for (int s = 1; s < AHEAD; ++s) issue(s, stages + s * T::STAGE, 0, LOADS);
     constexpr int PER = (LOADS + CG - 1) / CG;
     asm volatile("" : "+v"(held));
     if (t.rows > wm * 16 * NT) {
@@ -375,13 +377,6 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_deep_kerne
     const int64_t rows_all = p.token ? p.tokens : t.rows;
     const __amdgpu_buffer_rsrc_t a_buf = mx_buffer(t.a, (uint32_t)(rows_all * K)), w_buf = mx_buffer(t.w, (uint32_t)N * K),
                                  s_buf = mx_buffer(t.a_scales, (uint32_t)(rows_all * KB * 4));
-    uint32_t a_off[T::LOADS_A];
-#pragma unroll
-    for (int i = 0; i < T::LOADS_A; ++i) {
-        const uint32_t src = rows_source(p, t, 8 * (i * SET + sw) + lrow);
-        a_off[i] = src == kNoRow ? kBehind : src * K + 16 * chunk;
-    }
-    const uint32_t s_src = rows_source(p, t, 64 * sw + lane), s_off = s_src == kNoRow ? kBehind : s_src * (uint32_t)KB * 4;
     // Columns: half h of every wavefront column, eight at a time; in_tile: the first of the eight that instruction l of this wavefront brings.
     auto in_tile = [&](int h, int l) {
         const int j = l * SET + sw;
@@ -397,6 +392,15 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_deep_kerne
     auto issue_columns = [&](int s, int h, int l) {
         __builtin_amdgcn_raw_ptr_buffer_load_lds(w_buf, (mx_lds_void*)(smem + (s & 1) * T::STAGE + (BM + in_tile(h, l)) * 128), 16, (int)w_off[h][l], 128 * min(s, KB - 1), 0, COLD ? 2 : 0);
     };
+#pragma unroll
+    for (int j = 0; j < 2 * T::LOADS_H; ++j) issue_columns(0, j / T::LOADS_H, j % T::LOADS_H);
+    uint32_t a_off[T::LOADS_A];
+#pragma unroll
+    for (int i = 0; i < T::LOADS_A; ++i) {
+        const uint32_t src = rows_source(p, t, 8 * (i * SET + sw) + lrow);
+        a_off[i] = src == kNoRow ? kBehind : src * K + 16 * chunk;
+    }
+    const uint32_t s_src = rows_source(p, t, 64 * sw + lane), s_off = s_src == kNoRow ? kBehind : s_src * (uint32_t)KB * 4;
     auto issue_rows = [&](int s, int i) {
         __builtin_amdgcn_raw_ptr_buffer_load_lds(a_buf, (mx_lds_void*)(smem + (s & 1) * T::STAGE + (i * SET + sw) * 1024), 16, (int)a_off[i], 128 * min(s, KB - 1), 0, 0);
         if (i == 0)
@@ -437,13 +441,12 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_deep_kerne
             for (int j = T::LOADS_A * (n - HALF) / HALF; j < T::LOADS_A * (n - HALF + 1) / HALF; ++j) issue_rows(s + 2, j);
         }
     };
-    // what slabs -1 and -2 would have asked for
+    // what slabs -1 and -2 would have asked for, columns first: of rows that are fetched by index the indices have to come before
 #pragma unroll
     for (int i = 0; i < T::LOADS_A; ++i) issue_rows(0, i);
 #pragma unroll
-    for (int j = 0; j < 2 * T::LOADS_H; ++j) issue_columns(0, j / T::LOADS_H, j % T::LOADS_H);
-#pragma unroll
     for (int i = 0; i < T::LOADS_A; ++i) issue_rows(1, i);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(ROWS_IN_ALL) : "memory");      // (slab 0's rows came behind its columns)
     asm volatile("" : "+v"(held));
     if (t.rows > wm * 16 * NT) {
         mx_i32x8 x[NT], w[2];

@@ -15,6 +15,17 @@ constexpr int kRowChunk = 8;
 struct GroupedTask {
     int expert, row0, rows, ctile;
 };
+// The sum over this lane and those in front of it: DPP moves within rows of 16 lanes, then the last lane of one row to the next, and of one half
+// to the other.  (Six steps through LDS by __shfl_up take some 600 cycles, in which nothing of the tile is on its way.)
+__device__ __forceinline__ int lanes_before(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return v;
+}
 // Which tile workgroup `id` of a grouped product takes, from the experts' row counts alone; false: none.  Order: the row blocks of
 // full height, expert by expert, column tile by column tile, an expert's row blocks (kRowChunk of them) fastest (few row blocks stay in the
 // caches while its column tiles pass by); with 256-row blocks, behind them the remainders of at most 128 rows: the long tasks start
@@ -38,15 +49,10 @@ __device__ __forceinline__ bool grouped_task(const int32_t* __restrict__ count, 
     int big_sum = 0, left_sum = 0;         // full row blocks and remainders of all experts
     for (int c = 0; c < E; c += kWave) {
         const int n = rows_of(c), big = big_of(n);
-        big_sum += big;
-        left_sum += n > big * BIG ? 1 : 0;
+        big_sum += __builtin_amdgcn_readlane(lanes_before(big), kWave - 1);
+        left_sum += __popcll(__ballot(n > big * BIG));
     }
-#pragma unroll
-    for (int off = kWave / 2; off; off >>= 1) {
-        big_sum += __shfl_xor(big_sum, off, kWave);
-        left_sum += __shfl_xor(left_sum, off, kWave);
-    }
-    const int bigs = __builtin_amdgcn_readfirstlane(big_sum) * ncol, lefts = __builtin_amdgcn_readfirstlane(left_sum) * ncol;
+    const int bigs = big_sum * ncol, lefts = left_sum * ncol;
     const int big_share = (bigs + 7) / 8, left_share = (lefts + 7) / 8;
     if (id < 8 * big_share) {
         id = (id & 7) * big_share + (id >> 3);
@@ -60,12 +66,7 @@ __device__ __forceinline__ bool grouped_task(const int32_t* __restrict__ count, 
     int base = 0;                          // full row blocks of the experts in front
     for (int c = 0; c < E; c += kWave) {
         const int n = rows_of(c), o = offset_of(c), big = big_of(n);
-        int inc = big;
-#pragma unroll
-        for (int off = 1; off < kWave; off <<= 1) {
-            const int o = __shfl_up(inc, off, kWave);
-            if (lane >= off) inc += o;
-        }
+        const int inc = lanes_before(big);
         const int total = __builtin_amdgcn_readlane(inc, kWave - 1);
         if (id < (base + total) * ncol) {
             const int l = __builtin_ctzll(__ballot((base + inc) * ncol > id));
