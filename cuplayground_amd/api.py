@@ -1309,15 +1309,17 @@ def rms_norm_rows128(x, weight, eps: float = 1e-6, residual=None, want_rows: boo
     rows, H, dtype, wdtype = _norm_operands(x, weight, ("residual", residual))
     if H % 128:
         raise ValueError("rows of %d values: rows in e4m3 hold a multiple of 128" % H)
-    for name, t in (("x", x), ("weight", weight), ("residual", residual)):
-        if t is not None:
-            _on_16_bytes(name, t)
+    at, at_w, at_res = x.data_ptr(), weight.data_ptr(), None if residual is None else residual.data_ptr()
+    if (at | at_w | (at_res or 0)) & 15:
+        for name, t in (("x", x), ("weight", weight), ("residual", residual)):
+            if t is not None:
+                _on_16_bytes(name, t)
     shape, device = x.shape, x.device
     q = torch.empty(shape, dtype=torch.uint8, device=device)
     s = torch.empty((*shape[:-1], H // 128), dtype=torch.float32, device=device)
     out = torch.empty_like(x) if want_rows else None
     h = None if residual is None else torch.empty_like(x)
-    rc = load_library().moe_rms_norm(x.data_ptr(), None if residual is None else residual.data_ptr(), weight.data_ptr(), rows, H, eps, dtype, wdtype,
+    rc = load_library().moe_rms_norm(at, at_res, at_w, rows, H, eps, dtype, wdtype,
                                      None if h is None else h.data_ptr(), None if out is None else out.data_ptr(), q.data_ptr(), s.data_ptr(), _stream())
     if rc:
         raise MoEError(rc, "moe_rms_norm")
