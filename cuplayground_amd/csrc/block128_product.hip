@@ -28,34 +28,79 @@ struct RowsTask {
     const int32_t* token;     // of the block's rows, or null
     uint16_t* out;            // at the block's first row
     int rows, n0;
+    int kind;                 // a block of a tile's rows; with 256: kLeftRows at most; kPieceRows at most and half a tile's columns
 };
+enum { kBlockTask, kLeftTask, kPieceTask };
+constexpr int kLeftRows = 128, kPieceRows = 64;
 
+// The tiles of one matrix: blocks of BM rows; with 256 what is left of at most kLeftRows stands behind them, and the last round may be in smaller tiles, as of
+// experts (grouped_task.hpp).
+struct RowsDense {
+    int blocks, lefts;
+    int64_t share, halved, left_share;          // of an XCD
+    bool pieces;
+};
+__host__ __device__ __forceinline__ RowsDense rows_dense(const RowsProduct& p, int BM, int BN) {
+    const int ncol = (p.N + BN - 1) / BN;
+    RowsDense d;
+    d.blocks = (int)((p.M + BM - 1 - (BM == 256 ? kLeftRows : 0)) / BM);
+    const int64_t left = p.M - (int64_t)d.blocks * BM;
+    const int high = left <= 0 ? 0 : left <= kPieceRows ? 1 : 2;
+    d.share = ((int64_t)d.blocks * ncol + 7) / 8;
+    d.pieces = d.share % kXcdUnits == 0 && 2 * (int64_t)high * ncol <= kGroupedUnits;
+    d.lefts = high == 0 ? 0 : d.pieces ? 2 * high * ncol : ncol;
+    d.left_share = ((int64_t)d.lefts + 7) / 8;
+    d.halved = BM == 256 ? halved_blocks(d.share, d.left_share) : 0;
+    return d;
+}
 // Which block of BM rows and which BN columns a workgroup takes.
 template <int BM>
 __device__ __forceinline__ bool rows_task(const RowsProduct& p, int BN, RowsTask& t) {
     const int ncol = (p.N + BN - 1) / BN;
-    int expert = 0, ctile, rows;
+    constexpr bool LEFT = BM == 256;
+    int expert = 0, ctile, rows, kind = kBlockTask;
     int64_t row0;
     if (p.count) {
         GroupedTask g;
-        if (!grouped_task<BM>(p.count, p.offset, p.E, ncol, (int)blockIdx.x, g)) return false;
+        if (!grouped_task<BM, LEFT ? kPieceRows : 0>(p.count, p.offset, p.E, ncol, (int)blockIdx.x, g)) return false;
         expert = g.expert, ctile = g.ctile, row0 = g.row0, rows = g.rows;
+        if (LEFT) kind = g.piece ? kPieceTask : rows <= kLeftRows ? kLeftTask : kBlockTask;
         if (row0 < 0 || row0 + rows > p.M) return false;          // tables that are not this layer's: nothing behind the buffers is touched
     } else {
-        // an eighth of the tiles in a row for each XCD, kRowChunk row blocks at a time, as for the experts
-        const int blocks = (int)((p.M + BM - 1) / BM);
-        const int64_t total = (int64_t)blocks * ncol, share = (total + 7) / 8;
-        const int64_t id = (int64_t)(blockIdx.x & 7) * share + (blockIdx.x >> 3);
-        if ((int64_t)(blockIdx.x >> 3) >= share || id >= total) return false;
-        int rb = (int)(id / ((int64_t)kRowChunk * ncol)) * kRowChunk;
-        const int width = min(kRowChunk, blocks - rb), local = (int)(id - (int64_t)rb * ncol);
-        ctile = local / width;
-        rb += local - ctile * width;
-        row0 = (int64_t)rb * BM;
-        rows = (int)min((int64_t)BM, p.M - row0);
+        // an eighth of the tiles in a row for each XCD, kRowChunk row blocks at a time, then the same of the remainder, as for the experts
+        const RowsDense d = rows_dense(p, BM, BN);
+        int64_t id = blockIdx.x >> 3;
+        const int xcd = blockIdx.x & 7;
+        if (id < d.share + d.halved) {
+            const int64_t behind = id - (d.share - d.halved);
+            if (LEFT && behind >= 0) id -= (behind + 1) >> 1;
+            id += xcd * d.share;
+            if (id >= (int64_t)d.blocks * ncol) return false;
+            int rb = (int)(id / ((int64_t)kRowChunk * ncol)) * kRowChunk;
+            const int width = min(kRowChunk, d.blocks - rb), local = (int)(id - (int64_t)rb * ncol);
+            ctile = local / width;
+            rb += local - ctile * width;
+            row0 = (int64_t)rb * BM;
+            rows = (int)min((int64_t)BM, p.M - row0);
+            if (LEFT && behind >= 0) {
+                const int first = (int)(behind & 1) * kLeftRows;
+                row0 += first, rows = min(rows - first, kLeftRows), kind = kLeftTask;
+            }
+        } else {
+            id = id - d.share - d.halved + xcd * d.left_share;
+            const int cols = d.pieces ? 2 * ncol : ncol;
+            if (id >= d.lefts || id >= (xcd + 1) * d.left_share) return false;
+            const int rb = (int)id / cols;
+            ctile = (int)id - rb * cols;
+            row0 = (int64_t)d.blocks * BM + rb * kPieceRows;
+            rows = (int)(p.M - row0);
+            if (d.pieces) rows = min(rows, kPieceRows);
+            kind = d.pieces ? kPieceTask : kLeftTask;
+        }
     }
     // the same in every lane, and said so
     row0 = mx_uniform(row0), expert = __builtin_amdgcn_readfirstlane(expert), ctile = __builtin_amdgcn_readfirstlane(ctile), rows = __builtin_amdgcn_readfirstlane(rows);
+    kind = __builtin_amdgcn_readfirstlane(kind);
     const int KB = p.K >> 7;
     const int64_t first = p.token ? 0 : row0;
     t.a = p.a + first * p.K;
@@ -66,8 +111,9 @@ __device__ __forceinline__ bool rows_task(const RowsProduct& p, int BN, RowsTask
     t.token = p.token ? p.token + row0 : nullptr;
     t.out = p.out + row0 * p.N;
     t.rows = rows;
-    t.n0 = ctile * BN;
-    return true;
+    t.n0 = ctile * (kind == kPieceTask ? BN / 2 : BN);
+    t.kind = kind;
+    return t.n0 < p.N;        // (half tiles: the last one may have no column)
 }
 // Row r of the block as the buffers below count rows; kNoRow where there is none (an index that is no token's is none).
 constexpr uint32_t kNoRow = 0xFFFFFFFFu;
@@ -201,11 +247,8 @@ struct RowsTile {
 };
 
 template <class T, bool COLD>
-__global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_tile_kernel(RowsProduct p) {
-    extern __shared__ __align__(16) unsigned char smem[];
+__device__ __forceinline__ void rows_tile(const RowsProduct& p, const RowsTask& t, unsigned char* smem) {
     constexpr int NT = T::NT, CG = T::CG, KS = T::KS, SET = T::SET, BM = T::BM, BN = T::BN, AHEAD = T::AHEAD;
-    RowsTask t;
-    if (!rows_task<BM>(p, BN, t)) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ks = wave / SET, sw = wave % SET;
     const int wm = sw / T::CW, wn = sw % T::CW;
@@ -342,6 +385,13 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_tile_kerne
     mx_store_tile<NT, CG>(p, t, 16 * wm * NT + idx, c0 + 4 * q, acc, &bias);
 }
 
+template <class T, bool COLD>
+__global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_tile_kernel(RowsProduct p) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    RowsTask t;
+    if (rows_task<T::BM>(p, T::BN, t)) rows_tile<T, COLD>(p, t, smem);
+}
+
 // -- large tiles: halves of a slab --
 //
 // What bounded the tiles above at these sizes were their loads: two stages are all that LDS has room for, a stage could be filled again once the whole
@@ -368,11 +418,8 @@ struct RowsDeep {
 };
 
 template <class T, bool COLD>
-__global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_deep_kernel(RowsProduct p) {
-    extern __shared__ __align__(16) unsigned char smem[];
+__device__ __forceinline__ void rows_deep(const RowsProduct& p, const RowsTask& t, unsigned char* smem) {
     constexpr int NT = T::NT, CG = T::CG, SET = T::SET, BM = T::BM, BN = T::BN, HALF = T::HALF;
-    RowsTask t;
-    if (!rows_task<BM>(p, BN, t)) return;
     const int lane = threadIdx.x & 63, sw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = sw / T::CW, wn = sw % T::CW;
     const int idx = lane & 15, q = lane >> 4;
@@ -538,13 +585,42 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_deep_kerne
     else mx_store_tile<NT, CG>(p, t, 16 * wm * NT + idx, c0 + 4 * q, acc, EARLY ? &bias : nullptr);
 }
 
+// The last round of blocks of 256 rows in halves, and what such blocks leave of an expert or of the one matrix, by smaller tiles behind the large ones.  Large
+// tiles for all / this, us: 2037 x 10624 x 4608 115 / 103, 3678 x 9216 x 3840 150 / 137, 1435 x 14336 x 5376 129 / 113; 8 experts of 6016 x 5760, 3104 rows 150 /
+// 132, of 4096 x 14336, 16384 rows 950 / 925 (its pieces take 40 us; the rest is 2.2 PFLOP/s, 2.4 where all rows meet one matrix: weights of
+// eight experts come from memory, each for one XCD).
+typedef RowsDeep<2, 4, 4, 4> RowsLeft;
+typedef RowsTile<1, 4, 4, 2, 2, 2> RowsPiece;
+template <class T>
+constexpr int rows_lds() { return T::BM == 256 ? std::max(T::LDS, std::max(RowsLeft::LDS, RowsPiece::LDS)) : T::LDS; }
+
+template <class T, bool COLD>
+__global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void rows_deep_kernel(RowsProduct p) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    RowsTask t;
+    if (!rows_task<T::BM>(p, T::BN, t)) return;
+    if constexpr (T::BM == 256) {
+        static_assert(RowsLeft::BM == kLeftRows && RowsLeft::BN == T::BN && RowsLeft::THREADS == T::THREADS && RowsPiece::BM == kPieceRows && 2 * RowsPiece::BN == T::BN && RowsPiece::THREADS == T::THREADS, "");
+        if (t.kind == kLeftTask) return rows_deep<RowsLeft, COLD>(p, t, smem);
+        if (t.kind == kPieceTask) return rows_tile<RowsPiece, COLD>(p, t, smem);
+    }
+    rows_deep<T, COLD>(p, t, smem);
+}
+
 // ---- launches ----
 
 // Workgroups of a launch: blocks of BM rows times column tiles, in eight equal shares.  Experts' blocks are counted on the device; M rows on n experts
-// that have any fill (M + n (BM - 1)) / BM of them at most.
+// that have any fill (M + n (BM - 1)) / BM of them at most; with pieces, the blocks in front of those and a workgroup for each of them; with
+// halves, half a round more.
 int64_t rows_grid(const RowsProduct& p, int BM, int BN) {
-    const int64_t ncol = (p.N + BN - 1) / BN, n = p.count ? std::min<int64_t>(p.E, p.M) : 1, blocks = (p.M + n * (BM - 1)) / BM;
-    return (blocks * ncol + 7) / 8 * 8 + (p.count ? 16 : 0);
+    if (!p.count) {
+        const RowsDense d = rows_dense(p, BM, BN);
+        return 8 * (d.share + d.halved + d.left_share);
+    }
+    const int64_t ncol = (p.N + BN - 1) / BN, n = std::min<int64_t>(p.E, p.M);
+    int64_t tiles = (p.M + n * (BM - 1)) / BM * ncol;
+    if (BM == 256) tiles = std::max(tiles, (p.M + n * (BM - 1 - kLeftRows)) / BM * ncol + kGroupedUnits) + kGroupedUnits / 2;
+    return (tiles + 7) / 8 * 8 + 16;
 }
 
 // Weights that are not kept behind their one reading: more than the memory-side cache would hold for the next call, and about one block of
@@ -589,9 +665,9 @@ template <int RH, int NT, int CW, int CG, bool COLD>
 struct RowsKernel<RowsDeep<RH, NT, CW, CG>, COLD> { static constexpr void (*kernel)(RowsProduct) = rows_deep_kernel<RowsDeep<RH, NT, CW, CG>, COLD>; };
 template <class T, bool COLD>
 hipError_t launch_rows_tile(const RowsProduct& p, hipStream_t st) {
-    const hipError_t e = allow_lds(RowsKernel<T, COLD>::kernel, T::LDS);
+    const hipError_t e = allow_lds(RowsKernel<T, COLD>::kernel, rows_lds<T>());
     if (e != hipSuccess) return e;
-    RowsKernel<T, COLD>::kernel<<<(unsigned)rows_grid(p, T::BM, T::BN), T::THREADS, T::LDS, st>>>(p);
+    RowsKernel<T, COLD>::kernel<<<(unsigned)rows_grid(p, T::BM, T::BN), T::THREADS, rows_lds<T>(), st>>>(p);
     return hipGetLastError();
 }
 
@@ -631,7 +707,8 @@ int block_form(const RowsProduct& p) {
     int form = 0;
     for (int f = 1; f < (int)(sizeof kRowsTiles / sizeof kRowsTiles[0]); ++f) {
         const RowsCost& t = kRowsTiles[f];
-        const double tiles = std::ceil(row_blocks(t.rows) * ((p.N + t.columns - 1) / t.columns) / 256.0);      // of the compute unit that has most
+        double tiles = std::ceil(row_blocks(t.rows) * ((p.N + t.columns - 1) / t.columns) / 256.0);      // of the compute unit that has most
+        if (t.rows == 256 && tiles - row_blocks(t.rows) * ((p.N + t.columns - 1) / t.columns) / 256.0 >= 0.5) tiles -= 0.4;      // halves in the last round
         const double cost = t.launch + p.K / 128 * (t.slab + t.more * (tiles - 1));
         if (cost < best) best = cost, form = f;
     }

@@ -14,6 +14,7 @@ constexpr int kShareSlack = 14;      // workgroups without a tile, at most: the 
 constexpr int kRowChunk = 8;
 struct GroupedTask {
     int expert, row0, rows, ctile;
+    bool piece;      // (with PIECE) a remainder's piece: ctile counts half tiles
 };
 // The sum over this lane and those in front of it: DPP moves within rows of 16 lanes, then the last lane of one row to the next, and of one half
 // to the other.  (Six steps through LDS by __shfl_up take some 600 cycles, in which nothing of the tile is on its way.)
@@ -37,7 +38,14 @@ __device__ __forceinline__ int lanes_before(int v) {
 // The share of an XCD in a row, against the list dealt out to them: whole layers as two launches, 8 experts of 4096 x 14336, 2048 rows
 // 4679 -> 4431 us, 1024 rows 2860 -> 2484; 64 of 2048 x 1408, 1536 rows 1863 -> 1662, 750 rows 1089 -> 907; 12 of 1344 x 2752, 444 rows
 // 174 -> 165, 150 rows 125 -> 107.
-template <int BIG>
+// PIECE > 0: the last round of an XCD's compute units in smaller tiles, where it has a unit for each of those: blocks in halves, or, where no block is
+// in it, remainders in pieces of so many rows and half a tile's columns.
+constexpr int kGroupedUnits = 256, kXcdUnits = kGroupedUnits / 8;      // compute units
+__host__ __device__ __forceinline__ int64_t halved_blocks(int64_t share, int64_t left_share) {      // of the tiles of an XCD, the last ones
+    const int64_t rest = share % kXcdUnits;
+    return 2 * rest + left_share <= kXcdUnits ? rest : 0;
+}
+template <int BIG, int PIECE = 0>
 __device__ __forceinline__ bool grouped_task(const int32_t* __restrict__ count, const int32_t* __restrict__ offset, int E, int ncol, int id, GroupedTask& t) {
     constexpr int LEFT = BIG == 256 ? 128 : 0;          // rows up to which what is left of an expert is a block of its own kind
     const int lane = threadIdx.x & 63;
@@ -46,19 +54,25 @@ __device__ __forceinline__ bool grouped_task(const int32_t* __restrict__ count, 
     auto rows_of = [&](int c) { return c == 0 ? first_rows : c + lane < E ? max(count[c + lane], 0) : 0; };
     auto offset_of = [&](int c) { return c == 0 ? first_offset : c + lane < E ? offset[c + lane] : 0; };
     auto big_of = [&](int n) { return (n + BIG - 1 - LEFT) / BIG; };
-    int big_sum = 0, left_sum = 0;         // full row blocks and remainders of all experts
+    int big_sum = 0, left_sum = 0, piece_sum = 0;         // full row blocks and remainders of all experts
     for (int c = 0; c < E; c += kWave) {
         const int n = rows_of(c), big = big_of(n);
         big_sum += __builtin_amdgcn_readlane(lanes_before(big), kWave - 1);
         left_sum += __popcll(__ballot(n > big * BIG));
+        if (PIECE) piece_sum += __popcll(__ballot(n > big * BIG)) + __popcll(__ballot(n > big * BIG + PIECE));
     }
-    const int bigs = big_sum * ncol, lefts = left_sum * ncol;
-    const int big_share = (bigs + 7) / 8, left_share = (lefts + 7) / 8;
-    if (id < 8 * big_share) {
-        id = (id & 7) * big_share + (id >> 3);
+    const bool pieces = PIECE && (big_sum * ncol + 7) / 8 % kXcdUnits == 0 && 2 * piece_sum * ncol <= kGroupedUnits;
+    const int left_cols = pieces ? 2 * ncol : ncol, bigs = big_sum * ncol, lefts = (pieces ? piece_sum : left_sum) * left_cols;
+    const int big_share = (bigs + 7) / 8, left_share = (lefts + 7) / 8, halved = PIECE ? (int)halved_blocks(big_share, left_share) : 0;
+    int half = -1;
+    if (id < 8 * (big_share + halved)) {
+        int i = id >> 3;
+        const int whole = big_share - halved;
+        if (PIECE && i >= whole) half = (i - whole) & 1, i = whole + ((i - whole) >> 1);
+        id = (id & 7) * big_share + i;
         if (id >= bigs) return false;
     } else {
-        id -= 8 * big_share;
+        id -= 8 * (big_share + halved);
         if ((id >> 3) >= left_share) return false;
         id = (id & 7) * left_share + (id >> 3) + bigs;
         if (id >= bigs + lefts) return false;
@@ -82,23 +96,33 @@ __device__ __forceinline__ bool grouped_task(const int32_t* __restrict__ count, 
             t.expert = c + l;
             t.rows = min(BIG, __builtin_amdgcn_readlane(n, l) - rb * BIG);
             t.row0 = __builtin_amdgcn_readlane(o, l) + rb * BIG;
+            t.piece = false;
+            if (PIECE && half >= 0) t.row0 += half * (BIG / 2), t.rows = min(t.rows - half * (BIG / 2), BIG / 2);
             return true;
         }
         base += total;
     }
     if constexpr (LEFT > 0) {
-        int before = (id - base * ncol) / ncol;      // remainders in front of this one
-        t.ctile = (id - base * ncol) - before * ncol;
+        static_assert(PIECE == 0 || LEFT <= 2 * PIECE, "two pieces a remainder");
+        int before = (id - base * ncol) / left_cols;      // remainders, or pieces' rows, in front of this one
+        t.ctile = (id - base * ncol) - before * left_cols;
+        t.piece = pieces;
         for (int c = 0; c < E; c += kWave) {
             const int n = rows_of(c), o = offset_of(c), left = max(n - big_of(n) * BIG, 0);
-            const unsigned long long m = __ballot(left > 0);
-            const int here = __popcll(m);
+            unsigned long long m = __ballot(left > 0);
+            const int first = __popcll(m);
+            const unsigned long long m2 = pieces ? __ballot(left > PIECE) : 0;
+            const int here = first + __popcll(m2);
             if (before < here) {
+                const int behind = before < first ? 0 : PIECE;      // rows of the remainder in front
+                if (before >= first) m = m2, before -= first;
                 const int rank = __popcll(m & ((1ull << lane) - 1ull));
                 const int l = __builtin_ctzll(__ballot(((m >> lane) & 1) && rank == before));
                 t.expert = c + l;
                 t.rows = __builtin_amdgcn_readlane(left, l);
-                t.row0 = __builtin_amdgcn_readlane(o, l) + (__builtin_amdgcn_readlane(n, l) - t.rows);
+                t.row0 = __builtin_amdgcn_readlane(o, l) + (__builtin_amdgcn_readlane(n, l) - t.rows) + behind;
+                t.rows -= behind;
+                if (pieces) t.rows = min(t.rows, PIECE);
                 return true;
             }
             before -= here;

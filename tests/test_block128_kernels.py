@@ -79,3 +79,60 @@ def test_experts(M, N, K, E, kernel, how):
             _check(out[o:o + n], (q[o:o + n], s[o:o + n], w[e], ws[e]), b[e], api.ACT_NONE)
         o += n
     assert (out[o:] == 7).all()
+
+
+# The last round of the largest tiles (256 compute units, 32 of a share) in smaller ones: blocks of 256 rows in halves; what is left of up to 128 rows in
+# pieces of 64 x 128, where no block is beside it, or as a tile of its own.  M, N, K.
+LAST = [(2100, 8187, 384), (2148, 8136, 384), (2052, 8192, 512), (2148, 17617, 384), (2100, 5977, 384), (2204, 8190, 384), (2344, 8192, 384), (2177, 5976, 384),
+        (20564, 1000, 384), (2304, 8187, 512)]
+# rows of 70 experts (all rows are 40000), with remainders in both parts of the table, one behind another, and of one row: pieces; halves and tiles; tiles
+SOME = {3: 612, 4: 576, 5: 577, 20: 1, 21: 0, 22: 128, 23: 129, 63: 640, 64: 520, 66: 0, 67: 612, 69: 64}
+PIECES = tuple(SOME.get(e, 512 if e < 65 else 256) for e in range(70))
+HALVES = tuple(SOME.get(e, 512 if e < 69 else 300) for e in range(70))
+TILES_LEFT = tuple(257 + e % 128 if e % 3 else 700 for e in range(70))
+
+
+def _last(counts, N):
+    """(halves, pieces, tiles of what is left) of these row counts."""
+    ncol = (N + 255) // 256
+    share = -(-sum((n + 127) // 256 for n in counts) * ncol // 8)
+    left = [n % 256 for n in counts if 0 < n % 256 <= 128]
+    high = sum(1 if n <= 64 else 2 for n in left)
+    if share % 32 == 0 and 2 * high * ncol <= 256:
+        return 0, 2 * high * ncol, 0
+    rest, tiles = share % 32, len(left) * ncol
+    return (rest if 2 * rest + -(-tiles // 8) <= 32 else 0), 0, tiles
+
+
+def test_the_sizes_below_end_in_every_way():
+    assert all(_plan(M, N, K) == (256, 256, 1) for M, N, K in LAST) and _plan(40000, 512, 384, 70) == (256, 256, 1)
+    assert {tuple(v > 0 for v in _last((M,), N)) for M, N, K in LAST} >= {(False, True, False), (False, False, True), (True, False, True), (True, False, False)}
+    assert [tuple(v > 0 for v in _last(c, 512)) for c in (PIECES, HALVES, TILES_LEFT)] == [(False, True, False), (True, False, True), (False, False, True)]
+    assert max(sum(c) for c in (PIECES, HALVES, TILES_LEFT)) <= 40000
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K", LAST)
+def test_the_last_round(M, N, K):
+    q, s, w, ws, b = _operands(M, N, K, seed=M + N)
+    for bias, act in ((None, api.ACT_NONE), (b, api.ACT_GELU)):
+        _check(moe.gemm_block128(q, s, w, ws, bias=bias, act=act), (q, s, w, ws), bias, act)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("counts", [PIECES, HALVES, TILES_LEFT])
+@pytest.mark.parametrize("gather", [False, True])
+def test_the_last_round_of_experts(counts, gather):
+    M, N, K, E = 40000, 512, 384, 70
+    q, s, w, ws, b = _operands(M, N, K, E, seed=sum(counts))
+    layer = _layer(M, 1, E, N, K)
+    out = torch.full((M, N), 7.0, dtype=BF16, device=DEV)
+    rows = torch.randperm(M, generator=torch.Generator().manual_seed(5)).to(DEV) if gather else torch.arange(M, device=DEV)
+    layer.expert_gemm_block128(q, s, w, ws, b, *_tables(counts), out=out, token_indices=rows.int() if gather else None)
+    o = 0
+    for e, n in enumerate(counts):
+        if n:
+            r = rows[o:o + n]
+            _check(out[o:o + n], (q[r], s[r], w[e], ws[e]), b[e], api.ACT_NONE)
+        o += n
+    assert (out[o:] == 7).all()
