@@ -625,10 +625,12 @@ int64_t rows_grid(const RowsProduct& p, int BM, int BN) {
 
 // Weights that are not kept behind their one reading: more than the memory-side cache would hold for the next call, and about one block of
 // rows for each.  Kept / not, us: 65536 x 4096 for one row 51.5 / 46.4; 256 experts of 2048 x 7168, 128 rows 303 / 277, 512 rows 624 / 563; 8 of 14336 x
-// 4096, 128 rows 98 / 86 -- but 14336 x 4096 for 48 rows, which the cache holds, 12.4 / 15.3, and many rows on 8 of 4096 x 14336 1225 / 1640.
+// 4096, 128 rows 98 / 86 -- but 14336 x 4096 for 48 rows, which the cache holds, 12.4 / 15.3, and many rows on 8 of 4096 x 14336 1225 / 1640.  Between two
+// calls with an expert's matrix come those with the layer's others, so half of the cache is enough: 64 of 1408 x 2048, three layers in
+// turn, 30 rows each 39.8 / 35.5, 94 rows 50.1 / 48.7, 32 of 2048 x 4096, 12 rows 62.9 / 56.2 (a single matrix again and again 30.4 / 35.2, 40 / 44.5, 40.7 / 53.7).
 bool rows_cold(const RowsProduct& p, int block_rows) {
     const int64_t experts = p.count ? std::min<int64_t>(p.E, p.M) : 1;
-    return p.M <= experts * block_rows && experts * p.N * p.K > ((int64_t)256 << 20);
+    return p.M <= experts * block_rows && experts * p.N * p.K > ((int64_t)(p.count ? 128 : 256) << 20);
 }
 
 struct RowsCut {
@@ -687,7 +689,8 @@ auto with_rows_tile(int form, F f) {
 
 // What a tile costs, in us: a launch of its form; a slab of the contraction where a compute unit has one tile; the same for every further tile of the
 // unit.  Fitted to 575 products of 1 to 6000 rows, 4 to 1000 us, dense and of experts, evenly and not, each with every form: the choice by
-// these is 1.0 % behind the best of the forms on average, 35 % at worst (one row times 4352 x 6400).
+// these was 1.0 % behind the best of the forms on average.  Over 1324 others it is 0.9 % behind for one matrix and 1.9 % for experts (a fit
+// to those alone 0.9 and 1.3), 50 % at worst (23 rows on 4 experts of 1152 x 7168, 16.4 us).
 struct RowsCost {
     int rows, columns;
     float launch, slab, more;
