@@ -341,6 +341,13 @@ def _stream():
     return C.c_void_p(raw(device()) if raw and device else torch.cuda.current_stream().cuda_stream)
 
 
+def _stream_on(device: int) -> int:
+    """_stream() where a tensor on the current device is at hand (the runtime is up): 0.1 us."""
+    import torch
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(device) if raw else torch.cuda.current_stream().cuda_stream
+
+
 def _torch_act_dtype(torch_dtype: int):
     """Storage type of activations: the layer's own; fp32 for tf32 layers, bf16 for e4m3 layers."""
     import torch
@@ -1222,9 +1229,9 @@ def gemm_block128(A, a_scales, w, w_scales, bias=None, act: int = ACT_NONE):
             _device_operand("bias", bias, torch.bfloat16, (N,))
     _on_16_bytes("A", A)
     _on_16_bytes("w", w)
-    out = torch.empty((M, N), dtype=torch.bfloat16, device=A.device)
+    out = A.new_empty((M, N), dtype=torch.bfloat16)
     rc = load_library().moe_gemm_block128(A.data_ptr(), a_scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(), None if bias is None else bias.data_ptr(),
-                                          out.data_ptr(), M, N, K, act, _stream())
+                                          out.data_ptr(), M, N, K, act, _stream_on(A.get_device()))
     if rc:
         raise MoEError(rc, "moe_gemm_block128")
     return out
@@ -1278,7 +1285,7 @@ def rms_norm(x, weight, eps: float = 1e-6, residual=None):
     else:
         h = torch.empty_like(x)
         res, total = residual.data_ptr(), h.data_ptr()
-    rc = load_library().moe_rms_norm(x.data_ptr(), res, weight.data_ptr(), rows, H, eps, dtype, wdtype, total, out.data_ptr(), None, None, _stream())
+    rc = load_library().moe_rms_norm(x.data_ptr(), res, weight.data_ptr(), rows, H, eps, dtype, wdtype, total, out.data_ptr(), None, None, _stream_on(x.get_device()))
     if rc:
         raise MoEError(rc, "moe_rms_norm")
     return out if residual is None else (out, h)
@@ -1314,13 +1321,12 @@ def rms_norm_rows128(x, weight, eps: float = 1e-6, residual=None, want_rows: boo
         for name, t in (("x", x), ("weight", weight), ("residual", residual)):
             if t is not None:
                 _on_16_bytes(name, t)
-    shape, device = x.shape, x.device
-    q = torch.empty(shape, dtype=torch.uint8, device=device)
-    s = torch.empty((*shape[:-1], H // 128), dtype=torch.float32, device=device)
+    q = torch.empty_like(x, dtype=torch.uint8)      # (half of what torch.empty takes with a shape, a type and a device)
+    s = x.new_empty((*x.shape[:-1], H // 128), dtype=torch.float32)
     out = torch.empty_like(x) if want_rows else None
     h = None if residual is None else torch.empty_like(x)
     rc = load_library().moe_rms_norm(at, at_res, at_w, rows, H, eps, dtype, wdtype,
-                                     None if h is None else h.data_ptr(), None if out is None else out.data_ptr(), q.data_ptr(), s.data_ptr(), _stream())
+                                     None if h is None else h.data_ptr(), None if out is None else out.data_ptr(), q.data_ptr(), s.data_ptr(), _stream_on(x.get_device()))
     if rc:
         raise MoEError(rc, "moe_rms_norm")
     return q, s, out, h
@@ -1347,11 +1353,10 @@ def act_rows128(u_rows, g_rows, act: int, expert_count=None, expert_offset=None)
     for name, t in (("expert_count", expert_count), ("expert_offset", expert_offset)):
         if t is not None:
             _device_operand(name, t, torch.int32, (E,))
-    device = u_rows.device
-    q = torch.empty((R, I), dtype=torch.uint8, device=device)
-    s = torch.empty((R, I // 128), dtype=torch.float32, device=device)
+    q = torch.empty_like(u_rows, dtype=torch.uint8)
+    s = u_rows.new_empty((R, I // 128), dtype=torch.float32)
     rc = load_library().moe_act_rows128(u_rows.data_ptr(), None if g_rows is None else g_rows.data_ptr(), R, I, act, _ptr(expert_count), _ptr(expert_offset), E,
-                                        q.data_ptr(), s.data_ptr(), _stream())
+                                        q.data_ptr(), s.data_ptr(), _stream_on(u_rows.get_device()))
     if rc:
         raise MoEError(rc, "moe_act_rows128")
     return q, s
