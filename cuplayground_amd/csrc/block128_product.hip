@@ -377,12 +377,10 @@ __device__ __forceinline__ void rows_tile(const RowsProduct& p, const RowsTask& 
     if (!mx_join<KS, SET, NT, CG>(acc, ks, sw, smem, lane)) return;
     if constexpr (KS == 1) {
         mx_meet();                                // (requests for slabs behind the last one: zeros, but they write to LDS)
-        if (!(N & 7)) {
-            mx_store_rows<NT, CG, 16, 16>(p, t, smem + sw * mx_rows_lds<NT, CG, 16, 16>(), lane, idx, 4 * q, 16 * wm * NT, c0, acc, &bias);
-            return;
-        }
+        mx_store_rows<NT, CG, 16, 16>(p, t, smem + sw * mx_rows_lds<NT, CG, 16, 16>(), lane, idx, 4 * q, 16 * wm * NT, c0, acc, &bias);
+    } else {
+        mx_store_tile<NT, CG>(p, t, 16 * wm * NT + idx, c0 + 4 * q, acc, &bias);
     }
-    mx_store_tile<NT, CG>(p, t, 16 * wm * NT + idx, c0 + 4 * q, acc, &bias);
 }
 
 template <class T, bool COLD>
@@ -581,8 +579,7 @@ __device__ __forceinline__ void rows_deep(const RowsProduct& p, const RowsTask& 
         }
     }
     mx_meet();                                    // (the requests behind the last slab write to LDS)
-    if (!(N & 7)) mx_store_rows<NT, CG, 16, 16>(p, t, smem + sw * mx_rows_lds<NT, CG, 16, 16>(), lane, idx, 4 * q, 16 * wm * NT, c0, acc, EARLY ? &bias : nullptr);
-    else mx_store_tile<NT, CG>(p, t, 16 * wm * NT + idx, c0 + 4 * q, acc, EARLY ? &bias : nullptr);
+    mx_store_rows<NT, CG, 16, 16>(p, t, smem + sw * mx_rows_lds<NT, CG, 16, 16>(), lane, idx, 4 * q, 16 * wm * NT, c0, acc, EARLY ? &bias : nullptr);
 }
 
 // The last round of blocks of 256 rows in halves, and what such blocks leave of an expert or of the one matrix, by smaller tiles behind the large ones.  Large

@@ -293,13 +293,11 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void mx_tile_kernel(
     if constexpr (KS == 1) {
         constexpr int OWN = mx_rows_lds<NT, CG, 16, 16>();
         static_assert(T::SET * OWN <= T::LDS, "a place for every wavefront");
-        if (!(N & 7)) {
-            mx_meet();
-            mx_store_rows<NT, CG, 16, 16>(p, t, smem + sw * OWN, lane, idx, 4 * q, 16 * wm * NT, c0, acc);
-            return;
-        }
+        mx_meet();
+        mx_store_rows<NT, CG, 16, 16>(p, t, smem + sw * OWN, lane, idx, 4 * q, 16 * wm * NT, c0, acc);
+    } else {
+        mx_store_tile<NT, CG>(p, t, 16 * wm * NT + idx, c0 + 4 * q, acc);
     }
-    mx_store_tile<NT, CG>(p, t, 16 * wm * NT + idx, c0 + 4 * q, acc);
 }
 
 // -- rows in MXFP4 too --
@@ -466,13 +464,11 @@ __global__ __launch_bounds__(T::THREADS, T::WAVES_PER_SIMD) void mx_tile4_kernel
     if constexpr (KS == 1) {
         constexpr int OWN = mx_rows_lds<NT, 4 * CG, 32, 8>();
         static_assert(SET * OWN <= T::LDS, "a place for every wavefront");
-        if (!(N & 7)) {
-            mx_meet();
-            mx_store_rows<NT, 4 * CG, 32, 8>(p, t, smem + sw * OWN, lane, r32, 4 * b, wm * 32 * NT, t.n0 + wn * 32 * CG, sum);
-            return;
-        }
+        mx_meet();
+        mx_store_rows<NT, 4 * CG, 32, 8>(p, t, smem + sw * OWN, lane, r32, 4 * b, wm * 32 * NT, t.n0 + wn * 32 * CG, sum);
+    } else {
+        mx_store_tile<NT, 4 * CG, 32, 8>(p, t, wm * 32 * NT + r32, t.n0 + wn * 32 * CG + 4 * b, sum);
     }
-    mx_store_tile<NT, 4 * CG, 32, 8>(p, t, wm * 32 * NT + r32, t.n0 + wn * 32 * CG + 4 * b, sum);
 }
 
 // Workgroups of a launch: blocks of BM rows (an expert's last one is its own) times column tiles, in eight equal shares.

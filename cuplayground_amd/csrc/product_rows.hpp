@@ -26,9 +26,15 @@ struct MxBias {
         if (!any) return;
         if (p.N & 3) {
 #pragma unroll
-            for (int g = 0; g < CG; ++g)
+            for (int g = 0; g < CG; ++g) {
+                const int col = col0 + COLS * g;
+                if (col + 4 <= p.N) {
+                    __builtin_memcpy(raw[g], t.bias + col, 8);
+                } else {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) raw[g][r] = t.bias[min(col0 + COLS * g + r, p.N - 1)];
+                    for (int r = 0; r < 4; ++r) raw[g][r] = t.bias[min(col + r, p.N - 1)];
+                }
+            }
         } else {
 #pragma unroll
             for (int g = 0; g < CG; ++g) __builtin_memcpy(raw[g], t.bias + min(col0 + COLS * g, p.N - 4), 8);
@@ -50,7 +56,8 @@ __device__ __forceinline__ void mx_bias(const PRODUCT& p, const TASK& t, int col
     raw.fetch(p, t, col0);
     raw.widen(b);
 }
-// Four neighbouring columns of a token row, as the matrix instructions leave them in a lane.  whole: N is a multiple of 4.
+// Four neighbouring columns of a token row, as the matrix instructions leave them in a lane, in one store (memory takes 8 bytes at any address) but where
+// the row ends.  whole: N is a multiple of 4.
 template <int ACT, class TASK>
 __device__ __forceinline__ void mx_store4(const TASK& t, int N, bool whole, int row, int col, const mx_f32x4& u) {
     float v[4];
@@ -58,8 +65,9 @@ __device__ __forceinline__ void mx_store4(const TASK& t, int N, bool whole, int 
     for (int r = 0; r < 4; ++r) v[r] = ACT == MOE_ACT_GELU ? gelu16(u[r]) : ACT == MOE_ACT_RELU && u[r] < 0.0f ? 0.0f : u[r];      // a NaN stays a NaN
     const uint32_t lo = pack2_bf16(v[0], v[1]), hi = pack2_bf16(v[2], v[3]);
     uint16_t* o = t.out + (int64_t)row * N + col;
-    if (whole) {
-        *reinterpret_cast<uint2*>(o) = uint2{lo, hi};
+    if (whole || col + 4 <= N) {
+        const uint2 both{lo, hi};
+        __builtin_memcpy(o, &both, 8);
     } else {
         const uint32_t w[4] = {lo, lo >> 16, hi, hi >> 16};
 #pragma unroll
@@ -93,8 +101,8 @@ __device__ __forceinline__ void mx_store_tile(const PRODUCT& p, const TASK& t, i
     else all(std::integral_constant<int, MOE_ACT_NONE>{}, Whole{});
 }
 
-// mx_store_tile through LDS of the wavefront's own (mx_rows_lds bytes, where nothing else is read or written any more), for N of a multiple
-// of 8: as the instructions leave them, a store writes 16 or 32 bytes of 32 or 16 rows; this way it writes 64 to 256 bytes of a row.  Both rows in
+// mx_store_tile through LDS of the wavefront's own (mx_rows_lds bytes, where nothing else is read or written any more): as the instructions leave
+// them, a store writes 16 or 32 bytes of 32 or 16 rows; this way it writes 64 to 256 bytes of a row, from any address.  Both rows in
 // MXFP4, us, without / with: 8192 x 14336 x 4096 305 / 275, 1777 x 2752 x 1344 14.0 / 11.4; rows in bf16 672 / 657, 19.7 / 17.8.
 template <int NT, int CG, int ROWS, int COLS>
 __device__ __host__ constexpr int mx_rows_lds() { return ROWS * NT * (2 * COLS * CG + 16); }
@@ -126,7 +134,15 @@ __device__ __forceinline__ void mx_store_rows(const PRODUCT& p, const TASK& t, u
 #pragma unroll
     for (int r = 0; r < ROWS * NT; r += 64 / LANES) {
         const mx_u32x4 v = *reinterpret_cast<const mx_u32x4*>(own + (r + at) * PITCH + 16 * piece);
-        if (row0 + r + at < t.rows && c < p.N) *reinterpret_cast<mx_u32x4*>(t.out + (int64_t)(row0 + r + at) * p.N + c) = v;
+        if (row0 + r + at >= t.rows) continue;
+        uint16_t* const o = t.out + (int64_t)(row0 + r + at) * p.N + c;
+        if (c + 8 <= p.N) {
+            __builtin_memcpy(o, &v, 16);
+        } else {                                  // (with N a multiple of 8: behind the last column)
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (c + k < p.N) o[k] = (uint16_t)(v[k / 2] >> (16 * (k & 1)));
+        }
     }
 }
 
