@@ -686,8 +686,8 @@ auto with_rows_tile(int form, F f) {
 
 // What a tile costs, in us: a launch of its form; a slab of the contraction where a compute unit has one tile; the same for every further tile of the
 // unit.  Fitted to 575 products of 1 to 6000 rows, 4 to 1000 us, dense and of experts, evenly and not, each with every form: the choice by
-// these was 1.0 % behind the best of the forms on average.  Over 1324 others it is 0.9 % behind for one matrix and 1.9 % for experts (a fit
-// to those alone 0.9 and 1.3), 50 % at worst (23 rows on 4 experts of 1152 x 7168, 16.4 us).
+// these was 1.0 % behind the best of the forms on average.  Over some 1500 others it is 0.8 % behind for one matrix and 2.0 % for experts
+// (a fit to those alone 0.7 and 1.2), 50 % at worst (23 rows on 4 experts of 1152 x 7168, 16.4 us).
 struct RowsCost {
     int rows, columns;
     float launch, slab, more;
