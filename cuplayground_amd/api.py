@@ -7,6 +7,7 @@ torch is used for device memory and the current HIP stream only.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import json
 import os
 from dataclasses import asdict, dataclass
@@ -701,21 +702,24 @@ class MoELayer:
             raise ValueError("expert_gemm_block128 takes a matrix for every expert")
         (_, N, K), A = w.shape, self.S * self.k
         rows = A if token_indices is None else self.S
-        operands = (("w", w, 1, (self.E, N, K)), ("a_rows", a_rows, 1, (rows, K)), ("w_scales", w_scales, torch.float32, (self.E, (N + 127) // 128, K // 128)),
-                    ("a_scales", a_scales, torch.float32, (rows, K // 128)), ("bias", bias, torch.bfloat16, (self.E, N)),
-                    ("expert_count", expert_count, torch.int32, (self.E,)), ("expert_offset", expert_offset, torch.int32, (self.E,)),
-                    ("token_indices", token_indices, torch.int32, (A,)), ("out", out, torch.bfloat16, (A, N)))
-        if not _right([o[1:] for o in operands]):
-            for name, t, dtype, shape in operands:
+        E, kb = self.E, K // 128
+        operands = ((w, 1, (E, N, K)), (a_rows, 1, (rows, K)), (w_scales, torch.float32, (E, (N + 127) // 128, kb)), (a_scales, torch.float32, (rows, kb)),
+                    (expert_count, torch.int32, (E,)), (expert_offset, torch.int32, (E,)), (bias, torch.bfloat16, (E, N)),
+                    (token_indices, torch.int32, (A,)), (out, torch.bfloat16, (A, N)))
+        if not _right(operands):
+            for name, (t, dtype, shape) in zip(("w", "a_rows", "w_scales", "a_scales", "expert_count", "expert_offset", "bias", "token_indices", "out"), operands):
                 if t is not None:
                     _codes(name, t, shape) if dtype == 1 else _device_operand(name, t, dtype, shape)
-        for name, t in (("w", w), ("a_rows", a_rows), ("out", out)):
-            if t is not None:
-                _on_16_bytes(name, t)
         if out is None:
-            out = torch.empty((A, N), dtype=torch.bfloat16, device=w.device)
-        _check(self.L.moe_expert_gemm_block128(self._h, _ptr(a_rows), _ptr(a_scales), _ptr(token_indices), _ptr(w), _ptr(w_scales), _ptr(bias),
-                                               _ptr(expert_count), _ptr(expert_offset), N, K, act, _ptr(out), _stream()), "moe_expert_gemm_block128")
+            out = w.new_empty((A, N), dtype=torch.bfloat16)
+        at = [None if t is None else t.data_ptr() for t in (a_rows, a_scales, token_indices, w, w_scales, bias, expert_count, expert_offset, out)]
+        if ((at[0] or 0) | (at[3] or 0) | at[8]) & 15:
+            for name, t in (("w", w), ("a_rows", a_rows), ("out", out)):
+                if t is not None:
+                    _on_16_bytes(name, t)
+        rc = self.L.moe_expert_gemm_block128(self._h, *at[:8], N, K, act, at[8], _stream_on(w.get_device()))
+        if rc:
+            raise MoEError(rc, "moe_expert_gemm_block128")
         return out
 
     def forward_block128(self, x, weights: dict, norm_weight=None, eps: float = 1e-6, residual=None):
@@ -1227,10 +1231,12 @@ def gemm_block128(A, a_scales, w, w_scales, bias=None, act: int = ACT_NONE):
         _device_operand("a_scales", a_scales, torch.float32, (M, K // 128))
         if bias is not None:
             _device_operand("bias", bias, torch.bfloat16, (N,))
-    _on_16_bytes("A", A)
-    _on_16_bytes("w", w)
+    at_a, at_w = A.data_ptr(), w.data_ptr()
+    if (at_a | at_w) & 15:
+        _on_16_bytes("A", A)
+        _on_16_bytes("w", w)
     out = A.new_empty((M, N), dtype=torch.bfloat16)
-    rc = load_library().moe_gemm_block128(A.data_ptr(), a_scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(), None if bias is None else bias.data_ptr(),
+    rc = load_library().moe_gemm_block128(at_a, a_scales.data_ptr(), at_w, w_scales.data_ptr(), None if bias is None else bias.data_ptr(),
                                           out.data_ptr(), M, N, K, act, _stream_on(A.get_device()))
     if rc:
         raise MoEError(rc, "moe_gemm_block128")
@@ -1291,18 +1297,23 @@ def rms_norm(x, weight, eps: float = 1e-6, residual=None):
     return out if residual is None else (out, h)
 
 
+@functools.lru_cache(maxsize=64)
+def _norm_scratch(rows: int, H: int) -> int:
+    n = C.c_size_t(0)
+    _check(load_library().moe_rms_norm_scratch_bytes(rows, H, C.byref(n)), "moe_rms_norm_scratch_bytes")
+    return n.value
+
+
 def rms_norm_backward(dout, h, weight, eps: float = 1e-6, dsum=None):
     """(dx, dweight) of rms_norm: h is what was normalised (x, or the sum with the residual), dsum the gradient that h has from elsewhere
     (None: none).  dx is the gradient of x and of the residual alike; dweight has the weight's type."""
     import torch
     rows, H, dtype, wdtype = _norm_operands(h, weight, ("dout", dout), ("dsum", dsum))
-    L = load_library()
-    n = C.c_size_t(0)
-    _check(L.moe_rms_norm_scratch_bytes(rows, H, C.byref(n)), "moe_rms_norm_scratch_bytes")
-    scratch = torch.empty(n.value, dtype=torch.uint8, device=h.device)
+    size = _norm_scratch(rows, H)
+    scratch = h.new_empty(size, dtype=torch.uint8)
     dx, dweight = torch.empty_like(h), torch.empty_like(weight)
-    rc = L.moe_rms_norm_backward(dout.data_ptr(), h.data_ptr(), weight.data_ptr(), None if dsum is None else dsum.data_ptr(), rows, H, eps, dtype, wdtype,
-                                 dx.data_ptr(), dweight.data_ptr(), scratch.data_ptr(), n.value, _stream())
+    rc = load_library().moe_rms_norm_backward(dout.data_ptr(), h.data_ptr(), weight.data_ptr(), None if dsum is None else dsum.data_ptr(), rows, H, eps, dtype, wdtype,
+                                 dx.data_ptr(), dweight.data_ptr(), scratch.data_ptr(), size, _stream_on(h.get_device()))
     if rc:
         raise MoEError(rc, "moe_rms_norm_backward")
     return dx, dweight
