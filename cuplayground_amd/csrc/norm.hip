@@ -118,6 +118,13 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float* part) {
     }
 }
 
+// The squares' sum of a row may pass fp32 where their mean does not, and a value may be larger than any whose square fp32 holds.  Such a row is summed
+// again from its values times this: no sum is above 2^126 then, the product is exact but for values below 2^-54 (whose n is below 2^-111 in such a
+// row), and r takes the factor back (21 bits of it at least where r is below fp32's normal numbers).  fp16 has no such rows.
+constexpr float kFarRow = 0x1p-72f;
+template <class T> constexpr bool kHasFarRows = true;
+template <> constexpr bool kHasFarRows<f16_e> = false;
+
 // THREADS threads to a row, NV pieces each; of rows that a wavefront holds, four share a workgroup.
 template <int THREADS> constexpr int kNormBlock = THREADS == kWave ? 4 * kWave : THREADS;
 
@@ -149,7 +156,6 @@ __global__ __launch_bounds__(kNormBlock<THREADS>) void norm_rows_kernel(NormArgs
         const int c = (t + THREADS * i) * VEC;
         if (c < a.H) load_weights<T, WHOLE>(w[i], a.weight, a.weight_f32, c, a.H - c);
     }
-    float sum[1] = {0.0f};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (t + THREADS * i) * VEC;
@@ -160,13 +166,24 @@ __global__ __launch_bounds__(kNormBlock<THREADS>) void norm_rows_kernel(NormArgs
             store<T, WHOLE>(a.sum, at + c, a.H - c, x[i]);
         }
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-            h[i][k] = widen<T>(x[i].e[k]);
-            sum[0] = __builtin_fmaf(h[i][k], h[i][k], sum[0]);
-        }
+        for (int k = 0; k < VEC; ++k) h[i][k] = widen<T>(x[i].e[k]);
     }
-    row_sums<THREADS, 1>(sum, part);
-    const float r = 1.0f / sqrtf(sum[0] / (float)a.H + a.eps);
+    float sum[1], mean, far = 1.0f;
+    for (;;) {
+        sum[0] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if ((t + THREADS * i) * VEC >= a.H) continue;
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) sum[0] = __builtin_fmaf(h[i][k] * far, h[i][k] * far, sum[0]);
+        }
+        row_sums<THREADS, 1>(sum, part);
+        mean = sum[0] / (float)a.H + a.eps * far * far;
+        if (!kHasFarRows<T> || mean < INFINITY || far != 1.0f) break;      // (the same in all threads of the row)
+        far = kFarRow;
+        if (THREADS > kWave) __syncthreads();     // (everybody has read the sums)
+    }
+    const float r = 1.0f / sqrtf(mean) * far;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (t + THREADS * i) * VEC;
@@ -214,55 +231,75 @@ __global__ __launch_bounds__(kNormBlock<THREADS>) void norm_backward_kernel(Norm
         for (int k = 0; k < VEC; ++k) w[i][k] = dw[i][k] = 0.0f;
         if (c < a.H) load_weights<T, WHOLE>(w[i], a.weight, a.weight_f32, c, a.H - c);
     }
-    P h[NV], dy[NV], ds[NV];
-    auto fetch = [&](int64_t row) {
+    struct Operands { P h[NV], dy[NV], ds[NV]; };
+    auto fetch = [&](int64_t row, Operands& o) {
         if (row >= a.rows) return;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (t + THREADS * i) * VEC;
             if (c >= a.H) continue;
-            h[i] = load<T, WHOLE>(a.h, row * a.H + c, a.H - c);
-            dy[i] = load<T, WHOLE>(a.dy, row * a.H + c, a.H - c);
-            if (a.dsum) ds[i] = load<T, WHOLE>(a.dsum, row * a.H + c, a.H - c);
+            o.h[i] = load<T, WHOLE>(a.h, row * a.H + c, a.H - c);
+            o.dy[i] = load<T, WHOLE>(a.dy, row * a.H + c, a.H - c);
+            if (a.dsum) o.ds[i] = load<T, WHOLE>(a.dsum, row * a.H + c, a.H - c);
         }
+    };
+    auto times_far = [&](Operands& o) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if ((t + THREADS * i) * VEC < a.H)
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) o.h[i].e[k] = narrow<T>(widen<T>(o.h[i].e[k]) * kFarRow);
     };
     constexpr bool AHEAD = NV == 1;               // (wider rows: the registers do not hold two rows' operands)
     int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / THREADS;
-    if (AHEAD) fetch(row);
-    for (int turn = 0; row < a.rows; row += step, turn ^= 1) {
+    Operands next;
+    if (AHEAD) fetch(row, next);
+    float far = 1.0f;
+    for (int turn = 0; row < a.rows; turn ^= 1) {
         const int64_t at = row * a.H;
-        if (!AHEAD) fetch(row);
         float sums[2] = {0.0f, 0.0f};
-        P h_now[NV], dy_now[NV], ds_now[NV];
+        Operands now;
+        if (!AHEAD) {
+            fetch(row, now);
+            if (kHasFarRows<T> && far != 1.0f) times_far(now);
+        }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             if ((t + THREADS * i) * VEC >= a.H) continue;
-            h_now[i] = h[i], dy_now[i] = dy[i], ds_now[i] = ds[i];
+            if (AHEAD) now.h[i] = next.h[i], now.dy[i] = next.dy[i], now.ds[i] = next.ds[i];
 #pragma unroll
             for (int k = 0; k < VEC; ++k) {
-                const float hv = widen<T>(h[i].e[k]);
+                const float hv = widen<T>(now.h[i].e[k]);
                 sums[0] = __builtin_fmaf(hv, hv, sums[0]);
-                sums[1] = __builtin_fmaf(widen<T>(dy[i].e[k]) * w[i][k], hv, sums[1]);
+                sums[1] = __builtin_fmaf(widen<T>(now.dy[i].e[k]) * w[i][k], hv, sums[1]);
             }
         }
-        if (AHEAD) fetch(row + step);
+        if (AHEAD) fetch(row + step, next);
         row_sums<THREADS, 2>(sums, part[turn]);
-        const float r = 1.0f / sqrtf(sums[0] / (float)a.H + a.eps), along = sums[1] * r / (float)a.H;
+        const float mean = sums[0] / (float)a.H + a.eps * far * far;
+        if (kHasFarRows<T> && far == 1.0f && __builtin_amdgcn_readfirstlane(!(mean < INFINITY))) {      // another turn for this row (a wavefront's are one row's)
+            far = kFarRow;
+            if (AHEAD) fetch(row, next), times_far(next);
+            continue;
+        }
+        const float r = 1.0f / sqrtf(mean), along = sums[1] * r / (float)a.H, r_dx = r * far;      // (n = h r: h has the factor)
+        far = 1.0f;
+        row += step;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (t + THREADS * i) * VEC;
             if (c >= a.H) continue;
             if (!AHEAD) {                         // as fetched, and not widened since: of several pieces the registers do not hold both
-                asm volatile("" : "+v"(*reinterpret_cast<mx_u32x4*>(&h_now[i])));
-                asm volatile("" : "+v"(*reinterpret_cast<mx_u32x4*>(&dy_now[i])));
+                asm volatile("" : "+v"(*reinterpret_cast<mx_u32x4*>(&now.h[i])));
+                asm volatile("" : "+v"(*reinterpret_cast<mx_u32x4*>(&now.dy[i])));
             }
             P o;
 #pragma unroll
             for (int k = 0; k < VEC; ++k) {
-                const float n = widen<T>(h_now[i].e[k]) * r, d = widen<T>(dy_now[i].e[k]);
+                const float n = widen<T>(now.h[i].e[k]) * r, d = widen<T>(now.dy[i].e[k]);
                 dw[i][k] = __builtin_fmaf(d, n, dw[i][k]);
-                float v = r * (d * w[i][k] - n * along);
-                if (a.dsum) v += widen<T>(ds_now[i].e[k]);
+                float v = r_dx * (d * w[i][k] - n * along);
+                if (a.dsum) v += widen<T>(now.ds[i].e[k]);
                 o.e[k] = narrow<T>(v);
             }
             store<T, WHOLE>(a.dx, at + c, a.H - c, o);

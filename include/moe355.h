@@ -480,12 +480,14 @@ int moe_expert_gemm_block128(moe_handle* h, const void* a_rows, const float* a_s
  *   the row's h^2 + eps), in fp32.  x, residual, sum and out are [rows, H] in `dtype` (fp32, bf16, fp16), weight [H] in that type or in fp32
  *   (weight_dtype).  y goes to `out`, rounded once, and / or to q [rows, H] and scales [rows, H / 128] in e4m3 with a scale for 128 values, the
  *   format of moe_quant_rows128, from the fp32 values (scale = amax / 448, not below 2^-126): rows of a product with block scales.  Either may
- *   be NULL, not both.  sum may be x or residual; else nothing overlaps.  The squares' mean has to be a number of fp32.  H up to 16384; with q
- *   a multiple of 128, and x, residual, weight, sum and out 16-byte aligned (else elements may lie anywhere that whole ones can), q 8-byte.
+ *   be NULL, not both.  sum may be x or residual; else nothing overlaps.  A row may hold any finite values, also such that the mean
+ *   of their squares is no number of fp32.  H up to 16384; with q a multiple of 128, and x, residual, weight, sum and out 16-byte aligned (else
+ *   elements may lie anywhere that whole ones can), q 8-byte.
  *   rows < 2^22; 0: nothing is done.  MOE_ERR_UNSUPPORTED: other types, longer rows, more of them.
  * moe_rms_norm_backward: from dout = dL/dout, h (what was normalised: x, or `sum`) and, where h goes on to elsewhere, dsum = dL/dh from there
  *   (or NULL): dx [rows, H] = dL/dx (= dL/dresidual), rounded once, and dweight [H] in the weight's type.  Sums in fp32, in a fixed
- *   order: the same inputs give the same bits.  scratch: moe_rms_norm_scratch_bytes, 4-byte aligned, overwritten.  rows = 0: dweight = 0.
+ *   order: the same inputs give the same bits.  Any finite h, but a row's sum of dout * weight * h has to be a number of fp32 (where
+ *   the mean of h^2 + eps is none: 2^-72 times it).  scratch: moe_rms_norm_scratch_bytes, 4-byte aligned, overwritten.  rows = 0: dweight = 0.
  * moe_act_rows128: the experts' activation with its result in that format: silu(g) * u (act SWIGLU), gelu(u) or relu(u) (g = NULL) of bf16
  *   rows [rows, I], I a multiple of 128, u and g 16-byte aligned.  With expert_count / expert_offset [E] (of moe_route) only the packed rows
  *   that belong to an expert are read and written; NULL: all.  MOE_ERR_UNSUPPORTED: 2^24 * 2048 values and more. */
