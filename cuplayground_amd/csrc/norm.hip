@@ -354,11 +354,15 @@ __global__ __launch_bounds__(1024) void norm_weight_grad_kernel(const float* __r
 
 // ---- the experts' activation ----
 //
-// silu(g) u, gelu(u) or relu(u) of bf16 rows, to e4m3.  Hardware exp2 and reciprocal (1 ulp each): the result is off by about as much as with the
-// library's expf and a division -- the argument's rounding is ln 2 |g| 2^-24 of the exponential -- and four bits see neither.  What it saves is time:
-// the vector ALU, not memory, bounded the kernel with an exponential of an argument in two parts, a Newton step and clamps: 16384 x 14336
-// SwiGLU 234 us.  Out of range everything falls into place: exp2 gives infinity and the reciprocal 0 for far negative g, and NaN for -infinity.
-__device__ __forceinline__ float silu_to8(float g) { return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.4426950408889634f)); }
+// silu(g) u, gelu(u) or relu(u) of bf16 rows, to e4m3.  Hardware exp2 and reciprocal, 1 ulp each.  The exponential's argument is rounded once, so for
+// negative g the result is off by |g| 2^-24 and the constant's half of that, 1.45 |g| 2^-24 in all: 2^-17 at g = -88, which three bits behind the
+// first one see seldom.  What it saves is time: the vector ALU, not memory, bounded the kernel with an exponential of an argument in two parts, a
+// Newton step and clamps: 16384 x 14336 SwiGLU 234 us.
+// The quotient is made of quarters, 4 / (1 + e^-g): the hardware's reciprocal is 0 below fp32's normal numbers, and so is as wide as e^-g is one of
+// fp32, g > -88.72.  Behind that e^-g / 4 or the sum is too large or infinite and the result 0 (exact: below 2.6e-37); NaN for -infinity.
+__device__ __forceinline__ float silu_to8(float g) {
+    return 0.25f * g * __builtin_amdgcn_rcpf(0.25f + __builtin_amdgcn_exp2f(__builtin_fmaf(g, -1.4426950408889634f, -2.0f)));
+}
 
 // COLD: more rows than the memory-side cache holds, read past it (16384 x 14336 SwiGLU 196 -> 175 to 186 us; 6000 x 1408, which the products in front have
 // left there, 9.0 -> 9.8).  181 to 194 us are 6.1 to 6.5 TB/s.

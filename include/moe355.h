@@ -488,8 +488,8 @@ int moe_expert_gemm_block128(moe_handle* h, const void* a_rows, const float* a_s
  *   (or NULL): dx [rows, H] = dL/dx (= dL/dresidual), rounded once, and dweight [H] in the weight's type.  Sums in fp32, in a fixed
  *   order: the same inputs give the same bits.  Any finite h, but a row's sum of dout * weight * h has to be a number of fp32 (where
  *   the mean of h^2 + eps is none: 2^-72 times it).  scratch: moe_rms_norm_scratch_bytes, 4-byte aligned, overwritten.  rows = 0: dweight = 0.
- * moe_act_rows128: the experts' activation with its result in that format: silu(g) * u (act SWIGLU), gelu(u) or relu(u) (g = NULL) of bf16
- *   rows [rows, I], I a multiple of 128, u and g 16-byte aligned.  With expert_count / expert_offset [E] (of moe_route) only the packed rows
+ * moe_act_rows128: the experts' activation with its result in that format: silu(g) * u (act SWIGLU; 0 for g below -88.72, where silu is less than
+ *   2.6e-37 and e^-g no number of fp32), gelu(u) or relu(u) (g = NULL) of bf16 rows [rows, I], I a multiple of 128, u and g 16-byte aligned.  With expert_count / expert_offset [E] (of moe_route) only the packed rows
  *   that belong to an expert are read and written; NULL: all.  MOE_ERR_UNSUPPORTED: 2^24 * 2048 values and more. */
 int moe_rms_norm(const void* x, const void* residual, const void* weight, int64_t rows, int32_t H, float eps, int32_t dtype, int32_t weight_dtype,
                  void* sum, void* out, void* q, float* scales, void* stream);
