@@ -723,8 +723,8 @@ class MoELayer:
         return out
 
     def forward_block128(self, x, weights: dict, norm_weight=None, eps: float = 1e-6, residual=None):
-        """out[S,H] = MoE(x) of an e4m3 layer with the rows in e4m3 too, as rms_norm_rows128 and act_rows128 make them: for any number of tokens, the
-        stages one by one, the projections by expert_gemm_block128, which fetches its rows from the tokens'.  With norm_weight [H] (bf16 or fp32) the
+        """out[S,H] = MoE(x) of an e4m3 layer with the rows in e4m3 too, as rms_norm_rows128 and act_rows128 make them: the stages one by one, the
+        projections by expert_gemm_block128, which fetches its rows from the tokens'.  S H below 3 GiB, S k I below 2^35.  With norm_weight [H] (bf16 or fp32) the
         layer stands behind that norm, MoE(rms_norm(x)), its router on the bf16 rows of it; with a residual besides: (out, x + residual).
         Rows in e4m3 carry three bits where forward()'s bf16 rows carry seven: a token's answer is some 4 % from 64 bits instead of 0.3 %."""
         import torch
@@ -759,6 +759,7 @@ class MoELayer:
                 _on_16_bytes(name, t)
         _device_operand("x", x, torch.bfloat16, (self.S, H))
         _on_16_bytes("x", x)
+        _block128_layer_sizes(self.S, self.k, E, H, I)
         h = None
         if norm_weight is None:
             rows, (q, s) = x, quantize_rows128(x)
@@ -1241,6 +1242,19 @@ def gemm_block128(A, a_scales, w, w_scales, bias=None, act: int = ACT_NONE):
     if rc:
         raise MoEError(rc, "moe_gemm_block128")
     return out
+
+
+@functools.lru_cache(maxsize=64)
+def _block128_layer_sizes(S: int, k: int, E: int, H: int, I: int):
+    """What a stage of forward_block128 would refuse for its size, asked before the first one is launched."""
+    if S * H >= 3 << 30:
+        raise MoEError(_UNSUPPORTED, "%d tokens of %d values: rows fetched by index lie in less than 3 GiB" % (S, H))
+    if S * k * I > ((1 << 24) - 1) * 2048:
+        raise MoEError(_UNSUPPORTED, "%d rows of %d values: act_rows128 takes (2^24 - 1) * 2048 at most" % (S * k, I))
+    if S >= 1 << 24:
+        raise MoEError(_UNSUPPORTED, "%d tokens: combine takes less than 2^24" % S)
+    for N, K in ((I, H), (H, I)):
+        gemm_block128_plan(S * k, N, K, E)
 
 
 def gemm_block128_plan(M: int, N: int, K: int, experts: int = 0) -> dict:

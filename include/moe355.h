@@ -490,7 +490,7 @@ int moe_expert_gemm_block128(moe_handle* h, const void* a_rows, const float* a_s
  *   the mean of h^2 + eps is none: 2^-72 times it).  scratch: moe_rms_norm_scratch_bytes, 4-byte aligned, overwritten.  rows = 0: dweight = 0.
  * moe_act_rows128: the experts' activation with its result in that format: silu(g) * u (act SWIGLU; 0 for g below -88.72, where silu is less than
  *   2.6e-37 and e^-g no number of fp32), gelu(u) or relu(u) (g = NULL) of bf16 rows [rows, I], I a multiple of 128, u and g 16-byte aligned.  With expert_count / expert_offset [E] (of moe_route) only the packed rows
- *   that belong to an expert are read and written; NULL: all.  MOE_ERR_UNSUPPORTED: 2^24 * 2048 values and more. */
+ *   that belong to an expert are read and written; NULL: all.  MOE_ERR_UNSUPPORTED: more than (2^24 - 1) * 2048 values. */
 int moe_rms_norm(const void* x, const void* residual, const void* weight, int64_t rows, int32_t H, float eps, int32_t dtype, int32_t weight_dtype,
                  void* sum, void* out, void* q, float* scales, void* stream);
 int moe_rms_norm_scratch_bytes(int64_t rows, int32_t H, size_t* bytes);
