@@ -430,9 +430,13 @@ hipError_t launch_norm_type(const NormArgs& a, hipStream_t st) {
     });
 }
 
-// Rows of partial sums of dw, 1024 at most: workgroups of 4096 wavefronts in all (16 a compute unit: 8192 rows of 4096 47 us, 52 with twice as many, 62
-// with half), but not more than a quarter of the rows beyond one for each compute unit.
-int64_t norm_parts(int64_t rows, int threads) { return std::min<int64_t>(rows, std::min<int64_t>(4096 * 64 / std::max(threads, 256), std::max<int64_t>(256, rows / 4))); }
+// Rows of partial sums of dw, one a workgroup: at most 1024 of up to 256 threads, fewer of more, so that 4096 wavefronts are on their way (16 a compute unit: 8192
+// rows of 4096 47 us, 52 with twice as many, 62 with half; rows of 128 threads make 2048); no more than a quarter of the rows beyond one for each
+// compute unit; and none that has no row (of rows that a wavefront holds, a workgroup takes four).  threads = 0: the most of any.
+int64_t norm_parts(int64_t rows, int threads) {
+    const int64_t filled = threads == kWave ? (rows + 3) / 4 : rows;
+    return std::min<int64_t>(filled, std::min<int64_t>(4096 * 64 / std::max(threads, 256), std::max<int64_t>(256, rows / 4)));
+}
 
 template <class T>
 hipError_t launch_norm_backward_type(const NormBackwardArgs& a, hipStream_t st) {
