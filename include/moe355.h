@@ -455,10 +455,14 @@ int moe_forward_few(moe_handle* h, const void* x, const moe_weights* w, const mo
  * (moe_quant_block128).  No counterpart in the reference, whose dtypes stop at fp16.  Asynchronous on `stream`, no scratch, can be captured.
  *
  * moe_gemm_block128: out [M, N] (bf16) = act(a . w^T + bias), a [M, K] codes with a_scales [M, K / 128] fp32, w [N, K] codes with w_scales
- *   [ceil(N / 128), K / 128] fp32, bias [N] bf16 or NULL, act RELU, GELU or NONE.  Products and their sums in fp32, rounded once; the same call
- *   gives the same bits, but the order of a row's sums goes by the numbers of rows, of all experts together.  K a multiple of 128 up to 2^20, any
- *   N (a last block of fewer rows has scales too), any M below 2^31 (0: nothing is done); a, w and out 16-byte aligned.  MOE_ERR_UNSUPPORTED:
- *   a matrix of 3 GiB and more, more workgroups than a launch takes (2^22).
+ *   [ceil(N / 128), K / 128] fp32, bias [N] bf16 or NULL, act RELU, GELU or NONE.  Products are exact; the matrix instruction adds eight
+ *   neighbouring ones at a time and cuts each off below 2^-13 of the power of two that the largest of the eight begins with (where a value below
+ *   e4m3's normal numbers counts as the smallest of those); the rest is added up in fp32 and rounded once.  So a result is off by as much as
+ *   2^-10 of the sum, over the eights, of their largest product, whatever they add up to: on random rows by 2.7e-4 of the results in the
+ *   2-norm, beside 1.7e-3 of their rounding, but by more where a sum cancels.  The same call gives the same bits, but the order of a row's
+ *   sums goes by the numbers of rows, of all experts together.  K a multiple of 128 up to 2^20, any N (a last block of fewer rows has scales
+ *   too), any M below 2^31 (0: nothing is done); a, w and out 16-byte aligned.  MOE_ERR_UNSUPPORTED: a matrix of 3 GiB and more, more
+ *   workgroups than a launch takes (2^22).
  * moe_gemm_block128_plan: which kernel a product of these sizes takes, as moe_gemm_mxfp4_plan says it (16 x 16 or 16 x 32: the weight streamer).
  *   Host only.
  * moe_expert_gemm_block128: the rows of every expert of an e4m3 layer through its matrix, w [E, N, K], w_scales [E, N / 128, K / 128], bias [E, N]
