@@ -584,8 +584,8 @@ __device__ __forceinline__ void rows_deep(const RowsProduct& p, const RowsTask& 
 
 // The last round of blocks of 256 rows in halves, and what such blocks leave of an expert or of the one matrix, by smaller tiles behind the large ones.  Large
 // tiles for all / this, us: 2037 x 10624 x 4608 115 / 103, 3678 x 9216 x 3840 150 / 137, 1435 x 14336 x 5376 129 / 113; 8 experts of 6016 x 5760, 3104 rows 150 /
-// 132, of 4096 x 14336, 16384 rows 950 / 925 (its pieces take 40 us; the rest is 2.2 PFLOP/s, 2.4 where all rows meet one matrix: weights of
-// eight experts come from memory, each for one XCD).
+// 132, of 4096 x 14336, 16384 rows 950 / 925 (its pieces take 40 us, and the eight matrices' way from
+// memory 45: so much less where all of them lie at one address; the rest is 2.3 PFLOP/s).
 typedef RowsDeep<2, 4, 4, 4> RowsLeft;
 typedef RowsTile<1, 4, 4, 2, 2, 2> RowsPiece;
 template <class T>

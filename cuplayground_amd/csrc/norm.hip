@@ -5,8 +5,9 @@
 //   dx = r (dy w - n mean(dy w n)) + dsum,  n = h r;   dw = sum over rows of dy n
 //
 // Memory bounds all of it: every array passes once.  A row stays in the registers of the threads that fetched it, 16 bytes of every operand a
-// thread and step, from the sum of its squares to its results.  8192 rows of 4096 in bf16 with a residual: the norm 46 to 49 us (5.5 to 5.8 TB/s; a copy of
-// 1 GiB reaches 5.15 here, one of 128 MiB 7.2), in e4m3 and bf16 54 to 60, the gradients 51 to 53 and 4 for the weight's.
+// thread and step, from the sum of its squares to its results.  8192 rows of 4096 in bf16 with a residual, kernel times on three inputs in turn, least to
+// median: the norm 45 to 48 us (5.6 to 5.9 TB/s; a copy of 1 GiB reaches 5.15 here, one of 128 MiB 7.2), in e4m3 and bf16 55 to 59, the gradients 51 to 54
+// (with one of the sum; 44 to 46 without) and 4 for the weight's.
 #include "ffn_common.hpp"
 #include "mxfp4.hpp"
 #include "rows8.hpp"
@@ -214,8 +215,8 @@ __global__ __launch_bounds__(kNormBlock<THREADS>) void norm_rows_kernel(NormArgs
 
 // The gradients.  A workgroup takes every gridDim.x-th row (ROWS of them at a time) and keeps its threads' columns of dw in registers; what it has of dw
 // at the end is a row of `part`, and norm_weight_grad_kernel adds those up in their order: no atomics, the same bits every time.  The next
-// row's operands are on their way while a row's sums are made, where a thread's share of a row is small.  (Of fp32 rows above 8192 values some
-// registers spill to scratch memory.)
+// row's operands are on their way while a row's sums are made, where a thread's share of a row is small.  (Of fp32 rows above 8192 values 36 bytes a
+// lane spill to scratch memory, 44 where rows begin on no 16 bytes: 2048 x 16384 with a gradient of the sum 124 us, 4.3 TB/s.)
 template <class T, int NV, int THREADS, bool WHOLE>
 __global__ __launch_bounds__(kNormBlock<THREADS>) void norm_backward_kernel(NormBackwardArgs a) {
     constexpr int ROWS = kNormBlock<THREADS> / THREADS, VEC = kNormVec<T>;
@@ -396,8 +397,9 @@ __global__ __launch_bounds__(256) void act_rows128_kernel(const uint16_t* __rest
 
 // ---- launches ----
 
-// f(threads, pieces a thread), as types: one piece a thread, and as few wavefronts as that takes, up to 16; then two or four.  8192 rows in bf16, us, 256
-// threads of several pieces / this: norm of 4096 values 49 / 44, of 7168 97 / 88, to e4m3 56 / 51, gradients 64 / 47; 64 rows of 7168 5.0 / 3.6.
+// f(threads, pieces a thread), as types: one piece a thread, and as few wavefronts as that takes, up to 16; then two or four.  8192 rows in bf16, us a call in a row, 256
+// threads of several pieces / this: norm of 4096 values 49 / 44, of 7168 97 / 88, to e4m3 56 / 51, gradients without one of the sum 64 / 47; 64 rows of
+// 7168 5.0 / 3.6.
 // (BACKWARD: for wide rows eight wavefronts, which have twice the registers each that sixteen have.)
 template <class T, bool BACKWARD, class F>
 hipError_t with_norm_shape(int H, F f) {
@@ -431,7 +433,7 @@ hipError_t launch_norm_type(const NormArgs& a, hipStream_t st) {
 }
 
 // Rows of partial sums of dw, one a workgroup: at most 1024 of up to 256 threads, fewer of more, so that 4096 wavefronts are on their way (16 a compute unit: 8192
-// rows of 4096 47 us, 52 with twice as many, 62 with half; rows of 128 threads make 2048); no more than a quarter of the rows beyond one for each
+// rows of 4096 without a gradient of the sum 47 us, 52 with twice as many, 62 with half; rows of 128 threads make 2048); no more than a quarter of the rows beyond one for each
 // compute unit; and none that has no row (of rows that a wavefront holds, a workgroup takes four).  threads = 0: the most of any.
 int64_t norm_parts(int64_t rows, int threads) {
     const int64_t filled = threads == kWave ? (rows + 3) / 4 : rows;
